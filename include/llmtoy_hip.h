@@ -62,7 +62,12 @@ enum {
     LT_TYPE_Q5_0 = 6,
     LT_TYPE_Q5_1 = 7,
     LT_TYPE_Q3_K = 11,
-    LT_TYPE_IQ4_NL = 20
+    LT_TYPE_IQ4_NL = 20,
+    /* microscaled 4-bit floating point: 17 bytes per 32 elements, a scale
+     * byte e (2^(e - 127); 255: NaN) and 16 bytes of codes, element i in the
+     * low and 16 + i in the high half of byte i; a code is a sign and one of
+     * 0, .5, 1, 1.5, 2, 3, 4, 6.  No counterpart in the reference. */
+    LT_TYPE_MXFP4 = 39
 };
 
 /* Gated-FFN activation: SiLU (ops/math.zig:37-40) or GELU-tanh (math.zig:84-88). */
@@ -132,12 +137,18 @@ int lt_tensor_read(lt_ctx *ctx, const lt_tensor *t, void *host_bytes, size_t nby
  * rotate weight copies so that timing is not served from the 256 MB cache. */
 int lt_tensor_clone(lt_ctx *ctx, const lt_tensor *src, lt_tensor **out_tensor);
 int lt_tensor_free(lt_ctx *ctx, lt_tensor *t);
+/* An MXFP4 tensor of the given shape (as lt_tensor_upload's) holding zeros, for
+ * lt_quantize to fill; other types are LT_ERR_UNSUPPORTED.  Returns when the
+ * memory is cleared. */
+int lt_tensor_create(lt_ctx *ctx, uint32_t ggml_type, size_t rows, size_t cols, size_t n_experts,
+                     lt_tensor **out_tensor);
 /* Read nbytes (a positive multiple of 16) of device memory at buf (16-byte
  * aligned) once, with a streaming kernel of 16-byte loads, on the context's
  * stream.  No counterpart in the reference: bench.py times it as the read
  * ceiling of one launch that the decode kernels' streams are set against. */
 int lt_stream_read(lt_ctx *ctx, const void *buf, size_t nbytes);
-/* Device bytes held by the tensor (equal to the GGUF byte count). */
+/* The tensor's GGUF byte count, which is what it holds on the device (MXFP4: a
+ * little more there, rows padded to 16 an expert and to 128 columns). */
 size_t lt_tensor_bytes(const lt_tensor *t);
 
 /* out[rows] = W[rows x cols] * x[cols], fp32 accumulation.  Activations are
@@ -154,10 +165,41 @@ size_t lt_tensor_bytes(const lt_tensor *t);
  * sums give, which is NaN or an infinity (Q4_K and Q6_K subtract a block's
  * offset as a sum of its own, Q8_0 has none).  Q4_K and Q6_K activations below
  * about 2^-100 lose bits (their products are kept 2^-24 of their size).
+ * MXFP4 activations are exact to 2^-24 of the largest of each 32 and any NaN or
+ * infinity makes every output NaN.
  * Replaces quantMatvec / quantMatvecPar (ops/math.zig:133-171, 277-320) and
  * MatvecSession.run / runQ8_1Mv (gpu/matvec.zig:497-647,
  * gemma4/gpu_weights.zig:1573-1607).  W must be a 2-D tensor. */
 int lt_matvec(lt_ctx *ctx, float *out, const lt_tensor *W, const float *x, uint32_t flags);
+
+/* Rows row0 .. row0 + rows - 1 of an MXFP4 tensor (counted over all experts)
+ * from x [rows][cols]; the tensor's other rows stay as they are.  Per block of
+ * 32, with a = max |x|: the scale 2^e, e = floor(log2 a) - 2 (at least -127;
+ * a = 0: the least), and each element's nearest code to x / 2^e, a tie to the
+ * even code, 6 for what lies beyond (a itself falls in [4, 8)).  A negative
+ * value that rounds to zero keeps its sign.  A block with a NaN or an infinity
+ * becomes all NaN (scale byte 255, codes 0).  rows = 0 does nothing.  A device
+ * pointer x must be 16-byte aligned.  flags: LT_HOST_IO.  No counterpart in
+ * the reference. */
+int lt_quantize(lt_ctx *ctx, lt_tensor *t, const float *x, size_t row0, size_t rows, uint32_t flags);
+/* The values of those rows of an MXFP4 tensor: out [rows][cols], exact.  A
+ * device pointer out must be 16-byte aligned.  flags: LT_HOST_IO. */
+int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size_t rows, uint32_t flags);
+
+/* out [T][rows] = X [T][cols] W^T for T vectors at once, W an MXFP4 matrix (2-D,
+ * cols <= 16384, T <= 65536), X and out fp32: prompts, batched decode.  The
+ * products take each activation as five 6-bit limbs, exact to 2^-24 of the
+ * largest of its 32-element block, and are summed in fp32: the accuracy of
+ * lt_matvec, in another order of sums.  A NaN or an infinity in a vector makes that
+ * vector's outputs NaN and leaves the others.  T = 0 does nothing.  Device
+ * pointers X and out must be 16-byte aligned; out must not overlap X.  flags:
+ * LT_HOST_IO.  The reference calls quantMatvecPar once a vector
+ * (main.zig:1916-1922). */
+int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const float *X, uint32_t T, uint32_t flags);
+/* The same with X the first T rows of a 2-D MXFP4 tensor (4-bit activations, as
+ * lt_quantize makes them): out [T][rows], about five times lt_matmul's rate on
+ * long batches.  X may be W.  flags: LT_HOST_IO (out is host memory). */
+int lt_matmul_quantized(lt_ctx *ctx, float *out, const lt_tensor *W, const lt_tensor *X, uint32_t T, uint32_t flags);
 
 /* Dense gated FFN: out[d_model] = Wd * (act(Wg x) * (Wu x)).
  * Replaces the dense-FFN matvec chain (model/forward.zig:301-308,

@@ -2,6 +2,7 @@
 // into the planar device layout, argument validation, and kernel dispatch.
 #include "llmtoy_hip.h"
 #include "lt_internal.h"
+#include "lt_mx.h"
 
 #include <stdarg.h>
 #include <stdio.h>
@@ -63,7 +64,7 @@ struct lt_ctx {
     hipStream_t stream = nullptr;
     std::string err;
     // context-owned device scratch, grown on demand
-    DevBuf x, out, logits, h, ids, w, shared, g, u, ids_io, w_io, bias, eh, pf, nrm, sink;
+    DevBuf x, out, logits, h, ids, w, shared, g, u, ids_io, w_io, bias, eh, pf, nrm, sink, mx;
     // buffers replaced by larger ones; a HIP graph captured earlier may still
     // reference them, so they are released only by lt_destroy
     std::vector<void *> retired;
@@ -292,7 +293,8 @@ size_t block_elems(uint32_t type) {
     case LT_TYPE_Q3_K: return 256;
     case LT_TYPE_Q5_0:
     case LT_TYPE_Q5_1:
-    case LT_TYPE_IQ4_NL: return 32;
+    case LT_TYPE_IQ4_NL:
+    case LT_TYPE_MXFP4: return 32;
     default: return 0;
     }
 }
@@ -307,6 +309,7 @@ size_t block_bytes(uint32_t type) {
     case LT_TYPE_Q5_1: return 24;
     case LT_TYPE_IQ4_NL: return 18;
     case LT_TYPE_Q3_K: return 110;
+    case LT_TYPE_MXFP4: return lt::kMxBlockBytes;
     default: return 0;
     }
 }
@@ -343,8 +346,35 @@ void set_planes(DevTensor &t) {
         t.p2 = t.p1 + nblk * 32;
         t.p3 = t.p2 + nblk * 12;
         break;
+    case LT_TYPE_MXFP4: {  // operand order: codes, scales
+        const lt::MxDims d = lt::mx_dims(t.rows, t.blocks_per_row);
+        t.p1 = b + lt::mx_code_bytes(d, t.n_experts);
+        break;
+    }
     default: break;
     }
+}
+
+// A tensor's shape fields; its memory is the caller's to get.
+int shape_tensor(lt_ctx *ctx, DevTensor &t, uint32_t type, size_t rows, size_t cols, size_t n_experts) {
+    const size_t be = block_elems(type), bb = block_bytes(type);
+    if (!be) return fail(ctx, LT_ERR_UNSUPPORTED, "tensor type %u not supported by the device path", type);
+    if (rows == 0 || cols == 0 || n_experts == 0) return fail(ctx, LT_ERR_INVALID, "empty shape");
+    if (cols % be) return fail(ctx, LT_ERR_UNSUPPORTED, "cols %zu not a multiple of the %zu-element block", cols, be);
+    if ((double)rows * (double)cols * (double)n_experts > 1e15) return fail(ctx, LT_ERR_INVALID, "shape beyond any memory");
+    t.type = type;
+    t.rows = rows;
+    t.cols = cols;
+    t.n_experts = n_experts;
+    t.total_rows = rows * n_experts;
+    t.blocks_per_row = cols / be;
+    t.bytes = t.total_rows * t.blocks_per_row * bb;
+    t.held = t.bytes;
+    if (type == LT_TYPE_MXFP4) {
+        const lt::MxDims d = lt::mx_dims(rows, t.blocks_per_row);
+        t.held = lt::mx_code_bytes(d, n_experts) + lt::mx_scale_bytes(d, n_experts);
+    }
+    return LT_OK;
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
@@ -519,6 +549,7 @@ int matvec_dev(lt_ctx *ctx, const DevTensor &W, const float *x, float *y) {
     case LT_TYPE_Q8_0: e = lt::launch_matvec_q8_0(W, x, y, ctx->stream); break;
     case LT_TYPE_Q6_K: e = lt::launch_matvec_q6k(W, x, y, ctx->stream); break;
     case LT_TYPE_F32: e = lt::launch_matvec_f32(W, x, y, ctx->stream); break;
+    case LT_TYPE_MXFP4: e = lt::launch_matvec_mx(W, x, y, ctx->stream); break;
     case LT_TYPE_Q5_0:
     case LT_TYPE_Q5_1:
     case LT_TYPE_IQ4_NL:
@@ -576,7 +607,7 @@ extern "C" void lt_destroy(lt_ctx *ctx) {
     (void)hipStreamSynchronize(ctx->stream);
     DevBuf *bufs[] = {&ctx->x, &ctx->out, &ctx->logits, &ctx->h, &ctx->ids, &ctx->w,
                       &ctx->shared, &ctx->g, &ctx->u, &ctx->ids_io, &ctx->w_io, &ctx->bias, &ctx->eh, &ctx->pf,
-                      &ctx->nrm, &ctx->sink};
+                      &ctx->nrm, &ctx->sink, &ctx->mx};
     for (DevBuf *b : bufs)
         if (b->p) (void)hipFree(b->p);
     for (void *p : ctx->retired) (void)hipFree(p);
@@ -613,24 +644,14 @@ extern "C" int lt_tensor_upload(lt_ctx *ctx, const void *host_bytes, size_t nbyt
                                 size_t cols, size_t n_experts, lt_tensor **out_tensor) {
     if (!ctx || !host_bytes || !out_tensor) return fail(ctx, LT_ERR_INVALID, "null argument");
     *out_tensor = nullptr;
-    const size_t be = block_elems(type), bb = block_bytes(type);
-    if (!be) return fail(ctx, LT_ERR_UNSUPPORTED, "tensor type %u not supported by the device path", type);
-    if (rows == 0 || cols == 0 || n_experts == 0) return fail(ctx, LT_ERR_INVALID, "empty shape");
-    if (cols % be) return fail(ctx, LT_ERR_UNSUPPORTED, "cols %zu not a multiple of the %zu-element block", cols, be);
-    const size_t total_rows = rows * n_experts;
-    const size_t want = total_rows * (cols / be) * bb;
-    if (nbytes != want) return fail(ctx, LT_ERR_INVALID, "nbytes %zu != expected %zu", nbytes, want);
-    lt_tensor *t = new (std::nothrow) lt_tensor();
+    DevTensor shape{};
+    int rc = shape_tensor(ctx, shape, type, rows, cols, n_experts);
+    if (rc) return rc;
+    if (nbytes != shape.bytes) return fail(ctx, LT_ERR_INVALID, "nbytes %zu != expected %zu", nbytes, shape.bytes);
+    lt_tensor *t = new (std::nothrow) lt_tensor{shape};
     if (!t) return fail(ctx, LT_ERR_OOM, "host allocation failed");
-    t->t.type = type;
-    t->t.rows = rows;
-    t->t.cols = cols;
-    t->t.n_experts = n_experts;
-    t->t.total_rows = total_rows;
-    t->t.bytes = nbytes;
-    t->t.blocks_per_row = cols / be;
     hipError_t e = hipSetDevice(ctx->device);
-    if (e == hipSuccess) e = hipMalloc((void **)&t->t.base, nbytes);
+    if (e == hipSuccess) e = hipMalloc((void **)&t->t.base, t->t.held);
     if (e != hipSuccess) {
         delete t;
         return hip_fail(ctx, e, "hipMalloc(tensor)");
@@ -641,6 +662,33 @@ extern "C" int lt_tensor_upload(lt_ctx *ctx, const void *host_bytes, size_t nbyt
         (void)hipFree(t->t.base);
         delete t;
         return hip_fail(ctx, e, "tensor upload");
+    }
+    *out_tensor = t;
+    return LT_OK;
+}
+
+extern "C" int lt_tensor_create(lt_ctx *ctx, uint32_t type, size_t rows, size_t cols, size_t n_experts,
+                                lt_tensor **out_tensor) {
+    if (!ctx || !out_tensor) return fail(ctx, LT_ERR_INVALID, "null argument");
+    *out_tensor = nullptr;
+    if (type != LT_TYPE_MXFP4) return fail(ctx, LT_ERR_UNSUPPORTED, "tensors of type %u cannot be filled on the device", type);
+    DevTensor shape{};
+    int rc = shape_tensor(ctx, shape, type, rows, cols, n_experts);
+    if (rc) return rc;
+    lt_tensor *t = new (std::nothrow) lt_tensor{shape};
+    if (!t) return fail(ctx, LT_ERR_OOM, "host allocation failed");
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e == hipSuccess) e = hipMalloc((void **)&t->t.base, t->t.held);
+    if (e != hipSuccess) {
+        delete t;
+        return hip_fail(ctx, e, "hipMalloc(tensor)");
+    }
+    set_planes(t->t);
+    e = lt::zero_tensor(ctx->up, t->t);
+    if (e != hipSuccess) {
+        (void)hipFree(t->t.base);
+        delete t;
+        return hip_fail(ctx, e, "tensor clear");
     }
     *out_tensor = t;
     return LT_OK;
@@ -659,8 +707,8 @@ extern "C" int lt_tensor_clone(lt_ctx *ctx, const lt_tensor *src, lt_tensor **ou
     if (!ctx || !src || !out_tensor) return fail(ctx, LT_ERR_INVALID, "null argument");
     lt_tensor *t = new (std::nothrow) lt_tensor(*src);
     if (!t) return fail(ctx, LT_ERR_OOM, "host allocation failed");
-    hipError_t e = hipMalloc((void **)&t->t.base, src->t.bytes);
-    if (e == hipSuccess) e = hipMemcpy(t->t.base, src->t.base, src->t.bytes, hipMemcpyDeviceToDevice);
+    hipError_t e = hipMalloc((void **)&t->t.base, src->t.held);
+    if (e == hipSuccess) e = hipMemcpy(t->t.base, src->t.base, src->t.held, hipMemcpyDeviceToDevice);
     if (e != hipSuccess) {
         if (t->t.base != src->t.base) (void)hipFree(t->t.base);
         delete t;
@@ -717,6 +765,124 @@ extern "C" int lt_matvec(lt_ctx *ctx, float *out, const lt_tensor *W, const floa
 
 namespace {
 
+int check_rows(lt_ctx *ctx, const DevTensor &T, size_t row0, size_t rows, const void *p, uint32_t flags) {
+    if (T.type != LT_TYPE_MXFP4)
+        return fail(ctx, LT_ERR_UNSUPPORTED, "tensor type %u: only MXFP4 is quantised and read by rows", T.type);
+    if (row0 > T.total_rows || rows > T.total_rows - row0)
+        return fail(ctx, LT_ERR_INVALID, "rows %zu + %zu of a tensor of %zu", row0, rows, T.total_rows);
+    if (flags & ~(uint32_t)LT_HOST_IO) return fail(ctx, LT_ERR_INVALID, "unknown flags 0x%x", flags & ~(uint32_t)LT_HOST_IO);
+    if (!(flags & LT_HOST_IO) && !aligned16(p)) return fail(ctx, LT_ERR_INVALID, "the array must be 16-byte aligned");
+    return LT_OK;
+}
+
+}  // namespace
+
+extern "C" int lt_quantize(lt_ctx *ctx, lt_tensor *t, const float *x, size_t row0, size_t rows, uint32_t flags) {
+    if (!ctx || !t || !x) return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_rows(ctx, t->t, row0, rows, x, flags);
+    if (rc || rows == 0) return rc;
+    Span span_(ctx, "lt_quantize");
+    const float *dx = x;
+    if ((flags & LT_HOST_IO) && (rc = stage_in(ctx, ctx->x, x, rows * t->t.cols * 4, (const void **)&dx))) return rc;
+    if ((rc = launch_rc(ctx, lt::launch_mx_quantize(t->t, dx, row0, rows, ctx->stream), "quantize"))) return rc;
+    if (flags & LT_HOST_IO) {
+        if ((rc = host_sync(ctx))) return rc;
+        prof_harvest(ctx);
+    }
+    return LT_OK;
+}
+
+extern "C" int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size_t rows, uint32_t flags) {
+    if (!ctx || !t || !out) return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_rows(ctx, t->t, row0, rows, out, flags);
+    if (rc || rows == 0) return rc;
+    Span span_(ctx, "lt_dequantize");
+    const size_t bytes = rows * t->t.cols * 4;
+    float *dy = out;
+    if (flags & LT_HOST_IO) {
+        if ((rc = ensure(ctx, ctx->out, bytes))) return rc;
+        dy = (float *)ctx->out.p;
+    }
+    if ((rc = launch_rc(ctx, lt::launch_mx_dequantize(t->t, dy, row0, rows, ctx->stream), "dequantize"))) return rc;
+    if (flags & LT_HOST_IO) {
+        if ((rc = host_out(ctx, out, dy, bytes))) return rc;
+        prof_harvest(ctx);
+    }
+    return LT_OK;
+}
+
+namespace {
+
+constexpr uint32_t kMaxVectors = 65536;
+
+// What both batched products ask of their arguments.
+int check_matmul(lt_ctx *ctx, const DevTensor &W, uint32_t T, const float *out, uint32_t flags) {
+    if (W.type != LT_TYPE_MXFP4) return fail(ctx, LT_ERR_UNSUPPORTED, "matmul: type %u (device path: MXFP4)", W.type);
+    if (W.n_experts != 1) return fail(ctx, LT_ERR_INVALID, "matmul: W must be a 2-D tensor");
+    if (W.cols > kMaxQuantCols) return fail(ctx, LT_ERR_UNSUPPORTED, "row length %zu exceeds %zu", W.cols, kMaxQuantCols);
+    if (T > kMaxVectors) return fail(ctx, LT_ERR_INVALID, "T=%u out of range (0..%u)", T, kMaxVectors);
+    if (flags & ~(uint32_t)LT_HOST_IO) return fail(ctx, LT_ERR_INVALID, "unknown flags 0x%x", flags & ~(uint32_t)LT_HOST_IO);
+    if (!(flags & LT_HOST_IO) && !aligned16(out)) return fail(ctx, LT_ERR_INVALID, "out must be 16-byte aligned");
+    return LT_OK;
+}
+
+}  // namespace
+
+extern "C" int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const float *X, uint32_t T, uint32_t flags) {
+    if (!ctx || !out || !W || !X) return fail(ctx, LT_ERR_INVALID, "null argument");
+    const DevTensor &w = W->t;
+    int rc = check_matmul(ctx, w, T, out, flags);
+    if (rc) return rc;
+    const bool host = flags & LT_HOST_IO;
+    if (!host && !aligned16(X)) return fail(ctx, LT_ERR_INVALID, "X must be 16-byte aligned");
+    if (T == 0) return LT_OK;
+    Span span_(ctx, "lt_matmul");
+    const size_t bytes = (size_t)T * w.rows * 4;
+    const float *dx = X;
+    float *dy = out;
+    if (host) {
+        if ((rc = stage_in(ctx, ctx->x, X, (size_t)T * w.cols * 4, (const void **)&dx))) return rc;
+        if ((rc = ensure(ctx, ctx->out, bytes))) return rc;
+        dy = (float *)ctx->out.p;
+    }
+    if ((rc = ensure(ctx, ctx->mx, lt::matmul_mx_workspace(T, w.cols)))) return rc;
+    if ((rc = launch_rc(ctx, lt::launch_matmul_mx(w, dx, T, ctx->mx.p, dy, ctx->stream), "matmul"))) return rc;
+    if (host) {
+        if ((rc = host_out(ctx, out, dy, bytes))) return rc;
+        prof_harvest(ctx);
+    }
+    return LT_OK;
+}
+
+extern "C" int lt_matmul_quantized(lt_ctx *ctx, float *out, const lt_tensor *W, const lt_tensor *X, uint32_t T,
+                                   uint32_t flags) {
+    if (!ctx || !out || !W || !X) return fail(ctx, LT_ERR_INVALID, "null argument");
+    const DevTensor &w = W->t, &x = X->t;
+    int rc = check_matmul(ctx, w, T, out, flags);
+    if (rc) return rc;
+    if (x.type != LT_TYPE_MXFP4) return fail(ctx, LT_ERR_UNSUPPORTED, "matmul: X of type %u (device path: MXFP4)", x.type);
+    if (x.n_experts != 1 || x.cols != w.cols || T > x.rows)
+        return fail(ctx, LT_ERR_INVALID, "matmul: X is %zux%zux%zu, %u rows of %zu are needed", x.n_experts, x.rows, x.cols, T,
+                    w.cols);
+    if (T == 0) return LT_OK;
+    Span span_(ctx, "lt_matmul_quantized");
+    const size_t bytes = (size_t)T * w.rows * 4;
+    const bool host = flags & LT_HOST_IO;
+    float *dy = out;
+    if (host) {
+        if ((rc = ensure(ctx, ctx->out, bytes))) return rc;
+        dy = (float *)ctx->out.p;
+    }
+    if ((rc = launch_rc(ctx, lt::launch_matmul_mx_mx(w, x, T, dy, ctx->stream), "matmul_quantized"))) return rc;
+    if (host) {
+        if ((rc = host_out(ctx, out, dy, bytes))) return rc;
+        prof_harvest(ctx);
+    }
+    return LT_OK;
+}
+
+namespace {
+
 // act(g) * u elementwise, zero tail to n_out (generic dense-FFN path).
 __global__ void k_act_mul(const float *g, const float *u, int n, int n_out, uint32_t act, float *h) {
     int i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -741,6 +907,8 @@ int ffn_dense_dev(lt_ctx *ctx, const DevTensor &G, const DevTensor &U, const Dev
     if (G.type == LT_TYPE_Q8_0 && U.type == LT_TYPE_Q8_0 && Kd == F) {
         if ((rc = launch_rc(ctx, lt::launch_gate_up_q8_0(G, U, x, act, h, ctx->stream), "gate_up_q8_0")))
             return rc;
+    } else if (G.type == LT_TYPE_MXFP4 && U.type == LT_TYPE_MXFP4 && G.n_experts == 1 && U.n_experts == 1) {
+        if ((rc = launch_rc(ctx, lt::launch_gate_up_mx(G, U, x, act, (uint32_t)Kd, h, ctx->stream), "gate_up_mx"))) return rc;
     } else {
         if ((rc = ensure(ctx, ctx->g, F * 4)) || (rc = ensure(ctx, ctx->u, F * 4))) return rc;
         if ((rc = matvec_dev(ctx, G, x, (float *)ctx->g.p))) return rc;
@@ -854,19 +1022,19 @@ int copy_routing_out(lt_ctx *ctx, uint32_t k, uint32_t *ids, float *w, bool host
     return LT_OK;
 }
 
-// Expert formats: Q4_K (tuned kernels, single-launch layer) and the Gemma4
-// APEX formats Q3_K, Q5_0, Q5_1, IQ4_NL (lt_formats.hip).
+// Expert formats: Q4_K (tuned kernels, single-launch layer), the Gemma4 APEX
+// formats Q3_K, Q5_0, Q5_1, IQ4_NL (lt_formats.hip) and MXFP4 (lt_mx_matvec.hip).
 bool is_fmt(uint32_t t) {
     return t == LT_TYPE_Q5_0 || t == LT_TYPE_Q5_1 || t == LT_TYPE_IQ4_NL || t == LT_TYPE_Q3_K;
 }
-bool expert_type_ok(uint32_t t) { return t == LT_TYPE_Q4_K || is_fmt(t); }
+bool expert_type_ok(uint32_t t) { return t == LT_TYPE_Q4_K || t == LT_TYPE_MXFP4 || is_fmt(t); }
 
 int check_experts(lt_ctx *ctx, const lt_tensor *gate_up, const lt_tensor *down, size_t d_model, uint32_t d_expert,
                   size_t n_experts, uint32_t k = 0) {
     if (!gate_up || !down) return fail(ctx, LT_ERR_INVALID, "null expert tensor");
     const DevTensor &GU = gate_up->t, &D = down->t;
     if (!expert_type_ok(GU.type) || !expert_type_ok(D.type))
-        return fail(ctx, LT_ERR_UNSUPPORTED, "expert types %u/%u (device expert path: Q4_K, Q3_K, Q5_0, Q5_1, IQ4_NL)",
+        return fail(ctx, LT_ERR_UNSUPPORTED, "expert types %u/%u (device expert path: Q4_K, Q3_K, Q5_0, Q5_1, IQ4_NL, MXFP4)",
                     GU.type, D.type);
     if (GU.cols != d_model || GU.rows != 2 * (size_t)d_expert)
         return fail(ctx, LT_ERR_INVALID, "gate_up per-expert shape %zux%zu != %ux%zu", GU.rows, GU.cols,
@@ -881,10 +1049,17 @@ int check_experts(lt_ctx *ctx, const lt_tensor *gate_up, const lt_tensor *down, 
         return fail(ctx, LT_ERR_UNSUPPORTED, "d_model %zu too long for the gate/up kernel", GU.cols);
     if (D.type == LT_TYPE_Q4_K && D.blocks_per_row > 16)
         return fail(ctx, LT_ERR_UNSUPPORTED, "down row length %zu > 4096", D.cols);
+    if (D.type == LT_TYPE_MXFP4 && D.cols > kMaxQuantCols)
+        return fail(ctx, LT_ERR_UNSUPPORTED, "down row length %zu > %zu", D.cols, kMaxQuantCols);
     if (is_fmt(D.type) && (size_t)(k ? k : 1) * D.cols > 16384)
         return fail(ctx, LT_ERR_UNSUPPORTED, "k * down row length %zu > 16384 (LDS staging of h)",
                     (size_t)(k ? k : 1) * D.cols);
     return LT_OK;
+}
+
+// Whether the gate/up kernel selects the experts itself (else the router does).
+bool gate_up_routes(const DevTensor &GU, size_t n_experts) {
+    return n_experts <= kRoutedGateUpMaxExperts && GU.type != LT_TYPE_MXFP4;
 }
 
 // gate/up of the k selected experts into h [k][Kd] (ids on the device)
@@ -893,6 +1068,9 @@ int gate_up_dev(lt_ctx *ctx, const DevTensor &GU, const float *x, const uint32_t
     if (GU.type == LT_TYPE_Q4_K)
         return launch_rc(ctx, lt::launch_expert_gate_up_q4k(GU, x, ids, k, d_expert, Kd, act, h, ctx->stream),
                          "expert_gate_up");
+    if (GU.type == LT_TYPE_MXFP4)
+        return launch_rc(ctx, lt::launch_expert_gate_up_mx(GU, x, ids, k, d_expert, Kd, act, h, ctx->stream),
+                         "expert_gate_up_mx");
     return launch_rc(ctx, lt::launch_expert_gate_up_fmt(GU, x, ids, k, d_expert, Kd, act, h, ctx->stream),
                      "expert_gate_up_fmt");
 }
@@ -920,6 +1098,9 @@ int down_dev(lt_ctx *ctx, const DevTensor &D, const float *h, const uint32_t *id
     if (D.type == LT_TYPE_Q4_K)
         return launch_rc(ctx, lt::launch_expert_down_q4k(D, h, ids, w, k, base, accumulate, out, ctx->stream, dscale),
                          "expert_down");
+    if (D.type == LT_TYPE_MXFP4)
+        return launch_rc(ctx, lt::launch_expert_down_mx(D, h, ids, w, k, base, accumulate, dscale, out, ctx->stream),
+                         "expert_down_mx");
     return launch_rc(ctx, lt::launch_expert_down_fmt(D, h, ids, w, k, base, accumulate, dscale, out, ctx->stream),
                      "expert_down_fmt");
 }
@@ -1002,6 +1183,8 @@ extern "C" int lt_expert_down_id(lt_ctx *ctx, const lt_tensor *down, const float
     if (!expert_type_ok(D.type)) return fail(ctx, LT_ERR_UNSUPPORTED, "down type %u not on the device path", D.type);
     if (D.type == LT_TYPE_Q4_K && D.blocks_per_row > 16)
         return fail(ctx, LT_ERR_UNSUPPORTED, "down row length %zu > 4096", D.cols);
+    if (D.type == LT_TYPE_MXFP4 && D.cols > kMaxQuantCols)
+        return fail(ctx, LT_ERR_UNSUPPORTED, "down row length %zu > %zu", D.cols, kMaxQuantCols);
     if (is_fmt(D.type) && (size_t)k * D.cols > 16384)
         return fail(ctx, LT_ERR_UNSUPPORTED, "k * down row length > 16384 (LDS staging of h)");
     const bool host = flags & LT_HOST_IO;
@@ -1119,7 +1302,7 @@ int moe_dev(lt_ctx *ctx, float *out, const float *x, const DevTensor &R, const f
     }
     if ((rc = ensure(ctx, ctx->eh, (size_t)k * Kd * 4))) return rc;
     float *h = (float *)ctx->eh.p;
-    if (R.total_rows <= kRoutedGateUpMaxExperts) {
+    if (gate_up_routes(GU, R.total_rows)) {
         // logits only; each gate/up block selects its expert from them
         if ((rc = router_dev(ctx, R, x, bias, 0, flags, r))) return rc;
         rc = gate_up_routed_dev(ctx, GU, x, k, (flags & LT_MOE_NORM_TOPK) ? 1u : 0u, d_expert, (uint32_t)Kd, act, h,
@@ -1528,7 +1711,7 @@ extern "C" int lt_gemma4_moe_block(lt_ctx *ctx, float *x, const float *dense_ffn
     if ((rc = ensure(ctx, ctx->eh, (size_t)k * Kd * 4))) return rc;
     float *h = (float *)ctx->eh.p;
     const uint32_t norm = (flags & LT_MOE_NORM_TOPK) ? 1u : 0u;
-    if (E <= kRoutedGateUpMaxExperts) {
+    if (gate_up_routes(GU, E)) {
         if ((rc = router_dev(ctx, R, rin, nullptr, 0, flags, r, nullptr, fuse_prep ? &prep : nullptr))) return rc;
         rc = gate_up_routed_dev(ctx, GU, moe_in, k, norm, d_expert, (uint32_t)Kd, act, h, r);
     } else {

@@ -19,6 +19,8 @@
 //   Q3_K  qs [R][nsb][64], hmask [R][nsb][32], scales [R][nsb][12],
 //         d [R][nsb]                                      (110 B / 256)
 //   F32   [R][cols]
+//   MXFP4 codes and scales in the matrix instructions' operand order, rows
+//         padded to 16 an expert and blocks to 4 (lt_mx.h)  (17 B / 32)
 //
 // R = n_experts * rows (expert e owns rows [e*rows, (e+1)*rows)).
 #pragma once
@@ -38,11 +40,12 @@ struct DevTensor {
     size_t cols;        // GGUF row length (elements)
     size_t n_experts;   // 1 for 2-D tensors
     size_t total_rows;  // n_experts * rows
-    size_t bytes;       // == GGUF byte count
+    size_t bytes;       // GGUF byte count
+    size_t held;        // device bytes (== bytes, but for MXFP4's padding)
     uint8_t *base;      // device allocation (256-byte aligned)
     // plane pointers (into base)
-    const uint8_t *p0;  // Q4_K hdr | Q8_0 qs | Q6_K ql | F32 data
-    const uint8_t *p1;  // Q4_K qs  | Q8_0 d  | Q6_K qh
+    const uint8_t *p0;  // Q4_K hdr | Q8_0 qs | Q6_K ql | F32 data | MXFP4 codes
+    const uint8_t *p1;  // Q4_K qs  | Q8_0 d  | Q6_K qh | MXFP4 scales
     const uint8_t *p2;  // Q6_K sc
     const uint8_t *p3;  // Q6_K d
     size_t blocks_per_row;  // nsb (K-quants) or nb (Q8_0)
@@ -310,6 +313,7 @@ struct UploadStaging {
 };
 // t.base must hold t.bytes; src holds the tensor's GGUF blocks.  Returns
 // after every copy has finished.
+hipError_t zero_tensor(UploadStaging &S, const DevTensor &t);  // all held bytes; returns when done
 hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const uint8_t *src);
 // The inverse: the tensor's GGUF blocks into dst (t.bytes bytes).
 hipError_t download_planar(UploadStaging &S, const DevTensor &t, uint8_t *dst);
@@ -351,6 +355,27 @@ hipError_t launch_expert_gate_up_fmt_routed(const DevTensor &GU, const float *x,
 hipError_t launch_expert_down_fmt(const DevTensor &D, const float *h, const uint32_t *ids, const float *w,
                                   uint32_t k, const float *base, int accumulate, const float *dscale, float *out,
                                   hipStream_t s);
+// MXFP4 (lt_mx_quant.hip, lt_mx_matvec.hip, lt_mx_matmul.hip).  raw: nblk GGUF
+// blocks, blk0 .. of the tensor, readable and writable up to 3 bytes past
+// them; row0: over all experts' rows.
+constexpr uint32_t kMxBlockBytes = 17;
+hipError_t launch_mx_blocks(const DevTensor &t, uint8_t *raw, size_t nblk, size_t blk0, bool in, hipStream_t s);
+hipError_t launch_mx_quantize(const DevTensor &t, const float *x, size_t row0, size_t rows, hipStream_t s);
+hipError_t launch_mx_dequantize(const DevTensor &t, float *out, size_t row0, size_t rows, hipStream_t s);
+hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s);
+// act(G x) * (U x) of two 2-D tensors of the same shape, zeros from their rows to down_cols
+hipError_t launch_gate_up_mx(const DevTensor &G, const DevTensor &U, const float *x, uint32_t act, uint32_t down_cols,
+                             float *h, hipStream_t s);
+// Selected experts: row lengths up to 16384, any k and sizes.
+hipError_t launch_expert_gate_up_mx(const DevTensor &GU, const float *x, const uint32_t *ids, uint32_t k, uint32_t d_expert,
+                                    uint32_t down_cols, uint32_t act, float *h, hipStream_t s);
+hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint32_t *ids, const float *w, uint32_t k,
+                                 const float *base, int accumulate, const float *dscale, float *out, hipStream_t s);
+// out [T][rows] = X [T][cols] W^T; ws: matmul_mx_workspace(T, cols) bytes.
+size_t matmul_mx_workspace(size_t T, size_t cols);
+hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *ws, float *out, hipStream_t s);
+// The same with X the first T rows of an MXFP4 tensor.
+hipError_t launch_matmul_mx_mx(const DevTensor &W, const DevTensor &X, size_t T, float *out, hipStream_t s);
 hipError_t launch_gate_up_q8_0(const DevTensor &Wg, const DevTensor &Wu, const float *x, uint32_t act,
                                float *h, hipStream_t s);
 // Router logits (F32 or Q8_0 router, exact reference order) plus softmax /

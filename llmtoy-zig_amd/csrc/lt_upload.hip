@@ -162,16 +162,24 @@ void free_staging(UploadStaging &S) {
     S.workers = 0;
 }
 
+hipError_t zero_tensor(UploadStaging &S, const DevTensor &t) {
+    hipError_t e = ensure_staging(S, 1);
+    if (e == hipSuccess) e = hipMemsetAsync(t.base, 0, t.held, S.st[0]);
+    if (e == hipSuccess) e = hipStreamSynchronize(S.st[0]);
+    return e;
+}
+
 hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const uint8_t *src) {
     PlaneArgs pa{};
-    const bool f32 = t.type == LT_TYPE_F32;
-    if (!f32 && !plane_args(t, pa)) return hipErrorInvalidValue;
-    const uint32_t bb = f32 ? 4u : pa.bb;
+    const bool f32 = t.type == LT_TYPE_F32, mx = t.type == LT_TYPE_MXFP4;
+    if (!f32 && !mx && !plane_args(t, pa)) return hipErrorInvalidValue;
+    const uint32_t bb = f32 ? 4u : mx ? kMxBlockBytes : pa.bb;
     const size_t nblk = t.bytes / bb, CH = chunk_blocks(bb);
     if (nblk * bb != t.bytes || CH == 0) return hipErrorInvalidValue;
     const size_t nchunks = (nblk + CH - 1) / CH;
     const int W = (int)std::min<size_t>(kUpWorkers, nchunks);
     hipError_t e = ensure_staging(S, W);
+    if (e == hipSuccess && mx) e = zero_tensor(S, t);  // the padding of rows and blocks
     if (e != hipSuccess) return e;
     std::atomic<int> err{(int)hipSuccess};
 
@@ -190,7 +198,9 @@ hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const
                 e = hipMemcpyAsync(t.base + first * bb, S.pinned[slot], nb * bb, hipMemcpyHostToDevice, S.st[w]);
             } else {
                 e = hipMemcpyAsync(S.dev[slot], S.pinned[slot], nb * bb, hipMemcpyHostToDevice, S.st[w]);
-                if (e == hipSuccess) {
+                if (e == hipSuccess && mx) {
+                    e = launch_mx_blocks(t, S.dev[slot], nb, first, true, S.st[w]);
+                } else if (e == hipSuccess) {
                     k_blocks_to_planes<<<(unsigned)((nb + kBlkPerWG - 1) / kBlkPerWG), 256, 0, S.st[w]>>>(
                         S.dev[slot], nb, first, pa);
                     e = hipGetLastError();
@@ -218,9 +228,9 @@ hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const
 
 hipError_t download_planar(UploadStaging &S, const DevTensor &t, uint8_t *dst) {
     PlaneArgs pa{};
-    const bool f32 = t.type == LT_TYPE_F32;
-    if (!f32 && !plane_args(t, pa)) return hipErrorInvalidValue;
-    const uint32_t bb = f32 ? 4u : pa.bb;
+    const bool f32 = t.type == LT_TYPE_F32, mx = t.type == LT_TYPE_MXFP4;
+    if (!f32 && !mx && !plane_args(t, pa)) return hipErrorInvalidValue;
+    const uint32_t bb = f32 ? 4u : mx ? kMxBlockBytes : pa.bb;
     const size_t nblk = t.bytes / bb, CH = chunk_blocks(bb);
     if (nblk * bb != t.bytes || CH == 0) return hipErrorInvalidValue;
     hipError_t e = ensure_staging(S, 1);
@@ -229,9 +239,13 @@ hipError_t download_planar(UploadStaging &S, const DevTensor &t, uint8_t *dst) {
         if (f32) {
             e = hipMemcpyAsync(S.pinned[0], t.base + first * bb, nb * bb, hipMemcpyDeviceToHost, S.st[0]);
         } else {
-            k_planes_to_blocks<<<(unsigned)((nb + kBlkPerWG - 1) / kBlkPerWG), 256, 0, S.st[0]>>>(S.dev[0], nb,
-                                                                                               first, pa);
-            e = hipGetLastError();
+            if (mx) {
+                e = launch_mx_blocks(t, S.dev[0], nb, first, false, S.st[0]);
+            } else {
+                k_planes_to_blocks<<<(unsigned)((nb + kBlkPerWG - 1) / kBlkPerWG), 256, 0, S.st[0]>>>(S.dev[0], nb,
+                                                                                                   first, pa);
+                e = hipGetLastError();
+            }
             if (e == hipSuccess)
                 e = hipMemcpyAsync(S.pinned[0], S.dev[0], nb * bb, hipMemcpyDeviceToHost, S.st[0]);
         }

@@ -115,6 +115,7 @@ inline BlockSize block_size(uint32_t type) {
     case 18: return {98, 256};  // iq3_xxs
     case 21: return {110, 256}; // iq3_s
     case 20: return {18, 32};   // iq4_nl
+    case 39: return {17, 32};   // mxfp4 (no counterpart in the reference)
     case 23: return {136, 256}; // iq4_xs
     case 19: return {50, 256};  // iq1_s
     case 29: return {56, 256};  // iq1_m

@@ -48,7 +48,8 @@ namespace llmtoy {
 
 // GgmlType ids (gguf/types.zig:23-53) of the formats on this path.
 enum class GgmlType : uint32_t {
-    f32 = 0, f16 = 1, q5_0 = 6, q5_1 = 7, q8_0 = 8, q3_k = 11, q4_k = 12, q6_k = 14, iq4_nl = 20
+    f32 = 0, f16 = 1, q5_0 = 6, q5_1 = 7, q8_0 = 8, q3_k = 11, q4_k = 12, q6_k = 14, iq4_nl = 20,
+    mxfp4 = 39  // microscaled 4-bit floating point (no counterpart in the reference)
 };
 
 enum class Error { Unsupported, Invalid, NotOnGpu, ExpertNotOnGpu, Device, OutOfMemory };
@@ -91,6 +92,7 @@ inline size_t rowBytes(GgmlType t, size_t cols) {
     case GgmlType::q5_0: return (cols / 32) * 22;
     case GgmlType::q5_1: return (cols / 32) * 24;
     case GgmlType::iq4_nl: return (cols / 32) * 18;
+    case GgmlType::mxfp4: return (cols / 32) * 17;
     case GgmlType::q3_k: return (cols / 256) * 110;
     }
     throw Exception(Error::Unsupported, LT_ERR_UNSUPPORTED, "unsupported quant type in rowBytes");
@@ -262,7 +264,8 @@ class MatvecSession {
     static std::optional<MatvecSession> initFromRaw(GpuContext &g, const RawMatrix &m) {
         switch (m.type) {
         case GgmlType::f32: case GgmlType::q8_0: case GgmlType::q4_k: case GgmlType::q6_k:
-        case GgmlType::q5_0: case GgmlType::q5_1: case GgmlType::iq4_nl: case GgmlType::q3_k: break;
+        case GgmlType::q5_0: case GgmlType::q5_1: case GgmlType::iq4_nl: case GgmlType::q3_k:
+        case GgmlType::mxfp4: break;
         default: return std::nullopt;
         }
         try {
@@ -293,7 +296,7 @@ class GpuWeights {
             down_ = g.tensor(down_exps, n_experts);
             auto ok = [](GgmlType t) {
                 return t == GgmlType::q4_k || t == GgmlType::q3_k || t == GgmlType::q5_0 || t == GgmlType::q5_1 ||
-                       t == GgmlType::iq4_nl;
+                       t == GgmlType::iq4_nl || t == GgmlType::mxfp4;
             };
             on_gpu_ = ok(gate_up_exps.type) && ok(down_exps.type);
         } catch (const Exception &e) {

@@ -47,7 +47,7 @@ BLOCK = {
     0: (4, 1), 1: (2, 1), 30: (2, 1), 24: (1, 1), 25: (2, 1), 26: (4, 1), 27: (8, 1),
     2: (18, 32), 3: (20, 32), 6: (22, 32), 7: (24, 32), 8: (34, 32), 9: (40, 32),
     10: (84, 256), 11: (110, 256), 12: (144, 256), 13: (176, 256), 14: (210, 256), 15: (292, 256),
-    16: (66, 256), 17: (74, 256), 22: (82, 256), 18: (98, 256), 21: (110, 256), 20: (18, 32),
+    16: (66, 256), 17: (74, 256), 22: (82, 256), 18: (98, 256), 21: (110, 256), 20: (18, 32), 39: (17, 32),
     23: (136, 256), 19: (50, 256), 29: (56, 256),
 }
 

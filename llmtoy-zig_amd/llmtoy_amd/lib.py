@@ -67,7 +67,7 @@ _ERRS = {LT_ERR_UNSUPPORTED: UnsupportedError, LT_ERR_INVALID: InvalidError, LT_
 
 EXPORTS = [
     "lt_init", "lt_destroy", "lt_last_error", "lt_sync", "lt_stream", "lt_tensor_upload", "lt_tensor_read", "lt_tensor_clone",
-    "lt_tensor_free", "lt_tensor_bytes", "lt_stream_read", "lt_matvec", "lt_ffn_dense", "lt_moe_router_topk", "lt_expert_gate_up_id",
+    "lt_tensor_free", "lt_tensor_create", "lt_quantize", "lt_dequantize", "lt_matmul", "lt_matmul_quantized", "lt_tensor_bytes", "lt_stream_read", "lt_matvec", "lt_ffn_dense", "lt_moe_router_topk", "lt_expert_gate_up_id",
     "lt_expert_down_id", "lt_moe_forward", "lt_moe_forward_noalloc", "lt_moe_prefill", "lt_rmsnorm", "lt_add_rmsnorm",
     "lt_rmsnorm_weighted_raw_scaled", "lt_moe_tail", "lt_gemma4_moe_block", "lt_profile_report",
 ]
@@ -94,6 +94,11 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "lt_tensor_read": (i32, [vp, vp, vp, sz]),
         "lt_tensor_clone": (i32, [vp, vp, C.POINTER(vp)]),
         "lt_tensor_free": (i32, [vp, vp]),
+        "lt_tensor_create": (i32, [vp, u32, sz, sz, sz, C.POINTER(vp)]),
+        "lt_quantize": (i32, [vp, vp, vp, sz, sz, u32]),
+        "lt_dequantize": (i32, [vp, vp, vp, sz, sz, u32]),
+        "lt_matmul": (i32, [vp, vp, vp, vp, u32, u32]),
+        "lt_matmul_quantized": (i32, [vp, vp, vp, vp, u32, u32]),
         "lt_tensor_bytes": (sz, [vp]),
         "lt_stream_read": (i32, [vp, vp, sz]),
         "lt_matvec": (i32, [vp, vp, vp, vp, u32]),
@@ -219,6 +224,34 @@ class Context:
                                                n_experts, C.byref(h)))
         return Tensor(self, h, ggml_type, rows, cols, n_experts)
 
+    def create(self, ggml_type: int, rows: int, cols: int, n_experts: int = 1) -> Tensor:
+        """A tensor of zeros (MXFP4) for quantize() to fill."""
+        h = C.c_void_p()
+        self._check(self.lib.lt_tensor_create(self.ptr, ggml_type, rows, cols, n_experts, C.byref(h)))
+        return Tensor(self, h, ggml_type, rows, cols, n_experts)
+
+    def quantize(self, t: Tensor, x, row0: int = 0):
+        """Rows row0 .. of the MXFP4 tensor t from x ([cols] or [rows, cols], float32)."""
+        rows = self._rows_of(x, t.cols)
+        self._check(self.lib.lt_quantize(self.ptr, t.handle, _ptr(x)[0], row0, rows, self._io(x)))
+        return t
+
+    def dequantize(self, out, t: Tensor, row0: int = 0):
+        """The values of rows row0 .. of the MXFP4 tensor t into out ([cols] or [rows, cols], float32)."""
+        rows = self._rows_of(out, t.cols)
+        self._check(self.lib.lt_dequantize(self.ptr, _ptr(out)[0], t.handle, row0, rows, self._io(out)))
+        return out
+
+    @staticmethod
+    def _rows_of(a, cols: int) -> int:
+        """Rows of a float32 array [cols] or [rows, cols]."""
+        shape = tuple(a.shape)
+        if "float32" not in str(a.dtype):
+            raise InvalidError(f"float32 array expected, got {a.dtype}")
+        if len(shape) not in (1, 2) or shape[-1] != cols:
+            raise InvalidError(f"array of shape {shape}, rows of {cols} expected")
+        return shape[0] if len(shape) == 2 else 1
+
     # ---- op-level mirror ------------------------------------------------
     def _io(self, *arrays):
         kinds = {_ptr(a)[1] for a in arrays if a is not None}
@@ -230,6 +263,18 @@ class Context:
         """out[rows] = W . x (quantMatvec, ops/math.zig:133-171)."""
         fl = self._io(out, x)
         self._check(self.lib.lt_matvec(self.ptr, _ptr(out)[0], W.handle, _ptr(x)[0], fl))
+        return out
+
+    def quant_matmul(self, out, W: Tensor, X):
+        """out [T, rows] = X [T, cols] . W^T for an MXFP4 matrix W (lt_matmul); X may be an MXFP4
+        Tensor, of which the first T rows are taken (lt_matmul_quantized)."""
+        T = self._rows_of(out, W.rows)
+        if isinstance(X, Tensor):
+            self._check(self.lib.lt_matmul_quantized(self.ptr, _ptr(out)[0], W.handle, X.handle, T, self._io(out)))
+            return out
+        if self._rows_of(X, W.cols) != T:
+            raise InvalidError(f"out has {T} rows, X {self._rows_of(X, W.cols)}")
+        self._check(self.lib.lt_matmul(self.ptr, _ptr(out)[0], W.handle, _ptr(X)[0], T, self._io(out, X)))
         return out
 
     def stream_read(self, ptr: int, nbytes: int):

@@ -117,6 +117,16 @@ def q3k_matrix(g: np.random.Generator, rows: int, cols: int) -> np.ndarray:
     return blk.reshape(rows, nsb * 110)
 
 
+def mxfp4_matrix(g: np.random.Generator, rows: int, cols: int) -> np.ndarray:
+    """uint8 [rows, row_bytes] of MXFP4 blocks: uniform codes, scale bytes
+    119..122 (weights of about 0.03)."""
+    assert cols % 32 == 0
+    nb = cols // 32
+    blk = g.integers(0, 256, size=(rows, nb, 17), dtype=np.uint8)
+    blk[..., 0] = g.integers(119, 123, size=(rows, nb), dtype=np.uint8)
+    return blk.reshape(rows, nb * 17)
+
+
 def quant_matrix(g: np.random.Generator, gtype: int, rows: int, cols: int) -> np.ndarray:
     """Random rows of any device-path type."""
     if gtype == ggml.Q8_0:
@@ -127,6 +137,8 @@ def quant_matrix(g: np.random.Generator, gtype: int, rows: int, cols: int) -> np
         return q6k_matrix(g, rows, cols)
     if gtype == ggml.Q3_K:
         return q3k_matrix(g, rows, cols)
+    if gtype == ggml.MXFP4:
+        return mxfp4_matrix(g, rows, cols)
     return small_block_matrix(g, gtype, rows, cols)
 
 
