@@ -372,7 +372,7 @@ int shape_tensor(lt_ctx *ctx, DevTensor &t, uint32_t type, size_t rows, size_t c
     t.held = t.bytes;
     if (type == LT_TYPE_MXFP4) {
         const lt::MxDims d = lt::mx_dims(rows, t.blocks_per_row);
-        t.held = lt::mx_code_bytes(d, n_experts) + lt::mx_scale_bytes(d, n_experts);
+        t.held = lt::mx_code_bytes(d, n_experts) + lt::mx_scale_bytes(d, n_experts) + lt::mx_slack_bytes(d);
     }
     return LT_OK;
 }

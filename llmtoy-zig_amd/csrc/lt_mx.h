@@ -69,6 +69,9 @@ __host__ __device__ inline MxDims mx_dims(size_t rows, size_t nb) {
     d.tiles = (rows + 15) / 16;
     return d;
 }
+// Behind the planes a tile's codes more are allocated: kernels that take 32 rows
+// at once may read (never use) a tile past the last one.
+inline size_t mx_slack_bytes(const MxDims &d) { return (size_t)d.kg * 1024; }
 inline size_t mx_code_bytes(const MxDims &d, size_t n_experts) { return n_experts * d.tiles * d.kg * 1024; }
 inline size_t mx_scale_bytes(const MxDims &d, size_t n_experts) { return n_experts * d.tiles * d.kq * 256; }
 
