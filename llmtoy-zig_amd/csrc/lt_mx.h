@@ -69,9 +69,10 @@ __host__ __device__ inline MxDims mx_dims(size_t rows, size_t nb) {
     d.tiles = (rows + 15) / 16;
     return d;
 }
-// Behind the planes a tile's codes more are allocated: kernels that take 32 rows
-// at once may read (never use) a tile past the last one.
-inline size_t mx_slack_bytes(const MxDims &d) { return (size_t)d.kg * 1024; }
+// Behind the planes a tile's codes and 4 KiB more are allocated: the batched
+// product takes 32 rows at once, and its last loads run a few blocks past a
+// row's end, so it may read (never use) what is there.
+inline size_t mx_slack_bytes(const MxDims &d) { return (size_t)d.kg * 1024 + 4096; }
 inline size_t mx_code_bytes(const MxDims &d, size_t n_experts) { return n_experts * d.tiles * d.kg * 1024; }
 inline size_t mx_scale_bytes(const MxDims &d, size_t n_experts) { return n_experts * d.tiles * d.kq * 256; }
 

@@ -2,12 +2,28 @@
 // out[t][r] = sum_c W[r][c] X[t][c].
 //
 // X in fp32: a first launch turns its blocks into limbs (lt_mx.h) laid out as
-// matrix operands, [tile of 16 vectors][group of 4 blocks][limb][64 lanes],
-// and the product runs one matrix instruction a limb into the same sums.  X as
-// an MXFP4 tensor: its codes and scales are an operand already.
+// matrix operands, and the product runs one matrix instruction a limb into the
+// same sums.  X as an MXFP4 tensor: its codes and scales are an operand already.
+//
+// What bounds it.  4096 vectors by 8192 x 4096: 1.37 PFLOP of FP6 x FP4
+// products; the instructions alone, their operands held in registers, take 238
+// us at the clock that the card holds under them (5.8 PFLOP/s; 8.9 with
+// constant operands), the product with its loads from LDS 253 us, the whole
+// kernel 290 us, and the limbs 25 us before it (130 MB, the card's copy rate).
+// With 4-bit X 82 us, of which the instructions alone take 61.
+//
+// What made it fast, on that size: both operands through LDS by direct loads
+// instead of registers (1570 -> 335 us); uniform addresses that move on by one
+// addition a load, where computing each address anew had cost more issue slots
+// than the matrix instructions (a 256 x 64 tile's stage from 0.80 to 0.60 us);
+// 512 x 128 tiles with three stages (326 -> 316).  Holding the next stage's
+// operands in registers besides, s_setprio and forced interleaving changed
+// nothing or cost.
 #include "llmtoy_hip.h"
 #include "lt_internal.h"
 #include "lt_mx.h"
+
+#include <type_traits>
 
 namespace lt {
 
@@ -25,7 +41,10 @@ struct MxLimbs {
 };
 __host__ __device__ inline size_t limb_tiles(size_t T) { return (T + 63) / 64; }
 size_t limb_data_bytes(const MxDims &d, size_t T) { return limb_tiles(T) * 2 * d.kg * kPairBytes; }
-size_t limb_bytes(const MxDims &d, size_t T) { return limb_data_bytes(d, T) + limb_tiles(T) * 4 * d.kq * 256; }
+// the last loads of a product run past the data by up to kStages pairs
+constexpr int kStages = 4;
+size_t limb_scales_at(const MxDims &d, size_t T) { return limb_data_bytes(d, T) + kStages * kPairBytes; }
+size_t limb_bytes(const MxDims &d, size_t T) { return limb_scales_at(d, T) + limb_tiles(T) * 4 * d.kq * 256 + kStages * 256; }
 
 // A thread a block; vectors from T on and blocks from nb on are zeros.
 __global__ __launch_bounds__(256) void k_mx_limbs(const float *__restrict__ X, uint32_t T, MxDims d, MxLimbs p) {
@@ -61,138 +80,164 @@ struct MxSide {
     uint32_t last;  // the last tile of 32 rows (its second half may be past the rows: allocated, not used)
 };
 
-// The scale bytes of a lane's blocks in 16 groups' words: word h for the
-// blocks 2 h + lane / 32 of a group, byte g for group g.
-struct MxScales {
-    uint32_t w[2];
+// out[t][r]: a workgroup of WR x WC waves computes 32 WR MI rows of W by 32 WC NI
+// vectors, a wave MI x NI tiles of 32 x 32; a stage is a pair of blocks (64
+// columns) of both sides, of which NST are in LDS.  The vectors are the
+// instruction's rows and W's rows its columns: a store of sums is then 32
+// neighbouring rows of out for each of two vectors, whatever rows % 4 is.
+template <int NL, int WR, int WC, int MI, int NI, int NST>
+struct MxTile {
+    static constexpr int kWaves = WR * WC, kRows = WR * MI, kVecs = WC * NI;  // tiles of 32
+    // a stage in KiB: W's codes, its scale words (256 B a tile), X's operands, its scale words
+    static constexpr int kWS = kRows, kX = kWS + (kRows + 3) / 4;
+    static constexpr int kXS = kX + (NL == 1 ? kVecs : (kVecs + 1) / 2 * 15), kChunks = kXS + (kVecs + 3) / 4;
+    static constexpr int kEach = (kChunks + kWaves - 1) / kWaves;  // loads of a wave for a stage
+    static_assert((NST - 2) * kEach < 64, "the count of loads in flight");
+    static_assert(NST <= kStages, "the memory that the last loads run into");
 };
-__device__ __forceinline__ MxScales scales_at(const MxSide &p, uint32_t kq, uint32_t tile32, uint32_t q, uint32_t off) {
-    const uint8_t *w = p.scales + ((size_t)2 * min(tile32, p.last) * kq + q) * 256;  // (uniform)
-    return {{*reinterpret_cast<const uint32_t *>(w + off), *reinterpret_cast<const uint32_t *>(w + off + 128)}};
+
+// Until this wave has at most N loads in flight and no LDS access; then, behind
+// the barrier, every wave of the workgroup.
+template <int N>
+__device__ __forceinline__ void arrive() {
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | N >> 4 << 14);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-// out[t][r]: a workgroup of WR x WC waves computes 32 WR MI rows of W by 32 WC NI
-// vectors, a wave MI x NI tiles of 32 x 32, KS pairs of blocks (64 columns) a
-// stage.
-//
-// The vectors are the instruction's rows and W's rows its columns: a store of
-// the sums is then 32 neighbouring rows of out for each of two vectors.
-template <int NL, int WR, int WC, int MI, int NI, int KS>
-struct MxTile {
-    static constexpr int kRows = WR * MI, kVecs = WC * NI;  // tiles of 32
-    static constexpr int kWBytes = kRows * KS * 1024;
-    static constexpr int kXBytes = NL == 1 ? kVecs * KS * 1024 : kVecs / 2 * KS * (int)kPairBytes;
-    static constexpr int kChunks = (kWBytes + kXBytes) / 1024, kWaves = WR * WC;
-    static constexpr int kBytes = kWBytes + kXBytes;
-};
-
-template <int NL, int WR, int WC, int MI, int NI, int KS>
+template <int NL, int WR, int WC, int MI, int NI, int NST>
 __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x, uint32_t kg, uint32_t kq, uint32_t rows,
                                                              uint32_t T, uint32_t grid_m, uint32_t grid_n, float *out) {
-    using L = MxTile<NL, WR, WC, MI, NI, KS>;
-    __shared__ __attribute__((aligned(16))) uint8_t buf0[L::kBytes];
-    __shared__ __attribute__((aligned(16))) uint8_t buf1[L::kBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    using L = MxTile<NL, WR, WC, MI, NI, NST>;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NST * L::kChunks * 1024];
+    const uint32_t lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wc = wave / WR;
-    // blocks of one XCD (equal index % 8) take neighbouring tiles
+    // blocks of one XCD (equal index % 8) take neighbouring tiles, 8 of W's by as many of X's
     const uint32_t per = (grid_m * grid_n + 7) / 8;
     const uint32_t id = blockIdx.x % 8 * per + blockIdx.x / 8;
     if (id >= grid_m * grid_n) return;
-    const uint32_t m0 = id % grid_m * L::kRows, n0 = id / grid_m * L::kVecs;  // in tiles of 32
-    const uint32_t steps = 2 * kg / KS;
-    // a lane's place in a tile of 32's codes of a pair, and in its scale words
-    const uint32_t code_off = (uint32_t)(lane & 31) / 16 * kg * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
-    const uint32_t scale_off = (uint32_t)(lane & 31) / 16 * kq * 256 + (lane >> 5) * 64 + (lane & 15) * 4;
+    const uint32_t band = id / (8 * grid_n) * 8, wide = min(8u, grid_m - band), in = id % (8 * grid_n);
+    const uint32_t m0 = (band + in % wide) * L::kRows, n0 = in / wide * L::kVecs;  // in tiles of 32
+    const uint32_t steps = 2 * kg;
 
-    auto fetch = [&](uint32_t step, uint8_t *dst) {
+    // This wave's loads of a stage: a uniform address that moves on from stage
+    // to stage, and each lane's offset.
+    const uint8_t *src[L::kEach];
+    uint32_t off[L::kEach];
+    int stride[L::kEach], to[L::kEach];  // stride 0: scale words
 #pragma unroll
-        for (int c0 = 0; c0 < L::kChunks; c0 += L::kWaves) {
-            const int c = c0 + wave;
-            if (L::kChunks % L::kWaves && c >= L::kChunks) break;
-            const uint8_t *src;
-            if (c < L::kRows * KS || NL == 1) {  // codes: chunk = tile of 32 and pair of blocks
-                const bool isw = c < L::kRows * KS;
-                const MxSide &p = isw ? w : x;
-                const int i = isw ? c : c - L::kRows * KS;
-                const uint32_t t32 = min((isw ? m0 : n0) + i / KS, p.last), pair = step * KS + i % KS;
-                src = p.data + ((size_t)2 * t32 * kg + pair / 2) * 1024 + (pair % 2) * 512 + code_off;
-            } else {  // limbs: 15 chunks a tile of 64 and pair
-                const int i = c - L::kRows * KS;
-                const uint32_t t64 = min(n0 / 2 + i / (15 * KS), (uint32_t)limb_tiles(T) - 1), pair = step * KS + i / 15 % KS;
-                src = x.data + ((size_t)t64 * 2 * kg + pair) * kPairBytes + (i % 15) * 1024 + lane * 16;
-            }
-            to_lds(src, dst + c * 1024);
+    for (int i = 0; i < L::kEach; i++) {
+        const int c = min(wave + i * L::kWaves, L::kChunks - 1);  // (the last one again, the same bytes)
+        to[i] = c * 1024;
+        if (c < L::kWS || (NL == 1 && c >= L::kX && c < L::kXS)) {  // codes of a tile of 32
+            const MxSide &p = c < L::kWS ? w : x;
+            const uint32_t t32 = min(c < L::kWS ? m0 + c : n0 + c - L::kX, p.last);
+            src[i] = p.data + (size_t)2 * t32 * kg * 1024;
+            off[i] = lane % 32 / 16 * kg * 1024 + lane / 32 * 256 + lane % 16 * 16;
+            stride[i] = 512;
+        } else if (c >= L::kX && c < L::kXS) {  // limbs: 15 chunks a tile of 64
+            const uint32_t t64 = min(n0 / 2 + (c - L::kX) / 15, x.last / 2);
+            src[i] = x.data + (size_t)t64 * steps * kPairBytes + (c - L::kX) % 15 * 1024;
+            off[i] = lane * 16;
+            stride[i] = (int)kPairBytes;
+        } else {  // scale words: 8 lanes a tile of 16
+            const bool isw = c < L::kX;
+            const MxSide &p = isw ? w : x;
+            const uint32_t first = isw ? m0 + (c - L::kWS) * 4 : n0 + (c - L::kXS) * 4, t32 = min(first + lane / 16, p.last);
+            src[i] = p.scales;
+            off[i] = (2 * t32 + lane / 8 % 2) * kq * 256 + lane % 8 * 16;
+            stride[i] = 0;
         }
+    }
+    // (the last stages' loads run past the end by up to NST stages: allocated, not used)
+    uint32_t fetched = 0;
+    auto fetch_one = [&](int i, uint8_t *dst) { to_lds(src[i] + off[i], dst + to[i]); };
+    auto fetch_next = [&](bool odd) {  // odd: the stage just fetched was odd
+        fetched++;
+        const int sc = !odd || fetched % 8 == 0 ? 128 : -128;
+#pragma unroll
+        for (int i = 0; i < L::kEach; i++) off[i] += stride[i] ? stride[i] : sc;
     };
 
     mx_acc32 acc[MI][NI] = {};
-    MxScales sw[MI], sx[NI];
-    auto scales = [&](uint32_t q) {
-#pragma unroll
-        for (int i = 0; i < MI; i++) sw[i] = scales_at(w, kq, m0 + wr * MI + i, q, scale_off);
-#pragma unroll
-        for (int i = 0; i < NI; i++) sx[i] = scales_at(x, kq, n0 + wc * NI + i, q, scale_off);
+    auto operand = [&](const uint8_t *st, int v, int j) {
+        if (NL == 1) return mx_op4(*reinterpret_cast<const mx_u32x4 *>(st + (L::kX + v) * 1024 + lane * 16));
+        const uint8_t *u = st + L::kX * 1024 + v / 2 * (int)kPairBytes;
+        const int o = (v % 2 * kMxLimbs + j) * 64 + lane;
+        return mx_op6(reinterpret_cast<const mx_u32x4 *>(u)[o], reinterpret_cast<const mx_u32x2 *>(u + kPairLo)[o]);
     };
-    auto compute = [&](uint32_t step, const uint8_t *src) {
+    auto step = [&](auto odd, uint32_t pair, const uint8_t *st, uint8_t *dst) {
+        constexpr int ODD = decltype(odd)::value;
+        const uint32_t shift = pair / 2 % 4 * 8;
+        const uint32_t at = lane % 32 / 16 * 128 + lane / 32 * 64 + lane % 16 * 4;  // a lane's scale word
+        mx_op b[MI], a[NI], an[NI];
+        int sb[MI], sa[NI];
 #pragma unroll
-        for (int h = 0; h < KS; h++) {
-            const uint32_t pair = step * KS + h, shift = pair / 2 % 4 * 8;
-            const bool odd = KS == 2 ? h : pair % 2;
-            mx_op b[MI];
-            int sb[MI], sa[NI];
+        for (int i = 0; i < NI; i++) {
+            sa[i] = (int)(*reinterpret_cast<const uint32_t *>(st + L::kXS * 1024 + (wc * NI + i) * 256 + at) >> shift & 255u);
+            a[i] = operand(st, wc * NI + i, 0);
+        }
 #pragma unroll
-            for (int i = 0; i < MI; i++) {
-                b[i] = mx_op4(*reinterpret_cast<const mx_u32x4 *>(src + ((wr * MI + i) * KS + h) * 1024 + lane * 16));
-                sb[i] = (int)((odd ? sw[i].w[1] : sw[i].w[0]) >> shift);
-            }
+        for (int i = 0; i < MI; i++) {
+            b[i] = mx_op4(*reinterpret_cast<const mx_u32x4 *>(st + (wr * MI + i) * 1024 + lane * 16));
+            sb[i] = (int)(*reinterpret_cast<const uint32_t *>(st + L::kWS * 1024 + (wr * MI + i) * 256 + at) >> shift);
+        }
 #pragma unroll
-            for (int i = 0; i < NI; i++) sa[i] = (int)((odd ? sx[i].w[1] : sx[i].w[0]) >> shift & 255u);
+        for (int j = 0; j < NL; j++) {
+            if (j + 1 < NL)
 #pragma unroll
-            for (int j = 0; j < NL; j++) {
-                mx_op a[NI];
+                for (int i = 0; i < NI; i++) an[i] = operand(st, wc * NI + i, j + 1);
 #pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const int v = wc * NI + i;
-                    if (NL == 1) {
-                        a[i] = mx_op4(*reinterpret_cast<const mx_u32x4 *>(src + L::kWBytes + (v * KS + h) * 1024 + lane * 16));
-                    } else {
-                        const uint8_t *u = src + L::kWBytes + (v / 2 * KS + h) * (int)kPairBytes;
-                        const int at = (v % 2 * kMxLimbs + j) * 64 + lane;
-                        a[i] = mx_op6(reinterpret_cast<const mx_u32x4 *>(u)[at],
-                                      reinterpret_cast<const mx_u32x2 *>(u + kPairLo)[at]);
+            for (int n = 0; n < NI; n++)
+#pragma unroll
+                for (int m = 0; m < MI; m++) {
+                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        a[n], b[m], acc[m][n], NL == 1 ? kMxCbszFp4 : kMxCbszFp6, kMxCbszFp4, 0,
+                        sa[n] - (NL == 1 ? 0 : (int)kMxLimbShift[j]), 0, sb[m]);
+                    const int k = (j * NI + n) * MI + m + 1, total = NL * NI * MI;
+                    if (k * L::kEach / total > (k - 1) * L::kEach / total) {
+#pragma unroll
+                        for (int i = (k - 1) * L::kEach / total; i < k * L::kEach / total; i++) fetch_one(i, dst);
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < NI; n++)
-#pragma unroll
-                    for (int m = 0; m < MI; m++)
-                        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                            a[n], b[m], acc[m][n], NL == 1 ? kMxCbszFp4 : kMxCbszFp6, kMxCbszFp4, 0,
-                            sa[n] - (NL == 1 ? 0 : (int)kMxLimbShift[j]), 0, sb[m]);
-            }
+            for (int i = 0; i < NI; i++) a[i] = an[i];
         }
+        fetch_next((NST - 1 + ODD) % 2);
     };
 
-    fetch(0, buf0);
-    for (uint32_t s = 0; s < steps; s += 2) {  // (an even number of steps)
-        if (s * KS % 8 == 0) scales(s * KS / 8);
-        __syncthreads();
-        fetch(s + 1, buf1);
-        compute(s, buf0);
-        __syncthreads();
-        if (s + 2 < steps) fetch(s + 2, buf0);
-        compute(s + 1, buf1);
+    constexpr int kAhead = (NST - 2) * L::kEach, kStage = L::kChunks * 1024;
+    for (int i = 0; i < NST - 1; i++) {
+#pragma unroll
+        for (int c = 0; c < L::kEach; c++) fetch_one(c, lds + i * kStage);
+        fetch_next(i % 2);
     }
+    int now = 0, free = NST - 1;
+    auto turn = [&](auto odd, uint32_t s) {
+        // stage s is in LDS, and every wave is past stage s - 1, whose memory the
+        // loads of stage s + NST - 1 take
+        arrive<kAhead>();
+        step(odd, s, lds + now * kStage, lds + free * kStage);
+        free = now;
+        now = now + 1 == NST ? 0 : now + 1;
+    };
+    for (uint32_t s = 0; s < steps; s += 2) {
+        turn(std::integral_constant<int, 0>{}, s);
+        turn(std::integral_constant<int, 1>{}, s + 1);
+    }
+    arrive<0>();  // no load into LDS outlives the workgroup
 
 #pragma unroll
     for (int n = 0; n < NI; n++)
 #pragma unroll
         for (int m = 0; m < MI; m++) {
-            const uint32_t r = (m0 + wr * MI + m) * 32 + (lane & 31);
+            const uint32_t r = (m0 + wr * MI + m) * 32 + lane % 32;
             if (r >= rows) continue;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const uint32_t t = (n0 + wc * NI + n) * 32 + i / 4 * 8 + 4 * (lane >> 5) + i % 4;
+                const uint32_t t = (n0 + wc * NI + n) * 32 + i / 4 * 8 + 4 * (lane / 32) + i % 4;
                 if (t < T) out[(size_t)t * rows + r] = acc[m][n][i];
             }
         }
@@ -205,16 +250,29 @@ size_t batch_of(size_t T, size_t cols) {
     return T < fit ? T : fit;
 }
 
-template <int NL, int WR, int WC, int MI, int NI, int KS>
+template <int NL, int WR, int WC, int MI, int NI, int NST>
 hipError_t launch_gemm(const DevTensor &W, const MxSide &x, uint32_t T, float *out, hipStream_t s) {
-    using L = MxTile<NL, WR, WC, MI, NI, KS>;
+    using L = MxTile<NL, WR, WC, MI, NI, NST>;
     const MxDims d = mx_dims(W.rows, W.blocks_per_row);
     const MxSide w{W.p0, W.p1, (uint32_t)((d.tiles - 1) / 2)};
     const uint32_t gm = (uint32_t)((W.rows + 32 * L::kRows - 1) / (32 * L::kRows)), gn = (T + 32 * L::kVecs - 1) / (32 * L::kVecs);
     const uint32_t grid = (gm * gn + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_mx_gemm<NL, WR, WC, MI, NI, KS>), dim3(grid), dim3(64 * WR * WC), 0, s, w, x, d.kg, d.kq,
+    hipLaunchKernelGGL((k_mx_gemm<NL, WR, WC, MI, NI, NST>), dim3(grid), dim3(64 * WR * WC), 0, s, w, x, d.kg, d.kq,
                        (uint32_t)W.rows, T, gm, gn, out);
     return hipGetLastError();
+}
+
+constexpr size_t kCus = 256;
+size_t tiles_of(const DevTensor &W, size_t T, size_t m, size_t n) { return ((W.rows + m - 1) / m) * ((T + n - 1) / n); }
+
+// A stage of a 512 x 128 tile takes 1.13 us (one workgroup a CU), one of two 256
+// x 64 tiles on a CU 0.63 us: the fewer rounds' time.  4096 x 8192 x 4096: 316
+// and 348 us; 4095 x 7001 x 2816: 216 and 226; 1024 x 4096 x 4096: 105 and 66;
+// 509 x 4864 x 2816: 73 and 33.
+hipError_t limbs_product(const DevTensor &W, const MxSide &x, uint32_t T, float *out, hipStream_t s) {
+    const size_t large = (tiles_of(W, T, 512, 128) + kCus - 1) / kCus, mid = (tiles_of(W, T, 256, 64) + 2 * kCus - 1) / (2 * kCus);
+    if (large * 9 <= mid * 5) return launch_gemm<kMxLimbs, 4, 2, 4, 2, 3>(W, x, T, out, s);
+    return launch_gemm<kMxLimbs, 4, 2, 2, 1, 3>(W, x, T, out, s);
 }
 
 }  // namespace
@@ -229,13 +287,13 @@ hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *
     for (size_t t0 = 0; t0 < T; t0 += step) {
         const size_t n = T - t0 < step ? T - t0 : step;
         const MxDims d = mx_dims(limb_tiles(n) * 64, W.blocks_per_row);
-        const MxLimbs p{(uint8_t *)ws, (uint8_t *)ws + limb_data_bytes(d, n)};
+        const MxLimbs p{(uint8_t *)ws, (uint8_t *)ws + limb_scales_at(d, n)};
         hipLaunchKernelGGL(k_mx_limbs, dim3((unsigned)((limb_tiles(n) * 2 * d.kg * 128 + 255) / 256)), dim3(256), 0, s,
                            X + t0 * W.cols, (uint32_t)n, d, p);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         const MxSide x{p.data, p.scales, (uint32_t)((d.tiles - 1) / 2)};
-        e = launch_gemm<kMxLimbs, 4, 1, 4, 2, 1>(W, x, (uint32_t)n, out + t0 * W.rows, s);
+        e = limbs_product(W, x, (uint32_t)n, out + t0 * W.rows, s);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -244,7 +302,10 @@ hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *
 hipError_t launch_matmul_mx_mx(const DevTensor &W, const DevTensor &X, size_t T, float *out, hipStream_t s) {
     const MxDims d = mx_dims(X.rows, X.blocks_per_row);
     const MxSide x{X.p0, X.p1, (uint32_t)((d.tiles - 1) / 2)};
-    return launch_gemm<1, 2, 2, 4, 2, 1>(W, x, (uint32_t)T, out, s);
+    // 256 x 128 tiles once they fill the CUs: 4095 x 7001 x 2816 61 us (128 x 64: 72),
+    // 1024 x 4096 x 4096 (128 of them) 22.8 us (17.2)
+    if (tiles_of(W, T, 256, 128) >= kCus) return launch_gemm<1, 4, 2, 2, 2, 3>(W, x, (uint32_t)T, out, s);
+    return launch_gemm<1, 2, 2, 2, 1, 4>(W, x, (uint32_t)T, out, s);
 }
 
 }  // namespace lt
