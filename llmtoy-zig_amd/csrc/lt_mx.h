@@ -43,7 +43,7 @@ constexpr int kMxLimbs = 5;
 constexpr int kMxCbszFp6 = 2, kMxCbszFp4 = 4;  // operand formats of the instruction
 // scale exponents of the limbs below the first one's
 constexpr uint32_t kMxLimbShift[kMxLimbs] = {0, 4, 9, 14, 19};
-constexpr uint32_t kMxLeastScale = 19;  // keeps the last limb's exponent at 0 or more
+constexpr uint32_t kMxLeastScale = 20;  // keeps the last limb's unit a normal number
 
 typedef int mx_op __attribute__((ext_vector_type(8)));          // a matrix operand's registers
 typedef float mx_acc16 __attribute__((ext_vector_type(4)));     // 16 x 16 sums
@@ -91,9 +91,19 @@ __device__ __forceinline__ mx_op mx_op6(mx_u32x4 v, mx_u32x2 w) {
     return mx_op{(int)v[0], (int)v[1], (int)v[2], (int)v[3], (int)w[0], (int)w[1], 0, 0};
 }
 
-// The scale byte of a block of activations from the largest |x|'s bits: 255
-// (NaN) where a value is NaN or infinite.
-__device__ __forceinline__ uint32_t mx_limb_scale(uint32_t top) {
+// The largest |x| of a block; NaN where one is.
+__device__ __forceinline__ float mx_top(const mx_f32x16 &a, const mx_f32x16 &b) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(__builtin_fabsf(a[i]), __builtin_fabsf(b[i])));
+    return m;
+}
+
+// The scale byte of a block of activations: 255 (NaN) where a value is NaN or
+// infinite.
+__device__ __forceinline__ uint32_t mx_limb_scale(float largest) {
+    const uint32_t top = __float_as_uint(largest);
     if (top >= 0x7f800000u) return 255u;
     const uint32_t s = (top >> 23) + ((top & 0x7fffffu) > 0x780000u ? 1u : 0u);
     return s < kMxLeastScale + 2 ? kMxLeastScale : s - 2;
@@ -103,34 +113,21 @@ __device__ __forceinline__ uint32_t mx_limb_scale(uint32_t top) {
 // scale byte s; put(limb, operand words).
 template <typename Put>
 __device__ __forceinline__ void mx_limbs(mx_f32x16 a, mx_f32x16 b, uint32_t s, Put put) {
-    // (s = 255: the words do not matter, every product with the block is NaN)
-    const float inv = __uint_as_float((254u - (s > 253u ? 253u : s)) << 23);
-    a *= inv;
-    b *= inv;
 #pragma unroll
     for (int j = 0; j < kMxLimbs; j++) {
-        const mx_u32x6 q = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 1.0f);
+        // (s = 255: the words do not matter, every product with the block is NaN)
+        const float unit = __uint_as_float((min(s, 253u) - kMxLimbShift[j]) << 23);
+        const mx_u32x6 q = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, unit);
         put(j, q);
         if (j + 1 < kMxLimbs) {
-            const float up = j ? 32.0f : 16.0f;
-            const mx_f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q, up);  // q * up
+            const mx_f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q, unit);
 #pragma unroll
             for (int i = 0; i < 16; i++) {  // exact: the remainder has fewer bits
-                a[i] = __builtin_fmaf(a[i], up, -back[2 * i]);
-                b[i] = __builtin_fmaf(b[i], up, -back[2 * i + 1]);
+                a[i] -= back[2 * i];
+                b[i] -= back[2 * i + 1];
             }
         }
     }
-}
-
-__device__ __forceinline__ uint32_t mx_top(const mx_f32x16 &a, const mx_f32x16 &b) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        m = max(m, __float_as_uint(a[i]) & 0x7fffffffu);
-        m = max(m, __float_as_uint(b[i]) & 0x7fffffffu);
-    }
-    return m;
 }
 
 // 32 floats at x (16-byte aligned)

@@ -1,18 +1,24 @@
 // lt_mx_matvec.hip -- products of MXFP4 matrices with one vector: matvec, the
 // experts' gate/up and down by id.
 //
-//   y[r] = sum_b 2^(e_rb - 127) sum_i w_rbi x_bi,   x_bi = sum_j q_jbi s_b 2^(-shift_j)   (lt_mx.h)
+//   y[r] = sum_b 2^(e_rb - 127) sum_i w_rbi x_bi
 //
-// One v_mfma_scale_f32_16x16x128 takes 16 rows of 4 weight blocks, codes and
-// scales as they stand in memory, against a 128 x 16 operand whose columns 0..4
-// are the five limbs of those 128 activations (the other columns are zero): the
-// row's sum over the columns is the product with the fp32 activations.  No
-// weight is ever converted; a KiB of weights costs one matrix instruction (about
-// 18 cycles) and two LDS reads.
+// A weight times its block's scale is a bf16 number (2 bits times a power of
+// two), and v_cvt_scalef32_pk_bf16_fp4 makes two of them from a byte.  An
+// activation is the sum of three bf16 numbers of 8 bits each, cut off from the
+// top, exactly.  So v_mfma_f32_16x16x32_bf16 with 16 rows of weights on one
+// side and the three parts as columns on the other gives the products with the
+// fp32 activations; the row's sum over the columns is y.  (The scaled
+// instruction, which takes the codes as they are, needs activations in FP6:
+// their conversion is 32 values wide and cost every workgroup 0.7 us before its
+// first product, three parts cut off by masks 0.1.  FP8 operands converted in
+// pairs are no way out: sums with them were 1e-4 off.)
 //
-// A workgroup converts the vector once, while its first weights are on their
-// way, and its waves split a tile's row over groups of 16 blocks (one scale
-// word); what they summed meets in LDS in the waves' order.
+// Bound by the weights' bytes, and where there are few of those by the chain
+// launch - vector - product - sum over the waves.  A workgroup converts the
+// vector once, while its first weights are on their way.  A tile's rows are
+// split over S waves, 16 blocks (a scale word) at a time; what they summed
+// meets in LDS in the waves' order.
 #include "llmtoy_hip.h"
 #include "lt_internal.h"
 #include "lt_mx.h"
@@ -21,40 +27,37 @@ namespace lt {
 
 namespace {
 
-constexpr int kMvWaves = 8;
-constexpr int kMvThreads = 64 * kMvWaves;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// LDS of a vector's limbs: per block and limb 16 + 8 bytes of operand words,
-// per group of 16 blocks and lane group a word of four scale bytes.
-struct MxVec {
-    mx_u32x4 *hi;  // [4 kg][5]
-    mx_u32x2 *lo;  // [4 kg][5]
-    uint8_t *sc;   // [kq][4 lane groups][4]
+// A vector's three parts in LDS: [block][quarter][part], 8 bf16 each, in the
+// order of the codes (position 2 i: element i, 2 i + 1: element 16 + i).  (A wave's
+// reads, 4 blocks by 3 parts, fall on different banks.)
+constexpr int kParts = 3;
+__host__ __device__ inline size_t mx_vec_bytes(uint32_t kg) { return (size_t)kg * 4 * 4 * kParts * 16; }
+
+// Quarter u % 4 of block u / 4 (blocks from nb on: the last one again, against
+// weights of zero).
+struct MxQuarter {
+    float4 a, h;  // elements 4 m .. + 3 and 16 + 4 m .. + 3
 };
-__host__ __device__ inline size_t mx_vec_bytes(uint32_t kg) {
-    const size_t nb = 4 * (size_t)kg, kq = (kg + 3) / 4;
-    return nb * kMxLimbs * 24 + kq * 16;
+__device__ __forceinline__ MxQuarter mx_vec_load(const float *x, uint32_t u, uint32_t nb) {
+    const float *p = x + (size_t)min(u / 4, nb - 1) * 32 + u % 4 * 4;
+    return {ldg16f(p), ldg16f(p + 16)};
 }
-__device__ __forceinline__ MxVec mx_vec_at(uint8_t *lds, uint32_t kg) {
-    MxVec v;
-    v.hi = reinterpret_cast<mx_u32x4 *>(lds);
-    v.lo = reinterpret_cast<mx_u32x2 *>(lds + (size_t)4 * kg * kMxLimbs * 16);
-    v.sc = lds + (size_t)4 * kg * kMxLimbs * 24;
-    return v;
-}
-
-// Blocks [0, 4 kg) of x's limbs into v by the workgroup (blocks from nb on:
-// zeros).  Followed by a barrier.
-__device__ __forceinline__ void mx_vec_fill(const MxVec &v, const float *x, uint32_t nb, uint32_t kg) {
-    for (uint32_t b = threadIdx.x; b < 4 * kg; b += blockDim.x) {
-        mx_f32x16 lo = {}, hi = {};
-        if (b < nb) mx_load_block(x + (size_t)b * 32, lo, hi);
-        const uint32_t s = mx_limb_scale(mx_top(lo, hi));
-        v.sc[(b / 16) * 16 + (b % 4) * 4 + (b / 4) % 4] = (uint8_t)s;
-        mx_limbs(lo, hi, s, [&](int j, const mx_u32x6 &q) {
-            v.hi[b * kMxLimbs + j] = mx_u32x4{q[0], q[1], q[2], q[3]};
-            v.lo[b * kMxLimbs + j] = mx_u32x2{q[4], q[5]};
-        });
+__device__ __forceinline__ void mx_vec_put(mx_u32x4 *v, uint32_t u, const MxQuarter &x) {
+    float a[4] = {x.a.x, x.a.y, x.a.z, x.a.w}, h[4] = {x.h.x, x.h.y, x.h.z, x.h.w};
+#pragma unroll
+    for (int c = 0; c < kParts; c++) {
+        mx_u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t ua = __float_as_uint(a[i]), uh = __float_as_uint(h[i]);
+            w[i] = __builtin_amdgcn_perm(uh, ua, 0x07060302u);  // the upper halves
+            a[i] -= __uint_as_float(ua & 0xffff0000u);
+            h[i] -= __uint_as_float(uh & 0xffff0000u);
+        }
+        v[u * kParts + c] = w;
     }
 }
 
@@ -74,155 +77,249 @@ struct MxWords {
     mx_u32x4 c[4];
     uint32_t s;
 };
+// NT: read past the caches, which then keep what is read again (experts are).
+template <bool NT>
 __device__ __forceinline__ void mx_fetch(MxWords &w, const MxRow &r, uint32_t q, uint32_t kg) {
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++)
-        if (4 * q + j < kg) w.c[j] = *reinterpret_cast<const mx_u32x4 *>(r.codes + (size_t)(4 * q + j) * 1024);
+        if (4 * q + j < kg) {
+            const mx_u32x4 *p = reinterpret_cast<const mx_u32x4 *>(r.codes + (size_t)(4 * q + j) * 1024);
+            w.c[j] = NT ? __builtin_nontemporal_load(p) : *p;
+        }
     w.s = *reinterpret_cast<const uint32_t *>(r.scales + (size_t)q * 256);
 }
 
-// acc += the groups 4 q .. of the rows in w times the vector's.
+// acc += the groups 4 q .. of the rows in w times the vector's.  Columns from 3
+// on repeat the third: mx_rows leaves them out.
+struct MxSum {
+    mx_acc16 s[4];  // chains
+    __device__ __forceinline__ mx_acc16 all() const { return (s[0] + s[1]) + (s[2] + s[3]); }
+};
 template <int J>
-__device__ __forceinline__ mx_acc16 mx_step(const MxWords &w, const MxVec &v, uint32_t q, uint32_t sv, bool live, int limb,
-                                            int lane, mx_acc16 acc) {
-    mx_op x = {};
-    const uint32_t b = (4 * q + J) * 4 + (uint32_t)(lane >> 4);
-    if (live) x = mx_op6(v.hi[b * kMxLimbs + limb], v.lo[b * kMxLimbs + limb]);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op4(w.c[J]), x, acc, kMxCbszFp4, kMxCbszFp6, J, (int)w.s, J,
-                                                            (int)sv);
+__device__ __forceinline__ void mx_step(const MxWords &w, const mx_u32x4 *v, MxSum &acc) {
+    // a float whose exponent is the scale byte: 2^(e - 127), 255 makes NaN
+    const float scale = __uint_as_float((J < 3 ? w.s << (23 - 8 * J) : w.s >> 1) & 0x7f800000u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        union {
+            bf16x2 p[4];
+            bf16x8 v;
+        } m;
+        m.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 0);
+        m.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 1);
+        m.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 2);
+        m.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 3);
+        const bf16x8 x = __builtin_bit_cast(bf16x8, v[(16 * J + i) * kParts]);
+        acc.s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m.v, x, acc.s[i], 0, 0, 0);
+    }
 }
-__device__ __forceinline__ mx_acc16 mx_dot(const MxWords &w, const MxVec &v, uint32_t q, uint32_t kg, int lane,
-                                           mx_acc16 acc) {
-    const int col = lane & 15;
-    const bool live = col < kMxLimbs;
-    const int limb = live ? col : 0;
-    constexpr uint64_t shifts = 0ull | 4ull << 8 | 9ull << 16 | 14ull << 24 | 19ull << 32;
-    const uint32_t shift = (uint32_t)(shifts >> (8 * limb)) & 255u;
-    // the limb's scale bytes: every byte of the word is at least kMxLeastScale
-    const uint32_t sv = reinterpret_cast<const uint32_t *>(v.sc)[q * 4 + (lane >> 4)] - shift * 0x01010101u;
-    acc = mx_step<0>(w, v, q, sv, live, limb, lane, acc);
-    if (4 * q + 1 < kg) acc = mx_step<1>(w, v, q, sv, live, limb, lane, acc);
-    if (4 * q + 2 < kg) acc = mx_step<2>(w, v, q, sv, live, limb, lane, acc);
-    if (4 * q + 3 < kg) acc = mx_step<3>(w, v, q, sv, live, limb, lane, acc);
-    return acc;
+__device__ __forceinline__ void mx_dot(const MxWords &w, const mx_u32x4 *v, uint32_t q, uint32_t kg, int lane, MxSum &acc) {
+    v += ((16 * q + (uint32_t)(lane >> 4)) * 4) * kParts + min(lane & 15, kParts - 1);
+    mx_step<0>(w, v, acc);
+    if (4 * q + 1 < kg) mx_step<1>(w, v, acc);
+    if (4 * q + 2 < kg) mx_step<2>(w, v, acc);
+    if (4 * q + 3 < kg) mx_step<3>(w, v, acc);
 }
 
 // The sums over the columns: row 4 (lane / 16) + i in acc[i] of every lane of
 // the 16, then row lane % 16 from lanes of column i = row % 4.
 __device__ __forceinline__ float mx_rows(mx_acc16 acc, int lane, bool first) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = group_sum_dpp<16>(acc[i], first);
+    for (int i = 0; i < 4; i++) acc[i] = group_sum_dpp<16>((lane & 15) < kParts ? acc[i] : 0.0f, first);
     const int i = lane & 3;
     return i == 0 ? acc[0] : i == 1 ? acc[1] : i == 2 ? acc[2] : acc[3];
 }
 // the lane that holds row r of mx_rows is 16 (r / 4) + r % 4: lanes with
 // lane % 16 < 4 write row 4 (lane / 16) + lane % 4
 
-__global__ __launch_bounds__(kMvThreads) void k_mx_matvec(const uint8_t *codes, const uint8_t *scales, MxDims d,
-                                                          uint32_t rows, uint32_t expert_rows, const float *x, float *y) {
+// Loads stay behind this point, or before it.
+__device__ __forceinline__ void mx_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+constexpr int kMvWaves = 16;  // of a workgroup at most
+
+// Workgroups of S waves a tile (and blockDim / 64 / S tiles side by side) walk the
+// tiles.  Two items (16 rows by 16 blocks) of a wave are on their way, over the
+// tiles' ends, before the vector is converted and from then on.
+template <bool NT>
+__global__ __launch_bounds__(64 * kMvWaves) void k_mx_matvec(const uint8_t *codes, const uint8_t *scales, MxDims d,
+                                                             uint32_t ntiles, uint32_t expert_rows, uint32_t S,
+                                                             const float *x, float *y) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ float part[kMvWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float part[2][kMvWaves][16];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sp = wave % S, tp = wave / S;
+    const uint32_t TP = blockDim.x / 64 / S, stride = gridDim.x * TP, t0 = blockIdx.x * TP;
     const bool first = p32_first(lane);
-    const MxVec v = mx_vec_at(lds, d.kg);
-    mx_vec_fill(v, x, d.nb, d.kg);
+    mx_u32x4 *const v = reinterpret_cast<mx_u32x4 *>(lds);
+    const uint32_t units = 16 * d.kg;
+    MxQuarter xb;
+    if (threadIdx.x < units) xb = mx_vec_load(x, threadIdx.x, d.nb);
+    mx_order();
+
+    // every wave of the workgroup goes through the same number of tiles (past
+    // the last one: that one again, not written)
+    const uint32_t rounds = (ntiles - t0 + stride - 1) / stride, n = rounds * ((d.kq - sp + S - 1) / S);
+    uint32_t ft = t0 + tp, fq = sp;  // the next item to fetch
+    auto fetch = [&](MxWords &w) {
+        const uint32_t tile = min(ft, ntiles - 1);
+        const MxRow r{codes + ((size_t)tile * d.kg * 64 + lane) * 16, scales + ((size_t)tile * d.kq * 64 + lane) * 4};
+        mx_fetch<NT>(w, r, fq, d.kg);
+        if ((fq += S) >= d.kq) fq = sp, ft += stride;
+    };
+    MxWords w0, w1;
+    fetch(w0);
+    if (n > 1) fetch(w1);
+    mx_order();
+    if (threadIdx.x < units) mx_vec_put(v, threadIdx.x, xb);
+    for (uint32_t u = threadIdx.x + blockDim.x; u < units; u += blockDim.x) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
     __syncthreads();
-    const size_t ntiles = (size_t)(rows / expert_rows) * d.tiles;
-    for (size_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-        const size_t expert = tile / d.tiles;
-        const uint32_t row0 = (uint32_t)(tile % d.tiles) * 16;
-        const MxRow r = mx_row_at(codes, scales, d, expert, row0 + (uint32_t)(lane & 15), lane);
-        mx_acc16 acc = {};
-        for (uint32_t q = wave; q < d.kq; q += kMvWaves) {
-            MxWords w;
-            mx_fetch(w, r, q, d.kg);
-            acc = mx_dot(w, v, q, d.kg, lane, acc);
+
+    MxSum acc = {};
+    uint32_t tile = t0 + tp, q = sp, turn = 0;
+    auto use = [&](const MxWords &w) {
+        mx_dot(w, v, q, d.kg, lane, acc);
+        if ((q += S) < d.kq) return;
+        const uint32_t row0 = tile % d.tiles * 16;
+        float *out = y + (size_t)(tile / d.tiles) * expert_rows + row0;
+        const float t = mx_rows(acc.all(), lane, first);
+        const uint32_t r = 4 * (lane >> 4) + (lane & 3);
+        if (S == 1) {
+            if ((lane & 15) < 4 && tile < ntiles && row0 + r < expert_rows) out[r] = t;
+        } else {
+            if ((lane & 15) < 4) part[turn][wave][r] = t;
+            __syncthreads();
+            if (sp == 0 && lane < 16 && tile < ntiles && row0 + lane < expert_rows) {
+                float s = part[turn][wave][lane];
+                for (uint32_t i = 1; i < S; i++) s += part[turn][wave + i][lane];
+                out[lane] = s;
+            }
+            turn ^= 1;
         }
-        const float t = mx_rows(acc, lane, first);
-        if ((lane & 15) < 4) part[wave][4 * (lane >> 4) + (lane & 3)] = t;
-        __syncthreads();
-        if (threadIdx.x < 16 && row0 + threadIdx.x < expert_rows) {
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kMvWaves; i++) s += part[i][threadIdx.x];
-            y[expert * expert_rows + row0 + threadIdx.x] = s;
+        acc = MxSum{};
+        q = sp;
+        tile += stride;
+    };
+    for (uint32_t i = 0; i < n; i += 2) {
+        use(w0);
+        if (i + 2 < n) fetch(w0);
+        if (i + 1 < n) {
+            use(w1);
+            if (i + 3 < n) fetch(w1);
         }
-        __syncthreads();
     }
 }
 
 // h[slot][j] = act(G x)[j] (U x)[j] of expert ids[slot], zeros from F to
-// down_cols: waves 0-3 the 16 gate rows, 4-7 the up rows, which may begin
+// down_cols: S waves the 16 gate rows, S more the up rows, which may begin
 // inside a tile.  G and U are one tensor of 2 F rows an expert, or (ids null)
 // two tensors.
 struct MxPair {
     const uint8_t *codes[2], *scales[2];
-    uint32_t row0[2], rows;  // first row of either half; rows of an expert in memory
+    uint32_t row0[2];  // first row of either half
     MxDims d;
 };
-__global__ __launch_bounds__(kMvThreads) void k_mx_gate_up(MxPair p, const float *x, const uint32_t *ids, uint32_t n_experts,
-                                                           uint32_t F, uint32_t down_cols, uint32_t act, float *h) {
+constexpr int kPairWaves = 8;
+__global__ __launch_bounds__(64 * kPairWaves) void k_mx_gate_up(MxPair p, const float *x, const uint32_t *ids,
+                                                              uint32_t n_experts, uint32_t F, uint32_t down_cols,
+                                                              uint32_t act, float *h) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ float part[kMvWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t j0 = blockIdx.x * 16, expert = ids ? ids[blockIdx.y] : 0u;
+    __shared__ float part[kPairWaves][16];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), S = blockDim.x / 128, half = wave / S, sp = wave % S;
+    const uint32_t j0 = blockIdx.x * 16;
+    const MxDims &d = p.d;
+    const uint32_t units = 16 * d.kg;
+    MxQuarter xb;
+    if (threadIdx.x < units) xb = mx_vec_load(x, threadIdx.x, d.nb);
+    mx_order();
+    const uint32_t expert = ids ? ids[blockIdx.y] : 0u;
     float *out = h + (size_t)blockIdx.y * down_cols;
     if (j0 >= F || expert >= n_experts) {  // padding (or no such expert)
         if (threadIdx.x < 16 && j0 + threadIdx.x < down_cols) out[j0 + threadIdx.x] = 0.0f;
         return;
     }
     const bool first = p32_first(lane);
-    const MxVec v = mx_vec_at(lds, p.d.kg);
-    mx_vec_fill(v, x, p.d.nb, p.d.kg);
-    __syncthreads();
-    const int half = wave >> 2;
+    mx_u32x4 *const v = reinterpret_cast<mx_u32x4 *>(lds);
     const uint32_t j = min(j0 + (uint32_t)(lane & 15), F - 1);
-    const MxRow r = mx_row_at(p.codes[half], p.scales[half], p.d, expert, p.row0[half] + j, lane);
-    mx_acc16 acc = {};
-    for (uint32_t q = wave & 3; q < p.d.kq; q += 4) {
-        MxWords w;
-        mx_fetch(w, r, q, p.d.kg);
-        acc = mx_dot(w, v, q, p.d.kg, lane, acc);
+    const MxRow r = mx_row_at(half ? p.codes[1] : p.codes[0], half ? p.scales[1] : p.scales[0], d, expert,
+                              (half ? p.row0[1] : p.row0[0]) + j, lane);
+    MxWords w0, w1;
+    mx_fetch<false>(w0, r, sp, d.kg);
+    if (sp + S < d.kq) mx_fetch<false>(w1, r, sp + S, d.kg);
+    mx_order();
+    if (threadIdx.x < units) mx_vec_put(v, threadIdx.x, xb);
+    for (uint32_t u = threadIdx.x + blockDim.x; u < units; u += blockDim.x) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
+    __syncthreads();
+    MxSum acc = {};
+    for (uint32_t q = sp; q < d.kq; q += 2 * S) {
+        mx_dot(w0, v, q, d.kg, lane, acc);
+        if (q + 2 * S < d.kq) mx_fetch<false>(w0, r, q + 2 * S, d.kg);
+        if (q + S < d.kq) mx_dot(w1, v, q + S, d.kg, lane, acc);
+        if (q + 3 * S < d.kq) mx_fetch<false>(w1, r, q + 3 * S, d.kg);
     }
-    const float t = mx_rows(acc, lane, first);
+    const float t = mx_rows(acc.all(), lane, first);
     if ((lane & 15) < 4) part[wave][4 * (lane >> 4) + (lane & 3)] = t;
     __syncthreads();
     if (threadIdx.x < 16 && j0 + threadIdx.x < down_cols) {
         const uint32_t i = threadIdx.x;
-        const float g = ((part[0][i] + part[1][i]) + part[2][i]) + part[3][i];
-        const float u = ((part[4][i] + part[5][i]) + part[6][i]) + part[7][i];
+        float g = part[0][i], u = part[S][i];
+        for (uint32_t k = 1; k < S; k++) {
+            g += part[k][i];
+            u += part[S + k][i];
+        }
         out[j0 + i] = j0 + i < F ? act_apply(act, g) * u : 0.0f;
     }
 }
 
 // out[i] = sum over slots of w (D_id h[slot])[i]: the waves take the (slot, 16
-// blocks) pieces of a tile's rows in turn, `per` slots' limbs in LDS at once.
-__global__ __launch_bounds__(kMvThreads) void k_mx_down(const uint8_t *codes, const uint8_t *scales, MxDims d, uint32_t rows,
-                                                        uint32_t n_experts, const float *h, const uint32_t *ids,
-                                                        const float *wts, uint32_t k, uint32_t per, const float *base,
-                                                        int accumulate, const float *dscale, float *out) {
+// blocks) items of a tile's rows in turn, `per` slots' vectors in LDS at once.
+constexpr int kDownWaves = 16;
+__global__ __launch_bounds__(64 * kDownWaves) void k_mx_down(const uint8_t *codes, const uint8_t *scales, MxDims d,
+                                                             uint32_t rows, uint32_t n_experts, const float *h,
+                                                             const uint32_t *ids, const float *wts, uint32_t k,
+                                                             uint32_t per, const float *base, int accumulate,
+                                                             const float *dscale, float *out) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ float part[kMvWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float part[kDownWaves][16];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = blockDim.x / 64;
     const bool first = p32_first(lane);
-    const uint32_t row0 = blockIdx.x * 16;
-    const size_t vec = mx_vec_bytes(d.kg);
+    const uint32_t row0 = blockIdx.x * 16, vec = (uint32_t)mx_vec_bytes(d.kg), of = 16 * d.kg;
     mx_acc16 sum = {};
     for (uint32_t s0 = 0; s0 < k; s0 += per) {
-        const uint32_t n = min(per, k - s0);
+        const uint32_t n = min(per, k - s0), items = n * d.kq, units = n * of;
         if (s0) __syncthreads();
-        for (uint32_t i = 0; i < n; i++)
-            mx_vec_fill(mx_vec_at(lds + i * vec, d.kg), h + (size_t)(s0 + i) * d.nb * 32, d.nb, d.kg);
+        auto vec_of = [&](uint32_t i) { return reinterpret_cast<mx_u32x4 *>(lds + i * vec); };
+        auto load = [&](uint32_t u) { return mx_vec_load(h + (size_t)(s0 + u / of) * d.nb * 32, u % of, d.nb); };
+        auto put = [&](uint32_t u, const MxQuarter &x) { mx_vec_put(vec_of(u / of), u % of, x); };
+        MxQuarter xb;
+        if (threadIdx.x < units) xb = load(threadIdx.x);
+        mx_order();
+        auto fetch = [&](MxWords &w, uint32_t it) {
+            const uint32_t e = min(ids[s0 + it / d.kq], n_experts - 1);
+            mx_fetch<false>(w, mx_row_at(codes, scales, d, e, row0 + (uint32_t)(lane & 15), lane), it % d.kq, d.kg);
+        };
+        auto use = [&](const MxWords &w, uint32_t it) {
+            const uint32_t i = it / d.kq, e = ids[s0 + i];
+            MxSum t = {};
+            mx_dot(w, vec_of(i), it % d.kq, d.kg, lane, t);
+            if (e < n_experts) sum += t.all() * (dscale ? wts[s0 + i] * dscale[e] : wts[s0 + i]);
+        };
+        MxWords w0, w1;
+        if (wave < items) fetch(w0, wave);
+        if (wave + NW < items) fetch(w1, wave + NW);
+        mx_order();
+        if (threadIdx.x < units) put(threadIdx.x, xb);
+        for (uint32_t u = threadIdx.x + blockDim.x; u < units; u += blockDim.x) put(u, load(u));
         __syncthreads();
-        for (uint32_t it = wave; it < n * d.kq; it += kMvWaves) {
-            const uint32_t i = it / d.kq, q = it % d.kq, e = ids[s0 + i];
-            if (e >= n_experts) continue;
-            const MxRow r = mx_row_at(codes, scales, d, e, row0 + (uint32_t)(lane & 15), lane);
-            MxWords w;
-            mx_fetch(w, r, q, d.kg);
-            const mx_acc16 t = mx_dot(w, mx_vec_at(lds + i * vec, d.kg), q, d.kg, lane, mx_acc16{});
-            const float f = dscale ? wts[s0 + i] * dscale[e] : wts[s0 + i];
-            sum += t * f;
+        for (uint32_t it = wave; it < items; it += 2 * NW) {
+            use(w0, it);
+            if (it + 2 * NW < items) fetch(w0, it + 2 * NW);
+            if (it + NW < items) use(w1, it + NW);
+            if (it + 3 * NW < items) fetch(w1, it + 3 * NW);
         }
     }
     const float t = mx_rows(sum, lane, first);
@@ -230,16 +327,23 @@ __global__ __launch_bounds__(kMvThreads) void k_mx_down(const uint8_t *codes, co
     __syncthreads();
     const uint32_t row = row0 + threadIdx.x;
     if (threadIdx.x < 16 && row < rows) {
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kMvWaves; i++) s += part[i][threadIdx.x];
+        float s = part[0][threadIdx.x];
+        for (uint32_t i = 1; i < NW; i++) s += part[i][threadIdx.x];
         if (accumulate) s = out[row] + s;
         out[row] = base ? base[row] + s : s;
     }
 }
 
-// Limbs of this many bytes at most in a down block's LDS (two blocks a CU).
+// Parts of this many bytes at most in a down block's LDS (two blocks a CU).
 constexpr size_t kDownLds = 72 << 10;
+
+// Waves a tile: as many as it takes to have 4,096 (4 a SIMD), each with the same
+// number of items where they can; with few tiles a workgroup each, with many
+// 8 waves of several tiles, which walk on.
+constexpr size_t kMvTarget = 4096, kMvGroups = 1024;
+// Matrices from 8 MiB on are read past the caches: a model of them does not fit
+// the 256 MiB there are.
+constexpr size_t kNtBytes = 8u << 20;
 
 // Lets a kernel use the CU's LDS, once per kernel and device.
 hipError_t allow_lds(const void *fn, bool *set) {
@@ -257,13 +361,21 @@ hipError_t allow_lds(const void *fn, bool *set) {
 
 hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s) {
     const MxDims d = mx_dims(W.rows, W.blocks_per_row);
-    static bool set[64] = {};
-    hipError_t e = allow_lds((const void *)k_mx_matvec, set);
+    static bool set[2][64] = {};
+    const bool nt = W.bytes >= kNtBytes;
+    const auto kernel = nt ? k_mx_matvec<true> : k_mx_matvec<false>;
+    hipError_t e = allow_lds((const void *)kernel, set[nt]);
     if (e != hipSuccess) return e;
     const size_t tiles = W.n_experts * d.tiles;
-    const dim3 grid((unsigned)(tiles < 1024 ? tiles : 1024));
-    hipLaunchKernelGGL(k_mx_matvec, grid, dim3(kMvThreads), mx_vec_bytes(d.kg), s, W.p0, W.p1, d, (uint32_t)W.total_rows,
-                       (uint32_t)W.rows, x, y);
+    uint32_t S = (uint32_t)((kMvTarget + tiles - 1) / tiles);
+    S = S > (uint32_t)kMvWaves ? (uint32_t)kMvWaves : S;
+    S = S > d.kq ? d.kq : S;
+    const uint32_t each = (d.kq + S - 1) / S;
+    S = (d.kq + each - 1) / each;
+    const uint32_t TP = tiles * S <= kMvTarget || S > 4 ? 1 : 8 / S;
+    const size_t groups = (tiles + TP - 1) / TP;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kMvGroups ? groups : kMvGroups)), dim3(64 * S * TP),
+                       mx_vec_bytes(d.kg), s, W.p0, W.p1, d, (uint32_t)tiles, (uint32_t)W.rows, S, x, y);
     return hipGetLastError();
 }
 
@@ -273,20 +385,21 @@ static hipError_t launch_pair(const MxPair &p, const float *x, const uint32_t *i
     hipError_t e = allow_lds((const void *)k_mx_gate_up, set);
     if (e != hipSuccess) return e;
     const dim3 grid((down_cols + 15) / 16, k);
-    hipLaunchKernelGGL(k_mx_gate_up, grid, dim3(kMvThreads), mx_vec_bytes(p.d.kg), s, p, x, ids, n_experts, F, down_cols, act,
+    const uint32_t S = p.d.kq < (uint32_t)kPairWaves / 2 ? p.d.kq : (uint32_t)kPairWaves / 2;
+    hipLaunchKernelGGL(k_mx_gate_up, grid, dim3(128 * S), mx_vec_bytes(p.d.kg), s, p, x, ids, n_experts, F, down_cols, act,
                        h);
     return hipGetLastError();
 }
 
 hipError_t launch_gate_up_mx(const DevTensor &G, const DevTensor &U, const float *x, uint32_t act, uint32_t down_cols,
                              float *h, hipStream_t s) {
-    MxPair p{{G.p0, U.p0}, {G.p1, U.p1}, {0, 0}, (uint32_t)G.rows, mx_dims(G.rows, G.blocks_per_row)};
+    MxPair p{{G.p0, U.p0}, {G.p1, U.p1}, {0, 0}, mx_dims(G.rows, G.blocks_per_row)};
     return launch_pair(p, x, nullptr, 1, 1, (uint32_t)G.rows, down_cols, act, h, s);
 }
 
 hipError_t launch_expert_gate_up_mx(const DevTensor &GU, const float *x, const uint32_t *ids, uint32_t k, uint32_t d_expert,
                                     uint32_t down_cols, uint32_t act, float *h, hipStream_t s) {
-    MxPair p{{GU.p0, GU.p0}, {GU.p1, GU.p1}, {0, d_expert}, (uint32_t)GU.rows, mx_dims(GU.rows, GU.blocks_per_row)};
+    MxPair p{{GU.p0, GU.p0}, {GU.p1, GU.p1}, {0, d_expert}, mx_dims(GU.rows, GU.blocks_per_row)};
     return launch_pair(p, x, ids, (uint32_t)GU.n_experts, k, d_expert, down_cols, act, h, s);
 }
 
@@ -299,7 +412,8 @@ hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint3
     const size_t vec = mx_vec_bytes(d.kg);
     uint32_t per = (uint32_t)(kDownLds / vec);
     per = per < 1 ? 1 : per > k ? k : per;
-    hipLaunchKernelGGL(k_mx_down, dim3((unsigned)d.tiles), dim3(kMvThreads), per * vec, s, D.p0, D.p1, d, (uint32_t)D.rows,
+    const uint32_t items = per * d.kq, NW = items < (uint32_t)kDownWaves ? items : (uint32_t)kDownWaves;
+    hipLaunchKernelGGL(k_mx_down, dim3((unsigned)d.tiles), dim3(64 * NW), per * vec, s, D.p0, D.p1, d, (uint32_t)D.rows,
                        (uint32_t)D.n_experts, h, ids, w, k, per, base, accumulate, dscale, out);
     return hipGetLastError();
 }
