@@ -1057,11 +1057,6 @@ int check_experts(lt_ctx *ctx, const lt_tensor *gate_up, const lt_tensor *down, 
     return LT_OK;
 }
 
-// Whether the gate/up kernel selects the experts itself (else the router does).
-bool gate_up_routes(const DevTensor &GU, size_t n_experts) {
-    return n_experts <= kRoutedGateUpMaxExperts && GU.type != LT_TYPE_MXFP4;
-}
-
 // gate/up of the k selected experts into h [k][Kd] (ids on the device)
 int gate_up_dev(lt_ctx *ctx, const DevTensor &GU, const float *x, const uint32_t *ids, uint32_t k, uint32_t d_expert,
                 uint32_t Kd, uint32_t act, float *h) {
@@ -1087,6 +1082,11 @@ int gate_up_routed_dev(lt_ctx *ctx, const DevTensor &GU, const float *x, uint32_
                          lt::launch_expert_gate_up_q4k_routed(GU, x, logits, k, norm, d_expert, Kd, act, h, ids, w,
                                                               ctx->stream),
                          "expert_gate_up_routed");
+    if (GU.type == LT_TYPE_MXFP4)
+        return launch_rc(ctx,
+                         lt::launch_expert_gate_up_mx_routed(GU, x, logits, k, norm, d_expert, Kd, act, h, ids, w,
+                                                             ctx->stream),
+                         "expert_gate_up_mx_routed");
     return launch_rc(ctx,
                      lt::launch_expert_gate_up_fmt_routed(GU, x, logits, k, norm, d_expert, Kd, act, h, ids, w,
                                                           ctx->stream),
@@ -1302,7 +1302,7 @@ int moe_dev(lt_ctx *ctx, float *out, const float *x, const DevTensor &R, const f
     }
     if ((rc = ensure(ctx, ctx->eh, (size_t)k * Kd * 4))) return rc;
     float *h = (float *)ctx->eh.p;
-    if (gate_up_routes(GU, R.total_rows)) {
+    if (R.total_rows <= kRoutedGateUpMaxExperts) {
         // logits only; each gate/up block selects its expert from them
         if ((rc = router_dev(ctx, R, x, bias, 0, flags, r))) return rc;
         rc = gate_up_routed_dev(ctx, GU, x, k, (flags & LT_MOE_NORM_TOPK) ? 1u : 0u, d_expert, (uint32_t)Kd, act, h,
@@ -1711,7 +1711,7 @@ extern "C" int lt_gemma4_moe_block(lt_ctx *ctx, float *x, const float *dense_ffn
     if ((rc = ensure(ctx, ctx->eh, (size_t)k * Kd * 4))) return rc;
     float *h = (float *)ctx->eh.p;
     const uint32_t norm = (flags & LT_MOE_NORM_TOPK) ? 1u : 0u;
-    if (gate_up_routes(GU, E)) {
+    if (E <= kRoutedGateUpMaxExperts) {
         if ((rc = router_dev(ctx, R, rin, nullptr, 0, flags, r, nullptr, fuse_prep ? &prep : nullptr))) return rc;
         rc = gate_up_routed_dev(ctx, GU, moe_in, k, norm, d_expert, (uint32_t)Kd, act, h, r);
     } else {

@@ -369,6 +369,11 @@ hipError_t launch_gate_up_mx(const DevTensor &G, const DevTensor &U, const float
 // Selected experts: row lengths up to 16384, any k and sizes.
 hipError_t launch_expert_gate_up_mx(const DevTensor &GU, const float *x, const uint32_t *ids, uint32_t k, uint32_t d_expert,
                                     uint32_t down_cols, uint32_t act, float *h, hipStream_t s);
+// Selects the experts itself from the logits (n_experts <= 256), as
+// launch_expert_gate_up_q4k_routed.
+hipError_t launch_expert_gate_up_mx_routed(const DevTensor &GU, const float *x, const float *logits, uint32_t k, uint32_t norm,
+                                           uint32_t d_expert, uint32_t down_cols, uint32_t act, float *h, uint32_t *ids_out,
+                                           float *w_out, hipStream_t s);
 hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint32_t *ids, const float *w, uint32_t k,
                                  const float *base, int accumulate, const float *dscale, float *out, hipStream_t s);
 // out [T][rows] = X [T][cols] W^T; ws: matmul_mx_workspace(T, cols) bytes.
