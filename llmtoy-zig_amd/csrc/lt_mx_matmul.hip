@@ -243,6 +243,88 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x,
         }
 }
 
+// Few vectors, or few rows: a workgroup computes 16 RT rows by 16 NT vectors, its
+// waves split the columns and their sums meet in LDS.  Nothing is shared between
+// the waves, so both operands go from memory to registers, the next group of 4
+// blocks while one is computed: no barrier, and every CU has work where the
+// tiles above would be too few.
+constexpr int kThinWaves = 8;
+template <int NL, int RT, int NT>
+__global__ __launch_bounds__(64 * kThinWaves, 2) void k_mx_thin(MxSide w, MxSide x, uint32_t kg, uint32_t kq, uint32_t rows,
+                                                                uint32_t T, float *out) {
+    __shared__ float part[kThinWaves][RT][NT][16][17];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m0 = blockIdx.x * RT, n0 = blockIdx.y * NT;  // in tiles of 16
+    const uint32_t each = (kg + kThinWaves - 1) / kThinWaves, g0 = wave * each, g1 = min(g0 + each, kg);
+    struct Group {
+        mx_op w[RT], x[NL][NT];
+        uint32_t sw[RT], sx[NT];
+    };
+    auto fetch = [&](Group &r, uint32_t g) {
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const size_t tile = min(m0 + i, 2 * w.last + 1);
+            r.w[i] = mx_op4(*reinterpret_cast<const mx_u32x4 *>(w.data + (tile * kg + g) * 1024 + lane * 16));
+            r.sw[i] = *reinterpret_cast<const uint32_t *>(w.scales + (tile * kq + g / 4) * 256 + lane * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const size_t tile = min(n0 + i, 2 * x.last + 1);
+            r.sx[i] = *reinterpret_cast<const uint32_t *>(x.scales + (tile * kq + g / 4) * 256 + lane * 4);
+            if constexpr (NL == 1) {
+                r.x[0][i] = mx_op4(*reinterpret_cast<const mx_u32x4 *>(x.data + (tile * kg + g) * 1024 + lane * 16));
+            } else {
+                const uint8_t *u = x.data + (tile / 4 * 2 * kg + 2 * g + lane / 32) * kPairBytes;
+                const uint32_t at = tile % 4 / 2 * kMxLimbs * 64 + lane % 32 / 16 * 32 + tile % 2 * 16 + lane % 16;
+#pragma unroll
+                for (int j = 0; j < NL; j++)
+                    r.x[j][i] = mx_op6(reinterpret_cast<const mx_u32x4 *>(u)[at + j * 64],
+                                       reinterpret_cast<const mx_u32x2 *>(u + kPairLo)[at + j * 64]);
+            }
+        }
+    };
+    mx_acc16 acc[RT][NT] = {};
+    auto use = [&](const Group &r, uint32_t g) {
+        const uint32_t shift = g % 4 * 8;
+#pragma unroll
+        for (int j = 0; j < NL; j++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int m = 0; m < RT; m++)
+                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        r.x[j][n], r.w[m], acc[m][n], NL == 1 ? kMxCbszFp4 : kMxCbszFp6, kMxCbszFp4, 0,
+                        (int)(r.sx[n] >> shift & 255u) - (NL == 1 ? 0 : (int)kMxLimbShift[j]), 0, (int)(r.sw[m] >> shift));
+    };
+    if (g0 < g1) {  // (past the last group: that one again, not used)
+        Group r0, r1;
+        fetch(r0, g0);
+        for (uint32_t g = g0; g < g1; g += 2) {
+            fetch(r1, min(g + 1, g1 - 1));
+            use(r0, g);
+            fetch(r0, min(g + 2, g1 - 1));
+            if (g + 1 < g1) use(r1, g + 1);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < RT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) part[wave][m][n][4 * (lane / 16) + i][lane % 16] = acc[m][n][i];
+    __syncthreads();
+    for (uint32_t o = threadIdx.x; o < RT * NT * 256; o += 64 * kThinWaves) {
+        const uint32_t c = o % 16, m = o / 16 % RT, v = o / (16 * RT);  // rows of W side by side
+        const uint32_t row = (m0 + m) * 16 + c, t = n0 * 16 + v;
+        if (row >= rows || t >= T) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kThinWaves; k++) s += part[k][m][v / 16][v % 16][c];
+        out[(size_t)t * rows + row] = s;
+    }
+}
+
 // Vectors whose limbs are in the workspace at once: 128 MiB of it, half of the
 // last cache.
 size_t batch_of(size_t T, size_t cols) {
@@ -262,8 +344,24 @@ hipError_t launch_gemm(const DevTensor &W, const MxSide &x, uint32_t T, float *o
     return hipGetLastError();
 }
 
+template <int NL, int RT, int NT>
+hipError_t launch_thin(const DevTensor &W, const MxSide &x, uint32_t T, float *out, hipStream_t s) {
+    const MxDims d = mx_dims(W.rows, W.blocks_per_row);
+    const MxSide w{W.p0, W.p1, (uint32_t)((d.tiles - 1) / 2)};
+    const dim3 grid((unsigned)((W.rows + 16 * RT - 1) / (16 * RT)), (T + 16 * NT - 1) / (16 * NT));
+    hipLaunchKernelGGL((k_mx_thin<NL, RT, NT>), grid, dim3(64 * kThinWaves), 0, s, w, x, d.kg, d.kq, (uint32_t)W.rows, T, out);
+    return hipGetLastError();
+}
+
 constexpr size_t kCus = 256;
 size_t tiles_of(const DevTensor &W, size_t T, size_t m, size_t n) { return ((W.rows + m - 1) / m) * ((T + n - 1) / n); }
+
+// Up to 2^20 sums the thin kernel: 4096 x 4096 with T = 7 | 64 | 256 vectors 8.5 |
+// 13.4 | 35.6 us (tiles through LDS 32.8 | 33.9 | 36.8), 4-bit X 2.8 | 4.5 | 9.8
+// (11.2 | 11.3 | 12.3); twice as many sums would be 64 (37) and 17 (13).  16 rows
+// a workgroup for up to 16 vectors (T = 7: 8.5 us, 64 rows 10.2), unless there are
+// so many rows that reading the vectors for each 16 costs more.
+bool is_thin(const DevTensor &W, size_t T) { return (T + 15) / 16 * 16 * W.rows <= 1u << 20; }
 
 // A stage of a 512 x 128 tile takes 1.13 us (one workgroup a CU), one of two 256
 // x 64 tiles on a CU 0.63 us: the fewer rounds' time.  4096 x 8192 x 4096: 316
@@ -271,6 +369,9 @@ size_t tiles_of(const DevTensor &W, size_t T, size_t m, size_t n) { return ((W.r
 // 509 x 4864 x 2816: 73 and 33.
 hipError_t limbs_product(const DevTensor &W, const MxSide &x, uint32_t T, float *out, hipStream_t s) {
     const size_t large = (tiles_of(W, T, 512, 128) + kCus - 1) / kCus, mid = (tiles_of(W, T, 256, 64) + 2 * kCus - 1) / (2 * kCus);
+    if (is_thin(W, T))
+        return T <= 16 && W.rows <= 8192 ? launch_thin<kMxLimbs, 1, 1>(W, x, T, out, s)
+                                         : launch_thin<kMxLimbs, 4, 1>(W, x, T, out, s);
     if (large * 9 <= mid * 5) return launch_gemm<kMxLimbs, 4, 2, 4, 2, 3>(W, x, T, out, s);
     return launch_gemm<kMxLimbs, 4, 2, 2, 1, 3>(W, x, T, out, s);
 }
@@ -283,6 +384,7 @@ size_t matmul_mx_workspace(size_t T, size_t cols) {
 }
 
 hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *ws, float *out, hipStream_t s) {
+    if (T == 1) return launch_matvec_mx(W, X, out, s);
     const size_t step = batch_of(T, W.cols);
     for (size_t t0 = 0; t0 < T; t0 += step) {
         const size_t n = T - t0 < step ? T - t0 : step;
@@ -304,6 +406,9 @@ hipError_t launch_matmul_mx_mx(const DevTensor &W, const DevTensor &X, size_t T,
     const MxSide x{X.p0, X.p1, (uint32_t)((d.tiles - 1) / 2)};
     // 256 x 128 tiles once they fill the CUs: 4095 x 7001 x 2816 61 us (128 x 64: 72),
     // 1024 x 4096 x 4096 (128 of them) 22.8 us (17.2)
+    if (is_thin(W, T))
+        return T <= 16 && W.rows <= 8192 ? launch_thin<1, 1, 1>(W, x, (uint32_t)T, out, s)
+                                         : launch_thin<1, 2, 2>(W, x, (uint32_t)T, out, s);
     if (tiles_of(W, T, 256, 128) >= kCus) return launch_gemm<1, 4, 2, 2, 2, 3>(W, x, (uint32_t)T, out, s);
     return launch_gemm<1, 2, 2, 2, 1, 4>(W, x, (uint32_t)T, out, s);
 }

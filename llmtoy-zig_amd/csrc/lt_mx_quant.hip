@@ -56,54 +56,122 @@ __global__ __launch_bounds__(kMxStage) void k_mx_blocks(uint8_t *raw, size_t nbl
     }
 }
 
-// 8 lanes a block, a float4 each; lanes 0-3 hold the low halves of the code
-// bytes, lanes 4-7 the high ones.
-__global__ __launch_bounds__(256) void k_mx_quantize(const float *__restrict__ x, size_t row0, uint32_t rows,
-                                                     size_t expert_rows, MxDims d, uint8_t *codes, uint8_t *scales) {
-    const size_t unit = ((size_t)blockIdx.x * 256 + threadIdx.x) / 8;
-    const uint32_t j = threadIdx.x % 8;
-    if (unit >= (size_t)rows * d.nb) return;  // (whole groups of 8 lanes)
-    const uint32_t row = (uint32_t)(unit / d.nb), b = (uint32_t)(unit % d.nb);
-    const float4 v = ldg16f(x + unit * 32 + 4 * j);
-    uint32_t top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
-                       max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
-#pragma unroll
-    for (int off = 4; off; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 8));
-    const bool bad = top >= 0x7f800000u;
-    const int e = max((int)(top >> 23) - 2, 0);  // the scale byte
-    uint32_t q = 0;
-    if (!bad) {
-        const int up = 127 - e;
-        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, ldexpf(v.x, up), ldexpf(v.y, up), 1.0f, 0);
-        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, ldexpf(v.z, up), ldexpf(v.w, up), 1.0f, 1);
-        q = (q & 0xfu) | (q & 0xf0u) << 4 | (q & 0xf00u) << 8 | (q & 0xf000u) << 12;  // a nibble a byte
+// A workgroup a tile of 16 rows and a group of 16 blocks (512 columns): 32 KiB of
+// fp32 against 4 KiB of codes, which stand in a row, and a KiB's quarter of
+// scale words.  16 threads a row, 8 lanes a block with a float4 each; codes and
+// scales pass through LDS between a row's order and the tile's.  Bound by HBM:
+// XX.
+struct MxSpan {
+    size_t row0, rows;  // of the tensor, over all experts
+    size_t expert_rows;
+    uint32_t tile0;     // the first row's tile
+    MxDims d;
+};
+struct MxTileAt {
+    size_t tile;        // in the planes
+    size_t first;       // its row 0's place in the span's array, as row0 stands at 0 (may be before it)
+    __device__ __forceinline__ bool has(const MxSpan &p, uint32_t r, uint32_t in_expert) const {
+        const size_t at = first + r;  // (wraps below 0)
+        return in_expert + r < p.expert_rows && at < p.rows;
     }
-    const uint32_t hi = (uint32_t)__shfl_down((int)q, 4, 8);
-    const size_t all = row0 + row, r = all % expert_rows, tile = all / expert_rows * d.tiles + r / 16;
-    if (j < 4) reinterpret_cast<uint32_t *>(codes + mx_code_at(d, tile, (uint32_t)(r % 16), b))[j] = q | hi << 4;
-    if (j == 0) scales[mx_scale_at(d, tile, (uint32_t)(r % 16), b)] = bad ? (uint8_t)255 : (uint8_t)e;
+};
+
+__global__ __launch_bounds__(256) void k_mx_quantize(const float *__restrict__ x, MxSpan p, uint8_t *codes, uint8_t *scales) {
+    __shared__ uint32_t lc[16][16][5];  // [block][row][word], a word of padding
+    __shared__ uint8_t ls[16][4][4];    // [row][lane group][group of 4 blocks]
+    const uint32_t r = threadIdx.x / 16, l = threadIdx.x % 16, q = blockIdx.x;
+    const size_t tile = p.tile0 + blockIdx.y, expert = tile / p.d.tiles;
+    const uint32_t in = (uint32_t)(tile % p.d.tiles) * 16;
+    const MxTileAt t{tile, expert * p.expert_rows + in - p.row0};
+    if (t.has(p, r, in)) {
+        const float *row = x + (t.first + r) * p.d.nb * 32;
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (16 * q + 2 * i + l / 8 < p.d.nb) v[i] = ldg16f(row + 512 * q + 64 * i + 4 * l);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t b = 2 * i + l / 8, j = l % 8;
+            uint32_t word = 0, e = 0;
+            if (16 * q + b < p.d.nb) {  // (8 lanes together)
+                uint32_t top = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
+                                   max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
+#pragma unroll
+                for (int off = 4; off; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 8));
+                e = (uint32_t)max((int)(top >> 23) - 2, 0);
+                if (top >= 0x7f800000u) {
+                    e = 255;
+                } else {
+                    const int up = 127 - (int)e;
+                    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, ldexpf(v[i].x, up), ldexpf(v[i].y, up), 1.0f, 0);
+                    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, ldexpf(v[i].z, up), ldexpf(v[i].w, up), 1.0f, 1);
+                    word = (word & 0xfu) | (word & 0xf0u) << 4 | (word & 0xf00u) << 8 | (word & 0xf000u) << 12;  // a nibble a byte
+                }
+            }
+            const uint32_t hi = (uint32_t)__shfl_down((int)word, 4, 8);  // lanes 4-7: elements 16 on, the high halves
+            if (j < 4) lc[b][r][j] = word | hi << 4;
+            if (j == 0) ls[r][b % 4][b / 4] = (uint8_t)e;
+        }
+    }
+    __syncthreads();
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 16, g = 4 * q + wave;
+    if (!t.has(p, row, in)) return;
+    if (g < p.d.kg) {
+        const uint32_t *w = lc[4 * wave + lane / 16][row];
+        reinterpret_cast<uint4 *>(codes)[(tile * p.d.kg + g) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (wave == 0)
+        reinterpret_cast<uint32_t *>(scales)[(tile * p.d.kq + q) * 64 + lane] =
+            *reinterpret_cast<const uint32_t *>(ls[row][lane / 16]);
 }
 
-__global__ __launch_bounds__(256) void k_mx_dequantize(float *__restrict__ out, size_t row0, uint32_t rows,
-                                                       size_t expert_rows, MxDims d, const uint8_t *codes,
+__global__ __launch_bounds__(256) void k_mx_dequantize(float *__restrict__ out, MxSpan p, const uint8_t *codes,
                                                        const uint8_t *scales) {
-    const size_t unit = ((size_t)blockIdx.x * 256 + threadIdx.x) / 8;
-    const uint32_t j = threadIdx.x % 8;
-    if (unit >= (size_t)rows * d.nb) return;
-    const uint32_t row = (uint32_t)(unit / d.nb), b = (uint32_t)(unit % d.nb);
-    const size_t all = row0 + row, r = all % expert_rows, tile = all / expert_rows * d.tiles + r / 16;
-    const uint32_t w = reinterpret_cast<const uint32_t *>(codes + mx_code_at(d, tile, (uint32_t)(r % 16), b))[j % 4];
-    const uint32_t e = scales[mx_scale_at(d, tile, (uint32_t)(r % 16), b)];
-    const uint32_t n = (j < 4 ? w : w >> 4) & 0x0f0f0f0fu;
-    const uint32_t q = (n & 0xfu) | (n >> 4 & 0xf0u) | (n >> 8 & 0xf00u) | (n >> 12 & 0xf000u);
-    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
-    const int up = (int)e - 127;
-    float4 v = make_float4(ldexpf(lo[0], up), ldexpf(lo[1], up), ldexpf(hi[0], up), ldexpf(hi[1], up));
-    if (e == 255u) v = make_float4(NAN, NAN, NAN, NAN);
-    *reinterpret_cast<float4 *>(out + unit * 32 + 4 * j) = v;
+    __shared__ uint32_t lc[16][16][5];
+    __shared__ uint32_t ls[16][4];
+    const uint32_t r = threadIdx.x / 16, l = threadIdx.x % 16, q = blockIdx.x;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, g = 4 * q + wave;
+    const size_t tile = p.tile0 + blockIdx.y, expert = tile / p.d.tiles;
+    const uint32_t in = (uint32_t)(tile % p.d.tiles) * 16;
+    const MxTileAt t{tile, expert * p.expert_rows + in - p.row0};
+    if (g < p.d.kg) {
+        const uint4 w = reinterpret_cast<const uint4 *>(codes)[(tile * p.d.kg + g) * 64 + lane];
+        uint32_t *to = lc[4 * wave + lane / 16][lane % 16];
+        to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+    }
+    if (wave == 0) ls[lane % 16][lane / 16] = reinterpret_cast<const uint32_t *>(scales)[(tile * p.d.kq + q) * 64 + lane];
+    __syncthreads();
+    if (!t.has(p, r, in)) return;
+    float *row = out + (t.first + r) * p.d.nb * 32;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t b = 2 * i + l / 8, j = l % 8;
+        if (16 * q + b >= p.d.nb) continue;
+        const uint32_t w = lc[b][r][j % 4], n = (j < 4 ? w : w >> 4) & 0x0f0f0f0fu;
+        const uint32_t four = (n & 0xfu) | (n >> 4 & 0xf0u) | (n >> 8 & 0xf00u) | (n >> 12 & 0xf000u);
+        const uint32_t e = ls[r][b % 4] >> (b / 4 * 8) & 255u;
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 1);
+        const int up = (int)e - 127;
+        float4 v = make_float4(ldexpf(lo[0], up), ldexpf(lo[1], up), ldexpf(hi[0], up), ldexpf(hi[1], up));
+        if (e == 255u) v = make_float4(NAN, NAN, NAN, NAN);
+        *reinterpret_cast<float4 *>(row + 512 * q + 64 * i + 4 * l) = v;
+    }
 }
 
-unsigned grid_of(size_t units) { return (unsigned)((units * 8 + 255) / 256); }
+// One launch for each 65535 tiles (a grid's limit) of the rows.
+template <typename Launch>
+hipError_t over_tiles(const DevTensor &t, size_t row0, size_t rows, Launch launch) {
+    MxSpan p{row0, rows, t.rows, 0, mx_dims(t.rows, t.blocks_per_row)};
+    auto tile_of = [&](size_t row) { return row / t.rows * p.d.tiles + row % t.rows / 16; };
+    const size_t last = tile_of(row0 + rows - 1);
+    for (size_t first = tile_of(row0); first <= last; first += 65535) {
+        p.tile0 = (uint32_t)first;
+        launch(p, dim3(p.d.kq, (unsigned)(last - first + 1 < 65535 ? last - first + 1 : 65535)));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
 
 }  // namespace
 
@@ -119,17 +187,15 @@ hipError_t launch_mx_blocks(const DevTensor &t, uint8_t *raw, size_t nblk, size_
 }
 
 hipError_t launch_mx_quantize(const DevTensor &t, const float *x, size_t row0, size_t rows, hipStream_t s) {
-    const MxDims d = mx_dims(t.rows, t.blocks_per_row);
-    hipLaunchKernelGGL(k_mx_quantize, dim3(grid_of(rows * d.nb)), dim3(256), 0, s, x, row0, (uint32_t)rows,
-                       t.rows, d, const_cast<uint8_t *>(t.p0), const_cast<uint8_t *>(t.p1));
-    return hipGetLastError();
+    return over_tiles(t, row0, rows, [&](const MxSpan &p, dim3 grid) {
+        hipLaunchKernelGGL(k_mx_quantize, grid, dim3(256), 0, s, x, p, const_cast<uint8_t *>(t.p0), const_cast<uint8_t *>(t.p1));
+    });
 }
 
 hipError_t launch_mx_dequantize(const DevTensor &t, float *out, size_t row0, size_t rows, hipStream_t s) {
-    const MxDims d = mx_dims(t.rows, t.blocks_per_row);
-    hipLaunchKernelGGL(k_mx_dequantize, dim3(grid_of(rows * d.nb)), dim3(256), 0, s, out, row0, (uint32_t)rows,
-                       t.rows, d, t.p0, t.p1);
-    return hipGetLastError();
+    return over_tiles(t, row0, rows, [&](const MxSpan &p, dim3 grid) {
+        hipLaunchKernelGGL(k_mx_dequantize, grid, dim3(256), 0, s, out, p, t.p0, t.p1);
+    });
 }
 
 }  // namespace lt

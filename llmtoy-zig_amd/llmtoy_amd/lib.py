@@ -232,21 +232,21 @@ class Context:
 
     def quantize(self, t: Tensor, x, row0: int = 0):
         """Rows row0 .. of the MXFP4 tensor t from x ([cols] or [rows, cols], float32)."""
-        rows = self._rows_of(x, t.cols)
-        self._check(self.lib.lt_quantize(self.ptr, t.handle, _ptr(x)[0], row0, rows, self._io(x)))
+        rows, (p, host) = self._rows_of(x, t.cols), _ptr(x)
+        self._check(self.lib.lt_quantize(self.ptr, t.handle, p, row0, rows, LT_HOST_IO if host else 0))
         return t
 
     def dequantize(self, out, t: Tensor, row0: int = 0):
         """The values of rows row0 .. of the MXFP4 tensor t into out ([cols] or [rows, cols], float32)."""
-        rows = self._rows_of(out, t.cols)
-        self._check(self.lib.lt_dequantize(self.ptr, _ptr(out)[0], t.handle, row0, rows, self._io(out)))
+        rows, (p, host) = self._rows_of(out, t.cols), _ptr(out)
+        self._check(self.lib.lt_dequantize(self.ptr, p, t.handle, row0, rows, LT_HOST_IO if host else 0))
         return out
 
     @staticmethod
     def _rows_of(a, cols: int) -> int:
         """Rows of a float32 array [cols] or [rows, cols]."""
         shape = tuple(a.shape)
-        if "float32" not in str(a.dtype):
+        if a.dtype != np.float32 and str(a.dtype) != "torch.float32":
             raise InvalidError(f"float32 array expected, got {a.dtype}")
         if len(shape) not in (1, 2) or shape[-1] != cols:
             raise InvalidError(f"array of shape {shape}, rows of {cols} expected")
@@ -268,13 +268,16 @@ class Context:
     def quant_matmul(self, out, W: Tensor, X):
         """out [T, rows] = X [T, cols] . W^T for an MXFP4 matrix W (lt_matmul); X may be an MXFP4
         Tensor, of which the first T rows are taken (lt_matmul_quantized)."""
-        T = self._rows_of(out, W.rows)
+        T, (p, host) = self._rows_of(out, W.rows), _ptr(out)
         if isinstance(X, Tensor):
-            self._check(self.lib.lt_matmul_quantized(self.ptr, _ptr(out)[0], W.handle, X.handle, T, self._io(out)))
+            self._check(self.lib.lt_matmul_quantized(self.ptr, p, W.handle, X.handle, T, LT_HOST_IO if host else 0))
             return out
         if self._rows_of(X, W.cols) != T:
             raise InvalidError(f"out has {T} rows, X {self._rows_of(X, W.cols)}")
-        self._check(self.lib.lt_matmul(self.ptr, _ptr(out)[0], W.handle, _ptr(X)[0], T, self._io(out, X)))
+        px, host_x = _ptr(X)
+        if host != host_x:
+            raise InvalidError("mix of host and device arrays")
+        self._check(self.lib.lt_matmul(self.ptr, p, W.handle, px, T, LT_HOST_IO if host else 0))
         return out
 
     def stream_read(self, ptr: int, nbytes: int):

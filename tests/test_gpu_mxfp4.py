@@ -66,7 +66,7 @@ SPECIAL[9, 5] = -2 ** -149
 SPECIAL[10] = np.linspace(-6, 6, 32)
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 2816), (5, 96), (16, 128), (17, 160), (33, 4096), (300, 32)])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 2816), (5, 96), (16, 128), (17, 160), (33, 4096), (300, 32), (20, 1056)])
 @pytest.mark.parametrize("scale", [1.0, 3e-39, 1e36])
 def test_gpu_mx_quantize(ctx, rows, cols, scale):
     print(f"quantize {rows}x{cols} scale {scale}", flush=True)
@@ -228,7 +228,9 @@ def test_gpu_mx_matmul(ctx, T, rows, cols):
     xq.free(), t.free()
 
 
-@pytest.mark.parametrize("T,rows,cols", [(300, 700, 640), (513, 1030, 288), (1000, 300, 4096)])
+# past the thin kernel's range: each of the tiles, ragged on every side
+@pytest.mark.parametrize("T,rows,cols", [(300, 700, 640), (1000, 300, 4096), (1100, 1030, 288), (1300, 1000, 1056),
+                                         (130, 9001, 96), (9, 9001, 160), (2001, 8003, 96)])
 def test_gpu_mx_matmul_larger(ctx, T, rows, cols):
     test_gpu_mx_matmul(ctx, T, rows, cols)
 
@@ -245,19 +247,20 @@ def test_gpu_mx_matmul_more_vectors_than_the_workspace_holds(ctx):
     t.free()
 
 
-def test_gpu_mx_matmul_not_finite_stays_in_its_row(ctx):
+@pytest.mark.parametrize("T,rows", [(40, 50), (1100, 1000)])
+def test_gpu_mx_matmul_not_finite_stays_in_its_row(ctx, T, rows):
     g = gen(9)
-    m, x = synth.quant_matrix(g, MX, 50, 352), acts(g, 40, 352)
+    m, x = synth.quant_matrix(g, MX, rows, 352), acts(g, T, 352)
     x[3, 0], x[17, 351], x[39, 100] = np.nan, np.inf, -np.inf
-    m.reshape(50, 11, 17)[20, 10, 0] = 255
+    m.reshape(rows, 11, 17)[20, 10, 0] = 255
     bad_t, bad_r = [3, 17, 39], [20]
-    t = ctx.upload(m, MX, 50, 352)
-    y, z = np.empty((40, 50), np.float32), np.empty((40, 50), np.float32)
+    t = ctx.upload(m, MX, rows, 352)
+    y, z = np.empty((T, rows), np.float32), np.empty((T, rows), np.float32)
     ctx.quant_matmul(y, t, x)
-    xq = ctx.create(MX, 40, 352)
+    xq = ctx.create(MX, T, 352)
     ctx.quantize(xq, x)
     ctx.quant_matmul(z, t, xq)
-    keep_t, keep_r = np.setdiff1d(np.arange(40), bad_t), np.setdiff1d(np.arange(50), bad_r)
+    keep_t, keep_r = np.setdiff1d(np.arange(T), bad_t), np.setdiff1d(np.arange(rows), bad_r)
     w = mx.decode(m, 352)[keep_r]
     for got, xs in ((y, x[keep_t]), (z, mx.decode(mx.quantize(x), 352)[keep_t])):
         assert np.isnan(got[bad_t]).all() and np.isnan(got[:, bad_r]).all()
