@@ -130,6 +130,12 @@ __device__ __forceinline__ void mx_limbs(mx_f32x16 a, mx_f32x16 b, uint32_t s, P
     }
 }
 
+__device__ __forceinline__ float4 ldg16f_nt(const float *p) {
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p));
+    return make_float4(v.x, v.y, v.z, v.w);
+}
+
 // 32 floats at x (16-byte aligned)
 __device__ __forceinline__ void mx_load_block(const float *x, mx_f32x16 &a, mx_f32x16 &b) {
 #pragma unroll
