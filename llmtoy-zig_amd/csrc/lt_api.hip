@@ -371,6 +371,7 @@ int shape_tensor(lt_ctx *ctx, DevTensor &t, uint32_t type, size_t rows, size_t c
     t.bytes = t.total_rows * t.blocks_per_row * bb;
     t.held = t.bytes;
     if (type == LT_TYPE_MXFP4) {
+        if (t.total_rows > INT32_MAX) return fail(ctx, LT_ERR_UNSUPPORTED, "%zu rows of MXFP4 exceed 2^31 - 1", t.total_rows);
         const lt::MxDims d = lt::mx_dims(rows, t.blocks_per_row);
         t.held = lt::mx_code_bytes(d, n_experts) + lt::mx_scale_bytes(d, n_experts) + lt::mx_slack_bytes(d);
     }
@@ -778,7 +779,7 @@ int check_rows(lt_ctx *ctx, const DevTensor &T, size_t row0, size_t rows, const 
 }  // namespace
 
 extern "C" int lt_quantize(lt_ctx *ctx, lt_tensor *t, const float *x, size_t row0, size_t rows, uint32_t flags) {
-    if (!ctx || !t || !x) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (!ctx || !t || (!x && rows)) return fail(ctx, LT_ERR_INVALID, "null argument");
     int rc = check_rows(ctx, t->t, row0, rows, x, flags);
     if (rc || rows == 0) return rc;
     Span span_(ctx, "lt_quantize");
@@ -793,7 +794,7 @@ extern "C" int lt_quantize(lt_ctx *ctx, lt_tensor *t, const float *x, size_t row
 }
 
 extern "C" int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size_t rows, uint32_t flags) {
-    if (!ctx || !t || !out) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (!ctx || !t || (!out && rows)) return fail(ctx, LT_ERR_INVALID, "null argument");
     int rc = check_rows(ctx, t->t, row0, rows, out, flags);
     if (rc || rows == 0) return rc;
     Span span_(ctx, "lt_dequantize");
@@ -829,7 +830,7 @@ int check_matmul(lt_ctx *ctx, const DevTensor &W, uint32_t T, const float *out, 
 }  // namespace
 
 extern "C" int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const float *X, uint32_t T, uint32_t flags) {
-    if (!ctx || !out || !W || !X) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (!ctx || !W || (T && (!out || !X))) return fail(ctx, LT_ERR_INVALID, "null argument");
     const DevTensor &w = W->t;
     int rc = check_matmul(ctx, w, T, out, flags);
     if (rc) return rc;
@@ -856,7 +857,7 @@ extern "C" int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const floa
 
 extern "C" int lt_matmul_quantized(lt_ctx *ctx, float *out, const lt_tensor *W, const lt_tensor *X, uint32_t T,
                                    uint32_t flags) {
-    if (!ctx || !out || !W || !X) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (!ctx || !W || !X || (T && !out)) return fail(ctx, LT_ERR_INVALID, "null argument");
     const DevTensor &w = W->t, &x = X->t;
     int rc = check_matmul(ctx, w, T, out, flags);
     if (rc) return rc;

@@ -145,9 +145,10 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x,
         } else {  // scale words: 8 lanes a tile of 16
             const bool isw = c < L::kX;
             const MxSide &p = isw ? w : x;
-            const uint32_t first = isw ? m0 + (c - L::kWS) * 4 : n0 + (c - L::kXS) * 4, t32 = min(first + lane / 16, p.last);
-            src[i] = p.scales;
-            off[i] = (2 * t32 + lane / 8 % 2) * kq * 256 + lane % 8 * 16;
+            const uint32_t first = min(isw ? m0 + (c - L::kWS) * 4 : n0 + (c - L::kXS) * 4, p.last);
+            const uint32_t in = min(lane / 16, p.last - first);
+            src[i] = p.scales + (size_t)2 * first * kq * 256;
+            off[i] = (2 * in + lane / 8 % 2) * kq * 256 + lane % 8 * 16;
             stride[i] = 0;
         }
     }

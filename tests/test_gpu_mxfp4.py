@@ -279,6 +279,38 @@ def test_gpu_mx_matmul_of_a_tensor_with_itself(ctx):
     t.free()
 
 
+def test_gpu_mx_offsets_past_32_bits(ctx):
+    # codes of 4.3 GB: the last rows filled, all others zero
+    g = gen(17)
+    rows, cols, n, T = (1 << 19) + 32, 16384, 37, 20
+    t = ctx.create(MX, rows, cols)
+    w, x = g.standard_normal((n, cols)).astype(np.float32), acts(g, T, cols)
+    ctx.quantize(t, w, row0=rows - n)
+    m = mx.decode(mx.quantize(w), cols)
+    back = np.empty((n, cols), np.float32)
+    ctx.dequantize(back, t, row0=rows - n)
+    assert np.array_equal(back, m)
+    y, z = np.empty(rows, np.float32), np.empty((T, rows), np.float32)
+    ctx.quant_matvec(y, t, x[0])
+    ctx.quant_matmul(z, t, x)
+    for got, ref in ((y, x[0]), (z, x)):
+        assert not got[..., :rows - n].any()
+        close(got[..., rows - n:], *mx.product(m, ref))
+    t.free()
+
+
+def test_gpu_mx_clone_behind_a_quantisation(ctx):
+    # the copy is made of what the call before it has on its way
+    x = DeviceArray.from_numpy(acts(gen(18), 4096, 4096))
+    want = mx.quantize(x.numpy())
+    t = ctx.create(MX, 4096, 4096)
+    ctx.quantize(t, x)
+    c = t.clone()
+    assert np.array_equal(c.read().reshape(want.shape), want)
+    for a in (x, t, c):
+        a.free()
+
+
 # ------------------------------------------------------------------ experts
 def experts(ctx, g, E, D, F, Kd=None):
     Kd = Kd or F
@@ -505,6 +537,8 @@ def test_gpu_mx_refusals(ctx):
     I, U = ltlib.InvalidError, ltlib.UnsupportedError
     refused(U, lambda: ctx.create(ggml.Q8_0, 4, 64))
     refused(U, lambda: ctx.create(MX, 4, 48))
+    refused(U, lambda: ctx.create(MX, 1 << 31, 32))
+    refused(U, lambda: ctx.create(MX, 1 << 20, 32, 1 << 11))
     refused(I, lambda: ctx.create(MX, 0, 64))
     refused(I, lambda: ctx.create(MX, 1 << 40, 64, 1 << 40))
     refused(I, lambda: ctx.upload(np.zeros(33, np.uint8), MX, 1, 64))
@@ -530,6 +564,11 @@ def test_gpu_mx_refusals(ctx):
     assert lib.lt_quantize(ctx.ptr, t.handle, x.ctypes.data, 0, 2, 5) == ltlib.LT_ERR_INVALID
     ctx.quant_matmul(y[:0], t, x[:0])
     ctx.quant_matmul(y[:0], t, t)
+    assert lib.lt_matmul(ctx.ptr, None, t.handle, None, 0, 0) == lib.lt_matmul_quantized(ctx.ptr, None, t.handle, t.handle, 0, 0) == 0
+    assert lib.lt_quantize(ctx.ptr, t.handle, None, 20, 0, 0) == lib.lt_dequantize(ctx.ptr, None, t.handle, 0, 0, 0) == 0
+    for rc in (lib.lt_matmul(ctx.ptr, None, t.handle, x.ctypes.data, 2, 1), lib.lt_matmul(ctx.ptr, y.ctypes.data, t.handle, None, 2, 1),
+               lib.lt_quantize(ctx.ptr, t.handle, None, 0, 1, 1), lib.lt_dequantize(ctx.ptr, None, t.handle, 0, 1, 1)):
+        assert rc == ltlib.LT_ERR_INVALID
     refused(U, lambda: ctx.moe_forward_noalloc(DeviceArray((64,)), DeviceArray((64,)), ctx.upload(
         np.zeros((2, 64), np.float32), ggml.F32, 2, 64), ctx.create(MX, 64, 64, 2), ctx.create(MX, 64, 32, 2), 1, 32))
     for a in (t, e, q, wide, d):
