@@ -108,9 +108,9 @@ __global__ __launch_bounds__(256) void k_mx_quantize(const float *__restrict__ x
                 if (top >= 0x7f800000u) {
                     e = 255;
                 } else {
-                    const int up = 127 - (int)e;
-                    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, ldexpf(v[i].x, up), ldexpf(v[i].y, up), 1.0f, 0);
-                    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, ldexpf(v[i].z, up), ldexpf(v[i].w, up), 1.0f, 1);
+                    const float scale = __uint_as_float(e << 23);  // (its exponent is what counts: 0 is 2^-127)
+                    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[i].x, v[i].y, scale, 0);
+                    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[i].z, v[i].w, scale, 1);
                     word = (word & 0xfu) | (word & 0xf0u) << 4 | (word & 0xf00u) << 8 | (word & 0xf000u) << 12;  // a nibble a byte
                 }
             }
@@ -156,11 +156,9 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(float *__restrict__ out, 
         const uint32_t w = lc[b][r][j % 4], n = (j < 4 ? w : w >> 4) & 0x0f0f0f0fu;
         const uint32_t four = (n & 0xfu) | (n >> 4 & 0xf0u) | (n >> 8 & 0xf00u) | (n >> 12 & 0xf000u);
         const uint32_t e = ls[r][b % 4] >> (b / 4 * 8) & 255u;
-        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 1);
-        const int up = (int)e - 127;
-        float4 v = make_float4(ldexpf(lo[0], up), ldexpf(lo[1], up), ldexpf(hi[0], up), ldexpf(hi[1], up));
-        if (e == 255u) v = make_float4(NAN, NAN, NAN, NAN);
-        *reinterpret_cast<float4 *>(row + 512 * q + 64 * i + 4 * l) = v;
+        const float scale = __uint_as_float(e << 23);  // (255: every value NaN)
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, scale, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, scale, 1);
+        *reinterpret_cast<float4 *>(row + 512 * q + 64 * i + 4 * l) = make_float4(lo[0], lo[1], hi[0], hi[1]);
     }
 }
 
