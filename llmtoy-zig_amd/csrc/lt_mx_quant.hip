@@ -62,8 +62,10 @@ __global__ __launch_bounds__(kMxStage) void k_mx_blocks(uint8_t *raw, size_t nbl
 // scale words.  16 threads a row, 8 lanes a block with a float4 each; codes and
 // scales pass through LDS between a row's order and the tile's.  Bound by HBM:
 // 9728 x 4096 (181 MB) quantised in 30.8 us, 5.9 TB/s, with loads past the caches
-// (41.8 without; a block of 8 lanes on its own, with divisions, 43); read back in
-// 27.6.
+// (41.5 without; a block of 8 lanes on its own, with divisions, 43); read back in
+// 27.8.  What fits the L2s may be there still: 1024 x 4096 7.6 us past the caches,
+// 6.5 through them.
+constexpr size_t kMxNtBytes = 32 << 20;
 struct MxSpan {
     size_t row0, rows;  // of the tensor, over all experts
     size_t expert_rows;
@@ -79,6 +81,7 @@ struct MxTileAt {
     }
 };
 
+template <bool NT>
 __global__ __launch_bounds__(256) void k_mx_quantize(const float *__restrict__ x, MxSpan p, uint8_t *codes, uint8_t *scales) {
     __shared__ uint32_t lc[16][16][5];  // [block][row][word], a word of padding
     __shared__ uint8_t ls[16][4][4];    // [row][lane group][group of 4 blocks]
@@ -91,7 +94,7 @@ __global__ __launch_bounds__(256) void k_mx_quantize(const float *__restrict__ x
         float4 v[8];
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (16 * q + 2 * i + l / 8 < p.d.nb) v[i] = ldg16f_nt(row + 512 * q + 64 * i + 4 * l);
+            if (16 * q + 2 * i + l / 8 < p.d.nb) v[i] = NT ? ldg16f_nt(row + 512 * q + 64 * i + 4 * l) : ldg16f(row + 512 * q + 64 * i + 4 * l);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const uint32_t b = 2 * i + l / 8, j = l % 8;
@@ -191,8 +194,9 @@ hipError_t launch_mx_blocks(const DevTensor &t, uint8_t *raw, size_t nblk, size_
 }
 
 hipError_t launch_mx_quantize(const DevTensor &t, const float *x, size_t row0, size_t rows, hipStream_t s) {
+    const auto kernel = rows * t.cols * 4 > kMxNtBytes ? k_mx_quantize<true> : k_mx_quantize<false>;
     return over_tiles(t, row0, rows, [&](const MxSpan &p, dim3 grid) {
-        hipLaunchKernelGGL(k_mx_quantize, grid, dim3(256), 0, s, x, p, const_cast<uint8_t *>(t.p0), const_cast<uint8_t *>(t.p1));
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, x, p, const_cast<uint8_t *>(t.p0), const_cast<uint8_t *>(t.p1));
     });
 }
 
