@@ -119,10 +119,10 @@ void *lt_stream(lt_ctx *ctx);
  *                e * rows * rowBytes(type, cols).
  *   nbytes     : must equal n_experts * rows * rowBytes(type, cols)
  *                (ops/math.zig:194-208).
- * cols must be a multiple of the block size (32 for Q8_0, 256 for K-quants);
+ * cols must be a multiple of the block size (32 for Q8_0 and MXFP4, 256 for K-quants);
  * pad shorter rows with zero blocks.  The host buffer may be freed after the
  * call returns.  The device copy is repacked into a planar layout with the
- * same byte count: the GGUF bytes cross PCIe in 4 MiB pieces through pinned
+ * same byte count (MXFP4: into matrix operands, lt_tensor_bytes): the GGUF bytes cross PCIe in 4 MiB pieces through pinned
  * staging buffers (up to 8 in flight) and a device kernel splits them into
  * the planes.  The context keeps that staging (up to 64 MiB pinned host and
  * 64 MiB device memory) until lt_destroy. */
@@ -165,8 +165,8 @@ size_t lt_tensor_bytes(const lt_tensor *t);
  * sums give, which is NaN or an infinity (Q4_K and Q6_K subtract a block's
  * offset as a sum of its own, Q8_0 has none).  Q4_K and Q6_K activations below
  * about 2^-100 lose bits (their products are kept 2^-24 of their size).
- * MXFP4 activations are exact to 2^-24 of the largest of each 32 and any NaN or
- * infinity makes every output NaN.
+ * MXFP4 takes fp32 activations as they are, and any NaN or infinity among them
+ * makes every output NaN.
  * Replaces quantMatvec / quantMatvecPar (ops/math.zig:133-171, 277-320) and
  * MatvecSession.run / runQ8_1Mv (gpu/matvec.zig:497-647,
  * gemma4/gpu_weights.zig:1573-1607).  W must be a 2-D tensor. */
@@ -197,7 +197,7 @@ int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size
  * (main.zig:1916-1922). */
 int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const float *X, uint32_t T, uint32_t flags);
 /* The same with X the first T rows of a 2-D MXFP4 tensor (4-bit activations, as
- * lt_quantize makes them): out [T][rows], about five times lt_matmul's rate on
+ * lt_quantize makes them): out [T][rows], about four times lt_matmul's rate on
  * long batches.  X may be W.  flags: LT_HOST_IO (out is host memory). */
 int lt_matmul_quantized(lt_ctx *ctx, float *out, const lt_tensor *W, const lt_tensor *X, uint32_t T, uint32_t flags);
 

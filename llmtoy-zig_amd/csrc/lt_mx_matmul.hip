@@ -9,8 +9,11 @@
 // products; the instructions alone, their operands held in registers, take 238
 // us at the clock that the card holds under them (5.8 PFLOP/s; 8.9 with
 // constant operands), the product with its loads from LDS 253 us, the whole
-// kernel 290 us, and the limbs 25 us before it (130 MB, the card's copy rate).
-// With 4-bit X 82 us, of which the instructions alone take 61.
+// kernel 294 us, and the limbs 21 us before it (130 MB, 6.2 TB/s).  With 4-bit X
+// 82 us, of which the instructions alone take 61.  Middle sizes are bound by how
+// their tiles fall on the CUs: 509 x 4864 x 2816 is 152 of them on 256 CUs, 26 us
+// and the limbs 6 (smaller tiles, which need more waves or leave a SIMD with one,
+// 32.5 to 56 us in all against 31.6).
 //
 // What made it fast, on that size: both operands through LDS by direct loads
 // instead of registers (1570 -> 335 us); uniform addresses that move on by one
@@ -384,8 +387,8 @@ bool is_thin(const DevTensor &W, size_t T) { return (T + 15) / 16 * 16 * W.rows 
 
 // A stage of a 512 x 128 tile takes 1.13 us (one workgroup a CU), one of two 256
 // x 64 tiles on a CU 0.63 us: the fewer rounds' time.  4096 x 8192 x 4096: 316
-// and 348 us; 4095 x 7001 x 2816: 216 and 226; 1024 x 4096 x 4096: 105 and 66;
-// 509 x 4864 x 2816: 73 and 33.
+// and 348 us; 4095 x 7001 x 2816: 216 and 226; 1024 x 4096 x 4096: 105 and 62;
+// 509 x 4864 x 2816: 73 and 32.
 hipError_t limbs_product(const DevTensor &W, const MxSide &x, uint32_t T, float *out, hipStream_t s) {
     const size_t large = (tiles_of(W, T, 512, 128) + kCus - 1) / kCus, mid = (tiles_of(W, T, 256, 64) + 2 * kCus - 1) / (2 * kCus);
     if (is_thin(W, T))

@@ -14,11 +14,12 @@
 // first product, three parts cut off by masks 0.1.  FP8 operands converted in
 // pairs are no way out: sums with them were 1e-4 off.)
 //
-// Bound by the weights' bytes, and where there are few of those by the chain
-// launch - vector - product - sum over the waves.  A workgroup converts the
-// vector once, while its first weights are on their way.  A tile's rows are
-// split over S waves, 16 blocks (a scale word) at a time; what they summed
-// meets in LDS in the waves' order.
+// Bound by the weights' bytes (262144 x 2816, 392 MB: 65 us, 6.0 TB/s), and where
+// there are few of those by the chain launch - vector - product - sum over the
+// waves: 4096 x 4096 4.9 us a graph's node, of which an empty one has 1.8 and the
+// loads alone 4.4; 4865 x 896 3.6.  A workgroup converts the vector once, while its
+// first weights are on their way.  A tile's rows are split over S waves, 16 blocks
+// (a scale word) at a time; what they summed meets in LDS in the waves' order.
 #include "llmtoy_hip.h"
 #include "lt_internal.h"
 #include "lt_mx.h"
@@ -222,7 +223,11 @@ __global__ __launch_bounds__(64 * kMvWaves) void k_mx_matvec(const uint8_t *code
 // expert in the router's logits (up to 64 PER) itself, and a workgroup of its own
 // writes the selection and its weights for the down kernel.  Against the top-k
 // in the router's last workgroup, 128 experts of 768 by 2048, top 8: 18.4 -> 16.0
-// us a layer.
+// us a layer.  (One wave that selects for all eight: 6.45 us against 5.75, as the
+// others' weights then wait for it.)
+//
+// 13.4 MB of weights there: 5.4 us with the ids at hand, of which the launch has
+// 1.8, the weights at the rate of a copy 2.6.
 struct MxRoute {
     const float *logits;
     uint32_t k, norm, *ids;
@@ -304,6 +309,8 @@ __global__ __launch_bounds__(64 * kPairWaves) void k_mx_gate_up(MxPair p, const 
 
 // out[i] = sum over slots of w (D_id h[slot])[i]: the waves take the (slot, 16
 // blocks) items of a tile's rows in turn, `per` slots' vectors in LDS at once.
+// 8 x 2048 x 768 (6.7 MB): 5.7 us, a chain of launch (1.8), ids, weights, sums.  8
+// rows a workgroup, twice as many of them: 5.7, and 6.3 -> 10.4 on 4 x 2816 x 2112.
 constexpr int kDownWaves = 16;
 __global__ __launch_bounds__(64 * kDownWaves) void k_mx_down(const uint8_t *codes, const uint8_t *scales, MxDims d,
                                                              uint32_t rows, uint32_t n_experts, const float *h,
@@ -370,7 +377,7 @@ constexpr size_t kDownLds = 72 << 10;
 // 8 waves of several tiles, which walk on.
 constexpr size_t kMvTarget = 4096, kMvGroups = 1024;
 // Matrices from 8 MiB on are read past the caches: a model of them does not fit
-// the 256 MiB there are.
+// the 256 MiB there are (262144 x 2816 73 -> 65 us, 4096 x 4096 5.1 -> 4.9).
 constexpr size_t kNtBytes = 8u << 20;
 
 // Lets a kernel use the CU's LDS, once per kernel and device.
