@@ -148,13 +148,13 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x,
             src[i] = x.data + (size_t)t64 * steps * kPairBytes + (c - L::kX) % 15 * 1024;
             off[i] = lane * 16;
             stride[i] = (int)kPairBytes;
-        } else {  // scale words: 8 lanes a tile of 16
+        } else {  // scale words: 16 lanes a tile of 32, [block][row] of the pair
             const bool isw = c < L::kX;
             const MxSide &p = isw ? w : x;
             const uint32_t first = min(isw ? m0 + (c - L::kWS) * 4 : n0 + (c - L::kXS) * 4, p.last);
             const uint32_t in = min(lane / 16, p.last - first);
             src[i] = p.scales + (size_t)2 * first * kq * 256;
-            off[i] = (2 * in + lane / 8 % 2) * kq * 256 + lane % 8 * 16;
+            off[i] = (2 * in + lane / 4 % 2) * kq * 256 + lane / 8 % 2 * 64 + lane % 4 * 16;
             stride[i] = 0;
         }
     }
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x,
     auto step = [&](auto odd, uint32_t pair, const uint8_t *st, uint8_t *dst) {
         constexpr int ODD = decltype(odd)::value;
         const uint32_t shift = pair / 2 % 4 * 8;
-        const uint32_t at = lane % 32 / 16 * 128 + lane / 32 * 64 + lane % 16 * 4;  // a lane's scale word
+        const uint32_t at = lane * 4;  // a lane's scale word
         mx_op b[MI], a[NI], an[NI];
         int sb[MI], sa[NI];
 #pragma unroll
