@@ -102,6 +102,8 @@ struct MxTile {
     static_assert(NST <= kStages, "the memory that the last loads run into");
 };
 
+constexpr size_t kStageSums = 12 << 20;  // 48 MiB
+
 // Until this wave has at most N loads in flight and no LDS access; then, behind
 // the barrier, every wave of the workgroup.
 template <int N>
@@ -237,8 +239,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x,
     arrive<0>();  // no load into LDS outlives the workgroup
 
     // Past the caches where the stores are whole lines (4096 x 8192 x 4096 324 ->
-    // 316 us, 1024 x 4096 x 4096 with 4-bit X 20.1 -> 19.2); with rows that begin
-    // inside a line that would write each border twice (7001 rows: 68 -> 104).
+    // 316 us, 1024 x 4096 x 4096 with 4-bit X 20.1 -> 19.2).
     const bool lines = rows % 32 == 0 && ((uintptr_t)out & 127) == 0;
     auto store = [&](auto past) {
 #pragma unroll
@@ -259,10 +260,54 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_mx_gemm(MxSide w, MxSide x,
                 }
             }
     };
-    if (lines)
-        store(std::true_type{});
-    else
-        store(std::false_type{});
+    if (lines) return store(std::true_type{});
+    // (the smallest tiles' products have fewer)
+    if (L::kRows * L::kVecs <= 8 || (size_t)T * rows <= kStageSums) return store(std::false_type{});
+    // Rows that begin inside a line, and more sums than the L2s put together: the sums
+    // of 8 WC vectors at a time pass through LDS, where a vector's lie as its 16-byte
+    // pieces of out do, and a wave stores all of them in a row; past the caches but
+    // for the lines at both ends.  With 4-bit X, straight from the registers | this:
+    // 4095 x 7001 x 2816 67.8 | 62.0 us, 1100 x 30001 x 512 53.7 | 39.3; but 2000 x
+    // 5001 x 1024 (40 MB) 17.1 | 17.5, 500 x 4865 x 896 7.0 | 8.8.
+    constexpr uint32_t kR = 32 * L::kRows, kPitch = kR + 4;
+    static_assert(8 * WC * kPitch * 4 <= sizeof lds, "the sums take the stages' place");
+    float *const sums = reinterpret_cast<float *>(lds);
+    const int count = (int)min(kR, rows - m0 * 32);
+    const uint32_t base = (uint32_t)((uintptr_t)out / 4) + m0 * 32;  // (out is on 16 bytes)
+#pragma unroll
+    for (int n = 0; n < NI; n++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            if (n || g) arrive<63>();  // (not for the stores)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t v = wc * 8 + 4 * (lane / 32) + j, t = (n0 + wc * NI + n) * 32 + g * 8 + 4 * (lane / 32) + j;
+                float *to = sums + v * kPitch + (base + t * rows) % 4 + wr * MI * 32 + lane % 32;
+#pragma unroll
+                for (int m = 0; m < MI; m++) to[m * 32] = acc[m][n][g * 4 + j];
+            }
+            arrive<63>();
+            for (int v = wave; v < 8 * WC; v += L::kWaves) {
+                const uint32_t t = (n0 + v / 8 * NI + n) * 32 + g * 8 + v % 8;
+                if (t >= T) continue;
+                float *const to = out + (size_t)t * rows + m0 * 32;
+                const int q = (int)((base + t * rows) % 4);
+                const float *from = sums + v * kPitch;
+                for (int i = 4 * (int)lane; i + 4 <= count + q; i += 256) {
+                    if (i < q) continue;
+                    const mx_acc16 y = *reinterpret_cast<const mx_acc16 *>(from + i);
+                    mx_acc16 *at = reinterpret_cast<mx_acc16 *>(to - q + i);
+                    const int line = i - q - (int)((uintptr_t)at / 4 % 32);  // where its line begins
+                    if (line >= 0 && line + 32 <= count)
+                        __builtin_nontemporal_store(y, at);
+                    else
+                        *at = y;
+                }
+                // up to 3 at both ends
+                const int e = lane < 3 ? (int)lane : (count + q) / 4 * 4 - q + (int)lane - 3;
+                if (lane < 6 && e >= 0 && e < count && (lane >= 3 || e < (4 - q) % 4)) to[e] = from[q + e];
+            }
+        }
 }
 
 // Few vectors, or few rows: a workgroup computes 16 RT rows by 16 NT vectors, its

@@ -7,7 +7,7 @@ import llmtoy_amd as lt
 import mx_reference as mx
 from llmtoy_amd import ggml, synth
 from llmtoy_amd import lib as ltlib
-from llmtoy_amd.hip import DeviceArray, Graph
+from llmtoy_amd.hip import DeviceArray, DeviceView, Graph
 
 pytestmark = pytest.mark.gpu
 
@@ -233,6 +233,29 @@ def test_gpu_mx_matmul(ctx, T, rows, cols):
                                          (130, 9001, 96), (9, 9001, 160), (2001, 8003, 96)])
 def test_gpu_mx_matmul_larger(ctx, T, rows, cols):
     test_gpu_mx_matmul(ctx, T, rows, cols)
+
+
+# more sums than are stored from registers, rows that begin anywhere in a line
+@pytest.mark.parametrize("T,rows,cols,shift", [(2001, 8403, 32, 0), (1601, 8002, 64, 4), (3002, 4200, 32, 8), (1700, 8192, 64, 4),
+                                               (1537, 8193, 32, 12)])
+def test_gpu_mx_matmul_large_output(ctx, T, rows, cols, shift):
+    print(f"matmul T {T} {rows}x{cols} out + {shift}", flush=True)
+    g = gen(T, rows, cols, shift)
+    m, x = synth.quant_matrix(g, MX, rows, cols), acts(g, T, cols)
+    t = ctx.upload(m, MX, rows, cols)
+    xq = ctx.create(MX, T, cols)
+    ctx.quantize(xq, x)
+    dx = DeviceArray.from_numpy(x)
+    for X, xs in ((dx, x), (xq, mx.decode(mx.quantize(x), cols))):
+        buf = DeviceArray.from_numpy(np.full(T * rows + 64, 5.0, np.float32))
+        ctx.quant_matmul(DeviceView(buf.ptr + 4 * shift, (T, rows), np.float32), t, X)
+        ctx.sync()
+        got = buf.numpy()
+        assert (got[:shift] == 5).all() and (got[shift + T * rows:] == 5).all()
+        close(got[shift:shift + T * rows].reshape(T, rows), *mx.product(mx.decode(m, cols), xs))
+        buf.free()
+    for a in (dx, xq, t):
+        a.free()
 
 
 def test_gpu_mx_matmul_more_vectors_than_the_workspace_holds(ctx):
