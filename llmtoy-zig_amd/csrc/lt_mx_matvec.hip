@@ -140,25 +140,34 @@ __device__ __forceinline__ void mx_order() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// Division of u by a number that the host knows, as a multiplication: exact for
+// u d < 2^32.  (A division takes a chain of 30 instructions, and these stand
+// before a kernel's first loads.)
+struct MxDiv {
+    uint32_t d, m;
+    __device__ __forceinline__ uint32_t by(uint32_t u) const { return d == 1 ? u : __umulhi(u, m); }
+};
+MxDiv mx_div(uint32_t d) { return {d, (uint32_t)(((1ull << 32) + d - 1) / d)}; }
+
 constexpr int kMvWaves = 16;  // of a workgroup at most
 
-// Workgroups of S waves a tile (and blockDim / 64 / S tiles side by side) walk the
-// tiles.  Two items (16 rows by 16 blocks) of a wave are on their way, over the
+// Workgroups of S waves a tile (threadIdx.x; and TP tiles side by side, threadIdx.y)
+// walk the tiles.  Two items (16 rows by 16 blocks) of a wave are on their way, over the
 // tiles' ends, before the vector is converted and from then on.
 template <bool NT>
 __global__ __launch_bounds__(64 * kMvWaves) void k_mx_matvec(const uint8_t *codes, const uint8_t *scales, MxDims d,
-                                                             uint32_t ntiles, uint32_t expert_rows, uint32_t S,
+                                                             uint32_t ntiles, uint32_t expert_rows, uint32_t S, uint32_t TP,
                                                              const float *x, float *y) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ float part[2][kMvWaves][16];
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sp = wave % S, tp = wave / S;
-    const uint32_t TP = blockDim.x / 64 / S, stride = gridDim.x * TP, t0 = blockIdx.x * TP;
+    const uint32_t sp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tp = __builtin_amdgcn_readfirstlane(threadIdx.y);
+    const uint32_t wave = tp * S + sp, threads = 64 * S * TP, tid = 64 * wave + lane, stride = gridDim.x * TP, t0 = blockIdx.x * TP;
     const bool first = p32_first(lane);
     mx_u32x4 *const v = reinterpret_cast<mx_u32x4 *>(lds);
     const uint32_t units = 16 * d.kg;
     MxQuarter xb;
-    if (threadIdx.x < units) xb = mx_vec_load(x, threadIdx.x, d.nb);
+    if (tid < units) xb = mx_vec_load(x, tid, d.nb);
     mx_order();
 
     // every wave of the workgroup goes through the same number of tiles (past
@@ -175,8 +184,8 @@ __global__ __launch_bounds__(64 * kMvWaves) void k_mx_matvec(const uint8_t *code
     fetch(w0);
     if (n > 1) fetch(w1);
     mx_order();
-    if (threadIdx.x < units) mx_vec_put(v, threadIdx.x, xb);
-    for (uint32_t u = threadIdx.x + blockDim.x; u < units; u += blockDim.x) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
+    if (tid < units) mx_vec_put(v, tid, xb);
+    for (uint32_t u = tid + threads; u < units; u += threads) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
     __syncthreads();
 
     MxSum acc = {};
@@ -238,15 +247,16 @@ struct MxPair {
     uint32_t row0[2];  // first row of either half
     MxDims d;
 };
-constexpr int kPairWaves = 8;
+constexpr uint32_t kPairWaves = 8, kPairThreads = 64 * kPairWaves;
 template <int ROUTE>
 __global__ __launch_bounds__(64 * kPairWaves) void k_mx_gate_up(MxPair p, const float *x, const uint32_t *ids, MxRoute route,
                                                                 uint32_t n_experts, uint32_t F, uint32_t down_cols,
                                                                 uint32_t act, float *h) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ float part[kPairWaves][16];
+    constexpr uint32_t S = kPairWaves / 2;
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), S = blockDim.x / 128, half = wave / S, sp = wave % S;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave / S, sp = wave % S;
     const uint32_t j0 = blockIdx.x * 16;
     const MxDims &d = p.d;
     const uint32_t units = 16 * d.kg;
@@ -280,11 +290,11 @@ __global__ __launch_bounds__(64 * kPairWaves) void k_mx_gate_up(MxPair p, const 
     const MxRow r = mx_row_at(half ? p.codes[1] : p.codes[0], half ? p.scales[1] : p.scales[0], d, expert,
                               (half ? p.row0[1] : p.row0[0]) + j, lane);
     MxWords w0, w1;
-    mx_fetch<false>(w0, r, sp, d.kg);
+    if (sp < d.kq) mx_fetch<false>(w0, r, sp, d.kg);
     if (sp + S < d.kq) mx_fetch<false>(w1, r, sp + S, d.kg);
     mx_order();
     if (threadIdx.x < units) mx_vec_put(v, threadIdx.x, xb);
-    for (uint32_t u = threadIdx.x + blockDim.x; u < units; u += blockDim.x) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
+    for (uint32_t u = threadIdx.x + kPairThreads; u < units; u += kPairThreads) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
     __syncthreads();
     MxSum acc = {};
     for (uint32_t q = sp; q < d.kq; q += 2 * S) {
@@ -315,12 +325,13 @@ constexpr int kDownWaves = 16;
 __global__ __launch_bounds__(64 * kDownWaves) void k_mx_down(const uint8_t *codes, const uint8_t *scales, MxDims d,
                                                              uint32_t rows, uint32_t n_experts, const float *h,
                                                              const uint32_t *ids, const float *wts, uint32_t k,
-                                                             uint32_t per, const float *base, int accumulate,
-                                                             const float *dscale, float *out) {
+                                                             uint32_t per, uint32_t NW, MxDiv by_kq, MxDiv by_of,
+                                                             const float *base, int accumulate, const float *dscale,
+                                                             float *out) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ float part[kDownWaves][16];
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = blockDim.x / 64;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), threads = 64 * NW;
     const bool first = p32_first(lane);
     const uint32_t row0 = blockIdx.x * 16, vec = (uint32_t)mx_vec_bytes(d.kg), of = 16 * d.kg;
     mx_acc16 sum = {};
@@ -328,19 +339,22 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_mx_down(const uint8_t *code
         const uint32_t n = min(per, k - s0), items = n * d.kq, units = n * of;
         if (s0) __syncthreads();
         auto vec_of = [&](uint32_t i) { return reinterpret_cast<mx_u32x4 *>(lds + i * vec); };
-        auto load = [&](uint32_t u) { return mx_vec_load(h + (size_t)(s0 + u / of) * d.nb * 32, u % of, d.nb); };
-        auto put = [&](uint32_t u, const MxQuarter &x) { mx_vec_put(vec_of(u / of), u % of, x); };
+        auto load = [&](uint32_t u) {
+            const uint32_t i = by_of.by(u);
+            return mx_vec_load(h + (size_t)(s0 + i) * d.nb * 32, u - i * of, d.nb);
+        };
+        auto put = [&](uint32_t u, const MxQuarter &x) { mx_vec_put(vec_of(0), u, x); };  // (the vectors lie in a row)
         MxQuarter xb;
         if (threadIdx.x < units) xb = load(threadIdx.x);
         mx_order();
         auto fetch = [&](MxWords &w, uint32_t it) {
-            const uint32_t e = min(ids[s0 + it / d.kq], n_experts - 1);
-            mx_fetch<false>(w, mx_row_at(codes, scales, d, e, row0 + (uint32_t)(lane & 15), lane), it % d.kq, d.kg);
+            const uint32_t i = by_kq.by(it), e = min(ids[s0 + i], n_experts - 1);
+            mx_fetch<false>(w, mx_row_at(codes, scales, d, e, row0 + (uint32_t)(lane & 15), lane), it - i * d.kq, d.kg);
         };
         auto use = [&](const MxWords &w, uint32_t it) {
-            const uint32_t i = it / d.kq, e = ids[s0 + i];
+            const uint32_t i = by_kq.by(it), e = ids[s0 + i];
             MxSum t = {};
-            mx_dot(w, vec_of(i), it % d.kq, d.kg, lane, t);
+            mx_dot(w, vec_of(i), it - i * d.kq, d.kg, lane, t);
             if (e < n_experts) sum += t.all() * (dscale ? wts[s0 + i] * dscale[e] : wts[s0 + i]);
         };
         MxWords w0, w1;
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_mx_down(const uint8_t *code
         if (wave + NW < items) fetch(w1, wave + NW);
         mx_order();
         if (threadIdx.x < units) put(threadIdx.x, xb);
-        for (uint32_t u = threadIdx.x + blockDim.x; u < units; u += blockDim.x) put(u, load(u));
+        for (uint32_t u = threadIdx.x + threads; u < units; u += threads) put(u, load(u));
         __syncthreads();
         for (uint32_t it = wave; it < items; it += 2 * NW) {
             use(w0, it);
@@ -409,8 +423,8 @@ hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStr
     S = (d.kq + each - 1) / each;
     const uint32_t TP = tiles * S <= kMvTarget || S > 4 ? 1 : 8 / S;
     const size_t groups = (tiles + TP - 1) / TP;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kMvGroups ? groups : kMvGroups)), dim3(64 * S * TP),
-                       mx_vec_bytes(d.kg), s, W.p0, W.p1, d, (uint32_t)tiles, (uint32_t)W.rows, S, x, y);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kMvGroups ? groups : kMvGroups)), dim3(64 * S, TP),
+                       mx_vec_bytes(d.kg), s, W.p0, W.p1, d, (uint32_t)tiles, (uint32_t)W.rows, S, TP, x, y);
     return hipGetLastError();
 }
 
@@ -421,8 +435,7 @@ static hipError_t launch_pair(const MxPair &p, const float *x, const uint32_t *i
     hipError_t e = allow_lds((const void *)k_mx_gate_up<ROUTE>, set);
     if (e != hipSuccess) return e;
     const dim3 grid((down_cols + 15) / 16 + (ROUTE ? 1 : 0), k);
-    const uint32_t S = p.d.kq < (uint32_t)kPairWaves / 2 ? p.d.kq : (uint32_t)kPairWaves / 2;
-    hipLaunchKernelGGL(k_mx_gate_up<ROUTE>, grid, dim3(128 * S), mx_vec_bytes(p.d.kg), s, p, x, ids, route, n_experts, F,
+    hipLaunchKernelGGL(k_mx_gate_up<ROUTE>, grid, dim3(kPairThreads), mx_vec_bytes(p.d.kg), s, p, x, ids, route, n_experts, F,
                        down_cols, act, h);
     return hipGetLastError();
 }
@@ -461,7 +474,8 @@ hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint3
     per = per < 1 ? 1 : per > k ? k : per;
     const uint32_t items = per * d.kq, NW = items < (uint32_t)kDownWaves ? items : (uint32_t)kDownWaves;
     hipLaunchKernelGGL(k_mx_down, dim3((unsigned)d.tiles), dim3(64 * NW), per * vec, s, D.p0, D.p1, d, (uint32_t)D.rows,
-                       (uint32_t)D.n_experts, h, ids, w, k, per, base, accumulate, dscale, out);
+                       (uint32_t)D.n_experts, h, ids, w, k, per, NW, mx_div(d.kq), mx_div(16 * d.kg), base, accumulate, dscale,
+                       out);
     return hipGetLastError();
 }
 
