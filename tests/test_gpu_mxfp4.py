@@ -230,7 +230,8 @@ def test_gpu_mx_matmul(ctx, T, rows, cols):
 
 # past the thin kernel's range: each of the tiles, ragged on every side
 @pytest.mark.parametrize("T,rows,cols", [(300, 700, 640), (1000, 300, 4096), (1100, 1030, 288), (1300, 1000, 1056),
-                                         (130, 9001, 96), (9, 9001, 160), (2001, 8003, 96)])
+                                         (130, 9001, 96), (9, 9001, 160), (2001, 8003, 96), (65536, 9, 32),
+                                         (65536, 40, 64)])
 def test_gpu_mx_matmul_larger(ctx, T, rows, cols):
     test_gpu_mx_matmul(ctx, T, rows, cols)
 
@@ -319,6 +320,22 @@ def test_gpu_mx_offsets_past_32_bits(ctx):
     for got, ref in ((y, x[0]), (z, x)):
         assert not got[..., :rows - n].any()
         close(got[..., rows - n:], *mx.product(m, ref))
+    t.free()
+
+
+def test_gpu_mx_more_tiles_than_a_grid_holds(ctx):
+    # 68,750 tiles of 16 rows, from a row inside one on
+    rows, row0 = 1100000, 5
+    x = np.tile(acts(gen(19), 1000, 32), (rows // 1000, 1))
+    want = np.tile(mx.quantize(x[:1000]), (rows // 1000, 1))
+    t = ctx.create(MX, rows + 20, 32)
+    ctx.quantize(t, x, row0=row0)
+    got = t.read().reshape(-1, 17)
+    assert np.array_equal(got[row0:row0 + rows], want)
+    assert not got[:row0].any() and not got[row0 + rows:].any()
+    back = np.empty_like(x)
+    ctx.dequantize(back, t, row0=row0)
+    assert np.array_equal(back, np.tile(mx.decode(want[:1000], 32).astype(np.float32), (rows // 1000, 1)))
     t.free()
 
 
@@ -521,6 +538,31 @@ def test_gpu_mx_decode_and_prompt_in_one_graph(ctx):
     graph.destroy()
     for t in (GU, DN, W, R, xq, X, *outs):
         t.free()
+
+
+def test_gpu_mx_two_graphs_of_one_context(ctx):
+    # they share the context's workspace: replayed in turn, each with inputs of its own
+    g = gen(20)
+    W = ctx.upload(synth.quant_matrix(g, MX, 333, 640), MX, 333, 640)
+    Ts, xs, outs, want, graphs = (37, 90), [], [], [], []
+    for T in Ts:
+        x = acts(g, T, 640)
+        xs.append(DeviceArray.from_numpy(x))
+        outs.append(DeviceArray((T, 333)))
+        want.append(ctx.quant_matmul(np.empty((T, 333), np.float32), W, x).copy())
+        ctx.quant_matmul(outs[-1], W, xs[-1])
+        ctx.sync()
+        graphs.append(Graph(ctx.stream, lambda o=outs[-1], d=xs[-1]: ctx.quant_matmul(o, W, d)))
+    for i in (0, 1, 1, 0, 1, 0, 0):
+        graphs[i].launch()
+        graphs[1 - i].launch()
+        ctx.sync()
+        for w, o in zip(want, outs):
+            assert np.array_equal(w, o.numpy())
+    for a in (*graphs,):
+        a.destroy()
+    for a in (W, *xs, *outs):
+        a.free()
 
 
 def test_gpu_mx_two_contexts_side_by_side(ctx):
