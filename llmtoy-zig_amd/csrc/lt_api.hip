@@ -88,6 +88,13 @@ struct lt_ctx {
     // lt_moe_forward_noalloc
     uint8_t *na_base = nullptr;
     lt::FusedScratch na_fsc{};
+    // hand-over memory of the single-launch MXFP4 layer, one for each shape that
+    // came by (its epochs are counted by the shape's own grid)
+    struct MxHand {
+        size_t n_experts, k, d_model, down_cols;
+        uint8_t *p;
+    };
+    std::vector<MxHand> mx_hands;
     // hand-over memory of the single-launch dense FFN (allocated by lt_init)
     void *ffn = nullptr;
     lt::FfnScratch ffsc{};
@@ -473,6 +480,35 @@ int ensure_fused(lt_ctx *ctx) {
     return LT_OK;
 }
 
+// The same for the MXFP4 layer's, of one shape.
+int mx_hand_of(lt_ctx *ctx, size_t n_experts, size_t k, size_t d_model, size_t down_cols, uint8_t **out) {
+    for (const lt_ctx::MxHand &m : ctx->mx_hands)
+        if (m.n_experts == n_experts && m.k == k && m.d_model == d_model && m.down_cols == down_cols) {
+            *out = m.p;
+            return LT_OK;
+        }
+    if (capturing(ctx))
+        return fail(ctx, LT_ERR_INVALID,
+                    "the first MoE call of a shape with MXFP4 experts on a context cannot be captured into a graph: make one "
+                    "call before capturing");
+    try {
+        ctx->mx_hands.reserve(ctx->mx_hands.size() + 1);  // so that push_back below cannot throw
+    } catch (...) {
+        return fail(ctx, LT_ERR_OOM, "host allocation failed");
+    }
+    const size_t bytes = lt::moe_mx_bytes((uint32_t)n_experts, (uint32_t)k, d_model, down_cols);
+    void *p = nullptr;
+    LT_HIP(ctx, hipMalloc(&p, bytes));
+    const hipError_t e = hipMemset(p, 0, bytes);
+    if (e != hipSuccess) {
+        (void)hipFree(p);
+        return hip_fail(ctx, e, "hand-over memory");
+    }
+    ctx->mx_hands.push_back({n_experts, k, d_model, down_cols, (uint8_t *)p});
+    *out = (uint8_t *)p;
+    return LT_OK;
+}
+
 // lt_init's device set-up: the host-mapped error word, the address of this
 // device's static scratch, and the XCD placement probe (run once, into the
 // static scratch's probe area).  LT_FUSED_AGENT_HANDOVER=1 turns the same-XCD
@@ -620,6 +656,7 @@ extern "C" void lt_destroy(lt_ctx *ctx) {
     if (ctx->prof.stamps) (void)hipFree(ctx->prof.stamps);
     if (ctx->ticket) (void)hipFree(ctx->ticket);
     if (ctx->fused) (void)hipFree(ctx->fused);
+    for (const lt_ctx::MxHand &m : ctx->mx_hands) (void)hipFree(m.p);
     if (ctx->ffn) (void)hipFree(ctx->ffn);
     if (ctx->pin) (void)hipHostFree(ctx->pin);
     if (ctx->fused_err) (void)hipHostFree(ctx->fused_err);
@@ -1300,6 +1337,15 @@ int moe_dev(lt_ctx *ctx, float *out, const float *x, const DevTensor &R, const f
                                 (flags & LT_MOE_UNFUSED) != 0)))
             return rc;
         base = (const float *)ctx->shared.p;
+    }
+    if (lt::moe_mx_fits(R, GU, D, k) && !(flags & LT_MOE_UNFUSED)) {
+        uint8_t *hand = nullptr;
+        if ((rc = mx_hand_of(ctx, R.total_rows, k, D.rows, Kd, &hand))) return rc;
+        return launch_rc(ctx,
+                         lt::launch_moe_mx(R, bias, GU, D, x, k, (flags & LT_MOE_NORM_TOPK) ? 1u : 0u, d_expert, act, base,
+                                           (flags & LT_MOE_ACCUMULATE) ? 1 : 0, out, r.ids, r.w, hand, ctx->xcd_local,
+                                           ctx->err_dev, ctx->stream),
+                         "moe_mx");
     }
     if ((rc = ensure(ctx, ctx->eh, (size_t)k * Kd * 4))) return rc;
     float *h = (float *)ctx->eh.p;

@@ -376,6 +376,14 @@ hipError_t launch_expert_gate_up_mx_routed(const DevTensor &GU, const float *x, 
                                            float *w_out, hipStream_t s);
 hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint32_t *ids, const float *w, uint32_t k,
                                  const float *base, int accumulate, const float *dscale, float *out, hipStream_t s);
+// A layer in one launch (lt_mx_moe.hip): an F32 router (rows of a multiple of 256),
+// and slots that keep the XCDs busy (moe_mx_fits).  `hand` is moe_mx_bytes(shape),
+// zero at first and kept for calls of this shape.
+bool moe_mx_fits(const DevTensor &R, const DevTensor &GU, const DevTensor &D, uint32_t k);
+size_t moe_mx_bytes(uint32_t n_experts, uint32_t k, size_t d_model, size_t down_cols);
+hipError_t launch_moe_mx(const DevTensor &R, const float *bias, const DevTensor &GU, const DevTensor &D, const float *x, uint32_t k,
+                         uint32_t norm, uint32_t d_expert, uint32_t act, const float *base, int accumulate, float *out,
+                         uint32_t *ids, float *w, uint8_t *hand, int xcd_local, uint32_t *err, hipStream_t s);
 // out [T][rows] = X [T][cols] W^T; ws: matmul_mx_workspace(T, cols) bytes.
 size_t matmul_mx_workspace(size_t T, size_t cols);
 hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *ws, float *out, hipStream_t s);

@@ -438,6 +438,128 @@ def test_gpu_mx_moe_forward(ctx, E, D, F, k, norm, router):
         t.free()
 
 
+# the layer in one launch: slots for every XCD or nearly, rows and experts of every kind
+@pytest.mark.parametrize("E,D,F,Kd,k,act", [(6, 256, 40, 64, 6, 0), (7, 512, 32, 32, 7, 1), (128, 2048, 96, 96, 8, 0),
+                                            (256, 256, 160, 160, 8, 0), (40, 768, 80, 544, 14, 1), (255, 256, 64, 64, 15, 0),
+                                            (16, 1280, 48, 64, 16, 0), (9, 16384, 16, 32, 6, 0), (9, 256, 4100, 4128, 8, 0)])
+def test_gpu_mx_moe_one_launch(ctx, E, D, F, Kd, k, act):
+    print(f"one launch E {E} D {D} F {F} Kd {Kd} k {k}", flush=True)
+    g = gen(E, D, F, k, 21)
+    GU, DN, w = experts(ctx, g, E, D, F, Kd)
+    r, bias = (g.standard_normal((E, D)) * 0.05).astype(np.float32), g.standard_normal(E).astype(np.float32)
+    R, r64 = ctx.upload(r, ggml.F32, E, D), r.astype(np.float64)
+    for seed in range(3):
+        x, out = acts(gen(22, seed), D), g.standard_normal(D).astype(np.float32)
+        before, norm = out.astype(np.float64), seed % 2 == 0
+        ids, p = route(r64 @ x.astype(np.float64) + bias, k, norm)
+        _, ref, bound = expert_ref(w, x, ids, p, F, act)
+        got_ids, got_p = np.empty(k, np.uint32), np.empty(k, np.float32)
+        ctx.moe_forward(out, x, R, GU, DN, k, F, act=act, norm_topk=norm, accumulate=True, bias=bias, out_ids=got_ids, out_w=got_p)
+        assert got_ids.tolist() == ids.tolist()
+        slack = 2 * (D * 2.0 ** -24 * (np.abs(r64) @ np.abs(x)).max() + 2.0 ** -20)  # as above
+        assert (np.abs(got_p - p) <= slack * p).all()
+        more = slack * np.abs(ref) + slack * sum(q * np.abs(w["dn"][e]).sum(1) for e, q in zip(ids, p))
+        close(out, before + ref, bound + more + 2.0 ** -23 * (np.abs(before) + np.abs(ref)))
+        first = np.empty(D, np.float32)
+        for again in range(3):  # in the slots' order: the same bits
+            y = np.empty(D, np.float32)
+            ctx.moe_forward(y, x, R, GU, DN, k, F, act=act, norm_topk=norm, bias=bias)
+            if again == 0:
+                first = y
+            assert np.array_equal(first, y)
+        y = np.empty(D, np.float32)
+        ctx.moe_forward(y, x, R, GU, DN, k, F, act=act, norm_topk=norm, bias=bias, unfused=True)
+        assert np.linalg.norm(y - first) <= 2.0 ** -18 * np.linalg.norm(first)
+    for t in (R, GU, DN):
+        t.free()
+
+
+def test_gpu_mx_moe_one_launch_in_graphs(ctx, monkeypatch):
+    # two layers of different shapes and one of another k, eager and replayed in turn,
+    # h handed over inside an XCD and (the second context) past the L2s: the same bits
+    g = gen(23)
+    shapes = [(32, 512, 64, 8), (32, 512, 64, 7), (64, 256, 96, 16)]
+    layers, xs = [], [acts(g, 4, 512) for _ in range(3)]
+    for E, D, F, k in shapes:
+        layers.append(((g.standard_normal((E, D)) * 0.05).astype(np.float32), synth.quant_matrix(g, MX, E * 2 * F, D),
+                       synth.quant_matrix(g, MX, E * D, F)))
+    results = []
+    monkeypatch.setenv("LT_FUSED_AGENT_HANDOVER", "1")
+    with lt.Context(0) as other:
+        for c in (ctx, other):
+            ts = [(c.upload(r, ggml.F32, E, D), c.upload(a, MX, 2 * F, D, E), c.upload(b, MX, D, F, E))
+                  for (r, a, b), (E, D, F, k) in zip(layers, shapes)]
+            X = [DeviceArray((4, 512)) for _ in shapes]
+            outs = [DeviceArray((4, 512)) for _ in shapes]
+
+            def step():
+                for i in range(4):
+                    for (R, GU, DN), (E, D, F, k), x, o in zip(ts, shapes, X, outs):
+                        c.moe_forward(o.row(i), x.row(i), R, GU, DN, k, F, norm_topk=True)
+
+            def fill(seed):
+                import ctypes
+                from llmtoy_amd.hip import H2D, check, hip
+                for i, x in enumerate(X):
+                    v = xs[(i + seed) % 3]
+                    check(hip().hipMemcpy(x.ptr, v.ctypes.data_as(ctypes.c_void_p), v.nbytes, H2D))
+
+            fill(0)
+            step()
+            c.sync()
+            graph, got = Graph(c.stream, step), []
+            for seed in range(1, 4):
+                fill(seed)
+                step()
+                c.sync()
+                eager = [o.numpy()[:, :D] for o, (E, D, F, k) in zip(outs, shapes)]
+                fill(seed + 1)
+                graph.launch()
+                step()
+                c.sync()
+                fill(seed)
+                graph.launch()
+                graph.launch()
+                c.sync()
+                for a, o, (E, D, F, k) in zip(eager, outs, shapes):
+                    assert np.isfinite(a).all() and np.array_equal(a, o.numpy()[:, :D])
+                got += eager
+            results.append(got)
+            graph.destroy()
+            for t in (*[t for q in ts for t in q], *X, *outs):
+                t.free()
+    for a, b in zip(*results):
+        assert np.array_equal(a, b)
+
+
+def test_gpu_mx_moe_one_launch_first_call_in_a_capture(ctx):
+    g = gen(24)
+    E, D, F, k = 24, 256, 32, 7
+    GU, DN, _ = experts(ctx, g, E, D, F)
+    R = ctx.upload((g.standard_normal((E, D)) * 0.05).astype(np.float32), ggml.F32, E, D)
+    x, y = DeviceArray.from_numpy(acts(g, D)), DeviceArray((D,))
+    with lt.Context(0) as other:
+        tensors = [other.upload(t.read(), t.type, t.rows, t.cols, t.n_experts) for t in (R, GU, DN)]
+
+        def first():
+            with pytest.raises(ltlib.InvalidError):
+                other.moe_forward(y, x, *tensors, k, F)
+
+        Graph(other.stream, first).destroy()
+        other.moe_forward(y, x, *tensors, k, F)
+        other.sync()
+        want = y.numpy()
+        graph = Graph(other.stream, lambda: other.moe_forward(y, x, *tensors, k, F))
+        graph.launch()
+        other.sync()
+        assert np.array_equal(want, y.numpy())
+        graph.destroy()
+        for t in tensors:
+            t.free()
+    for t in (R, GU, DN, x, y):
+        t.free()
+
+
 def test_gpu_mx_experts_beside_other_formats(ctx):
     # gate/up in one format, down in another, a dense FFN of MXFP4 beside them
     g = gen(11)
