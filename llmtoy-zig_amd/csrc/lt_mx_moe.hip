@@ -20,13 +20,14 @@
 // its launches: the memory belongs to one shape, whose grid is always the same.
 //
 // Bound by a chain of latencies.  128 experts of 768 by 2048, top 8, us from the
-// start: logits made 2.1 and seen 3.6, experts known 3.9-4.9, h made 7, read 8, rows
-// published 9.5, summed 11.  13.1 us a token in a graph against 14.5 in three launches
-// (32 of 2112 by 2816, top 8: 26.3 | 28.7; 64 of 512 by 1024: 11.0 | 12.9).  A slot has
-// one XCD's share of the memory's rate, so slots that leave XCDs without one cost: with
-// 4 slots of 2112 by 2816 22.9 | 18.9, with 10 of 768 by 2048 16.6 | 15.5, with 6 12.7 |
-// 13.6 and 24.3 | 24.9: taken where at most two XCDs of a turn are idle.  Three
-// workgroups a CU, which the registers' 24 spilled bytes buy: 13.2 us, two 15.0.
+// start: logits made 2.0 and seen 3.2, experts known 3.5-4.5 (a round of the selection
+// 0.13), h made 7, read 8, rows published 9, summed 10.5.  us a token in a graph, this |
+// three launches: 13.0 | 14.6, top 6 12.6 | 13.7, top 16 18.6 | 20.8; 32 of 2112 by 2816,
+// top 8, 25.3 | 28.8; 64 of 512 by 1024, top 8, 10.8 | 12.9; 60 of 1408 by 2048, top 8,
+// 16.9 | 17.3.  A slot has one XCD's share of the memory's rate, so slots that leave XCDs
+// without one cost: top 4 of 32 of 2112 by 2816 22.9 | 19.0, top 10 of 128 of 768 by 2048
+// 16.6 | 15.5.  So it is taken where at most two XCDs of a turn are idle.  Three
+// workgroups a CU, which 24 spilled bytes a lane buy: 13.2 us, two without them 15.0.
 #include "llmtoy_hip.h"
 #include "lt_dotf32.h"
 #include "lt_internal.h"
@@ -58,14 +59,14 @@ struct MxLayer {
     uint64_t *pl;  // [slot][row]
 };
 
-// Waits until every lane's N words (its pointer p, stride apart; lanes without
-// `on` have none) carry the epoch.  False after the limit.
+// Waits until every lane's words (up to N, `have` of them from its pointer p on,
+// stride apart) carry the epoch; the others are 0.  False after the limit.
 template <int N>
-__device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, bool on, uint32_t ep, uint64_t t0, float (&v)[N]) {
+__device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N]) {
     while (true) {
         uint64_t w[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) w[i] = on ? hand_get(p + i * stride) : (uint64_t)ep << 32;
+        for (int i = 0; i < N; i++) w[i] = (uint32_t)i < have ? hand_get(p + i * stride) : (uint64_t)ep << 32;
         bool good = true;
 #pragma unroll
         for (int i = 0; i < N; i++) good = good && tag_is(w[i], ep);
@@ -73,7 +74,6 @@ __device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, boo
         for (int i = 0; i < N; i++) v[i] = good ? __uint_as_float((uint32_t)w[i]) : NAN;
         if (__all(good)) return true;
         if (wall_clock64() - t0 > kMxWaitTicks) return false;
-        __builtin_amdgcn_s_sleep(1);
     }
 }
 __device__ __forceinline__ void mx_late(const MxLayer &a, uint32_t code, uint32_t ep, int lane) {
@@ -87,13 +87,10 @@ template <int PER>
 __device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t ep, uint64_t t0, float (&v)[PER], int lane) {
     const uint64_t *w = a.lg + (blockIdx.x & 7) * kMxMaxLogits;
     float one[1];
-    bool good = mx_await<1>(w + (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one);  // then all of them
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        float y[1] = {NAN};
-        if (good) good = mx_await<1>(w + min((uint32_t)lane + 64u * i, a.n_experts - 1), 0, true, ep, t0, y);
-        v[i] = y[0];
-    }
+    for (int i = 0; i < PER; i++) v[i] = 0.0f;
+    const bool good = mx_await<1>(w + (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one) &&  // then all of them
+                      mx_await<PER>(w + lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v);
     if (!good) mx_late(a, 1u, ep, lane);
     return good;
 }
@@ -181,10 +178,9 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     for (uint32_t q = threadIdx.x; __any(q < 16 * a.d.kg); q += kPairThreads) {
         float y[8];
         const bool on = q < 4 * a.d.nb;
-        if (!mx_await<8>(a.hl + (size_t)slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on, ep, t0, y)) good = false;
+        if (!mx_await<8>(a.hl + (size_t)slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y)) good = false;
         if (q < 16 * a.d.kg)
-            mx_vec_put(v, q, {make_float4(on ? y[0] : 0.0f, on ? y[1] : 0.0f, on ? y[2] : 0.0f, on ? y[3] : 0.0f),
-                              make_float4(on ? y[4] : 0.0f, on ? y[5] : 0.0f, on ? y[6] : 0.0f, on ? y[7] : 0.0f)});
+            mx_vec_put(v, q, {make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7])});
     }
     __syncthreads();
     MxSum acc = {};
