@@ -257,7 +257,7 @@ int lt_expert_down_id(lt_ctx *ctx, const lt_tensor *down, const float *h, const 
  * launch), or Q3_K / Q4_K gate_up with IQ4_NL, Q5_0 or Q5_1 down (atomic
  * combine, the shared FFN then first, as the base).  MXFP4 experts with an F32
  * router, d_model a multiple of 256, <= 256 experts and k of 6 to 8 or 14 to 16
- * take a launch of their own, which adds in slot order (the shared FFN first, as
+ * (or experts of up to about 1 MB) take a launch of their own, which adds in slot order (the shared FFN first, as
  * the base).  Other expert types and shapes, and LT_MOE_UNFUSED, run router,
  * gate/up and down as separate launches. */
 int lt_moe_forward(lt_ctx *ctx, float *out, const float *x, const lt_tensor *router, const float *router_bias,

@@ -26,8 +26,11 @@
 // top 8, 25.3 | 28.8; 64 of 512 by 1024, top 8, 10.8 | 12.9; 60 of 1408 by 2048, top 8,
 // 16.9 | 17.3.  A slot has one XCD's share of the memory's rate, so slots that leave XCDs
 // without one cost: top 4 of 32 of 2112 by 2816 22.9 | 19.0, top 10 of 128 of 768 by 2048
-// 16.6 | 15.5.  So it is taken where at most two XCDs of a turn are idle.  Three
-// workgroups a CU, which 24 spilled bytes a lane buy: 13.2 us, two without them 15.0.
+// 16.6 | 15.5.  So it is taken where at most two XCDs of a turn are idle, or the slots
+// are small: 64 of 512 by 1024 (0.8 MB a slot) top 1 8.3 | 10.2, top 4 10.4 | 11.0, top 9
+// 11.1 | 13.4; 60 of 320 by 2048 (1.04 MB) top 4 10.7 | 11.4, but top 9 13.4 | 12.8.  h past
+// the L2s instead, as it is without the placement: 12.9 -> 14.4 us.  Three workgroups a
+// CU, which 24 spilled bytes a lane buy: 13.2 us, two without them 15.0.
 #include "llmtoy_hip.h"
 #include "lt_dotf32.h"
 #include "lt_internal.h"
@@ -234,7 +237,8 @@ uint32_t layer_groups(uint32_t n_experts, uint32_t k, size_t d_model, size_t dow
 
 bool moe_mx_fits(const DevTensor &R, const DevTensor &GU, const DevTensor &D, uint32_t k) {
     return GU.type == LT_TYPE_MXFP4 && D.type == LT_TYPE_MXFP4 && R.type == LT_TYPE_F32 && GU.cols % 256 == 0 &&
-           GU.n_experts <= kMxMaxLogits && k <= 16 && (k + 7) / 8 * 8 - k <= 2;
+           GU.n_experts <= kMxMaxLogits && k <= 16 &&
+           ((k + 7) / 8 * 8 - k <= 2 || (GU.bytes + D.bytes) / GU.n_experts <= (k <= 8 ? 1u << 20 : 7u << 17));
 }
 
 size_t moe_mx_bytes(uint32_t n_experts, uint32_t k, size_t d_model, size_t down_cols) {
