@@ -376,6 +376,11 @@ hipError_t launch_expert_gate_up_mx_routed(const DevTensor &GU, const float *x, 
                                            float *w_out, hipStream_t s);
 hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint32_t *ids, const float *w, uint32_t k,
                                  const float *base, int accumulate, const float *dscale, float *out, hipStream_t s);
+// out [T][rows] = X [T][cols] W^T of up to kMxFew vectors (as columns of the same
+// instructions), where they fit the LDS.
+constexpr size_t kMxFew = 5;
+bool matvecs_mx_fit(const DevTensor &W, size_t T);
+hipError_t launch_matvecs_mx(const DevTensor &W, const float *X, size_t T, float *out, hipStream_t s);
 // A layer in one launch (lt_mx_moe.hip): an F32 router (rows of a multiple of 256),
 // and slots that keep the XCDs busy (moe_mx_fits).  `hand` is moe_mx_bytes(shape),
 // zero at first and kept for calls of this shape.

@@ -1,4 +1,4 @@
-// lt_mx_dot.h -- products of rows of MXFP4 with a vector, as the matvec, the experts'
+// lt_mx_dot.h -- products of rows of MXFP4 with a vector or a few, as the matvec, the experts'
 // kernels and the single-launch layer have them.
 //
 //   y[r] = sum_b 2^(e_rb - 127) sum_i w_rbi x_bi
@@ -38,7 +38,9 @@ __device__ __forceinline__ MxQuarter mx_vec_load(const float *x, uint32_t u, uin
     const float *p = x + (size_t)min(u / 4, nb - 1) * 32 + u % 4 * 4;
     return {ldg16f(p), ldg16f(p + 16)};
 }
-__device__ __forceinline__ void mx_vec_put(mx_u32x4 *v, uint32_t u, const MxQuarter &x) {
+// NV vectors side by side: vector n's parts are 3 n .. of [block][quarter][3 NV].
+template <int NV = 1>
+__device__ __forceinline__ void mx_vec_put(mx_u32x4 *v, uint32_t u, const MxQuarter &x, int n = 0) {
     float a[4] = {x.a.x, x.a.y, x.a.z, x.a.w}, h[4] = {x.h.x, x.h.y, x.h.z, x.h.w};
 #pragma unroll
     for (int c = 0; c < kParts; c++) {
@@ -50,7 +52,7 @@ __device__ __forceinline__ void mx_vec_put(mx_u32x4 *v, uint32_t u, const MxQuar
             a[i] -= __uint_as_float(ua & 0xffff0000u);
             h[i] -= __uint_as_float(uh & 0xffff0000u);
         }
-        v[u * kParts + c] = w;
+        v[u * (kParts * NV) + kParts * n + c] = w;
     }
 }
 
@@ -88,7 +90,7 @@ struct MxSum {
     mx_acc16 s[4];  // chains
     __device__ __forceinline__ mx_acc16 all() const { return (s[0] + s[1]) + (s[2] + s[3]); }
 };
-template <int J>
+template <int J, int NV>
 __device__ __forceinline__ void mx_step(const MxWords &w, const mx_u32x4 *v, MxSum &acc) {
     // a float whose exponent is the scale byte: 2^(e - 127), 255 makes NaN
     const float scale = __uint_as_float((J < 3 ? w.s << (23 - 8 * J) : w.s >> 1) & 0x7f800000u);
@@ -102,16 +104,17 @@ __device__ __forceinline__ void mx_step(const MxWords &w, const mx_u32x4 *v, MxS
         m.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 1);
         m.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 2);
         m.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.c[J][i], scale, 3);
-        const bf16x8 x = __builtin_bit_cast(bf16x8, v[(16 * J + i) * kParts]);
+        const bf16x8 x = __builtin_bit_cast(bf16x8, v[(16 * J + i) * (kParts * NV)]);
         acc.s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m.v, x, acc.s[i], 0, 0, 0);
     }
 }
+template <int NV = 1>
 __device__ __forceinline__ void mx_dot(const MxWords &w, const mx_u32x4 *v, uint32_t q, uint32_t kg, int lane, MxSum &acc) {
-    v += ((16 * q + (uint32_t)(lane >> 4)) * 4) * kParts + min(lane & 15, kParts - 1);
-    mx_step<0>(w, v, acc);
-    if (4 * q + 1 < kg) mx_step<1>(w, v, acc);
-    if (4 * q + 2 < kg) mx_step<2>(w, v, acc);
-    if (4 * q + 3 < kg) mx_step<3>(w, v, acc);
+    v += ((16 * q + (uint32_t)(lane >> 4)) * 4) * (kParts * NV) + min(lane & 15, kParts * NV - 1);
+    mx_step<0, NV>(w, v, acc);
+    if (4 * q + 1 < kg) mx_step<1, NV>(w, v, acc);
+    if (4 * q + 2 < kg) mx_step<2, NV>(w, v, acc);
+    if (4 * q + 3 < kg) mx_step<3, NV>(w, v, acc);
 }
 
 // The sums over the columns: row 4 (lane / 16) + i in acc[i] of every lane of
@@ -124,6 +127,17 @@ __device__ __forceinline__ float mx_rows(mx_acc16 acc, int lane, bool first) {
 }
 // the lane that holds row r of mx_rows is 16 (r / 4) + r % 4: lanes with
 // lane % 16 < 4 write row 4 (lane / 16) + lane % 4
+
+// Of several vectors: the sum over the three columns of vector n in lanes of column
+// 3 n, row 4 (lane / 16) + i in [i].
+__device__ __forceinline__ mx_acc16 mx_rows_of(mx_acc16 acc) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float one = dpp<0x101>(acc[i]), two = dpp<0x102>(acc[i]);  // lanes + 1, + 2
+        acc[i] = (acc[i] + one) + two;
+    }
+    return acc;
+}
 
 // Loads stay behind this point, or before it.
 __device__ __forceinline__ void mx_order() {

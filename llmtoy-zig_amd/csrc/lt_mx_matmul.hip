@@ -451,7 +451,7 @@ size_t matmul_mx_workspace(size_t T, size_t cols) {
 }
 
 hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *ws, float *out, hipStream_t s) {
-    if (T == 1) return launch_matvec_mx(W, X, out, s);
+    if (matvecs_mx_fit(W, T)) return launch_matvecs_mx(W, X, T, out, s);
     const size_t step = batch_of(T, W.cols);
     for (size_t t0 = 0; t0 < T; t0 += step) {
         const size_t n = T - t0 < step ? T - t0 : step;

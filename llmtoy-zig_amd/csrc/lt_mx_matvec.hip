@@ -21,20 +21,28 @@ constexpr int kMvWaves = 16;  // of a workgroup at most
 // Workgroups of S waves a tile (threadIdx.x; and TP tiles side by side, threadIdx.y)
 // walk the tiles.  Two items (16 rows by 16 blocks) of a wave are on their way, over the
 // tiles' ends, before the vector is converted and from then on.
-template <bool NT>
+//
+// NV vectors at once, [NV][cols] to [NV][rows] of a matrix: their parts are columns of
+// the same instructions, of which there are 16.  1 | 2 | 5 vectors of 4096 x 4096 5.2 |
+// 5.4 | 6.6 us a graph's node (limbs and the thin product 9.3), of 262144 x 2816 64 |
+// 64 | 69 (limbs and tiles 113), of 11008 x 4096 8.4 | 9.1 | 9.2 (12.8).
+template <bool NT, int NV>
 __global__ __launch_bounds__(64 * kMvWaves) void k_mx_matvec(const uint8_t *codes, const uint8_t *scales, MxDims d,
                                                              uint32_t ntiles, uint32_t expert_rows, uint32_t S, uint32_t TP,
                                                              const float *x, float *y) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ float part[2][kMvWaves][16];
+    __shared__ float part[2][kMvWaves][NV][16];
     const int lane = threadIdx.x & 63;
     const uint32_t sp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tp = __builtin_amdgcn_readfirstlane(threadIdx.y);
     const uint32_t wave = tp * S + sp, threads = 64 * S * TP, tid = 64 * wave + lane, stride = gridDim.x * TP, t0 = blockIdx.x * TP;
     const bool first = p32_first(lane);
     mx_u32x4 *const v = reinterpret_cast<mx_u32x4 *>(lds);
     const uint32_t units = 16 * d.kg;
-    MxQuarter xb;
-    if (tid < units) xb = mx_vec_load(x, tid, d.nb);
+    MxQuarter xb[NV];
+    const size_t cols = (size_t)d.nb * 32;
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+        if (tid < units) xb[n] = mx_vec_load(x + n * cols, tid, d.nb);
     mx_order();
 
     // every wave of the workgroup goes through the same number of tiles (past
@@ -51,29 +59,50 @@ __global__ __launch_bounds__(64 * kMvWaves) void k_mx_matvec(const uint8_t *code
     fetch(w0);
     if (n > 1) fetch(w1);
     mx_order();
-    if (tid < units) mx_vec_put(v, tid, xb);
-    for (uint32_t u = tid + threads; u < units; u += threads) mx_vec_put(v, u, mx_vec_load(x, u, d.nb));
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+        if (tid < units) mx_vec_put<NV>(v, tid, xb[n], n);
+        for (uint32_t u = tid + threads; u < units; u += threads) mx_vec_put<NV>(v, u, mx_vec_load(x + n * cols, u, d.nb), n);
+    }
     __syncthreads();
 
     MxSum acc = {};
     uint32_t tile = t0 + tp, q = sp, turn = 0;
     auto use = [&](const MxWords &w) {
-        mx_dot(w, v, q, d.kg, lane, acc);
+        mx_dot<NV>(w, v, q, d.kg, lane, acc);
         if ((q += S) < d.kq) return;
         const uint32_t row0 = tile % d.tiles * 16;
         float *out = y + (size_t)(tile / d.tiles) * expert_rows + row0;
-        const float t = mx_rows(acc.all(), lane, first);
-        const uint32_t r = 4 * (lane >> 4) + (lane & 3);
-        if (S == 1) {
-            if ((lane & 15) < 4 && tile < ntiles && row0 + r < expert_rows) out[r] = t;
-        } else {
-            if ((lane & 15) < 4) part[turn][wave][r] = t;
-            __syncthreads();
-            if (sp == 0 && lane < 16 && tile < ntiles && row0 + lane < expert_rows) {
-                float s = part[turn][wave][lane];
-                for (uint32_t i = 1; i < S; i++) s += part[turn][wave + i][lane];
-                out[lane] = s;
+        if constexpr (NV == 1) {
+            const float t = mx_rows(acc.all(), lane, first);
+            const uint32_t r = 4 * (lane >> 4) + (lane & 3);
+            if (S == 1) {
+                if ((lane & 15) < 4 && tile < ntiles && row0 + r < expert_rows) out[r] = t;
+            } else if ((lane & 15) < 4) {
+                part[turn][wave][0][r] = t;
             }
+        } else {
+            const mx_acc16 t = mx_rows_of(acc.all());
+            const uint32_t n = (uint32_t)(lane & 15) / 3, r = 4 * (lane >> 4);
+            if ((lane & 15) % 3 == 0 && n < NV) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (S > 1)
+                        part[turn][wave][n][r + i] = t[i];
+                    else if (tile < ntiles && row0 + r + i < expert_rows)
+                        out[(size_t)n * expert_rows + r + i] = t[i];
+                }
+            }
+        }
+        if (S > 1) {
+            __syncthreads();
+            if (sp == 0 && tile < ntiles)
+                for (uint32_t e = lane; e < 16 * NV; e += 64) {
+                    const uint32_t n = e / 16, r = e % 16;
+                    float s = part[turn][wave][n][r];
+                    for (uint32_t i = 1; i < S; i++) s += part[turn][wave + i][n][r];
+                    if (row0 + r < expert_rows) out[(size_t)n * expert_rows + r] = s;
+                }
             turn ^= 1;
         }
         acc = MxSum{};
@@ -230,11 +259,12 @@ constexpr size_t kNtBytes = 8u << 20;
 
 }  // namespace
 
-hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s) {
+template <int NV>
+static hipError_t launch_matvec(const DevTensor &W, const float *x, float *y, hipStream_t s) {
     const MxDims d = mx_dims(W.rows, W.blocks_per_row);
     static bool set[2][64] = {};
     const bool nt = W.bytes >= kNtBytes;
-    const auto kernel = nt ? k_mx_matvec<true> : k_mx_matvec<false>;
+    const auto kernel = nt ? k_mx_matvec<true, NV> : k_mx_matvec<false, NV>;
     hipError_t e = allow_lds((const void *)kernel, set[nt]);
     if (e != hipSuccess) return e;
     const size_t tiles = W.n_experts * d.tiles;
@@ -243,11 +273,39 @@ hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStr
     S = S > d.kq ? d.kq : S;
     const uint32_t each = (d.kq + S - 1) / S;
     S = (d.kq + each - 1) / each;
-    const uint32_t TP = tiles * S <= kMvTarget || S > 4 ? 1 : 8 / S;
+    uint32_t TP = tiles * S <= kMvTarget || S > 4 ? 1 : 8 / S;
+    size_t most = kMvGroups;
+    const size_t lds = NV * mx_vec_bytes(d.kg), fit = (150 << 10) / (lds + sizeof(float) * 2 * kMvWaves * NV * 16);
+    // few workgroups a CU: of 16 waves between them, if there are tiles for that (11008
+    // x 4096 with 4 vectors 17.5 -> 8.7 us)
+    if (NV > 1 && fit < 4) {
+        most = 256 * fit;
+        const size_t each_gets = (tiles + most - 1) / most;
+        TP = (uint32_t)kMvWaves / (uint32_t)fit / S;
+        TP = TP < 1 ? 1 : TP > each_gets ? (uint32_t)each_gets : TP;
+    }
     const size_t groups = (tiles + TP - 1) / TP;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kMvGroups ? groups : kMvGroups)), dim3(64 * S, TP),
-                       mx_vec_bytes(d.kg), s, W.p0, W.p1, d, (uint32_t)tiles, (uint32_t)W.rows, S, TP, x, y);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < most ? groups : most)), dim3(64 * S, TP), lds, s, W.p0, W.p1, d,
+                       (uint32_t)tiles, (uint32_t)W.rows, S, TP, x, y);
     return hipGetLastError();
+}
+
+hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s) { return launch_matvec<1>(W, x, y, s); }
+
+bool matvecs_mx_fit(const DevTensor &W, size_t T) {
+    return T <= kMxFew && T * mx_vec_bytes(mx_dims(W.rows, W.blocks_per_row).kg) <= (128 << 10);
+}
+
+hipError_t launch_matvecs_mx(const DevTensor &W, const float *X, size_t T, float *out, hipStream_t s) {
+    if (W.n_experts != 1 || !matvecs_mx_fit(W, T)) return hipErrorInvalidValue;
+    switch (T) {
+    case 1: return launch_matvec<1>(W, X, out, s);
+    case 2: return launch_matvec<2>(W, X, out, s);
+    case 3: return launch_matvec<3>(W, X, out, s);
+    case 4: return launch_matvec<4>(W, X, out, s);
+    case 5: return launch_matvec<5>(W, X, out, s);
+    default: return hipErrorInvalidValue;
+    }
 }
 
 template <int ROUTE>

@@ -228,6 +228,33 @@ def test_gpu_mx_matmul(ctx, T, rows, cols):
     xq.free(), t.free()
 
 
+# a few vectors beside each other in the matvec's instructions, up to what the LDS holds
+@pytest.mark.parametrize("T", [2, 3, 4, 5])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (33, 544), (5000, 96), (17000, 64), (4099, 2048), (700, 4096), (300, 4384),
+                                       (100, 10912), (50, 16384), (9000, 512)])
+def test_gpu_mx_matmul_few(ctx, T, rows, cols):
+    print(f"few T {T} {rows}x{cols}", flush=True)
+    g = gen(T, rows, cols, 25)
+    m, x = synth.quant_matrix(g, MX, rows, cols), acts(g, T, cols)
+    t = ctx.upload(m, MX, rows, cols)
+    buf = DeviceArray.from_numpy(np.full(T * rows + 16, 5.0, np.float32))
+    dx = DeviceArray.from_numpy(x)
+    ctx.quant_matmul(DeviceView(buf.ptr, (T, rows), np.float32), t, dx)
+    ctx.sync()
+    got = buf.numpy()
+    assert (got[T * rows:] == 5).all()
+    w = mx.decode(m, cols)
+    close(got[:T * rows].reshape(T, rows), *mx.product(w, x))
+    x[T - 2, cols // 2] = np.inf  # in one vector: the others keep theirs
+    y = np.empty((T, rows), np.float32)
+    ctx.quant_matmul(y, t, x)
+    assert np.isnan(y[T - 2]).all()
+    keep = [n for n in range(T) if n != T - 2]
+    close(y[keep], *mx.product(w, x[keep]))
+    for a in (buf, dx, t):
+        a.free()
+
+
 # past the thin kernel's range: each of the tiles, ragged on every side
 @pytest.mark.parametrize("T,rows,cols", [(300, 700, 640), (1000, 300, 4096), (1100, 1030, 288), (1300, 1000, 1056),
                                          (130, 9001, 96), (9, 9001, 160), (2001, 8003, 96), (65536, 9, 32),
