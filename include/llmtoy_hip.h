@@ -256,10 +256,11 @@ int lt_expert_down_id(lt_ctx *ctx, const lt_tensor *down, const float *h, const 
  * 256 experts, k <= 16): Q4_K experts (with a Q8_0 shared FFN in the same
  * launch), or Q3_K / Q4_K gate_up with IQ4_NL, Q5_0 or Q5_1 down (atomic
  * combine, the shared FFN then first, as the base).  MXFP4 experts with an F32
- * router, d_model a multiple of 256, <= 256 experts and k of 6 to 8 or 14 to 16
- * (or experts of up to about 1 MB) take a launch of their own, which adds in slot order (the shared FFN first, as
- * the base).  Other expert types and shapes, and LT_MOE_UNFUSED, run router,
- * gate/up and down as separate launches. */
+ * router and <= 256 experts take a launch of their own, which adds in slot order
+ * (the shared FFN first, as the base), where the slots keep the chip's eight
+ * parts busy (k = 8 or 16, 6 and 7 of moderate size) or are small (up to about 1
+ * MB each).  Other expert types and shapes, and LT_MOE_UNFUSED, run
+ * router, gate/up and down as separate launches. */
 int lt_moe_forward(lt_ctx *ctx, float *out, const float *x, const lt_tensor *router, const float *router_bias,
                    const lt_tensor *gate_up, const lt_tensor *down, const lt_tensor *sh_gate,
                    const lt_tensor *sh_up, const lt_tensor *sh_down, uint32_t k, uint32_t d_expert, uint32_t act,

@@ -381,7 +381,7 @@ hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint3
 constexpr size_t kMxFew = 5;
 bool matvecs_mx_fit(const DevTensor &W, size_t T);
 hipError_t launch_matvecs_mx(const DevTensor &W, const float *X, size_t T, float *out, hipStream_t s);
-// A layer in one launch (lt_mx_moe.hip): an F32 router (rows of a multiple of 256),
+// A layer in one launch (lt_mx_moe.hip): an F32 router, MXFP4 experts, up to 256 of them,
 // and slots that keep the XCDs busy (moe_mx_fits).  `hand` is moe_mx_bytes(shape),
 // zero at first and kept for calls of this shape.
 bool moe_mx_fits(const DevTensor &R, const DevTensor &GU, const DevTensor &D, uint32_t k);

@@ -22,15 +22,19 @@
 // Bound by a chain of latencies.  128 experts of 768 by 2048, top 8, us from the
 // start: logits made 2.0 and seen 3.2, experts known 3.5-4.5 (a round of the selection
 // 0.13), h made 7, read 8, rows published 9, summed 10.5.  us a token in a graph, this |
-// three launches: 13.0 | 14.6, top 6 12.6 | 13.7, top 16 18.6 | 20.8; 32 of 2112 by 2816,
-// top 8, 25.3 | 28.8; 64 of 512 by 1024, top 8, 10.8 | 12.9; 60 of 1408 by 2048, top 8,
-// 16.9 | 17.3.  A slot has one XCD's share of the memory's rate, so slots that leave XCDs
-// without one cost: top 4 of 32 of 2112 by 2816 22.9 | 19.0, top 10 of 128 of 768 by 2048
-// 16.6 | 15.5.  So it is taken where at most two XCDs of a turn are idle, or the slots
-// are small: 64 of 512 by 1024 (0.8 MB a slot) top 1 8.3 | 10.2, top 4 10.4 | 11.0, top 9
-// 11.1 | 13.4; 60 of 320 by 2048 (1.04 MB) top 4 10.7 | 11.4, but top 9 13.4 | 12.8.  h past
-// the L2s instead, as it is without the placement: 12.9 -> 14.4 us.  Three workgroups a
-// CU, which 24 spilled bytes a lane buy: 13.2 us, two without them 15.0.
+// three launches: 13.0 | 14.5, top 6 12.5 | 13.7, top 16 18.4 | 20.6; 128 of 704 by 2816,
+// top 8, 15.4 | 16.5; 32 of 2112 by 2816, top 8, 25.0 | 28.1; 64 of 512 by 1024, top 8,
+// 10.9 | 12.9; 60 of 1408 by 2048, top 8, 16.9 | 17.4.
+//
+// A slot has one XCD's share of the memory's rate, so slots that leave XCDs without
+// one cost: top 4 of 32 of 2112 by 2816 22.9 | 19.0, top 10 of 128 of 768 by 2048 16.6 |
+// 15.5; and with more workgroups than are there at once fewer idle ones do: top 6 of 8
+// of 1024 by 2400 17.1 | 15.4, top 8 18.3 | 17.5 (8 of 2048 by 1024 16.7 | 19.5).  So it
+// is taken where no XCD of a turn is idle, or at most two and all are there at once, or
+// the slots are small: 64 of 512 by 1024 (0.8 MB a slot) top 1 8.3 | 10.2, top 4 10.0 |
+// 10.9, top 9 11.1 | 13.4; 60 of 320 by 2048 (1.04 MB) top 4 10.7 | 11.4, but top 9 13.4 |
+// 12.8.  h past the L2s instead, as it is without the placement: 12.9 -> 14.4 us.  Three
+// workgroups a CU: 13.2 us, two 15.0.
 #include "llmtoy_hip.h"
 #include "lt_dotf32.h"
 #include "lt_internal.h"
@@ -45,6 +49,7 @@ namespace {
 
 constexpr uint64_t kMxWaitTicks = 20000000;  // 200 ms of the 100 MHz wall clock
 constexpr uint32_t kMxMaxLogits = 256, kMxDownRows = 64;
+constexpr uint32_t kMxAtOnce = 96;  // workgroups of a group on its 32 CUs
 struct MxLayer {
     const float *router, *bias, *x, *base;
     MxPair gu;
@@ -116,7 +121,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     };
     if (i < a.NR) {
         const uint32_t row = 4 * b + wave / 2, at = min(row, a.n_experts - 1);
-        const float y = dotf32_pair(a.router + (size_t)at * a.gu.d.nb * 32, a.x, a.bias ? a.bias + at : nullptr, (int)a.gu.d.nb,
+        const float y = dotf32_pair_any<true>(a.router + (size_t)at * a.gu.d.nb * 32, a.x, a.bias ? a.bias + at : nullptr, (int)a.gu.d.nb,
                                     (int)(wave & 1), lane, reinterpret_cast<float *>(lds) + wave * 512, part[wave / 2]);
         if ((wave & 1) == 0 && lane < 8 && row < a.n_experts)
             hand_put(a.lg + lane * kMxMaxLogits + row, __float_as_uint(y), ep);
@@ -236,9 +241,12 @@ uint32_t layer_groups(uint32_t n_experts, uint32_t k, size_t d_model, size_t dow
 }  // namespace
 
 bool moe_mx_fits(const DevTensor &R, const DevTensor &GU, const DevTensor &D, uint32_t k) {
-    return GU.type == LT_TYPE_MXFP4 && D.type == LT_TYPE_MXFP4 && R.type == LT_TYPE_F32 && GU.cols % 256 == 0 &&
-           GU.n_experts <= kMxMaxLogits && k <= 16 &&
-           ((k + 7) / 8 * 8 - k <= 2 || (GU.bytes + D.bytes) / GU.n_experts <= (k <= 8 ? 1u << 20 : 7u << 17));
+    uint32_t NR, J, ND, SPG;
+    const uint32_t n = (uint32_t)GU.n_experts, idle = (k + 7) / 8 * 8 - k;
+    return GU.type == LT_TYPE_MXFP4 && D.type == LT_TYPE_MXFP4 && R.type == LT_TYPE_F32 &&
+           GU.n_experts <= kMxMaxLogits && k >= 1 && k <= 16 &&
+           (idle == 0 || (idle <= 2 && layer_groups(n, k, D.rows, D.cols, NR, J, ND, SPG) <= kMxAtOnce) ||
+            (GU.bytes + D.bytes) / n <= (k <= 8 ? 1u << 20 : 7u << 17));
 }
 
 size_t moe_mx_bytes(uint32_t n_experts, uint32_t k, size_t d_model, size_t down_cols) {

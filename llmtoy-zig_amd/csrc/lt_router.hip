@@ -131,10 +131,12 @@ __global__ void __launch_bounds__(64) k_router_f32(const float *__restrict__ W, 
     last_block_topk(logits, rows, ta);
 }
 
-// The same logits for rows of a multiple of 256 elements and x on a 16-byte
+// The same logits for rows of a multiple of 32 elements and x on a 16-byte
 // boundary, two rows a block, two wavefronts a row (dotf32_pair).  Bound by the
 // launch, one round trip to memory and the chain of adds (64 a row of 2,048):
-// 128 x 2,048 4.7 -> 3.35 us, 64 x 1,024 3.8 -> 2.9 against k_router_f32.
+// 128 x 2,048 4.7 -> 3.35 us, 64 x 1,024 3.8 -> 2.9 against k_router_f32 (with the
+// top-k 128 x 2,880 8.6 -> 5.7, 60 x 1,056 5.5 -> 4.6).
+template <bool EIGHTS>
 __global__ void __launch_bounds__(256) k_router_f32_pair(const float *__restrict__ W, const float *__restrict__ x,
                                                          const float *__restrict__ bias, float *__restrict__ logits,
                                                          int rows, int cols, TopkArgs ta) {
@@ -143,8 +145,9 @@ __global__ void __launch_bounds__(256) k_router_f32_pair(const float *__restrict
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int h = wave & 1, rl = wave >> 1, row = 2 * blockIdx.x + rl;
     const bool valid = row < rows;
-    const float sum = dotf32_pair(W + (size_t)(valid ? row : 0) * cols, x, bias ? bias + (valid ? row : 0) : nullptr, cols >> 5,
-                                  h, lane, prod_all[wave], xch[rl]);
+    const float *wr = W + (size_t)(valid ? row : 0) * cols, *br = bias ? bias + (valid ? row : 0) : nullptr;
+    const float sum = EIGHTS ? dotf32_pair(wr, x, br, cols >> 5, h, lane, prod_all[wave], xch[rl])
+                             : dotf32_pair_any<false>(wr, x, br, cols >> 5, h, lane, prod_all[wave], xch[rl]);
     if (h == 0 && lane == 0 && valid) put_logit(logits + row, sum);
     last_block_topk(logits, rows, ta);
 }
@@ -288,9 +291,9 @@ hipError_t launch_router(const DevTensor &R, const float *x, const float *bias, 
         // A router's few rows (other row lengths have a tail in dotf32's
         // order, and 4-byte loads take any x).  Large matrices fill the chip
         // either way: 32,000 x 2,048 takes 43.5 us in pairs, 42.6 without.
-        if (rows <= 1024 && cols % 256 == 0 && ((uintptr_t)x & 15u) == 0)
-            hipLaunchKernelGGL(k_router_f32_pair, dim3((rows + 1) / 2), dim3(256), 0, s, (const float *)R.p0, x, bias,
-                               logits, rows, cols, ta);
+        if (rows <= 1024 && cols % 32 == 0 && ((uintptr_t)x & 15u) == 0)
+            hipLaunchKernelGGL(cols % 256 ? k_router_f32_pair<false> : k_router_f32_pair<true>, dim3((rows + 1) / 2), dim3(256),
+                               0, s, (const float *)R.p0, x, bias, logits, rows, cols, ta);
         else
             hipLaunchKernelGGL(k_router_f32<64>, dim3((rows + 1) / 2), dim3(64), 0, s, (const float *)R.p0, x, bias,
                                logits, rows, cols, ta);

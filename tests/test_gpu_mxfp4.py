@@ -468,7 +468,9 @@ def test_gpu_mx_moe_forward(ctx, E, D, F, k, norm, router):
 # the layer in one launch: slots for every XCD or nearly, rows and experts of every kind
 @pytest.mark.parametrize("E,D,F,Kd,k,act", [(6, 256, 40, 64, 6, 0), (7, 512, 32, 32, 7, 1), (128, 2048, 96, 96, 8, 0),
                                             (256, 256, 160, 160, 8, 0), (40, 768, 80, 544, 14, 1), (255, 256, 64, 64, 15, 0),
-                                            (16, 1280, 48, 64, 16, 0), (9, 16384, 16, 32, 6, 0), (9, 256, 4100, 4128, 8, 0)])
+                                            (16, 1280, 48, 64, 16, 0), (9, 16384, 16, 32, 6, 0), (9, 256, 4100, 4128, 8, 0),
+                                            (8, 2880, 96, 96, 8, 1), (7, 96, 32, 32, 7, 0), (20, 32, 64, 64, 3, 0),
+                                            (60, 1056, 64, 64, 6, 0), (33, 544, 64, 64, 9, 0), (4, 224, 32, 32, 1, 0)])
 def test_gpu_mx_moe_one_launch(ctx, E, D, F, Kd, k, act):
     print(f"one launch E {E} D {D} F {F} Kd {Kd} k {k}", flush=True)
     g = gen(E, D, F, k, 21)
