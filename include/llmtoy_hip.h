@@ -188,9 +188,9 @@ int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size
 
 /* out [T][rows] = X [T][cols] W^T for T vectors at once, W an MXFP4 matrix (2-D,
  * cols <= 16384, T <= 65536), X and out fp32: prompts, batched decode.  The
- * products take each activation as five 6-bit limbs, exact to 2^-24 of the
- * largest of its 32-element block, and are summed in fp32: the accuracy of
- * lt_matvec, in another order of sums.  A NaN or an infinity in a vector makes that
+ * products take each activation to 2^-24 of the largest of its 32-element block
+ * (five 6-bit limbs; up to five vectors as lt_matvec does) and are summed in
+ * fp32: the accuracy of lt_matvec, in another order of sums.  A NaN or an infinity in a vector makes that
  * vector's outputs NaN and leaves the others.  T = 0 does nothing.  Device
  * pointers X and out must be 16-byte aligned; out must not overlap X.  flags:
  * LT_HOST_IO.  The reference calls quantMatvecPar once a vector

@@ -4,6 +4,7 @@
 // X in fp32: a first launch turns its blocks into limbs (lt_mx.h) laid out as
 // matrix operands, and the product runs one matrix instruction a limb into the
 // same sums.  X as an MXFP4 tensor: its codes and scales are an operand already.
+// (Up to five vectors of fp32 that fit the LDS go to the matvec's kernel.)
 //
 // What bounds it.  4096 vectors by 8192 x 4096: 1.37 PFLOP of FP6 x FP4
 // products; the instructions alone, their operands held in registers, take 238
