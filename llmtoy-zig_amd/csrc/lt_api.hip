@@ -883,7 +883,8 @@ extern "C" int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const floa
         if ((rc = ensure(ctx, ctx->out, bytes))) return rc;
         dy = (float *)ctx->out.p;
     }
-    if ((rc = ensure(ctx, ctx->mx, lt::matmul_mx_workspace(T, w.cols)))) return rc;
+    const size_t ws = lt::matmul_mx_workspace(w, T);
+    if (ws && (rc = ensure(ctx, ctx->mx, ws))) return rc;
     if ((rc = launch_rc(ctx, lt::launch_matmul_mx(w, dx, T, ctx->mx.p, dy, ctx->stream), "matmul"))) return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dy, bytes))) return rc;

@@ -389,8 +389,8 @@ size_t moe_mx_bytes(uint32_t n_experts, uint32_t k, size_t d_model, size_t down_
 hipError_t launch_moe_mx(const DevTensor &R, const float *bias, const DevTensor &GU, const DevTensor &D, const float *x, uint32_t k,
                          uint32_t norm, uint32_t d_expert, uint32_t act, const float *base, int accumulate, float *out,
                          uint32_t *ids, float *w, uint8_t *hand, int xcd_local, uint32_t *err, hipStream_t s);
-// out [T][rows] = X [T][cols] W^T; ws: matmul_mx_workspace(T, cols) bytes.
-size_t matmul_mx_workspace(size_t T, size_t cols);
+// out [T][rows] = X [T][cols] W^T; ws: matmul_mx_workspace(W, T) bytes.
+size_t matmul_mx_workspace(const DevTensor &W, size_t T);
 hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *ws, float *out, hipStream_t s);
 // The same with X the first T rows of an MXFP4 tensor.
 hipError_t launch_matmul_mx_mx(const DevTensor &W, const DevTensor &X, size_t T, float *out, hipStream_t s);

@@ -446,8 +446,9 @@ hipError_t limbs_product(const DevTensor &W, const MxSide &x, uint32_t T, float 
 
 }  // namespace
 
-size_t matmul_mx_workspace(size_t T, size_t cols) {
-    const size_t n = batch_of(T, cols);
+size_t matmul_mx_workspace(const DevTensor &W, size_t T) {
+    if (matvecs_mx_fit(W, T)) return 0;
+    const size_t cols = W.cols, n = batch_of(T, cols);
     return limb_bytes(mx_dims(n, cols / 32), n);
 }
 
