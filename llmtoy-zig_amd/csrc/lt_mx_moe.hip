@@ -18,6 +18,9 @@
 // index, and workgroups start in that order, so every wait ends; a limit on the clock
 // ends it too (NaN, and the error word).  The epoch is each workgroup's own count of
 // its launches: the memory belongs to one shape, whose grid is always the same.
+// (Two such launches at once, from two contexts, could each fill an XCD that the
+// other's first workgroups need, and end at the limit with the error: one context a
+// device at a time.)
 //
 // Bound by a chain of latencies.  128 experts of 768 by 2048, top 8, us from the
 // start: logits made 2.0 and seen 3.2, experts known 3.5-4.5 (a round of the selection
