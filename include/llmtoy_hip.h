@@ -66,7 +66,11 @@ enum {
     /* microscaled 4-bit floating point: 17 bytes per 32 elements, a scale
      * byte e (2^(e - 127); 255: NaN) and 16 bytes of codes, element i in the
      * low and 16 + i in the high half of byte i; a code is a sign and one of
-     * 0, .5, 1, 1.5, 2, 3, 4, 6.  No counterpart in the reference. */
+     * 0, .5, 1, 1.5, 2, 3, 4, 6.  Scale bytes 253 and 254 have values of 2^128
+     * and more: products take them as they are (a tensor uploaded with such a
+     * byte goes to the batched product's kernels), lt_dequantize gives
+     * infinities, and as experts (or more than one matrix) such a tensor is
+     * LT_ERR_UNSUPPORTED.  No counterpart in the reference. */
     LT_TYPE_MXFP4 = 39
 };
 
@@ -182,7 +186,8 @@ int lt_matvec(lt_ctx *ctx, float *out, const lt_tensor *W, const float *x, uint3
  * pointer x must be 16-byte aligned.  flags: LT_HOST_IO.  No counterpart in
  * the reference. */
 int lt_quantize(lt_ctx *ctx, lt_tensor *t, const float *x, size_t row0, size_t rows, uint32_t flags);
-/* The values of those rows of an MXFP4 tensor: out [rows][cols], exact.  A
+/* The values of those rows of an MXFP4 tensor: out [rows][cols], exact (2^128 and
+ * more: an infinity).  A
  * device pointer out must be 16-byte aligned.  flags: LT_HOST_IO. */
 int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size_t rows, uint32_t flags);
 

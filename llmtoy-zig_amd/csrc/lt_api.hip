@@ -380,7 +380,7 @@ int shape_tensor(lt_ctx *ctx, DevTensor &t, uint32_t type, size_t rows, size_t c
     if (type == LT_TYPE_MXFP4) {
         if (t.total_rows > INT32_MAX) return fail(ctx, LT_ERR_UNSUPPORTED, "%zu rows of MXFP4 exceed 2^31 - 1", t.total_rows);
         const lt::MxDims d = lt::mx_dims(rows, t.blocks_per_row);
-        t.held = lt::mx_code_bytes(d, n_experts) + lt::mx_scale_bytes(d, n_experts) + lt::mx_slack_bytes(d);
+        t.held = lt::mx_code_bytes(d, n_experts) + lt::mx_scale_bytes(d, n_experts) + lt::mx_slack_bytes(d) + lt::kMxFlagBytes;
     }
     return LT_OK;
 }
@@ -586,7 +586,17 @@ int matvec_dev(lt_ctx *ctx, const DevTensor &W, const float *x, float *y) {
     case LT_TYPE_Q8_0: e = lt::launch_matvec_q8_0(W, x, y, ctx->stream); break;
     case LT_TYPE_Q6_K: e = lt::launch_matvec_q6k(W, x, y, ctx->stream); break;
     case LT_TYPE_F32: e = lt::launch_matvec_f32(W, x, y, ctx->stream); break;
-    case LT_TYPE_MXFP4: e = lt::launch_matvec_mx(W, x, y, ctx->stream); break;
+    case LT_TYPE_MXFP4:
+        if (W.beyond) {  // (the scaled instruction takes any scale)
+            if (W.n_experts != 1)
+                return fail(ctx, LT_ERR_UNSUPPORTED, "matvec: MXFP4 weights of 2^128 and more in a 3-D tensor");
+            const int rc = ensure(ctx, ctx->mx, lt::matmul_mx_workspace(W, 1));
+            if (rc) return rc;
+            e = lt::launch_matmul_mx(W, x, 1, ctx->mx.p, y, ctx->stream);
+            break;
+        }
+        e = lt::launch_matvec_mx(W, x, y, ctx->stream);
+        break;
     case LT_TYPE_Q5_0:
     case LT_TYPE_Q5_1:
     case LT_TYPE_IQ4_NL:
@@ -946,7 +956,8 @@ int ffn_dense_dev(lt_ctx *ctx, const DevTensor &G, const DevTensor &U, const Dev
     if (G.type == LT_TYPE_Q8_0 && U.type == LT_TYPE_Q8_0 && Kd == F) {
         if ((rc = launch_rc(ctx, lt::launch_gate_up_q8_0(G, U, x, act, h, ctx->stream), "gate_up_q8_0")))
             return rc;
-    } else if (G.type == LT_TYPE_MXFP4 && U.type == LT_TYPE_MXFP4 && G.n_experts == 1 && U.n_experts == 1) {
+    } else if (G.type == LT_TYPE_MXFP4 && U.type == LT_TYPE_MXFP4 && G.n_experts == 1 && U.n_experts == 1 && !G.beyond &&
+               !U.beyond) {
         if ((rc = launch_rc(ctx, lt::launch_gate_up_mx(G, U, x, act, (uint32_t)Kd, h, ctx->stream), "gate_up_mx"))) return rc;
     } else {
         if ((rc = ensure(ctx, ctx->g, F * 4)) || (rc = ensure(ctx, ctx->u, F * 4))) return rc;
@@ -1068,6 +1079,11 @@ bool is_fmt(uint32_t t) {
 }
 bool expert_type_ok(uint32_t t) { return t == LT_TYPE_Q4_K || t == LT_TYPE_MXFP4 || is_fmt(t); }
 
+// (their kernels take weights as bf16 numbers)
+int check_beyond(lt_ctx *ctx, const DevTensor &T) {
+    return T.beyond ? fail(ctx, LT_ERR_UNSUPPORTED, "MXFP4 experts with weights of 2^128 and more (scale bytes 253, 254)") : LT_OK;
+}
+
 int check_experts(lt_ctx *ctx, const lt_tensor *gate_up, const lt_tensor *down, size_t d_model, uint32_t d_expert,
                   size_t n_experts, uint32_t k = 0) {
     if (!gate_up || !down) return fail(ctx, LT_ERR_INVALID, "null expert tensor");
@@ -1093,7 +1109,8 @@ int check_experts(lt_ctx *ctx, const lt_tensor *gate_up, const lt_tensor *down, 
     if (is_fmt(D.type) && (size_t)(k ? k : 1) * D.cols > 16384)
         return fail(ctx, LT_ERR_UNSUPPORTED, "k * down row length %zu > 16384 (LDS staging of h)",
                     (size_t)(k ? k : 1) * D.cols);
-    return LT_OK;
+    if (const int rc = check_beyond(ctx, GU)) return rc;
+    return check_beyond(ctx, D);
 }
 
 // gate/up of the k selected experts into h [k][Kd] (ids on the device)
@@ -1190,6 +1207,7 @@ extern "C" int lt_expert_gate_up_id(lt_ctx *ctx, const lt_tensor *gate_up, const
         return fail(ctx, LT_ERR_INVALID, "down_cols %u", down_cols);
     if (GU.cols > (GU.type == LT_TYPE_Q4_K ? 8192u : 16384u))
         return fail(ctx, LT_ERR_UNSUPPORTED, "d_model %zu too long for the gate/up kernel", GU.cols);
+    if (const int rc = check_beyond(ctx, GU)) return rc;
     const bool host = flags & LT_HOST_IO;
     const float *dx = x;
     const uint32_t *dids = ids;
@@ -1226,6 +1244,7 @@ extern "C" int lt_expert_down_id(lt_ctx *ctx, const lt_tensor *down, const float
         return fail(ctx, LT_ERR_UNSUPPORTED, "down row length %zu > %zu", D.cols, kMaxQuantCols);
     if (is_fmt(D.type) && (size_t)k * D.cols > 16384)
         return fail(ctx, LT_ERR_UNSUPPORTED, "k * down row length > 16384 (LDS staging of h)");
+    if (const int rc = check_beyond(ctx, D)) return rc;
     const bool host = flags & LT_HOST_IO;
     const float *dh = h, *dw = weights;
     Span span_(ctx, "lt_expert_down_id");

@@ -49,6 +49,7 @@ struct DevTensor {
     const uint8_t *p2;  // Q6_K sc
     const uint8_t *p3;  // Q6_K d
     size_t blocks_per_row;  // nsb (K-quants) or nb (Q8_0)
+    bool beyond;            // MXFP4: uploaded with weights of 2^128 and more (scale bytes 253, 254)
 };
 
 // ---------------------------------------------------------------- helpers
@@ -312,9 +313,9 @@ struct UploadStaging {
     hipEvent_t ev[kUpSlots] = {};
 };
 // t.base must hold t.bytes; src holds the tensor's GGUF blocks.  Returns
-// after every copy has finished.
+// after every copy has finished; sets t.beyond.
 hipError_t zero_tensor(UploadStaging &S, const DevTensor &t);  // all held bytes; returns when done
-hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const uint8_t *src);
+hipError_t upload_planar(UploadStaging &S, int device, DevTensor &t, const uint8_t *src);
 // The inverse: the tensor's GGUF blocks into dst (t.bytes bytes).
 hipError_t download_planar(UploadStaging &S, const DevTensor &t, uint8_t *dst);
 void free_staging(UploadStaging &S);
@@ -359,9 +360,15 @@ hipError_t launch_expert_down_fmt(const DevTensor &D, const float *h, const uint
 // blocks, blk0 .. of the tensor, readable and writable up to 3 bytes past
 // them; row0: over all experts' rows.
 constexpr uint32_t kMxBlockBytes = 17;
+// The word at a tensor's end that launch_mx_blocks (in) sets where a block has a scale
+// byte of 253 or 254; it stands on its own.
+constexpr size_t kMxFlagBytes = 256;
+inline uint32_t *mx_beyond_flag(const DevTensor &t) { return reinterpret_cast<uint32_t *>(t.base + t.held - kMxFlagBytes); }
 hipError_t launch_mx_blocks(const DevTensor &t, uint8_t *raw, size_t nblk, size_t blk0, bool in, hipStream_t s);
 hipError_t launch_mx_quantize(const DevTensor &t, const float *x, size_t row0, size_t rows, hipStream_t s);
 hipError_t launch_mx_dequantize(const DevTensor &t, float *out, size_t row0, size_t rows, hipStream_t s);
+// (these and the experts' take weights as bf16 numbers: not of a tensor `beyond`, which goes
+// to launch_matmul_mx)
 hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s);
 // act(G x) * (U x) of two 2-D tensors of the same shape, zeros from their rows to down_cols
 hipError_t launch_gate_up_mx(const DevTensor &G, const DevTensor &U, const float *x, uint32_t act, uint32_t down_cols,
@@ -377,7 +384,7 @@ hipError_t launch_expert_gate_up_mx_routed(const DevTensor &GU, const float *x, 
 hipError_t launch_expert_down_mx(const DevTensor &D, const float *h, const uint32_t *ids, const float *w, uint32_t k,
                                  const float *base, int accumulate, const float *dscale, float *out, hipStream_t s);
 // out [T][rows] = X [T][cols] W^T of up to kMxFew vectors (as columns of the same
-// instructions), where they fit the LDS.
+// instructions), where they fit the LDS and the weights are bf16 numbers.
 constexpr size_t kMxFew = 5;
 bool matvecs_mx_fit(const DevTensor &W, size_t T);
 hipError_t launch_matvecs_mx(const DevTensor &W, const float *X, size_t T, float *out, hipStream_t s);

@@ -293,7 +293,7 @@ static hipError_t launch_matvec(const DevTensor &W, const float *x, float *y, hi
 hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s) { return launch_matvec<1>(W, x, y, s); }
 
 bool matvecs_mx_fit(const DevTensor &W, size_t T) {
-    return T <= kMxFew && T * mx_vec_bytes(mx_dims(W.rows, W.blocks_per_row).kg) <= (128 << 10);
+    return T <= kMxFew && !W.beyond && T * mx_vec_bytes(mx_dims(W.rows, W.blocks_per_row).kg) <= (128 << 10);
 }
 
 hipError_t launch_matvecs_mx(const DevTensor &W, const float *X, size_t T, float *out, hipStream_t s) {

@@ -22,7 +22,7 @@ namespace {
 constexpr int kMxStage = 256;
 template <bool IN>
 __global__ __launch_bounds__(kMxStage) void k_mx_blocks(uint8_t *raw, size_t nblk, size_t blk0, size_t rows, MxDims d,
-                                                        uint8_t *codes, uint8_t *scales) {
+                                                        uint8_t *codes, uint8_t *scales, uint32_t *beyond) {
     __shared__ uint32_t lds[kMxStage * kMxBlockBytes / 4];
     const size_t b0 = (size_t)blockIdx.x * kMxStage;
     const uint32_t n = nblk - b0 < (size_t)kMxStage ? (uint32_t)(nblk - b0) : (uint32_t)kMxStage;
@@ -41,6 +41,7 @@ __global__ __launch_bounds__(kMxStage) void k_mx_blocks(uint8_t *raw, size_t nbl
         uint8_t *scale = scales + mx_scale_at(d, tile, (uint32_t)(r % 16), b);
         if (IN) {
             *scale = mine[0];
+            if (mine[0] == 253 || mine[0] == 254) *beyond = 1;
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 code[i] = (uint32_t)mine[4 * i + 1] | (uint32_t)mine[4 * i + 2] << 8 | (uint32_t)mine[4 * i + 3] << 16 |
@@ -187,9 +188,10 @@ hipError_t launch_mx_blocks(const DevTensor &t, uint8_t *raw, size_t nblk, size_
     const dim3 grid((unsigned)((nblk + kMxStage - 1) / kMxStage));
     uint8_t *codes = const_cast<uint8_t *>(t.p0), *scales = const_cast<uint8_t *>(t.p1);
     if (in)
-        hipLaunchKernelGGL(k_mx_blocks<true>, grid, dim3(kMxStage), 0, s, raw, nblk, blk0, t.rows, d, codes, scales);
+        hipLaunchKernelGGL(k_mx_blocks<true>, grid, dim3(kMxStage), 0, s, raw, nblk, blk0, t.rows, d, codes, scales,
+                           mx_beyond_flag(t));
     else
-        hipLaunchKernelGGL(k_mx_blocks<false>, grid, dim3(kMxStage), 0, s, raw, nblk, blk0, t.rows, d, codes, scales);
+        hipLaunchKernelGGL(k_mx_blocks<false>, grid, dim3(kMxStage), 0, s, raw, nblk, blk0, t.rows, d, codes, scales, nullptr);
     return hipGetLastError();
 }
 

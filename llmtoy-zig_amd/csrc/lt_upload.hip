@@ -169,7 +169,7 @@ hipError_t zero_tensor(UploadStaging &S, const DevTensor &t) {
     return e;
 }
 
-hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const uint8_t *src) {
+hipError_t upload_planar(UploadStaging &S, int device, DevTensor &t, const uint8_t *src) {
     PlaneArgs pa{};
     const bool f32 = t.type == LT_TYPE_F32, mx = t.type == LT_TYPE_MXFP4;
     if (!f32 && !mx && !plane_args(t, pa)) return hipErrorInvalidValue;
@@ -223,7 +223,14 @@ hipError_t upload_planar(UploadStaging &S, int device, const DevTensor &t, const
         for (int w = 0; w < W; w++) th.emplace_back(work, w, true);
         for (auto &x : th) x.join();
     }
-    return (hipError_t)err.load();
+    e = (hipError_t)err.load();
+    if (e == hipSuccess && mx) {
+        uint32_t flag = 0;
+        e = hipMemcpyAsync(&flag, mx_beyond_flag(t), 4, hipMemcpyDeviceToHost, S.st[0]);
+        if (e == hipSuccess) e = hipStreamSynchronize(S.st[0]);
+        t.beyond = flag != 0;
+    }
+    return e;
 }
 
 hipError_t download_planar(UploadStaging &S, const DevTensor &t, uint8_t *dst) {
