@@ -95,6 +95,7 @@ struct lt_ctx {
         uint8_t *p;
     };
     std::vector<MxHand> mx_hands;
+    uint32_t mx_wait = lt::kMxWaitTicks;
     // hand-over memory of the single-launch dense FFN (allocated by lt_init)
     void *ffn = nullptr;
     lt::FfnScratch ffsc{};
@@ -512,7 +513,7 @@ int mx_hand_of(lt_ctx *ctx, size_t n_experts, size_t k, size_t d_model, size_t d
 // lt_init's device set-up: the host-mapped error word, the address of this
 // device's static scratch, and the XCD placement probe (run once, into the
 // static scratch's probe area).  LT_FUSED_AGENT_HANDOVER=1 turns the same-XCD
-// hand-over off (testing).
+// hand-over off, LT_MX_WAIT_TICKS (10 ns each) limits the MXFP4 layer's waits (testing).
 hipError_t init_device_state(lt_ctx *ctx) {
     void *hp = nullptr, *dp = nullptr;
     hipError_t e = hipHostMalloc(&hp, 64, hipHostMallocMapped);
@@ -532,6 +533,8 @@ hipError_t init_device_state(lt_ctx *ctx) {
     const char *agent = getenv("LT_FUSED_AGENT_HANDOVER");
     if (agent && agent[0] == '1') local = 0;
     ctx->xcd_local = local;
+    const char *wait = getenv("LT_MX_WAIT_TICKS");
+    if (wait && wait[0]) ctx->mx_wait = (uint32_t)std::min<unsigned long>(strtoul(wait, nullptr, 10), lt::kMxWaitTicks);
     ctx->na_fsc = lt::fused_scratch_at(ctx->na_base, ctx->err_dev, local);
     if ((e = hipMalloc(&ctx->ffn, lt::kFfnScratchBytes)) != hipSuccess) return e;
     if ((e = hipMemset(ctx->ffn, 0, lt::kFfnScratchBytes)) != hipSuccess) return e;
@@ -1364,7 +1367,7 @@ int moe_dev(lt_ctx *ctx, float *out, const float *x, const DevTensor &R, const f
         return launch_rc(ctx,
                          lt::launch_moe_mx(R, bias, GU, D, x, k, (flags & LT_MOE_NORM_TOPK) ? 1u : 0u, d_expert, act, base,
                                            (flags & LT_MOE_ACCUMULATE) ? 1 : 0, out, r.ids, r.w, hand, ctx->xcd_local,
-                                           ctx->err_dev, ctx->stream),
+                                           ctx->mx_wait, ctx->err_dev, ctx->stream),
                          "moe_mx");
     }
     if ((rc = ensure(ctx, ctx->eh, (size_t)k * Kd * 4))) return rc;

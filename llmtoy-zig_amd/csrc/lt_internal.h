@@ -395,7 +395,8 @@ bool moe_mx_fits(const DevTensor &R, const DevTensor &GU, const DevTensor &D, ui
 size_t moe_mx_bytes(uint32_t n_experts, uint32_t k, size_t d_model, size_t down_cols);
 hipError_t launch_moe_mx(const DevTensor &R, const float *bias, const DevTensor &GU, const DevTensor &D, const float *x, uint32_t k,
                          uint32_t norm, uint32_t d_expert, uint32_t act, const float *base, int accumulate, float *out,
-                         uint32_t *ids, float *w, uint8_t *hand, int xcd_local, uint32_t *err, hipStream_t s);
+                         uint32_t *ids, float *w, uint8_t *hand, int xcd_local, uint32_t wait, uint32_t *err, hipStream_t s);
+constexpr uint32_t kMxWaitTicks = 20000000;  // its waits' limit: 200 ms of the 100 MHz wall clock
 // out [T][rows] = X [T][cols] W^T; ws: matmul_mx_workspace(W, T) bytes.
 size_t matmul_mx_workspace(const DevTensor &W, size_t T);
 hipError_t launch_matmul_mx(const DevTensor &W, const float *X, size_t T, void *ws, float *out, hipStream_t s);

@@ -50,7 +50,6 @@ namespace lt {
 
 namespace {
 
-constexpr uint64_t kMxWaitTicks = 20000000;  // 200 ms of the 100 MHz wall clock
 constexpr uint32_t kMxMaxLogits = 256, kMxDownRows = 64;
 constexpr uint32_t kMxAtOnce = 96;  // workgroups of a group on its 32 CUs
 struct MxLayer {
@@ -63,6 +62,7 @@ struct MxLayer {
     uint32_t NR, J, ND, SPG;
     MxDiv by_j, by_nd;
     int accumulate, local;
+    uint32_t wait;  // a wait's limit, ticks of the 100 MHz wall clock
     float *out;
     uint32_t *counters, *err;
     uint64_t *lg;  // [8][kMxMaxLogits]
@@ -70,10 +70,15 @@ struct MxLayer {
     uint64_t *pl;  // [slot][row]
 };
 
+// What a wait that ran out was for, in the error word (each bit's meaning stands in its text).
+enum : uint32_t { kMxGateLogits = 1, kMxDownLogits = 2, kMxH = 4, kMxRows = 8 };
+
 // Waits until every lane's words (up to N, `have` of them from its pointer p on,
-// stride apart) carry the epoch; the others are 0.  False after the limit.
+// stride apart) carry the epoch; the others are 0.  False after the limit: then
+// a late word is reported, by its place from `base` on.
 template <int N>
-__device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N]) {
+__device__ __forceinline__ bool mx_await(const MxLayer &a, uint32_t what, const uint64_t *base, const uint64_t *p, uint32_t stride,
+                                         uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N]) {
     while (true) {
         uint64_t w[N];
 #pragma unroll
@@ -84,26 +89,28 @@ __device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, uin
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = good ? __uint_as_float((uint32_t)w[i]) : NAN;
         if (__all(good)) return true;
-        if (wall_clock64() - t0 > kMxWaitTicks) return false;
+        if (wall_clock64() - t0 <= a.wait) continue;
+        if ((threadIdx.x & 63) == (uint32_t)__builtin_ctzll(__ballot(!good))) {
+            uint32_t at = 0, saw = 0;
+#pragma unroll
+            for (int i = N - 1; i >= 0; i--)
+                if (!tag_is(w[i], ep)) at = i * stride, saw = (uint32_t)(w[i] >> 32);
+            report_timeout(a.err, what);
+            report_detail(a.err, (int)blockIdx.x, what, (uint32_t)(p - base) + at, saw, ep);
+        }
+        return false;
     }
-}
-__device__ __forceinline__ void mx_late(const MxLayer &a, uint32_t code, uint32_t ep, int lane) {
-    if (lane) return;
-    report_timeout(a.err, code);
-    report_detail(a.err, (int)blockIdx.x, code, 0u, 0u, ep);
 }
 
 // One wave: logit lane + 64 i in v[i], from the group's copy.
 template <int PER>
-__device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t ep, uint64_t t0, float (&v)[PER], int lane) {
+__device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t what, uint32_t ep, uint64_t t0, float (&v)[PER], int lane) {
     const uint64_t *w = a.lg + (blockIdx.x & 7) * kMxMaxLogits;
     float one[1];
 #pragma unroll
     for (int i = 0; i < PER; i++) v[i] = 0.0f;
-    const bool good = mx_await<1>(w + (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one) &&  // then all of them
-                      mx_await<PER>(w + lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v);
-    if (!good) mx_late(a, 1u, ep, lane);
-    return good;
+    return mx_await<1>(a, what, w, w + (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one) &&  // then all of them
+           mx_await<PER>(a, what, w, w + lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v);
 }
 
 template <int ROUTE>
@@ -147,7 +154,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
         for (uint32_t q = threadIdx.x; q < units; q += kPairThreads) mx_vec_put(v, q, mx_vec_load(a.x, q, a.gu.d.nb));
         if (wave == 0) {
             float logit[ROUTE];
-            const bool good = mx_logits<ROUTE>(a, ep, t0, logit, lane);
+            const bool good = mx_logits<ROUTE>(a, kMxGateLogits, ep, t0, logit, lane);
             const int e = topk_index_at<ROUTE>(logit, (int)a.n_experts, (int)slot, lane);
             if (lane == 0) s_ids[0] = (uint32_t)e, s_good = good;
         }
@@ -165,7 +172,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     }
     if (wave == 0) {
         float logit[ROUTE];
-        const bool good = mx_logits<ROUTE>(a, ep, t0, logit, lane);
+        const bool good = mx_logits<ROUTE>(a, kMxDownLogits, ep, t0, logit, lane);
         uint32_t key[ROUTE];
         int e;
         float w;
@@ -185,11 +192,10 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     MxWords w0;
     if (half < a.d.kq) mx_fetch<false>(w0, rw, half, a.d.kg);
     mx_order();
-    bool good = s_good;
     for (uint32_t q = threadIdx.x; __any(q < 16 * a.d.kg); q += kPairThreads) {
         float y[8];
         const bool on = q < 4 * a.d.nb;
-        if (!mx_await<8>(a.hl + (size_t)slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y)) good = false;
+        (void)mx_await<8>(a, kMxH, a.hl, a.hl + (size_t)slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y);
         if (q < 16 * a.d.kg)
             mx_vec_put(v, q, {make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7])});
     }
@@ -216,7 +222,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
             const uint32_t row = row0 + q % kMxDownRows;
             const bool mine = q < slot * kMxDownRows, on = mine && row < a.rows;
             float y[1];
-            if (!mx_await<1>(a.pl + (size_t)(q / kMxDownRows) * a.rows + row, 0, on, ep, t0, y)) good = false;
+            (void)mx_await<1>(a, kMxRows, a.pl, a.pl + (size_t)(q / kMxDownRows) * a.rows + row, 0, on, ep, t0, y);
             if (mine) sums[q] = y[0];
         }
         __syncthreads();
@@ -228,7 +234,6 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
             a.out[row] = a.base ? a.base[row] + y : y;
         }
     }
-    if (!good) mx_late(a, 4u, ep, lane);
     done();
 }
 
@@ -260,7 +265,7 @@ size_t moe_mx_bytes(uint32_t n_experts, uint32_t k, size_t d_model, size_t down_
 
 hipError_t launch_moe_mx(const DevTensor &R, const float *bias, const DevTensor &GU, const DevTensor &D, const float *x, uint32_t k,
                          uint32_t norm, uint32_t d_expert, uint32_t act, const float *base, int accumulate, float *out,
-                         uint32_t *ids, float *w, uint8_t *hand, int xcd_local, uint32_t *err, hipStream_t s) {
+                         uint32_t *ids, float *w, uint8_t *hand, int xcd_local, uint32_t wait, uint32_t *err, hipStream_t s) {
     MxLayer a{};
     const uint32_t n = (uint32_t)GU.n_experts;
     if (!moe_mx_fits(R, GU, D, k) || R.total_rows != n) return hipErrorInvalidValue;
@@ -271,7 +276,7 @@ hipError_t launch_moe_mx(const DevTensor &R, const float *bias, const DevTensor 
     a.n_experts = n, a.F = d_expert, a.down_cols = (uint32_t)D.cols, a.rows = (uint32_t)D.rows, a.act = act;
     const unsigned grid = 8 * layer_groups(n, k, D.rows, D.cols, a.NR, a.J, a.ND, a.SPG);
     a.by_j = mx_div(a.J), a.by_nd = mx_div(a.ND);
-    a.accumulate = accumulate, a.local = xcd_local, a.out = out, a.err = err;
+    a.accumulate = accumulate, a.local = xcd_local, a.wait = wait, a.out = out, a.err = err;
     a.lg = reinterpret_cast<uint64_t *>(hand);
     a.hl = reinterpret_cast<uint64_t *>(hand + kMxLgBytes);
     a.pl = a.hl + (size_t)k * D.cols;
