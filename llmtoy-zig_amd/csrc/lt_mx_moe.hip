@@ -72,45 +72,58 @@ struct MxLayer {
 
 // What a wait that ran out was for, in the error word (each bit's meaning stands in its text).
 enum : uint32_t { kMxGateLogits = 1, kMxDownLogits = 2, kMxH = 4, kMxRows = 8 };
+// The first wait of a workgroup that ran out, in LDS: what for, a late word's place and
+// the tag that it had.  (Reported at the workgroup's end: the report's instructions beside
+// each wait spilled scalars.)
+typedef uint32_t mx_late __attribute__((ext_vector_type(4)));
 
-// Waits until every lane's words (up to N, `have` of them from its pointer p on,
-// stride apart) carry the epoch; the others are 0.  False after the limit: then
-// a late word is reported, by its place from `base` on.
+// Waits until every lane's words (up to N, `have` of them from words + first on, stride
+// apart) carry the epoch; the others are 0.  After the limit `good` becomes false.
 template <int N>
-__device__ __forceinline__ bool mx_await(const MxLayer &a, uint32_t what, const uint64_t *base, const uint64_t *p, uint32_t stride,
-                                         uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N]) {
+__device__ __forceinline__ void mx_await(const MxLayer &a, uint32_t what, const uint64_t *words, uint32_t first, uint32_t stride,
+                                         uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N], bool &good, mx_late &late) {
+    const uint64_t *const p = words + first;
     while (true) {
         uint64_t w[N];
 #pragma unroll
         for (int i = 0; i < N; i++) w[i] = (uint32_t)i < have ? hand_get(p + i * stride) : (uint64_t)ep << 32;
-        bool good = true;
+        bool here = true;
 #pragma unroll
-        for (int i = 0; i < N; i++) good = good && tag_is(w[i], ep);
+        for (int i = 0; i < N; i++) here = here && tag_is(w[i], ep);
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = good ? __uint_as_float((uint32_t)w[i]) : NAN;
-        if (__all(good)) return true;
+        for (int i = 0; i < N; i++) v[i] = here ? __uint_as_float((uint32_t)w[i]) : NAN;
+        if (__all(here)) return;
         if (wall_clock64() - t0 <= a.wait) continue;
-        if ((threadIdx.x & 63) == (uint32_t)__builtin_ctzll(__ballot(!good))) {
-            uint32_t at = 0, saw = 0;
+        if (good && (threadIdx.x & 63) == (uint32_t)__builtin_ctzll(__ballot(!here))) {
+            uint32_t i = 0, saw = (uint32_t)(w[0] >> 32);
 #pragma unroll
-            for (int i = N - 1; i >= 0; i--)
-                if (!tag_is(w[i], ep)) at = i * stride, saw = (uint32_t)(w[i] >> 32);
-            report_timeout(a.err, what);
-            report_detail(a.err, (int)blockIdx.x, what, (uint32_t)(p - base) + at, saw, ep);
+            for (int j = 1; j < N; j++)
+                if (saw == ep) i = j, saw = (uint32_t)(w[j] >> 32);
+            late = mx_late{what, first + i * stride, saw, 0};
         }
-        return false;
+        good = false;
+        return;
     }
 }
+__device__ __forceinline__ void mx_report(const MxLayer &a, const mx_late &late, uint32_t ep) {
+    report_timeout(a.err, late[0]);
+    report_detail(a.err, (int)blockIdx.x, late[0], late[1], late[2], ep);
+}
 
-// One wave: logit lane + 64 i in v[i], from the group's copy.
+// One wave: logit lane + 64 i in v[i], from the group's copy.  Late ones make all of them
+// NaN (those that came in time might select another expert), and so the weights.
 template <int PER>
-__device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t what, uint32_t ep, uint64_t t0, float (&v)[PER], int lane) {
+__device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t what, uint32_t ep, uint64_t t0, float (&v)[PER], int lane,
+                                          mx_late &late) {
     const uint64_t *w = a.lg + (blockIdx.x & 7) * kMxMaxLogits;
     float one[1];
+    bool good = true;
+    mx_await<1>(a, what, w, (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one, good, late);  // then all of them
+    mx_await<PER>(a, what, w, (uint32_t)lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v, good, late);
+    if (!good)
 #pragma unroll
-    for (int i = 0; i < PER; i++) v[i] = 0.0f;
-    return mx_await<1>(a, what, w, w + (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one) &&  // then all of them
-           mx_await<PER>(a, what, w, w + lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v);
+        for (int i = 0; i < PER; i++) v[i] = NAN;
+    return good;
 }
 
 template <int ROUTE>
@@ -119,6 +132,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     __shared__ float part[kPairWaves][16];
     __shared__ uint32_t s_ids[16], s_good;
     __shared__ float s_w[16];
+    __shared__ mx_late s_late;
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.x, group = b % 8;
     mx_u32x4 *const v = reinterpret_cast<mx_u32x4 *>(lds);
@@ -154,7 +168,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
         for (uint32_t q = threadIdx.x; q < units; q += kPairThreads) mx_vec_put(v, q, mx_vec_load(a.x, q, a.gu.d.nb));
         if (wave == 0) {
             float logit[ROUTE];
-            const bool good = mx_logits<ROUTE>(a, kMxGateLogits, ep, t0, logit, lane);
+            const bool good = mx_logits<ROUTE>(a, kMxGateLogits, ep, t0, logit, lane, s_late);
             const int e = topk_index_at<ROUTE>(logit, (int)a.n_experts, (int)slot, lane);
             if (lane == 0) s_ids[0] = (uint32_t)e, s_good = good;
         }
@@ -162,6 +176,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
         mx_gate_rows(
             a.gu, (uint32_t)__builtin_amdgcn_readfirstlane(s_ids[0]), j0, a.F, a.down_cols, a.act, v, part, [] {},
             [&](uint32_t r, float y) { put(r, s_good ? y : NAN); });
+        if (threadIdx.x == 0 && !s_good) mx_report(a, s_late, ep);
         return done();
     }
     i -= a.SPG * a.J;
@@ -172,7 +187,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     }
     if (wave == 0) {
         float logit[ROUTE];
-        const bool good = mx_logits<ROUTE>(a, kMxDownLogits, ep, t0, logit, lane);
+        const bool good = mx_logits<ROUTE>(a, kMxDownLogits, ep, t0, logit, lane, s_late);
         uint32_t key[ROUTE];
         int e;
         float w;
@@ -192,10 +207,11 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     MxWords w0;
     if (half < a.d.kq) mx_fetch<false>(w0, rw, half, a.d.kg);
     mx_order();
+    bool good = s_good;
     for (uint32_t q = threadIdx.x; __any(q < 16 * a.d.kg); q += kPairThreads) {
         float y[8];
         const bool on = q < 4 * a.d.nb;
-        (void)mx_await<8>(a, kMxH, a.hl, a.hl + (size_t)slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y);
+        mx_await<8>(a, kMxH, a.hl, slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y, good, s_late);
         if (q < 16 * a.d.kg)
             mx_vec_put(v, q, {make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7])});
     }
@@ -222,7 +238,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
             const uint32_t row = row0 + q % kMxDownRows;
             const bool mine = q < slot * kMxDownRows, on = mine && row < a.rows;
             float y[1];
-            (void)mx_await<1>(a, kMxRows, a.pl, a.pl + (size_t)(q / kMxDownRows) * a.rows + row, 0, on, ep, t0, y);
+            mx_await<1>(a, kMxRows, a.pl, q / kMxDownRows * a.rows + row, 0, on, ep, t0, y, good, s_late);
             if (mine) sums[q] = y[0];
         }
         __syncthreads();
@@ -234,6 +250,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
             a.out[row] = a.base ? a.base[row] + y : y;
         }
     }
+    if (!good && lane == 0) mx_report(a, s_late, ep);
     done();
 }
 
