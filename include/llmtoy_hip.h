@@ -138,7 +138,9 @@ int lt_tensor_upload(lt_ctx *ctx, const void *host_bytes, size_t nbytes, uint32_
  * byte for byte. */
 int lt_tensor_read(lt_ctx *ctx, const lt_tensor *t, void *host_bytes, size_t nbytes);
 /* Copy an uploaded tensor (same layout) to a new device allocation; used to
- * rotate weight copies so that timing is not served from the 256 MB cache. */
+ * rotate weight copies so that timing is not served from the 256 MB cache.
+ * Returns when the copy is made; not while the stream is captured
+ * (LT_ERR_INVALID). */
 int lt_tensor_clone(lt_ctx *ctx, const lt_tensor *src, lt_tensor **out_tensor);
 int lt_tensor_free(lt_ctx *ctx, lt_tensor *t);
 /* An MXFP4 tensor of the given shape (as lt_tensor_upload's) holding zeros, for

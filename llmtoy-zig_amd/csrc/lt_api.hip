@@ -756,12 +756,19 @@ extern "C" int lt_tensor_read(lt_ctx *ctx, const lt_tensor *t, void *host_bytes,
 
 extern "C" int lt_tensor_clone(lt_ctx *ctx, const lt_tensor *src, lt_tensor **out_tensor) {
     if (!ctx || !src || !out_tensor) return fail(ctx, LT_ERR_INVALID, "null argument");
+    *out_tensor = nullptr;
+    if (capturing(ctx)) return fail(ctx, LT_ERR_INVALID, "a tensor cannot be cloned while the stream is captured");
+    LT_HIP(ctx, hipSetDevice(ctx->device));
     lt_tensor *t = new (std::nothrow) lt_tensor(*src);
     if (!t) return fail(ctx, LT_ERR_OOM, "host allocation failed");
+    t->t.base = nullptr;
+    // behind what is enqueued, and waited for: a copy inside the device may outlive its
+    // hipMemcpy, and lt_tensor_read's streams wait for no other
     hipError_t e = hipMalloc((void **)&t->t.base, src->t.held);
-    if (e == hipSuccess) e = hipMemcpy(t->t.base, src->t.base, src->t.held, hipMemcpyDeviceToDevice);
+    if (e == hipSuccess) e = hipMemcpyAsync(t->t.base, src->t.base, src->t.held, hipMemcpyDeviceToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) {
-        if (t->t.base != src->t.base) (void)hipFree(t->t.base);
+        if (t->t.base) (void)hipFree(t->t.base);
         delete t;
         return hip_fail(ctx, e, "tensor clone");
     }
