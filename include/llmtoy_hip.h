@@ -171,8 +171,9 @@ size_t lt_tensor_bytes(const lt_tensor *t);
  * sums give, which is NaN or an infinity (Q4_K and Q6_K subtract a block's
  * offset as a sum of its own, Q8_0 has none).  Q4_K and Q6_K activations below
  * about 2^-100 lose bits (their products are kept 2^-24 of their size).
- * MXFP4 takes fp32 activations as they are, and any NaN or infinity among them
- * makes every output NaN.
+ * MXFP4 takes fp32 activations as they are (below 2^-110 to the nearest lower
+ * multiple of 2^-133), and any NaN or infinity among them makes every output
+ * NaN; so do the experts' calls.
  * Replaces quantMatvec / quantMatvecPar (ops/math.zig:133-171, 277-320) and
  * MatvecSession.run / runQ8_1Mv (gpu/matvec.zig:497-647,
  * gemma4/gpu_weights.zig:1573-1607).  W must be a 2-D tensor. */
@@ -197,8 +198,10 @@ int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t row0, size
  * cols <= 16384, T <= 65536), X and out fp32: prompts, batched decode.  The
  * products take each activation to 2^-24 of the largest of its 32-element block
  * (five 6-bit limbs; up to five vectors as lt_matvec does) and are summed in
- * fp32: the accuracy of lt_matvec, in another order of sums.  A NaN or an infinity in a vector makes that
- * vector's outputs NaN and leaves the others.  T = 0 does nothing.  Device
+ * fp32: the accuracy of lt_matvec, in another order of sums.  Blocks whose
+ * largest is below 2^-105 lose bits: activations are kept to 2^-129 there.  A
+ * NaN or an infinity in a vector makes that vector's outputs NaN and leaves the
+ * others.  T = 0 does nothing.  Device
  * pointers X and out must be 16-byte aligned; out must not overlap X.  flags:
  * LT_HOST_IO.  The reference calls quantMatvecPar once a vector
  * (main.zig:1916-1922). */

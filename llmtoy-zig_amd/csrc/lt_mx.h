@@ -43,7 +43,9 @@ constexpr int kMxLimbs = 5;
 constexpr int kMxCbszFp6 = 2, kMxCbszFp4 = 4;  // operand formats of the instruction
 // scale exponents of the limbs below the first one's
 constexpr uint32_t kMxLimbShift[kMxLimbs] = {0, 4, 9, 14, 19};
-constexpr uint32_t kMxLeastScale = 20;  // keeps the last limb's unit a normal number
+// keeps the last limb's unit a normal number: of blocks below 2^-105, 2^-129 may be lost
+// (more than 2^-24 of the largest)
+constexpr uint32_t kMxLeastScale = 20;
 
 typedef int mx_op __attribute__((ext_vector_type(8)));          // a matrix operand's registers
 typedef float mx_acc16 __attribute__((ext_vector_type(4)));     // 16 x 16 sums

@@ -6,7 +6,7 @@
 // A weight times its block's scale is a bf16 number (2 bits times a power of
 // two; scale bytes 253 and 254 have weights beyond them, see DevTensor::beyond), and v_cvt_scalef32_pk_bf16_fp4 makes two of them from a byte.  An
 // activation is the sum of three bf16 numbers of 8 bits each, cut off from the
-// top, exactly.  So v_mfma_f32_16x16x32_bf16 with 16 rows of weights on one
+// top, exactly (from 2^-110 on; bits below 2^-133 are no bf16 number's).  So v_mfma_f32_16x16x32_bf16 with 16 rows of weights on one
 // side and the three parts as columns on the other gives the products with the
 // fp32 activations; the row's sum over the columns is y.  (The scaled
 // instruction, which takes the codes as they are, needs activations in FP6:

@@ -1,7 +1,9 @@
-"""MXFP4 products at the ends of the numbers' ranges."""
+"""MXFP4 products at the ends of the numbers' ranges: every scale byte, activations
+from the least to the largest."""
 import numpy as np
 import pytest
 
+import mx_accuracy as acc
 import mx_reference as mx
 from llmtoy_amd import ggml, synth
 from llmtoy_amd import lib as ltlib
@@ -135,3 +137,46 @@ def test_gpu_mx_weights_beyond_bf16(ctx):
     assert np.isfinite(y).all()
     for t in (*ts, c, R, GU, DE, GB, DB):
         t.free()
+
+
+@pytest.mark.parametrize("xs", [1e-30, 1e30, 2e-38, 3e38])
+@pytest.mark.parametrize("T,rows", [(4, 40), (17, 40), (1100, 1030)])
+def test_gpu_mx_matmul_magnitudes(ctx, T, rows, xs):
+    print(f"magnitudes {xs} T {T} rows {rows}", flush=True)
+    g = gen(T, rows, 43)
+    m = synth.quant_matrix(g, MX, rows, 320)
+    m.reshape(rows, 10, 17)[..., 0] = g.integers(110, 120 if xs > 1e35 else 140, (rows, 10))
+    x = acts(g, T, 320)
+    x = (x / np.abs(x).max() if xs > 1e35 else x) * np.float32(xs)
+    t = ctx.upload(m, MX, rows, 320)
+    y = np.empty((T, rows), np.float32)
+    ctx.quant_matmul(y, t, x)
+    w = mx.decode(m, 320)
+    ref, bound = mx.product(w, x)
+    # the last limb's remainder of the least scale is 2^-129, a vector's third part is cut at 2^-133; subnormal sums
+    close(y, ref, bound + np.abs(w).sum(1) * 2.0 ** -129 + 2.0 ** -126)
+    t.free()
+
+
+@pytest.mark.parametrize("T,rows,least", [(1, 130, -109), (4, 130, -109), (17, 130, -104), (1100, 1030, -104)])
+def test_gpu_mx_least_activations_in_full(ctx, T, rows, least):
+    # the smallest that are taken in full: the elements themselves for a vector's parts, the
+    # blocks' largest for limbs; a step below, no more than the documented remainder is lost
+    print(f"least T {T} rows {rows}", flush=True)
+    g = gen(T, rows, 45)
+    m, x = synth.quant_matrix(g, MX, rows, 320), acts(g, T, 320)
+    m.reshape(rows, 10, 17)[..., 0] = g.integers(130, 134, (rows, 10))
+    x = np.copysign(1 + np.abs(x), x).astype(np.float32)  # no element and no block below 1
+    t, w = ctx.upload(m, MX, rows, 320), mx.decode(m, 320)
+    for e in (least, least - 12):
+        xs, y = x * np.float32(2.0 ** e), np.empty((T, rows), np.float32)
+        if T == 1:
+            ctx.quant_matvec(y[0], t, xs[0])
+        else:
+            ctx.quant_matmul(y, t, xs)
+        if e == least:
+            assert acc.within_l2(y, w, xs).max() <= 1
+        ref, _ = mx.product(w, xs)
+        lost = np.abs(w).sum(1) * 2.0 ** (-133 if T < 6 else -129) if e < least else 0
+        assert (np.linalg.norm(y - ref, axis=-1) <= acc.l2_limit(w, xs) + np.linalg.norm(lost)).all()
+    t.free()
