@@ -1,4 +1,5 @@
-"""The MXFP4 layer in one launch: waits that end at their limit."""
+"""The MXFP4 layer: which shapes are one launch, routing and activations that are not finite,
+waits that end at their limit."""
 import re
 
 import numpy as np
@@ -7,7 +8,8 @@ import pytest
 import llmtoy_amd as lt
 from llmtoy_amd import ggml, synth
 from llmtoy_amd import lib as ltlib
-from test_gpu_mxfp4 import acts, gen
+from llmtoy_amd.hip import DeviceArray, Graph
+from test_gpu_mxfp4 import acts, close, expert_ref, experts, gen, route
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +52,83 @@ def test_gpu_mx_layer_names_the_waits_that_ran_out(ctx, monkeypatch):
     assert np.linalg.norm(out - want) <= 2.0 ** -18 * np.linalg.norm(want)
     for t in ts:
         t.free()
+
+
+# (E, D, F, Kd, k): those that test_gpu_mx_moe_one_launch computes, and larger ones
+ONE = [(6, 256, 40, 64, 6), (7, 512, 32, 32, 7), (128, 2048, 96, 96, 8), (256, 256, 160, 160, 8), (40, 768, 80, 544, 14), (255, 256, 64, 64, 15),
+       (16, 1280, 48, 64, 16), (9, 16384, 16, 32, 6), (9, 256, 4100, 4128, 8), (8, 2880, 96, 96, 8), (7, 96, 32, 32, 7), (20, 32, 64, 64, 3),
+       (60, 1056, 64, 64, 6), (33, 544, 64, 64, 9), (4, 224, 32, 32, 1), (16, 2048, 768, 768, 8), (8, 2816, 2112, 2112, 8)]
+THREE = [(8, 2816, 2112, 2112, 4), (16, 2048, 768, 768, 10), (300, 256, 64, 64, 8), (8, 2880, 1024, 1024, 6)]
+
+
+def test_gpu_mx_layer_one_launch_or_three(ctx):
+    # the hand-over memory of a shape's single launch is set up by its first call, which therefore
+    # cannot be captured; three launches can be
+    x, y = DeviceArray((16384,)), DeviceArray((16384,))
+    with lt.Context(0) as c:
+        for shapes, refused in ((ONE, True), (THREE, False)):
+            for E, D, F, Kd, k in shapes:
+                ts = (c.upload(np.zeros((E, D), np.float32), ggml.F32, E, D), c.create(MX, 2 * F, D, E), c.create(MX, D, Kd, E))
+                seen = []
+
+                def first():
+                    try:
+                        c.moe_forward(y, x, *ts, k, F)
+                        seen.append(False)
+                    except ltlib.InvalidError:
+                        seen.append(True)
+
+                Graph(c.stream, first).destroy()
+                assert seen == [refused], (E, D, F, Kd, k)
+                for t in ts:
+                    t.free()
+    x.free(), y.free()
+
+
+@pytest.mark.parametrize("unfused", [False, True])
+@pytest.mark.parametrize("E,k", [(9, 8), (200, 8), (300, 6)])
+def test_gpu_mx_layer_not_finite(ctx, E, k, unfused):
+    print(f"not finite E {E} k {k} unfused {unfused}", flush=True)
+    D, F = 256, 64
+    g = gen(E, k, 53)
+    GU, DN, w = experts(ctx, g, E, D, F)
+    r, x = (g.standard_normal((E, D)) * 0.05).astype(np.float32), acts(g, D)
+    x[7] = 1.0
+    out, ids, p = np.empty(D, np.float32), np.empty(k, np.uint32), np.empty(k, np.float32)
+
+    def call(r, x):
+        R = ctx.upload(r, ggml.F32, E, D)
+        ctx.moe_forward(out, x, R, GU, DN, k, F, norm_topk=True, out_ids=ids, out_w=p, unfused=unfused)
+        R.free()
+        assert len(set(ids.tolist())) == k and (ids < E).all()
+
+    def finite(r, x, logits):
+        call(r, x)
+        want, wts = route(logits, k, True)
+        assert ids.tolist() == want.tolist()
+        _, ref, bound = expert_ref(w, x, want, wts, F, 0)
+        slack = 2 * (D * 2.0 ** -24 * (np.abs(r[want].astype(np.float64)) @ np.abs(x)).max() + 2.0 ** -20)  # the weights', as in the layer's tests
+        close(out, ref, bound + slack * np.abs(ref) + slack * sum(q * np.abs(w["dn"][e]).sum(1) for e, q in zip(want, wts)))
+
+    logits = r.astype(np.float64) @ x
+    finite(r, x, logits)
+    for bad in (np.nan, np.inf, -np.inf):
+        b = x.copy()
+        b[100] = bad
+        call(r, b)
+        assert np.isnan(out).all()
+    every = np.full_like(r, np.nan)  # all logits rank as -inf: the lowest indices
+    call(every, x)
+    assert ids.tolist() == list(range(k)) and np.isnan(p).all() and np.isnan(out).all()
+    for bad in (np.nan, -np.inf):  # one expert's logit: it is not selected, the others as ever
+        b, best = r.copy(), int(np.argmax(logits))
+        b[best, 7] = bad
+        rest = logits.copy()
+        rest[best] = -np.inf
+        finite(b, x, rest)
+    b = r.copy()  # +inf: it is selected first, and no weight is a number
+    b[E - 1, 7] = np.inf
+    call(b, x)
+    assert ids[0] == E - 1 and np.isnan(out).all()
+    finite(r, x, logits)
+    GU.free(), DN.free()
