@@ -573,13 +573,15 @@ int check_fused_err(lt_ctx *ctx) {
     // Later launches publish h through memory (agent scope) instead of an
     // XCD's L2, in case the placement the one-time probe saw has changed.
     ctx->xcd_local = ctx->fsc.xcd_local = ctx->na_fsc.xcd_local = ctx->ffsc.xcd_local = 0;
+    char word[64] = "word and tag not recorded";
+    if (d[2] != lt::kErrNotRecorded) snprintf(word, sizeof word, "index %u, saw %u", d[2], d[3]);
     return fail(ctx, LT_ERR_DEVICE,
                 "single-launch kernel: a hand-over wait timed out (code 0x%x: 1 gate/up logits, 2 down logits, 4 down "
                 "h records, 8 combine, 0x10 shared-FFN logits or last h word, 0x20 shared-FFN h, 0x40 dense-FFN h, "
                 "0x80 dense-FFN start values, 0x100 prefill f16 saturation, 0x200 Gemma4 tail, 0x400 prefill chunk "
-                "activations; first recorded: block %d, site 0x%x, index %u, saw %u, expected epoch or count %u); "
+                "activations; first recorded: block %d, site 0x%x, %s, expected epoch or count %u); "
                 "outputs of that call are NaN (prefill: wrong)",
-                v, (int)d[0] - 1, d[1], d[2], d[3], d[4]);
+                v, (int)d[0] - 1, d[1], word, d[4]);
 }
 
 int matvec_dev(lt_ctx *ctx, const DevTensor &W, const float *x, float *y) {

@@ -271,7 +271,8 @@ __device__ __forceinline__ void report_timeout(uint32_t *err, uint32_t code) {
 }
 // The first timed-out wait of a call also leaves what it saw in err[2..6]:
 // block + 1, site code, the word index, the word's epoch tag (or count)
-// seen, and the epoch expected.
+// seen (both may be kErrNotRecorded), and the epoch expected.
+constexpr uint32_t kErrNotRecorded = 0xffffffffu;
 __device__ __forceinline__ void report_detail(uint32_t *err, int bid, uint32_t code, uint32_t index, uint32_t seen,
                                               uint32_t ep) {
     uint32_t zero = 0;

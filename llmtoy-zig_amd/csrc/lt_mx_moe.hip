@@ -62,7 +62,7 @@ struct MxLayer {
     uint32_t NR, J, ND, SPG;
     MxDiv by_j, by_nd;
     int accumulate, local;
-    uint32_t wait;  // a wait's limit, ticks of the 100 MHz wall clock
+    uint32_t wait;  // the waits' limit, up to kMxWaitTicks
     float *out;
     uint32_t *counters, *err;
     uint64_t *lg;  // [8][kMxMaxLogits]
@@ -70,59 +70,48 @@ struct MxLayer {
     uint64_t *pl;  // [slot][row]
 };
 
-// What a wait that ran out was for, in the error word (each bit's meaning stands in its text).
-enum : uint32_t { kMxGateLogits = 1, kMxDownLogits = 2, kMxH = 4, kMxRows = 8 };
-// The first wait of a workgroup that ran out, in LDS: what for, a late word's place and
-// the tag that it had.  (Reported at the workgroup's end: the report's instructions beside
-// each wait spilled scalars.)
-typedef uint32_t mx_late __attribute__((ext_vector_type(4)));
-
-// Waits until every lane's words (up to N, `have` of them from words + first on, stride
-// apart) carry the epoch; the others are 0.  After the limit `good` becomes false.
+// Waits until every lane's words (up to N, `have` of them from its pointer p on,
+// stride apart) carry the epoch; the others are 0.  False after the limit.
 template <int N>
-__device__ __forceinline__ void mx_await(const MxLayer &a, uint32_t what, const uint64_t *words, uint32_t first, uint32_t stride,
-                                         uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N], bool &good, mx_late &late) {
-    const uint64_t *const p = words + first;
+__device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, uint32_t have, uint32_t ep, uint64_t t0, float (&v)[N]) {
     while (true) {
         uint64_t w[N];
 #pragma unroll
         for (int i = 0; i < N; i++) w[i] = (uint32_t)i < have ? hand_get(p + i * stride) : (uint64_t)ep << 32;
-        bool here = true;
+        bool good = true;
 #pragma unroll
-        for (int i = 0; i < N; i++) here = here && tag_is(w[i], ep);
+        for (int i = 0; i < N; i++) good = good && tag_is(w[i], ep);
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = here ? __uint_as_float((uint32_t)w[i]) : NAN;
-        if (__all(here)) return;
-        if (wall_clock64() - t0 <= a.wait) continue;
-        if (good && (threadIdx.x & 63) == (uint32_t)__builtin_ctzll(__ballot(!here))) {
-            uint32_t i = 0, saw = (uint32_t)(w[0] >> 32);
-#pragma unroll
-            for (int j = 1; j < N; j++)
-                if (saw == ep) i = j, saw = (uint32_t)(w[j] >> 32);
-            late = mx_late{what, first + i * stride, saw, 0};
-        }
-        good = false;
-        return;
+        for (int i = 0; i < N; i++) v[i] = good ? __uint_as_float((uint32_t)w[i]) : NAN;
+        if (__all(good)) return true;
+        if (wall_clock64() - t0 > kMxWaitTicks) return false;
     }
 }
-__device__ __forceinline__ void mx_report(const MxLayer &a, const mx_late &late, uint32_t ep) {
-    report_timeout(a.err, late[0]);
-    report_detail(a.err, (int)blockIdx.x, late[0], late[1], late[2], ep);
+// What a wait that ran out was for, in the error word (each bit's meaning stands in its text).
+enum : uint32_t { kMxGateLogits = 1, kMxDownLogits = 2, kMxH = 4, kMxRows = 8 };
+// (Which word was late, and its tag, are not recorded: every form of that cost 0.1 to 0.25
+// us a layer where nothing is late.)
+__device__ __forceinline__ void mx_late(const MxLayer &a, uint32_t what, uint32_t ep, int lane) {
+    if (lane) return;
+    report_timeout(a.err, what);
+    report_detail(a.err, (int)blockIdx.x, what, kErrNotRecorded, kErrNotRecorded, ep);
 }
 
 // One wave: logit lane + 64 i in v[i], from the group's copy.  Late ones make all of them
 // NaN (those that came in time might select another expert), and so the weights.
 template <int PER>
-__device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t what, uint32_t ep, uint64_t t0, float (&v)[PER], int lane,
-                                          mx_late &late) {
+__device__ __forceinline__ bool mx_logits(const MxLayer &a, uint32_t what, uint32_t ep, uint64_t t0, float (&v)[PER], int lane) {
     const uint64_t *w = a.lg + (blockIdx.x & 7) * kMxMaxLogits;
     float one[1];
-    bool good = true;
-    mx_await<1>(a, what, w, (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one, good, late);  // then all of them
-    mx_await<PER>(a, what, w, (uint32_t)lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v, good, late);
-    if (!good)
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = 0.0f;
+    const bool good = mx_await<1>(w + (blockIdx.x >> 3) % a.n_experts, 0, lane == 0, ep, t0, one) &&  // then all of them
+                      mx_await<PER>(w + lane, 64, (a.n_experts + 63u - lane) / 64, ep, t0, v);
+    if (__builtin_expect(!good, 0)) {
+        mx_late(a, what, ep, lane);
 #pragma unroll
         for (int i = 0; i < PER; i++) v[i] = NAN;
+    }
     return good;
 }
 
@@ -132,12 +121,11 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     __shared__ float part[kPairWaves][16];
     __shared__ uint32_t s_ids[16], s_good;
     __shared__ float s_w[16];
-    __shared__ mx_late s_late;
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.x, group = b % 8;
     mx_u32x4 *const v = reinterpret_cast<mx_u32x4 *>(lds);
     const uint32_t ep = a.counters[b] + 1u;
-    const uint64_t t0 = wall_clock64();
+    const uint64_t t0 = wall_clock64() - (kMxWaitTicks - a.wait);  // (where kMxWaitTicks before the limit is)
     uint32_t i = b / 8;
     // (behind a barrier: every wave has read the count)
     auto done = [&] {
@@ -168,7 +156,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
         for (uint32_t q = threadIdx.x; q < units; q += kPairThreads) mx_vec_put(v, q, mx_vec_load(a.x, q, a.gu.d.nb));
         if (wave == 0) {
             float logit[ROUTE];
-            const bool good = mx_logits<ROUTE>(a, kMxGateLogits, ep, t0, logit, lane, s_late);
+            const bool good = mx_logits<ROUTE>(a, kMxGateLogits, ep, t0, logit, lane);
             const int e = topk_index_at<ROUTE>(logit, (int)a.n_experts, (int)slot, lane);
             if (lane == 0) s_ids[0] = (uint32_t)e, s_good = good;
         }
@@ -176,7 +164,6 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
         mx_gate_rows(
             a.gu, (uint32_t)__builtin_amdgcn_readfirstlane(s_ids[0]), j0, a.F, a.down_cols, a.act, v, part, [] {},
             [&](uint32_t r, float y) { put(r, s_good ? y : NAN); });
-        if (threadIdx.x == 0 && !s_good) mx_report(a, s_late, ep);
         return done();
     }
     i -= a.SPG * a.J;
@@ -187,7 +174,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     }
     if (wave == 0) {
         float logit[ROUTE];
-        const bool good = mx_logits<ROUTE>(a, kMxDownLogits, ep, t0, logit, lane, s_late);
+        const bool good = mx_logits<ROUTE>(a, kMxDownLogits, ep, t0, logit, lane);
         uint32_t key[ROUTE];
         int e;
         float w;
@@ -207,11 +194,11 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
     MxWords w0;
     if (half < a.d.kq) mx_fetch<false>(w0, rw, half, a.d.kg);
     mx_order();
-    bool good = s_good;
+    uint32_t late = 0;
     for (uint32_t q = threadIdx.x; __any(q < 16 * a.d.kg); q += kPairThreads) {
         float y[8];
         const bool on = q < 4 * a.d.nb;
-        mx_await<8>(a, kMxH, a.hl, slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y, good, s_late);
+        if (!mx_await<8>(a.hl + (size_t)slot * 8 * (4 * a.d.nb) + q, 4 * a.d.nb, on ? 8 : 0, ep, t0, y)) late |= kMxH;
         if (q < 16 * a.d.kg)
             mx_vec_put(v, q, {make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7])});
     }
@@ -238,7 +225,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
             const uint32_t row = row0 + q % kMxDownRows;
             const bool mine = q < slot * kMxDownRows, on = mine && row < a.rows;
             float y[1];
-            mx_await<1>(a, kMxRows, a.pl, q / kMxDownRows * a.rows + row, 0, on, ep, t0, y, good, s_late);
+            if (!mx_await<1>(a.pl + (size_t)(q / kMxDownRows) * a.rows + row, 0, on, ep, t0, y)) late |= kMxRows;
             if (mine) sums[q] = y[0];
         }
         __syncthreads();
@@ -250,7 +237,7 @@ __global__ __launch_bounds__(kPairThreads, 6) void k_mx_moe(MxLayer a) {
             a.out[row] = a.base ? a.base[row] + y : y;
         }
     }
-    if (!good && lane == 0) mx_report(a, s_late, ep);
+    if (__builtin_expect(late != 0, 0)) mx_late(a, late, ep, lane);
     done();
 }
 
