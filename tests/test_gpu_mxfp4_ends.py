@@ -7,6 +7,7 @@ import mx_accuracy as acc
 import mx_reference as mx
 from llmtoy_amd import ggml, synth
 from llmtoy_amd import lib as ltlib
+from llmtoy_amd.hip import DeviceArray, DeviceView
 from test_gpu_mxfp4 import acts, close, gen, route
 
 pytestmark = pytest.mark.gpu
@@ -180,3 +181,21 @@ def test_gpu_mx_least_activations_in_full(ctx, T, rows, least):
         lost = np.abs(w).sum(1) * 2.0 ** (-133 if T < 6 else -129) if e < least else 0
         assert (np.linalg.norm(y - ref, axis=-1) <= acc.l2_limit(w, xs) + np.linalg.norm(lost)).all()
     t.free()
+
+
+@pytest.mark.parametrize("rows", [130, 70001])
+def test_gpu_mx_matvec_beyond_bf16_to_any_address(ctx, rows):
+    # lt_matvec asks nothing of out's address: through the thin product and the tiles
+    g = gen(rows, 46)
+    m, x = synth.quant_matrix(g, MX, rows, 160), acts(g, 160) * np.float32(2.0 ** -40)
+    m.reshape(rows, 5, 17)[[3, rows - 1], [0, 4], 0] = 254
+    t, dx = ctx.upload(m, MX, rows, 160), DeviceArray.from_numpy(x)
+    for shift in (1, 2, 3):
+        buf = DeviceArray.from_numpy(np.full(rows + 8, 5.0, np.float32))
+        ctx.quant_matvec(DeviceView(buf.ptr + 4 * shift, (rows,), np.float32), t, dx)
+        ctx.sync()
+        got = buf.numpy()
+        assert (got[:shift] == 5).all() and (got[shift + rows:] == 5).all()
+        close(got[shift:shift + rows], *mx.product(mx.decode(m, 160), x))
+        buf.free()
+    t.free(), dx.free()

@@ -130,3 +130,26 @@ def test_gpu_mx_layer_not_finite(ctx, E, k, unfused):
     assert ids[0] == E - 1 and np.isnan(out).all()
     finite(r, x, logits)
     GU.free(), DN.free()
+
+
+@pytest.mark.parametrize("unfused", [False, True])
+@pytest.mark.parametrize("E,D,F,Kd,k", [(1, 96, 1, 32, 1), (8, 64, 5, 64, 8), (9, 512, 33, 64, 7), (16, 2048, 96, 96, 16)])
+def test_gpu_mx_layer_into_its_own_input(ctx, E, D, F, Kd, k, unfused):
+    # x += layer(x) on the device, experts of one row and of odd numbers of them, one expert
+    print(f"in place E {E} D {D} F {F} Kd {Kd} k {k} unfused {unfused}", flush=True)
+    g = gen(E, D, F, k, 54)
+    GU, DN, w = experts(ctx, g, E, D, F, Kd)
+    r, x = (g.standard_normal((E, D)) * 0.05).astype(np.float32), acts(g, D)
+    R, d = ctx.upload(r, ggml.F32, E, D), DeviceArray.from_numpy(x)
+    for accumulate in (True, False):
+        now = d.numpy()
+        ids, p = route(r.astype(np.float64) @ now.astype(np.float64), k, True)
+        _, ref, bound = expert_ref(w, now, ids, p, F, 0)
+        ctx.moe_forward(d, d, R, GU, DN, k, F, norm_topk=True, accumulate=accumulate, unfused=unfused)
+        ctx.sync()
+        want = ref + now if accumulate else ref
+        slack = 2 * (D * 2.0 ** -24 * (np.abs(r.astype(np.float64)) @ np.abs(now)).max() + 2.0 ** -20)  # the weights', as in the layer's tests
+        close(d.numpy(), want, bound + slack * np.abs(ref) + slack * sum(q * np.abs(w["dn"][e]).sum(1) for e, q in zip(ids, p))
+              + 2.0 ** -23 * (np.abs(now) + np.abs(ref)))
+    for t in (GU, DN, R, d):
+        t.free()
