@@ -10,11 +10,11 @@
 // products; the instructions alone, their operands held in registers, take 238
 // us at the clock that the card holds under them (5.8 PFLOP/s; 8.9 with
 // constant operands), the product with its loads from LDS 253 us, the whole
-// kernel 294 us, and the limbs 21 us before it (130 MB, 6.2 TB/s).  With 4-bit X
-// 82 us, of which the instructions alone take 61.  Middle sizes are bound by how
-// their tiles fall on the CUs: 509 x 4864 x 2816 is 152 of them on 256 CUs, 26 us
-// and the limbs 6 (smaller tiles, which need more waves or leave a SIMD with one,
-// 32.5 to 56 us in all against 31.6).
+// kernel 294 to 309 us (cards differ), and the limbs 21 us before it (130 MB, 6.2
+// TB/s).  With 4-bit X 82 us, of which the instructions alone take 61.  Middle sizes
+// are bound by how their tiles fall on the CUs: 509 x 4864 x 2816 is 152 of them on
+// 256 CUs, 27 us and the limbs 7 (smaller tiles, which need more waves or leave a
+// SIMD with one, 32.5 to 56 us in all against 31.6).
 //
 // What made it fast, on that size: both operands through LDS by direct loads
 // instead of registers (1570 -> 335 us); uniform addresses that move on by one

@@ -3,8 +3,8 @@
 //
 // Bound by the weights' bytes (262144 x 2816, 392 MB: 65 us, 6.0 TB/s), and where
 // there are few of those by the chain launch - vector - product - sum over the
-// waves: 4096 x 4096 4.9 us a graph's node, of which an empty one has 1.8 and the
-// loads alone 4.4; 4865 x 896 3.6.  A workgroup converts the vector once, while its
+// waves: 4096 x 4096 4.9 to 5.2 us a graph's node (cards differ), of which an empty
+// one has 1.8 and, at 4.9, the loads alone 4.4; 4865 x 896 3.6 to 4.0.  A workgroup converts the vector once, while its
 // first weights are on their way.  A tile's rows are split over S waves, 16 blocks
 // (a scale word) at a time; what they summed meets in LDS in the waves' order.
 #include "llmtoy_hip.h"
@@ -292,6 +292,9 @@ static hipError_t launch_matvec(const DevTensor &W, const float *x, float *y, hi
 
 hipError_t launch_matvec_mx(const DevTensor &W, const float *x, float *y, hipStream_t s) { return launch_matvec<1>(W, x, y, s); }
 
+// Vectors whose parts fit the LDS together (768 B a vector for 128 columns).  At the edge, 4096
+// rows, this | limbs and the thin product for 32 columns more: 2 of 10880 10.2 | 16.3 us, 3 of
+// 7168 8.5 | 13.3, 4 of 5376 8.0 | 11.6, 5 of 4352 7.8 | 10.5.
 bool matvecs_mx_fit(const DevTensor &W, size_t T) {
     return T <= kMxFew && !W.beyond && T * mx_vec_bytes(mx_dims(W.rows, W.blocks_per_row).kg) <= (128 << 10);
 }
