@@ -89,7 +89,7 @@ __device__ __forceinline__ bool mx_await(const uint64_t *p, uint32_t stride, uin
 }
 // What a wait that ran out was for, in the error word (each bit's meaning stands in its text).
 enum : uint32_t { kMxGateLogits = 1, kMxDownLogits = 2, kMxH = 4, kMxRows = 8 };
-// (Which word was late, and its tag, are not recorded: every form of that cost 0.1 to 0.25
+// (Which word was late, and its tag, are not recorded: every form of that cost 0.2 to 0.3
 // us a layer where nothing is late.)
 __device__ __forceinline__ void mx_late(const MxLayer &a, uint32_t what, uint32_t ep, int lane) {
     if (lane) return;
