@@ -390,6 +390,139 @@ int lt_gemma4_moe_block(lt_ctx *ctx, float *x, const float *dense_ffn, const lt_
                         const float *post_ffw_norm, float layer_output_scale, float eps, uint32_t k,
                         uint32_t d_expert, uint32_t act, uint32_t flags, uint32_t *out_ids, float *out_w);
 
+/* ---- Attention of a decode step or a prompt (between the QKV products and the output product) ----
+ * Queries, keys and values are fp32, a head's head_dim elements in a row, the
+ * heads of a token one after the other, tokens a stride apart (counted in
+ * floats; 0: the heads' own length), so that they may be read where a fused
+ * projection left them.  Device pointers must be 16-byte aligned and strides
+ * multiples of 4 where not said otherwise.  One call is one layer.
+ *
+ * The cache is made of blocks of LT_KV_BLOCK tokens that belong to one sequence
+ * each; any free block may be a sequence's next one (block tables).  Keys and
+ * values are held in 8 bits: for each block and head, keys and values have a scale
+ * s = max |x| / 127 over the block's tokens so far (fp32) and a code
+ * round(x / s), a tie to the even one, an element.  The tokens of a sequence's last two
+ * blocks are kept in fp32 beside it, so that a block is always coded from its
+ * tokens: what the cache holds does not depend on how many came at a time.  A
+ * block and head with a NaN or an infinity among its keys (values) becomes all
+ * NaN there.
+ *
+ * Lengths, tables and maps are device arrays that kernels read, so a captured
+ * decode step may be replayed as sequences grow.  What is wrong with them is found
+ * on the device, by bounds checks: the calls below say what becomes of the
+ * sequences concerned, the others are served, and the next lt_sync (or
+ * LT_HOST_IO call) returns LT_ERR_DEVICE with the reason. */
+enum { LT_KV_BLOCK = 32 };
+#define LT_KV_NONE 0xffffffffu /* no block, no slot */
+
+/* Rotation of pairs of a head's first n_rot elements: (i, i + n_rot / 2), or
+ * (2 i, 2 i + 1) (rope.zig:14-77: NeoX and normal). */
+enum { LT_ROPE_NEOX = 0, LT_ROPE_PAIRS = 1 };
+
+enum { LT_ROPE_NO_NORM = 1u << 7 }; /* lt_qk_norm_rope: rotate only */
+
+typedef struct lt_rope lt_rope;
+typedef struct lt_kv lt_kv;
+
+/* A batch: the tokens start[i] .. start[i + 1] - 1 of the arrays are sequence
+ * i's last ones, at the positions len[i] - (start[i + 1] - start[i]) .. len[i] - 1;
+ * position p lies in block table[i * max_blocks + p / LT_KV_BLOCK].  start does not
+ * fall and ends at n_tokens or before; tokens behind the last sequence belong to nobody
+ * and are left alone.  A sequence with no token in the batch is idle.  The pointers are
+ * host memory with LT_HOST_IO, device memory (4-byte aligned) otherwise. */
+typedef struct {
+    uint32_t n_seqs;     /* 1 .. 4096 */
+    uint32_t n_tokens;   /* tokens that the arrays have room for, up to 2^24 */
+    uint32_t max_blocks; /* entries of a sequence's row of table, up to 2^24 */
+    uint32_t max_new;    /* no sequence has more tokens than this in the batch (1: a decode step); 0: not known */
+    uint32_t *start;     /* [n_seqs + 1] */
+    uint32_t *len;       /* [n_seqs] */
+    uint32_t *table;     /* [n_seqs][max_blocks] */
+} lt_kv_batch;
+
+/* What lt_qk_norm_rope rotates by: pair i turns by
+ * position * base^(-2 i / n_rot) / freq_factors[i] (host array of n_rot / 2
+ * positive values, an infinity for a pair that stays; NULL: all 1).  head_dim: even, up
+ * to 512; n_rot: even, 0 .. head_dim (elements from n_rot on are only
+ * normalised).  Not while the stream is captured.  Replaces rope.zig's tables. */
+int lt_rope_create(lt_ctx *ctx, uint32_t head_dim, uint32_t n_rot, double base, const float *freq_factors,
+                   uint32_t style, lt_rope **out_rope);
+int lt_rope_free(lt_ctx *ctx, lt_rope *rope);
+
+/* The norms of queries and keys for each head and the position rotation in one
+ * pass: y = rotate(x * rms_inv * w), with rms_inv = 1 / sqrt(mean(x^2) + eps) over
+ * the head and w = wq or wk [head_dim] (NULL: not multiplied; device pointers of any
+ * alignment).  q, q_out: n_tokens x n_heads heads; k, k_out: n_tokens x n_kv_heads
+ * (either number may be 0, then its pointers are not used).  positions:
+ * [n_tokens].  Outputs may be their inputs where the strides are alike; otherwise they must
+ * not overlap.  Angles are taken in 64 bits, so positions up to 2^32 - 1 keep fp32's
+ * accuracy.  Pointers need 4-byte alignment (16, with strides of whole 4 floats and
+ * head_dim and n_rot of whole 8, are faster).  flags: LT_HOST_IO,
+ * LT_NORM_ONE_PLUS_W, LT_ROPE_NO_NORM.  Replaces the per-head norms and rotations of
+ * gemma4/forward.zig (rmsnorm_perhead, rope_* pipelines). */
+int lt_qk_norm_rope(lt_ctx *ctx, float *q_out, float *k_out, const float *q, const float *k, const float *wq,
+                    const float *wk, const uint32_t *positions, const lt_rope *rope, uint32_t n_tokens,
+                    uint32_t n_heads, uint32_t n_kv_heads, size_t q_stride, size_t k_stride, size_t q_out_stride,
+                    size_t k_out_stride, float eps, uint32_t flags);
+
+/* A cache of n_blocks blocks for one layer, for up to n_seqs sequences (the rows
+ * of a batch).  head_dim: 64, 96, 128, 192, 256 or 512; n_kv_heads: 1 .. 256.  Not while the stream
+ * is captured.  Replaces KvCache (model/kv_cache.zig, gemma4/kv_cache.zig). */
+int lt_kv_create(lt_ctx *ctx, uint32_t n_blocks, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_seqs,
+                 lt_kv **out_kv);
+int lt_kv_free(lt_ctx *ctx, lt_kv *kv);
+/* Device bytes of the cache: codes, scales, and the fp32 tokens of the last two blocks. */
+size_t lt_kv_bytes(const lt_kv *kv);
+
+/* One step's batch from the lengths of its sequences: sequence i holds len_in[i]
+ * tokens and gets n_new[i] more (0: idle).
+ *   batch->start, batch->len  the batch's layout, tokens in the order of the sequences
+ *   batch->table              blocks for the new tokens: the sequences in order take those
+ *                             of free_blocks from entry used_in[0] on; other entries stay
+ *   used_out[0]               entries of free_blocks taken so far
+ *   positions, slots          [batch->n_tokens]: each token's position, and block *
+ *                             LT_KV_BLOCK + offset (tokens behind the last sequence: 0 and LT_KV_NONE)
+ * len_in may be batch->len and used_in used_out: a replayed graph then moves on by
+ * itself.  A sequence whose blocks free_blocks does not have, or whose row of the
+ * table is full, gets LT_KV_NONE for all its new blocks and its tokens there, and so do the later
+ * ones that need blocks; its length counts on (the caller that is told sets it
+ * back).  Tokens beyond n_tokens have no place in the maps.  Both are reported.
+ * flags: LT_HOST_IO. */
+int lt_kv_plan(lt_ctx *ctx, const lt_kv_batch *batch, const uint32_t *len_in, const uint32_t *n_new,
+               const uint32_t *free_blocks, uint32_t n_free, const uint32_t *used_in, uint32_t *used_out,
+               uint32_t *positions, uint32_t *slots, uint32_t flags);
+
+/* The batch's tokens into the cache: k, v n_tokens x n_kv_heads heads.  Where a sequence's
+ * tokens begin inside a block, that block's earlier tokens are taken from their
+ * fp32 copies, which are there for the last two blocks that were appended to: a
+ * sequence may be shortened (len set back) by up to LT_KV_BLOCK tokens, or to the start of any block, and go
+ * on from there (until then its last block stays coded beside the tokens taken back).  A block that is appended to must be in one sequence's table only; full
+ * blocks may be shared.  Codes, scales and copies of the tokens appended are
+ * written, nothing else.  A sequence that contradicts itself (more tokens than len, ...) or has more than
+ * max_new of them is left out and reported; a block that is not in the cache
+ * is not written, a block whose earlier tokens are not held becomes all NaN, both are reported.
+ * flags: LT_HOST_IO. */
+int lt_kv_append(lt_ctx *ctx, lt_kv *kv, const float *k, const float *v, size_t k_stride, size_t v_stride,
+                 const lt_kv_batch *batch, uint32_t flags);
+/* The values that n slots stand for (lt_kv_plan's slots, or block * LT_KV_BLOCK +
+ * offset): k_out, v_out [n][n_kv_heads][head_dim].  A slot outside the cache gives
+ * NaN.  flags: LT_HOST_IO (slots and outputs are host memory). */
+int lt_kv_read(lt_ctx *ctx, float *k_out, float *v_out, const lt_kv *kv, const uint32_t *slots, uint32_t n,
+               uint32_t flags);
+
+/* out [n_tokens][n_heads][head_dim]: for each query of the batch, at position p of
+ * its sequence, softmax(scale * q k^T) v over the keys at positions 0 .. p, or
+ * max(0, p - window + 1) .. p with window > 0.  The batch's own tokens have been appended.
+ * q: n_tokens x n_heads heads; heads h * n_heads / n_kv_heads .. share the cache's head
+ * h (n_heads up to 128 times n_kv_heads).  Products take queries and weights to 2^-22 of the largest of a
+ * row and are summed in fp32.  NaN comes out where a query, or a key or value that it sees, is not finite (a block
+ * is all NaN then); what it does not see changes nothing.  Where the table has no block of the cache for a key,
+ * the queries that see it get NaN; so do the tokens of a sequence that contradicts itself (those
+ * beyond max_new: are left as they were); both are reported.  out must not overlap q.  flags:
+ * LT_HOST_IO.  Replaces sdpAttn (ops/attn.zig:13-44) over all heads, and the attn_* pipelines. */
+int lt_attention(lt_ctx *ctx, float *out, const float *q, const lt_kv *kv, const lt_kv_batch *batch,
+                 uint32_t n_heads, size_t q_stride, float scale, uint32_t window, uint32_t flags);
+
 #ifdef __cplusplus
 }
 #endif

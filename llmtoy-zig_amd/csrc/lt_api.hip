@@ -2,8 +2,10 @@
 // into the planar device layout, argument validation, and kernel dispatch.
 #include "llmtoy_hip.h"
 #include "lt_internal.h"
+#include "lt_kv.h"
 #include "lt_mx.h"
 
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -19,6 +21,15 @@ using lt::DevTensor;
 
 struct lt_tensor {
     DevTensor t;
+};
+
+struct lt_rope {
+    lt::RopeDev r;
+};
+
+struct lt_kv {
+    lt::KvDev d;
+    size_t bytes;
 };
 
 namespace {
@@ -64,7 +75,7 @@ struct lt_ctx {
     hipStream_t stream = nullptr;
     std::string err;
     // context-owned device scratch, grown on demand
-    DevBuf x, out, logits, h, ids, w, shared, g, u, ids_io, w_io, bias, eh, pf, nrm, sink, mx;
+    DevBuf x, out, logits, h, ids, w, shared, g, u, ids_io, w_io, bias, eh, pf, nrm, sink, mx, attn, attn_io;
     // buffers replaced by larger ones; a HIP graph captured earlier may still
     // reference them, so they are released only by lt_destroy
     std::vector<void *> retired;
@@ -554,6 +565,33 @@ hipError_t init_device_state(lt_ctx *ctx) {
     return hipSuccess;
 }
 
+// What the cache's kernels found wrong with a batch (lt_kv.h, KvErr): reported,
+// and cleared, by the next synchronising call.
+int check_kv_err(lt_ctx *ctx) {
+    if (!ctx->fused_err) return LT_OK;
+    static const char *const what[] = {
+        "plan: no blocks left in the free list, or no room in the table's row",
+        "plan: more tokens than the maps have room for",
+        "the table has no block of the cache for a token",
+        "append: the block's earlier tokens are not held (shortened too far, or never appended)",
+        "the batch contradicts itself: start falls or passes n_tokens, len is less than the tokens or more than the "
+        "table holds, or more tokens than max_new",
+    };
+    std::string text;
+    for (int k = lt::kKvErrPool; k < lt::kKvErrEnd; k++) {
+        const uint32_t row = __atomic_exchange_n(ctx->fused_err + k, 0u, __ATOMIC_SEQ_CST);
+        if (!row) continue;
+        char buf[240];
+        snprintf(buf, sizeof buf, "%ssequence %u: %s", text.empty() ? "" : "; ", row - 1, what[k - lt::kKvErrPool]);
+        try {
+            text += buf;
+        } catch (...) {
+            return fail(ctx, LT_ERR_OOM, "host allocation failed");
+        }
+    }
+    return text.empty() ? LT_OK : fail(ctx, LT_ERR_DEVICE, "%s", text.c_str());
+}
+
 // A fused-kernel wait that ran into its time limit (the outputs of that
 // call are NaN); reported, and cleared, by the next synchronising call.
 int check_fused_err(lt_ctx *ctx) {
@@ -659,7 +697,7 @@ extern "C" void lt_destroy(lt_ctx *ctx) {
     (void)hipStreamSynchronize(ctx->stream);
     DevBuf *bufs[] = {&ctx->x, &ctx->out, &ctx->logits, &ctx->h, &ctx->ids, &ctx->w,
                       &ctx->shared, &ctx->g, &ctx->u, &ctx->ids_io, &ctx->w_io, &ctx->bias, &ctx->eh, &ctx->pf,
-                      &ctx->nrm, &ctx->sink, &ctx->mx};
+                      &ctx->nrm, &ctx->sink, &ctx->mx, &ctx->attn, &ctx->attn_io};
     for (DevBuf *b : bufs)
         if (b->p) (void)hipFree(b->p);
     for (void *p : ctx->retired) (void)hipFree(p);
@@ -687,7 +725,9 @@ extern "C" int lt_sync(lt_ctx *ctx) {
     int rc = host_sync(ctx);
     if (rc) return rc;
     prof_harvest(ctx);
-    return check_fused_err(ctx);
+    const int kv = check_kv_err(ctx);
+    rc = check_fused_err(ctx);
+    return rc ? rc : kv;
 }
 
 extern "C" void *lt_stream(lt_ctx *ctx) { return ctx ? (void *)ctx->stream : nullptr; }
@@ -1809,6 +1849,377 @@ extern "C" int lt_gemma4_moe_block(lt_ctx *ctx, float *x, const float *dense_ffn
         prof_harvest(ctx);
     }
     return LT_OK;
+}
+
+// ------------------------------------------------------------------ attention
+namespace {
+
+// The context's device as the current one for a call; the caller's afterwards.
+struct OnDevice {
+    int before = -1;
+    hipError_t e;
+    explicit OnDevice(const lt_ctx *ctx) {
+        e = hipGetDevice(&before);
+        if (e == hipSuccess && before != ctx->device) e = hipSetDevice(ctx->device);
+        else before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// Host arrays of a LT_HOST_IO call in ctx->attn_io: rows of `width` floats (or
+// words), `pitch` apart on the host, packed on the device.
+struct HostArrays {
+    struct Item {
+        void *host;
+        size_t width, pitch, rows, at;
+    };
+    lt_ctx *ctx;
+    Item items[12];
+    int n = 0;
+    size_t bytes = 0;
+    explicit HostArrays(lt_ctx *c) : ctx(c) {}
+    int add(const void *host, size_t rows, size_t width, size_t pitch = 0) {
+        items[n] = {const_cast<void *>(host), width * 4, (pitch ? pitch : width) * 4, rows, bytes};
+        bytes += (rows * width * 4 + 255) & ~(size_t)255;
+        return n++;
+    }
+    int open() { return ensure(ctx, ctx->attn_io, bytes); }
+    template <typename T>
+    T *dev(int i) const {
+        return items[i].host ? reinterpret_cast<T *>((uint8_t *)ctx->attn_io.p + items[i].at) : nullptr;
+    }
+    int copy(int i, bool in) {
+        const Item &t = items[i];
+        if (!t.host || !t.rows || !t.width) return LT_OK;
+        void *d = dev<uint8_t>(i);
+        if (t.pitch == t.width) {
+            LT_HIP(ctx, hipMemcpyAsync(in ? d : t.host, in ? t.host : d, t.rows * t.width,
+                                       in ? hipMemcpyHostToDevice : hipMemcpyDeviceToHost, ctx->stream));
+        } else {
+            LT_HIP(ctx, hipMemcpy2DAsync(in ? d : t.host, in ? t.width : t.pitch, in ? t.host : d, in ? t.pitch : t.width,
+                                         t.width, t.rows, in ? hipMemcpyHostToDevice : hipMemcpyDeviceToHost, ctx->stream));
+        }
+        return LT_OK;
+    }
+    int finish() {
+        const int rc = host_sync(ctx);
+        if (rc) return rc;
+        prof_harvest(ctx);
+        return check_kv_err(ctx);
+    }
+};
+
+int check_flags(lt_ctx *ctx, uint32_t flags, uint32_t allowed) {
+    return flags & ~allowed ? fail(ctx, LT_ERR_INVALID, "unknown flags 0x%x", flags & ~allowed) : LT_OK;
+}
+
+// A token's stride (0: packed) against its heads' own length.
+int check_stride(lt_ctx *ctx, const char *what, size_t &stride, size_t own) {
+    if (stride == 0) stride = own;
+    if (stride < own || stride > ((size_t)1 << 32))
+        return fail(ctx, LT_ERR_INVALID, "%s: a stride of %zu floats for %zu a token", what, stride, own);
+    return LT_OK;
+}
+
+int check_batch(lt_ctx *ctx, const lt_kv_batch *b, uint32_t flags) {
+    if (!b || !b->start || !b->len || !b->table) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (b->n_seqs == 0 || b->n_seqs > lt::kKvMaxSeqs)
+        return fail(ctx, LT_ERR_INVALID, "batch: n_seqs=%u out of range (1..%u)", b->n_seqs, lt::kKvMaxSeqs);
+    if (b->n_tokens > lt::kKvMaxTokens)
+        return fail(ctx, LT_ERR_INVALID, "batch: n_tokens=%u out of range (0..%u)", b->n_tokens, lt::kKvMaxTokens);
+    if (b->max_blocks == 0 || b->max_blocks > (1u << 24))
+        return fail(ctx, LT_ERR_INVALID, "batch: max_blocks=%u out of range (1..%u)", b->max_blocks, 1u << 24);
+    if (!(flags & LT_HOST_IO) && (((uintptr_t)b->start | (uintptr_t)b->len | (uintptr_t)b->table) & 3u))
+        return fail(ctx, LT_ERR_INVALID, "batch: arrays must be 4-byte aligned");
+    return LT_OK;
+}
+
+lt::KvBatchDev batch_dev(const lt_kv_batch &b) {
+    return {b.n_seqs, b.n_tokens, b.max_blocks, b.max_new, b.start, b.len, b.table};
+}
+
+// The batch's arrays as inputs of a LT_HOST_IO call: their places, then (staged) the device's.
+struct HostBatch {
+    int start, len, table;
+    HostBatch(HostArrays &io, const lt_kv_batch &b)
+        : start(io.add(b.start, 1, (size_t)b.n_seqs + 1)), len(io.add(b.len, 1, b.n_seqs)),
+          table(io.add(b.table, 1, (size_t)b.n_seqs * b.max_blocks)) {}
+    int stage(HostArrays &io, lt::KvBatchDev &d) const {
+        int rc;
+        if ((rc = io.copy(start, true)) || (rc = io.copy(len, true)) || (rc = io.copy(table, true))) return rc;
+        d.start = io.dev<uint32_t>(start), d.len = io.dev<uint32_t>(len), d.table = io.dev<uint32_t>(table);
+        return LT_OK;
+    }
+};
+
+}  // namespace
+
+extern "C" int lt_rope_create(lt_ctx *ctx, uint32_t head_dim, uint32_t n_rot, double base, const float *freq_factors,
+                              uint32_t style, lt_rope **out_rope) {
+    if (!ctx || !out_rope) return fail(ctx, LT_ERR_INVALID, "null argument");
+    *out_rope = nullptr;
+    if (head_dim == 0 || head_dim % 2 || head_dim > 512)
+        return fail(ctx, LT_ERR_UNSUPPORTED, "rope: head_dim %u (device path: even, 2..512)", head_dim);
+    if (n_rot % 2 || n_rot > head_dim) return fail(ctx, LT_ERR_INVALID, "rope: n_rot %u of head_dim %u", n_rot, head_dim);
+    if (!(base > 0.0) || base > 1e300) return fail(ctx, LT_ERR_INVALID, "rope: base must be positive and finite");
+    if (style != LT_ROPE_NEOX && style != LT_ROPE_PAIRS) return fail(ctx, LT_ERR_INVALID, "rope: unknown style %u", style);
+    if (capturing(ctx)) return fail(ctx, LT_ERR_INVALID, "a rotation cannot be made while the stream is captured");
+    double turns[256];
+    for (uint32_t i = 0; i < n_rot / 2; i++) {
+        const double f = freq_factors ? (double)freq_factors[i] : 1.0;
+        if (!(f > 0.0)) return fail(ctx, LT_ERR_INVALID, "rope: frequency factor %u must be positive", i);
+        turns[i] = pow(base, -2.0 * i / n_rot) / f / 6.283185307179586477;
+        if (!(turns[i] <= 1e12)) return fail(ctx, LT_ERR_INVALID, "rope: pair %u turns too fast", i);
+    }
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    lt_rope *r = new (std::nothrow) lt_rope{{nullptr, head_dim, n_rot, style}};
+    if (!r) return fail(ctx, LT_ERR_OOM, "host allocation failed");
+    void *p = nullptr;
+    hipError_t e = hipMalloc(&p, sizeof turns);
+    if (e == hipSuccess) e = hipMemcpy(p, turns, sizeof turns, hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        if (p) (void)hipFree(p);
+        delete r;
+        return hip_fail(ctx, e, "rotation table");
+    }
+    r->r.turns = (const double *)p;
+    *out_rope = r;
+    return LT_OK;
+}
+
+extern "C" int lt_rope_free(lt_ctx *ctx, lt_rope *rope) {
+    if (!rope) return LT_OK;
+    if (ctx) (void)hipStreamSynchronize(ctx->stream);
+    (void)hipFree(const_cast<double *>(rope->r.turns));
+    delete rope;
+    return LT_OK;
+}
+
+extern "C" int lt_qk_norm_rope(lt_ctx *ctx, float *q_out, float *k_out, const float *q, const float *k, const float *wq,
+                               const float *wk, const uint32_t *positions, const lt_rope *rope, uint32_t n_tokens,
+                               uint32_t n_heads, uint32_t n_kv_heads, size_t q_stride, size_t k_stride,
+                               size_t q_out_stride, size_t k_out_stride, float eps, uint32_t flags) {
+    if (!ctx || !rope || (n_tokens && !positions)) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (n_tokens && ((n_heads && (!q || !q_out)) || (n_kv_heads && (!k || !k_out)))) return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_flags(ctx, flags, LT_HOST_IO | LT_NORM_ONE_PLUS_W | LT_ROPE_NO_NORM);
+    if (rc) return rc;
+    if (!(eps >= 0.0f) || eps > 1.0f) return fail(ctx, LT_ERR_INVALID, "eps must be in [0, 1]");
+    if (n_tokens > lt::kKvMaxTokens) return fail(ctx, LT_ERR_INVALID, "n_tokens=%u out of range (0..%u)", n_tokens, lt::kKvMaxTokens);
+    if (n_heads > 1024 || n_kv_heads > 1024) return fail(ctx, LT_ERR_INVALID, "%u and %u heads (up to 1024)", n_heads, n_kv_heads);
+    const uint32_t D = rope->r.D;
+    const size_t qw = (size_t)n_heads * D, kw = (size_t)n_kv_heads * D;
+    if ((rc = check_stride(ctx, "q", q_stride, qw)) || (rc = check_stride(ctx, "k", k_stride, kw)) ||
+        (rc = check_stride(ctx, "q_out", q_out_stride, qw)) || (rc = check_stride(ctx, "k_out", k_out_stride, kw)))
+        return rc;
+    if (n_tokens == 0 || (n_heads == 0 && n_kv_heads == 0)) return LT_OK;
+    if (n_heads == 0) q = nullptr, q_out = nullptr, wq = nullptr, q_stride = q_out_stride = 0;
+    if (n_kv_heads == 0) k = nullptr, k_out = nullptr, wk = nullptr, k_stride = k_out_stride = 0;
+    const bool host = flags & LT_HOST_IO;
+    if (!host) {
+        const void *ptr[] = {q, k, wq, wk, positions, q_out, k_out};
+        for (const void *p : ptr)
+            if ((uintptr_t)p & 3u) return fail(ctx, LT_ERR_INVALID, "arrays must be 4-byte aligned");
+    }
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    Span span_(ctx, "lt_qk_norm_rope");
+    const bool norm = !(flags & LT_ROPE_NO_NORM), one = flags & LT_NORM_ONE_PLUS_W;
+    if (!host) {
+        const size_t st[4] = {q_stride, k_stride, q_out_stride, k_out_stride};
+        return launch_rc(ctx, lt::launch_qk_norm_rope(rope->r, q_out, k_out, q, k, wq, wk, positions, n_tokens, n_heads,
+                                                      n_kv_heads, st, eps, norm, one, ctx->stream), "qk_norm_rope");
+    }
+    HostArrays io(ctx);
+    const int iq = io.add(q, n_tokens, qw, q_stride), ik = io.add(k, n_tokens, kw, k_stride);
+    const int iwq = io.add(wq, 1, D), iwk = io.add(wk, 1, D), ip = io.add(positions, 1, n_tokens);
+    const int oq = io.add(q_out, n_tokens, qw, q_out_stride), ok = io.add(k_out, n_tokens, kw, k_out_stride);
+    if ((rc = io.open())) return rc;
+    for (int i : {iq, ik, iwq, iwk, ip})
+        if ((rc = io.copy(i, true))) return rc;
+    const size_t st[4] = {qw, kw, qw, kw};
+    if ((rc = launch_rc(ctx, lt::launch_qk_norm_rope(rope->r, io.dev<float>(oq), io.dev<float>(ok), io.dev<float>(iq),
+                                                     io.dev<float>(ik), io.dev<float>(iwq), io.dev<float>(iwk),
+                                                     io.dev<uint32_t>(ip), n_tokens, n_heads, n_kv_heads, st, eps, norm, one,
+                                                     ctx->stream), "qk_norm_rope")) ||
+        (rc = io.copy(oq, false)) || (rc = io.copy(ok, false)))
+        return rc;
+    return io.finish();
+}
+
+extern "C" int lt_kv_create(lt_ctx *ctx, uint32_t n_blocks, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_seqs,
+                            lt_kv **out_kv) {
+    if (!ctx || !out_kv) return fail(ctx, LT_ERR_INVALID, "null argument");
+    *out_kv = nullptr;
+    if (!lt::attention_head_dim(head_dim))
+        return fail(ctx, LT_ERR_UNSUPPORTED, "cache: head_dim %u (device path: 64, 96, 128, 192, 256, 512)", head_dim);
+    if (n_kv_heads == 0 || n_kv_heads > 256) return fail(ctx, LT_ERR_INVALID, "cache: n_kv_heads=%u out of range (1..256)", n_kv_heads);
+    if (n_blocks == 0 || n_blocks >= lt::kKvNone / lt::kKvBlock)
+        return fail(ctx, LT_ERR_INVALID, "cache: n_blocks=%u out of range", n_blocks);
+    if (n_seqs == 0 || n_seqs > lt::kKvMaxSeqs)
+        return fail(ctx, LT_ERR_INVALID, "cache: n_seqs=%u out of range (1..%u)", n_seqs, lt::kKvMaxSeqs);
+    if (capturing(ctx)) return fail(ctx, LT_ERR_INVALID, "a cache cannot be made while the stream is captured");
+    const auto round = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t bh = (size_t)n_blocks * n_kv_heads, sh = (size_t)n_seqs * n_kv_heads;
+    const size_t codes = round(bh * 2 * lt::kKvBlock * head_dim), scales = round(bh * sizeof(float2));
+    const size_t open = round(sh * 4 * lt::kKvBlock * head_dim * 4), tags = round(sh * 4 * sizeof(uint2));
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    lt_kv *kv = new (std::nothrow) lt_kv{};
+    if (!kv) return fail(ctx, LT_ERR_OOM, "host allocation failed");
+    uint8_t *p = nullptr;
+    hipError_t e = hipMalloc((void **)&p, codes + scales + open + tags);
+    // no token is held yet; behind what is enqueued, and waited for
+    if (e == hipSuccess) e = hipMemsetAsync(p + codes + scales + open, 0, tags, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        if (p) (void)hipFree(p);
+        delete kv;
+        return hip_fail(ctx, e, "cache");
+    }
+    kv->bytes = codes + scales + open + tags;
+    kv->d = {p, (float2 *)(p + codes), (float *)(p + codes + scales), (uint2 *)(p + codes + scales + open),
+             n_blocks, n_kv_heads, head_dim, n_seqs};
+    *out_kv = kv;
+    return LT_OK;
+}
+
+extern "C" int lt_kv_free(lt_ctx *ctx, lt_kv *kv) {
+    if (!kv) return LT_OK;
+    if (ctx) (void)hipStreamSynchronize(ctx->stream);
+    (void)hipFree(kv->d.codes);
+    delete kv;
+    return LT_OK;
+}
+
+extern "C" size_t lt_kv_bytes(const lt_kv *kv) { return kv ? kv->bytes : 0; }
+
+extern "C" int lt_kv_plan(lt_ctx *ctx, const lt_kv_batch *batch, const uint32_t *len_in, const uint32_t *n_new,
+                          const uint32_t *free_blocks, uint32_t n_free, const uint32_t *used_in, uint32_t *used_out,
+                          uint32_t *positions, uint32_t *slots, uint32_t flags) {
+    if (!ctx || !len_in || !n_new || (n_free && !free_blocks) || !used_in || !used_out)
+        return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_batch(ctx, batch, flags);
+    if (rc || (rc = check_flags(ctx, flags, LT_HOST_IO))) return rc;
+    const lt_kv_batch &b = *batch;
+    if (b.n_tokens && (!positions || !slots)) return fail(ctx, LT_ERR_INVALID, "null argument");
+    const bool host = flags & LT_HOST_IO;
+    if (!host) {
+        const void *ptr[] = {len_in, n_new, free_blocks, used_in, used_out, positions, slots};
+        for (const void *p : ptr)
+            if ((uintptr_t)p & 3u) return fail(ctx, LT_ERR_INVALID, "arrays must be 4-byte aligned");
+    }
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    Span span_(ctx, "lt_kv_plan");
+    lt::KvPlanArgs a{b.n_seqs, b.max_blocks, b.n_tokens, n_free, len_in, n_new, free_blocks, used_in,
+                     b.table, b.len, b.start, used_out, positions, slots, ctx->err_dev};
+    if (!host) return launch_rc(ctx, lt::launch_kv_plan(a, ctx->stream), "kv_plan");
+    HostArrays io(ctx);
+    const int il = io.add(len_in, 1, b.n_seqs), in = io.add(n_new, 1, b.n_seqs), iff = io.add(free_blocks, 1, n_free);
+    const int iu = io.add(used_in, 1, 1), it = io.add(b.table, 1, (size_t)b.n_seqs * b.max_blocks);
+    const int ol = io.add(b.len, 1, b.n_seqs), os = io.add(b.start, 1, (size_t)b.n_seqs + 1), ou = io.add(used_out, 1, 1);
+    const int op = io.add(positions, 1, b.n_tokens), osl = io.add(slots, 1, b.n_tokens);
+    if ((rc = io.open())) return rc;
+    for (int i : {il, in, iff, iu, it})
+        if ((rc = io.copy(i, true))) return rc;
+    a.len_in = io.dev<uint32_t>(il), a.n_new = io.dev<uint32_t>(in), a.free_blocks = io.dev<uint32_t>(iff);
+    a.used_in = io.dev<uint32_t>(iu), a.table = io.dev<uint32_t>(it), a.len = io.dev<uint32_t>(ol);
+    a.start = io.dev<uint32_t>(os), a.used = io.dev<uint32_t>(ou), a.pos = io.dev<uint32_t>(op), a.slot = io.dev<uint32_t>(osl);
+    if ((rc = launch_rc(ctx, lt::launch_kv_plan(a, ctx->stream), "kv_plan"))) return rc;
+    for (int i : {it, ol, os, ou, op, osl})
+        if ((rc = io.copy(i, false))) return rc;
+    return io.finish();
+}
+
+extern "C" int lt_kv_append(lt_ctx *ctx, lt_kv *kv, const float *k, const float *v, size_t k_stride, size_t v_stride,
+                            const lt_kv_batch *batch, uint32_t flags) {
+    if (!ctx || !kv) return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_batch(ctx, batch, flags);
+    if (rc || (rc = check_flags(ctx, flags, LT_HOST_IO))) return rc;
+    if (batch->n_tokens && (!k || !v)) return fail(ctx, LT_ERR_INVALID, "null argument");
+    if (batch->n_seqs > kv->d.n_seqs)
+        return fail(ctx, LT_ERR_INVALID, "append: %u sequences in a cache for %u", batch->n_seqs, kv->d.n_seqs);
+    const size_t width = (size_t)kv->d.n_kv * kv->d.D;
+    if ((rc = check_stride(ctx, "k", k_stride, width)) || (rc = check_stride(ctx, "v", v_stride, width))) return rc;
+    const bool host = flags & LT_HOST_IO;
+    if (!host && (!aligned16(k) || !aligned16(v) || k_stride % 4 || v_stride % 4))
+        return fail(ctx, LT_ERR_INVALID, "k and v must be 16-byte aligned, their strides multiples of 4");
+    if (batch->n_tokens == 0) return LT_OK;
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    Span span_(ctx, "lt_kv_append");
+    lt::KvBatchDev b = batch_dev(*batch);
+    if (!host) return launch_rc(ctx, lt::launch_kv_append(kv->d, b, k, v, k_stride, v_stride, ctx->err_dev, ctx->stream), "kv_append");
+    HostArrays io(ctx);
+    const int ik = io.add(k, b.n_tokens, width, k_stride), iv = io.add(v, b.n_tokens, width, v_stride);
+    const HostBatch hb(io, *batch);
+    if ((rc = io.open()) || (rc = io.copy(ik, true)) || (rc = io.copy(iv, true)) || (rc = hb.stage(io, b))) return rc;
+    if ((rc = launch_rc(ctx, lt::launch_kv_append(kv->d, b, io.dev<float>(ik), io.dev<float>(iv), width, width, ctx->err_dev,
+                                                  ctx->stream), "kv_append")))
+        return rc;
+    return io.finish();
+}
+
+extern "C" int lt_kv_read(lt_ctx *ctx, float *k_out, float *v_out, const lt_kv *kv, const uint32_t *slots, uint32_t n,
+                          uint32_t flags) {
+    if (!ctx || !kv || (n && (!k_out || !v_out || !slots))) return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_flags(ctx, flags, LT_HOST_IO);
+    if (rc) return rc;
+    if (n > lt::kKvMaxTokens) return fail(ctx, LT_ERR_INVALID, "n=%u out of range (0..%u)", n, lt::kKvMaxTokens);
+    const bool host = flags & LT_HOST_IO;
+    if (!host && (!aligned16(k_out) || !aligned16(v_out) || ((uintptr_t)slots & 3u)))
+        return fail(ctx, LT_ERR_INVALID, "outputs must be 16-byte aligned, slots 4-byte");
+    if (n == 0) return LT_OK;
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    Span span_(ctx, "lt_kv_read");
+    if (!host) return launch_rc(ctx, lt::launch_kv_read(kv->d, slots, n, k_out, v_out, ctx->stream), "kv_read");
+    HostArrays io(ctx);
+    const size_t width = (size_t)kv->d.n_kv * kv->d.D;
+    const int is = io.add(slots, 1, n), ok = io.add(k_out, n, width), ov = io.add(v_out, n, width);
+    if ((rc = io.open()) || (rc = io.copy(is, true))) return rc;
+    if ((rc = launch_rc(ctx, lt::launch_kv_read(kv->d, io.dev<uint32_t>(is), n, io.dev<float>(ok), io.dev<float>(ov), ctx->stream),
+                        "kv_read")) ||
+        (rc = io.copy(ok, false)) || (rc = io.copy(ov, false)))
+        return rc;
+    return io.finish();
+}
+
+extern "C" int lt_attention(lt_ctx *ctx, float *out, const float *q, const lt_kv *kv, const lt_kv_batch *batch,
+                            uint32_t n_heads, size_t q_stride, float scale, uint32_t window, uint32_t flags) {
+    if (!ctx || !kv) return fail(ctx, LT_ERR_INVALID, "null argument");
+    int rc = check_batch(ctx, batch, flags);
+    if (rc || (rc = check_flags(ctx, flags, LT_HOST_IO))) return rc;
+    if (batch->n_tokens && (!out || !q)) return fail(ctx, LT_ERR_INVALID, "null argument");
+    const uint32_t n_kv = kv->d.n_kv;
+    if (n_heads == 0 || n_heads % n_kv || n_heads / n_kv > 128)
+        return fail(ctx, LT_ERR_INVALID, "attention: %u heads over %u of the cache", n_heads, n_kv);
+    if (!(scale - scale == 0.0f)) return fail(ctx, LT_ERR_INVALID, "attention: scale must be finite");
+    const size_t width = (size_t)n_heads * kv->d.D;
+    if ((rc = check_stride(ctx, "q", q_stride, width))) return rc;
+    const bool host = flags & LT_HOST_IO;
+    if (!host && (!aligned16(out) || !aligned16(q) || q_stride % 4))
+        return fail(ctx, LT_ERR_INVALID, "out and q must be 16-byte aligned, q's stride a multiple of 4");
+    if (batch->n_tokens == 0) return LT_OK;
+    OnDevice dev(ctx);
+    LT_HIP(ctx, dev.e);
+    Span span_(ctx, "lt_attention");
+    lt::AttnArgs a{};
+    a.kv = kv->d, a.b = batch_dev(*batch), a.q = q, a.out = out, a.q_stride = q_stride;
+    a.n_heads = n_heads, a.group = n_heads / n_kv, a.window = window, a.scale = scale, a.err = ctx->err_dev;
+    if ((rc = ensure(ctx, ctx->attn, lt::attention_workspace(a)))) return rc;
+    a.work = ctx->attn.p;
+    if (!host) return launch_rc(ctx, lt::launch_attention(a, ctx->stream), "attention");
+    HostArrays io(ctx);
+    const int iq = io.add(q, a.b.n_tokens, width, q_stride), oo = io.add(out, a.b.n_tokens, width);
+    const HostBatch hb(io, *batch);
+    if ((rc = io.open()) || (rc = io.copy(iq, true)) || (rc = io.copy(oo, true)) || (rc = hb.stage(io, a.b))) return rc;
+    a.q = io.dev<float>(iq), a.out = io.dev<float>(oo), a.q_stride = width;
+    if ((rc = launch_rc(ctx, lt::launch_attention(a, ctx->stream), "attention")) || (rc = io.copy(oo, false))) return rc;
+    return io.finish();
 }
 
 // ------------------------------------------------------------------ profiling

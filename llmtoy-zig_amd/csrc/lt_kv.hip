@@ -1,0 +1,355 @@
+// lt_kv.hip -- block tables and slot maps from request lengths, and tokens into
+// and out of the 8-bit cache (layout: lt_kv.h).
+#include "llmtoy_hip.h"
+#include "lt_kv.h"
+
+namespace lt {
+
+namespace {
+
+// ------------------------------------------------------------------- the plan
+// With total = len + n_new of a row, it needs blocks for the indices
+// ceil(len / 32) .. ceil(total / 32) - 1; the rows take them from the free list in
+// order, and their tokens lie in the batch in order.  Both are prefix sums over
+// the rows, which one workgroup takes (kPlanRows a thread); new blocks and
+// tokens then look their row up in the sums.  Bound by its chain of latencies:
+// the lengths, the sums, the table's entry, the slot.
+constexpr uint32_t kPlanThreads = 1024, kPlanRows = kKvMaxSeqs / kPlanThreads;
+// Tokens of a batch that the one workgroup maps; more go to a grid of their own
+// behind it (k_kv_slots).
+constexpr uint32_t kPlanTokens = 2048;
+
+__device__ __forceinline__ uint32_t sat32(uint64_t v) { return v < kKvNone ? (uint32_t)v : kKvNone; }
+
+// The last row whose sum in first[0 .. n - 1] is <= u (first[0] = 0).
+__device__ __forceinline__ uint32_t plan_row(const uint32_t *first, uint32_t n, uint32_t u) {
+    uint32_t lo = 0, hi = n;  // first[lo] <= u < first[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (first[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ uint32_t plan_slot(const KvPlanArgs &a, uint32_t row, uint32_t pos) {
+    const uint32_t j = pos / kKvBlock;
+    const uint32_t b = j < a.max_blocks ? a.table[(size_t)row * a.max_blocks + j] : kKvNone;
+    return b < kKvNone / kKvBlock ? b * kKvBlock + pos % kKvBlock : kKvNone;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
+    __shared__ uint32_t s_first[kKvMaxSeqs], s_need[kKvMaxSeqs], s_block[kKvMaxSeqs], s_pos[kKvMaxSeqs];
+    __shared__ uint64_t s_wave[2][kPlanThreads / kWave];
+    __shared__ uint32_t s_used;
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const uint32_t used = a.used_in[0];
+    uint32_t len[kPlanRows], add[kPlanRows];
+    uint64_t tok = 0, need = 0;
+    for (uint32_t i = 0; i < kPlanRows; i++) {
+        const uint32_t r = tid * kPlanRows + i;
+        len[i] = r < a.n_seqs ? a.len_in[r] : 0;
+        add[i] = r < a.n_seqs ? a.n_new[r] : 0;
+        tok += add[i];
+        need += ((uint64_t)len[i] + add[i] + kKvBlock - 1) / kKvBlock - ((uint64_t)len[i] + kKvBlock - 1) / kKvBlock;
+    }
+    // sums before this thread's rows
+    uint64_t itok = tok, ineed = need;
+    for (int off = 1; off < kWave; off <<= 1) {
+        const uint64_t p = __shfl_up(itok, off, kWave), q = __shfl_up(ineed, off, kWave);
+        if ((int)lane >= off) itok += p, ineed += q;
+    }
+    if (lane == kWave - 1) s_wave[0][wave] = itok, s_wave[1][wave] = ineed;
+    if (tid == 0) s_used = used;
+    __syncthreads();  // (every length is read: len and len_in may be one array, so may used and used_in)
+    uint64_t btok = itok - tok, bneed = ineed - need;
+    for (uint32_t w = 0; w < wave; w++) btok += s_wave[0][w], bneed += s_wave[1][w];
+    uint64_t all = 0, fresh = 0;
+    for (uint32_t w = 0; w < kPlanThreads / kWave; w++) all += s_wave[0][w], fresh += s_wave[1][w];
+    uint32_t most = used;
+    for (uint32_t i = 0; i < kPlanRows; i++) {
+        const uint32_t r = tid * kPlanRows + i;
+        const uint64_t total = (uint64_t)len[i] + add[i];
+        const uint64_t b0 = ((uint64_t)len[i] + kKvBlock - 1) / kKvBlock, b1 = (total + kKvBlock - 1) / kKvBlock;
+        if (r < a.n_seqs) {
+            a.start[r] = sat32(btok);
+            a.len[r] = sat32(total);
+            s_first[r] = sat32(btok);
+            s_pos[r] = len[i];
+            s_need[r] = sat32(bneed);
+            const bool room = b1 <= a.max_blocks, served = room && used + bneed + (b1 - b0) <= a.n_free;
+            s_block[r] = served ? (uint32_t)b0 : kKvNone;
+            if (served) most = max(most, (uint32_t)(used + bneed + (b1 - b0)));
+            else if (b1 > b0) kv_report(a.err, kKvErrPool, r);
+            if (!served)  // (its new entries: nothing; the entries of a served row are written below)
+                for (uint64_t j = b0; j < b1 && j < a.max_blocks; j++) a.table[(size_t)r * a.max_blocks + j] = kKvNone;
+        }
+        btok += add[i];
+        bneed += b1 - b0;
+    }
+    atomicMax(&s_used, most);
+    __syncthreads();
+    if (tid == 0) {
+        a.start[a.n_seqs] = sat32(all);
+        a.used[0] = s_used;
+        if (all > a.n_tokens) kv_report(a.err, kKvErrRoom, a.n_seqs - 1);
+    }
+    const uint64_t left = used < a.n_free ? a.n_free - used : 0;  // (blocks beyond the list are nobody's)
+    const uint32_t blocks = (uint32_t)(fresh < left ? fresh : left);
+    for (uint32_t k = tid; k < blocks; k += kPlanThreads) {
+        const uint32_t r = plan_row(s_need, a.n_seqs, k), b0 = s_block[r];
+        if (b0 != kKvNone) a.table[(size_t)r * a.max_blocks + b0 + (k - s_need[r])] = a.free_blocks[used + k];
+    }
+    if (a.n_tokens > kPlanTokens) return;
+    __syncthreads();
+    __threadfence_block();
+    const uint32_t end = (uint32_t)(all < a.n_tokens ? all : a.n_tokens);
+    for (uint32_t t = tid; t < a.n_tokens; t += kPlanThreads) {
+        uint32_t pos = 0, slot = kKvNone;
+        if (t < end) {
+            const uint32_t r = plan_row(s_first, a.n_seqs, t);
+            pos = s_pos[r] + (t - s_first[r]);
+            slot = plan_slot(a, r, pos);
+        }
+        a.pos[t] = pos;
+        a.slot[t] = slot;
+    }
+}
+
+// The maps of a large batch.  A workgroup's tokens begin in the row that its
+// first wavefront finds and mostly end there; each thread goes on from it.
+__global__ __launch_bounds__(256) void k_kv_slots(KvPlanArgs a) {
+    const uint32_t t0 = blockIdx.x * 256, t = t0 + threadIdx.x;
+    uint32_t r = kv_row(a.n_seqs, t0, [&](uint32_t i) { return a.start[i]; });
+    if (t >= a.n_tokens) return;
+    uint32_t pos = 0, slot = kKvNone;
+    const uint32_t all = a.start[a.n_seqs];
+    if (t < all) {
+        uint32_t next = a.start[r + 1];
+        while (next <= t) next = a.start[++r + 1];  // (t < all: ends at the last row)
+        pos = a.len[r] - (next - t);
+        slot = plan_slot(a, r, pos);
+    }
+    a.pos[t] = pos;
+    a.slot[t] = slot;
+}
+
+// ------------------------------------------------------------------- appending
+// A (sequence, block) that the batch touches is one unit; unit u belongs to the
+// last row with first / 32 + 2 r <= u, which leaves every row as many units as
+// its tokens can touch blocks.
+__host__ __device__ __forceinline__ uint32_t append_units(uint32_t n_tokens, uint32_t n_seqs) {
+    return n_tokens / kKvBlock + 2 * n_seqs;
+}
+
+// round(x / s), ties to even, |x| <= 127.5 s: the product with 1 / s is at most
+// one code off, and what remains of x beside code * s is exact.
+__device__ __forceinline__ int kv_code(float x, float s, float inv) {
+    float q = rintf(x * inv);
+    q = fminf(fmaxf(q, -127.0f), 127.0f);
+    const float r = fmaf(-q, s, x), h = 0.5f * s;
+    if (r > h || (r == h && ((int)q & 1))) q += 1.0f;
+    else if (r < -h || (r == -h && ((int)q & 1))) q -= 1.0f;
+    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+__device__ __forceinline__ size_t open_at(const KvDev &kv, uint32_t seq, uint32_t h, uint32_t which, uint32_t block) {
+    return ((((size_t)seq * kv.n_kv + h) * 2 + which) * 2 + (block & 1)) * kKvBlock * kv.D;
+}
+
+// Grid: units, heads, keys or values.  A workgroup takes the block's tokens into
+// registers as the layout's pieces (16 elements a thread and step: two runs of
+// eight channels for keys, two of eight tokens for values), finds the largest,
+// and writes the codes.  The unit of a row's first block alone keeps that
+// row's fp32 tokens, after it has read those from before.
+// Bound by the reads of the new tokens; a single token by its chain of
+// latencies.
+constexpr int kAppendThreads = 256;
+template <int D>
+__global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchDev b, const float *k, const float *v,
+                                                              size_t k_stride, size_t v_stride, uint32_t *err) {
+    constexpr int kPieces = 2 * D, kSteps = (kPieces + kAppendThreads - 1) / kAppendThreads;
+    const uint32_t h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+    const uint32_t r = kv_row(b.n_seqs, blockIdx.x, [&](uint32_t i) {
+        const uint32_t s = b.start[i];
+        return (s < b.n_tokens ? s : b.n_tokens) / kKvBlock + 2 * i;
+    });
+    const KvRow row = kv_row_of(b, r);
+    if (row.n == 0) {
+        if (row.falls && tid == 0) kv_report(err, kKvErrRows, r);
+        return;
+    }
+    if (row.bad || r >= kv.n_seqs) {
+        if (tid == 0) kv_report(err, kKvErrRows, r);
+        return;
+    }
+    const uint32_t begin = row.len - row.n, first = begin / kKvBlock, last = (row.len - 1) / kKvBlock;
+    const uint32_t j = blockIdx.x - (row.first / kKvBlock + 2 * r) + first;
+    if (j < first || j > last) return;  // (more units than blocks; start that falls)
+    const uint32_t page = b.table[(size_t)r * b.max_blocks + j];
+    const bool lost = page >= kv.n_blocks;
+    if (lost && tid == 0) kv_report(err, kKvErrBlock, r);
+    const float *src = which ? v : k;
+    const size_t stride = which ? v_stride : k_stride;
+    src += (size_t)row.first * stride + (size_t)h * D;  // token i of the row at i * stride
+    const uint32_t base = j * kKvBlock;                 // position of the block's first token
+    const uint32_t from = begin > base ? begin - base : 0;  // its first token in the batch
+    const uint32_t held = row.len - base < kKvBlock ? row.len - base : kKvBlock;
+    uint2 *tag = kv.tags + (((size_t)r * kv.n_kv + h) * 2 + which) * 2;
+    float *open = kv.open + open_at(kv, r, h, which, j);
+    bool stale = false;
+    if (from) {
+        const uint2 t = tag[j & 1];
+        stale = t.x != j || t.y < from;
+        if (stale && tid == 0) kv_report(err, kKvErrOpen, r);
+    }
+    // the block's tokens from before lie in the open block, the batch's in src; none: the first of them, to be cleared
+    const auto at = [&](uint32_t token) -> const float * {
+        return token < from ? open + (size_t)token * D : src + (size_t)(base + (token < held ? token : held - 1) - begin) * stride;
+    };
+    float x[kSteps][16];
+    float top = 0.0f;
+    bool finite = !stale;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        const uint32_t p = tid + i * kAppendThreads, lane = p % kWave, c = p / kWave, g = lane / 16, n = lane % 16;
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[i][e] = 0.0f;
+        if (p >= (uint32_t)kPieces) continue;
+        if (which == 0) {
+#pragma unroll
+            for (int hi = 0; hi < 2; hi++) {
+                const float4 *row4 = reinterpret_cast<const float4 *>(at(n + 16 * hi) + 32 * c + 8 * g);
+                const float4 u = row4[0], w = row4[1];
+                const float e8[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int f = 0; f < 8; f++) x[i][8 * hi + f] = n + 16 * hi < held ? e8[f] : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; f++) {
+                const uint32_t token = 4 * g + f % 4 + 16 * (f / 4);
+                const float *row1 = at(token) + 32 * c + n;
+                const float lo = row1[0], hi = row1[16];
+                x[i][f] = token < held ? lo : 0.0f;
+                x[i][8 + f] = token < held ? hi : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            finite &= fabsf(x[i][e]) <= 3.402823466e38f;
+            top = fmaxf(top, fabsf(x[i][e]));
+        }
+    }
+    __shared__ float s_top[kAppendThreads / kWave];
+    __shared__ int s_bad[kAppendThreads / kWave];
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+    const bool all_finite = __all(finite);
+    if (tid % kWave == 0) s_top[tid / kWave] = top, s_bad[tid / kWave] = !all_finite;
+    __syncthreads();  // (and every earlier token of the block is read)
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kAppendThreads / kWave; i++) top = fmaxf(top, s_top[i]), bad |= s_bad[i] != 0;
+    if (!lost) {
+        const float s = bad ? __builtin_nanf("") : top / 127.0f;
+        const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+        // (next to the subnormal numbers the remainders of kv_code would not be exact: scaled up by 2^100 they are)
+        const bool tiny = s < 0x1p-100f;
+        uint4 *out = reinterpret_cast<uint4 *>(kv.codes + (((size_t)page * kv.n_kv + h) * 2 + which) * kKvBlock * D);
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+            const uint32_t p = tid + i * kAppendThreads;
+            if (p >= (uint32_t)kPieces) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                w[e] = 0;
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    const float y = x[i][4 * e + f];
+                    int code = 0;
+                    if (s > 0.0f) code = tiny ? kv_code(y * 0x1p100f, s * 0x1p100f, 1.0f / (s * 0x1p100f)) : kv_code(y, s, inv);
+                    w[e] |= (uint32_t)(code + 128) << (8 * f);
+                }
+            }
+            out[p] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (tid == 0) {
+            float *sc = reinterpret_cast<float *>(kv.scales + (size_t)page * kv.n_kv + h);
+            sc[which] = s;
+        }
+    }
+    if (j != first) return;
+    // the fp32 tokens of the row's last two blocks
+    for (uint32_t o = last > first ? last - 1 : last; o <= last; o++) {
+        const uint32_t b0 = o * kKvBlock, f = begin > b0 ? begin - b0 : 0;
+        const uint32_t e = row.len - b0 < kKvBlock ? row.len - b0 : kKvBlock;
+        float *dst = kv.open + open_at(kv, r, h, which, o);
+        for (uint32_t i = f * D + tid; i < e * D; i += kAppendThreads)
+            dst[i] = src[(size_t)(b0 + i / D - begin) * stride + i % D];
+        if (tid == 0 && !(o == first && stale)) tag[o & 1] = make_uint2(o, e);
+    }
+}
+
+// ------------------------------------------------------------------- reading
+// The values of single tokens: a thread four channels of a (slot, head).  Bound
+// by the writes.
+__global__ __launch_bounds__(256) void k_kv_read(KvDev kv, const uint32_t *slots, uint32_t n, float *k, float *v) {
+    const uint32_t quads = kv.D / 4;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (size_t)n * kv.n_kv * quads) return;
+    const uint32_t d = (uint32_t)(i % quads) * 4;
+    const size_t th = i / quads;
+    const uint32_t h = (uint32_t)(th % kv.n_kv), slot = slots[th / kv.n_kv], page = slot / kKvBlock, t = slot % kKvBlock;
+    const float nan = __builtin_nanf("");
+    float4 ko = make_float4(nan, nan, nan, nan), vo = ko;
+    if (page < kv.n_blocks) {
+        const float2 s = kv.scales[(size_t)page * kv.n_kv + h];
+        const uint8_t *kc = kv.codes + ((size_t)page * kv.n_kv + h) * 2 * kKvBlock * kv.D, *vc = kc + kKvBlock * kv.D;
+        const uint32_t c = d / 32;
+        // keys: four channels of one token in a row
+        const uint32_t kb = *reinterpret_cast<const uint32_t *>(
+            kc + (c * kWave + (d % 32) / 8 * 16 + t % 16) * 16 + (t / 16) * 8 + d % 8);
+        // values: token t is byte (t % 4) + 4 (t / 16) of lane group (t % 16) / 4
+        const uint8_t *vb = vc + (c * kWave + (t % 16) / 4 * 16 + d % 16) * 16 + (d % 32) / 16 * 8 + t % 4 + 4 * (t / 16);
+        const auto val = [](uint32_t byte, float scale) { return (float)((int)byte - 128) * scale; };
+        ko = make_float4(val(kb & 255, s.x), val(kb >> 8 & 255, s.x), val(kb >> 16 & 255, s.x), val(kb >> 24, s.x));
+        vo = make_float4(val(vb[0], s.y), val(vb[16], s.y), val(vb[32], s.y), val(vb[48], s.y));
+    }
+    const size_t at = th * kv.D + d;
+    *reinterpret_cast<float4 *>(k + at) = ko;
+    *reinterpret_cast<float4 *>(v + at) = vo;
+}
+
+}  // namespace
+
+hipError_t launch_kv_plan(const KvPlanArgs &a, hipStream_t s) {
+    if (a.n_seqs == 0 || a.n_seqs > kKvMaxSeqs) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(kPlanThreads), 0, s, a);
+    if (a.n_tokens > kPlanTokens) hipLaunchKernelGGL(k_kv_slots, dim3((a.n_tokens + 255) / 256), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvDev &kv, const KvBatchDev &b, const float *k, const float *v, size_t k_stride,
+                            size_t v_stride, uint32_t *err, hipStream_t s) {
+    const dim3 grid(append_units(b.n_tokens, b.n_seqs), kv.n_kv, 2), block(kAppendThreads);
+    switch (kv.D) {
+    case 64: hipLaunchKernelGGL(k_kv_append<64>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    case 96: hipLaunchKernelGGL(k_kv_append<96>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    case 128: hipLaunchKernelGGL(k_kv_append<128>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    case 192: hipLaunchKernelGGL(k_kv_append<192>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    case 256: hipLaunchKernelGGL(k_kv_append<256>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    case 512: hipLaunchKernelGGL(k_kv_append<512>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_read(const KvDev &kv, const uint32_t *slots, uint32_t n, float *k, float *v, hipStream_t s) {
+    const size_t threads = (size_t)n * kv.n_kv * (kv.D / 4);
+    hipLaunchKernelGGL(k_kv_read, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, kv, slots, n, k, v);
+    return hipGetLastError();
+}
+
+}  // namespace lt

@@ -31,7 +31,10 @@ LT_MOE_UNFUSED = 1 << 3
 LT_MOE_DETERMINISTIC = 1 << 4
 LT_NORM_PRECISE = 1 << 5
 LT_NORM_ONE_PLUS_W = 1 << 6
+LT_ROPE_NO_NORM = 1 << 7
 ACT_SILU, ACT_GELU_TANH = 0, 1
+ROPE_NEOX, ROPE_PAIRS = 0, 1
+KV_BLOCK, KV_NONE = 32, 0xFFFFFFFF
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "libllmtoy_hip.so")
@@ -70,7 +73,16 @@ EXPORTS = [
     "lt_tensor_free", "lt_tensor_create", "lt_quantize", "lt_dequantize", "lt_matmul", "lt_matmul_quantized", "lt_tensor_bytes", "lt_stream_read", "lt_matvec", "lt_ffn_dense", "lt_moe_router_topk", "lt_expert_gate_up_id",
     "lt_expert_down_id", "lt_moe_forward", "lt_moe_forward_noalloc", "lt_moe_prefill", "lt_rmsnorm", "lt_add_rmsnorm",
     "lt_rmsnorm_weighted_raw_scaled", "lt_moe_tail", "lt_gemma4_moe_block", "lt_profile_report",
+    "lt_rope_create", "lt_rope_free", "lt_qk_norm_rope", "lt_kv_create", "lt_kv_free", "lt_kv_bytes", "lt_kv_plan",
+    "lt_kv_append", "lt_kv_read", "lt_attention",
 ]
+
+
+class KvBatchStruct(C.Structure):
+    """lt_kv_batch"""
+    _fields_ = [("n_seqs", C.c_uint32), ("n_tokens", C.c_uint32), ("max_blocks", C.c_uint32), ("max_new", C.c_uint32),
+                ("start", C.c_void_p), ("len", C.c_void_p), ("table", C.c_void_p)]
+
 
 _lib = None
 
@@ -116,6 +128,16 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "lt_profile_report": (sz, [vp, vp, sz]),
         "lt_gemma4_moe_block": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_float, C.c_float, u32, u32,
                                       u32, u32, vp, vp]),
+        "lt_rope_create": (i32, [vp, u32, u32, C.c_double, vp, u32, C.POINTER(vp)]),
+        "lt_rope_free": (i32, [vp, vp]),
+        "lt_qk_norm_rope": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, sz, sz, sz, sz, C.c_float, u32]),
+        "lt_kv_create": (i32, [vp, u32, u32, u32, u32, C.POINTER(vp)]),
+        "lt_kv_free": (i32, [vp, vp]),
+        "lt_kv_bytes": (sz, [vp]),
+        "lt_kv_plan": (i32, [vp, C.POINTER(KvBatchStruct), vp, vp, vp, u32, vp, vp, vp, vp, u32]),
+        "lt_kv_append": (i32, [vp, vp, vp, vp, sz, sz, C.POINTER(KvBatchStruct), u32]),
+        "lt_kv_read": (i32, [vp, vp, vp, vp, vp, u32, u32]),
+        "lt_attention": (i32, [vp, vp, vp, vp, C.POINTER(KvBatchStruct), u32, sz, C.c_float, u32, u32]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -171,6 +193,113 @@ class Tensor:
     def free(self):
         if self.handle:
             self.ctx.lib.lt_tensor_free(self.ctx.ptr, self.handle)
+            self.handle = None
+
+
+def _words(a, n: int, what: str):
+    """A contiguous array of n 32-bit whole numbers."""
+    if a is None:
+        raise InvalidError(f"{what}: an array of {n} is needed")
+    if str(a.dtype).replace("torch.", "") not in ("int32", "uint32"):
+        raise InvalidError(f"{what}: 32-bit whole numbers expected, got {a.dtype}")
+    if int(np.prod(tuple(a.shape))) != n:
+        raise InvalidError(f"{what}: {tuple(a.shape)}, {n} entries expected")
+    return a
+
+
+def _heads(a, what: str):
+    """(pointer, is_host, tokens, heads, head_dim, floats from token to token) of a float32 array
+    [tokens, heads, head_dim] whose heads lie in a row; the tokens may be a stride apart."""
+    if a.dtype != np.float32 and str(a.dtype) != "torch.float32":
+        raise InvalidError(f"{what}: float32 expected, got {a.dtype}")
+    if len(a.shape) != 3:
+        raise InvalidError(f"{what}: [tokens, heads, head_dim] expected, got {tuple(a.shape)}")
+    T, H, D = (int(n) for n in a.shape)
+    if _is_torch(a):
+        st, p, host = a.stride(), a.data_ptr(), not a.is_cuda
+    elif isinstance(a, np.ndarray):
+        st, p, host = [n // 4 for n in a.strides], a.ctypes.data, True
+    else:
+        st, (p, host) = (H * D, D, 1), _ptr(a)
+    if T and (D > 1 and st[2] != 1 or H > 1 and st[1] != D or T > 1 and st[0] < H * D):
+        raise InvalidError(f"{what}: a token's heads must lie in a row (strides {tuple(st)})")
+    return p, host, T, H, D, int(st[0]) if T > 1 else H * D
+
+
+class Rope:
+    """A rotation (lt_rope_create)."""
+
+    def __init__(self, ctx: "Context", handle, head_dim):
+        self.ctx, self.handle, self.head_dim = ctx, handle, head_dim
+
+    def free(self):
+        if self.handle:
+            self.ctx.lib.lt_rope_free(self.ctx.ptr, self.handle)
+            self.handle = None
+
+
+class KvBatch:
+    """A batch of sequences (lt_kv_batch): start [n + 1], len [n], table [n, max_blocks], arrays of 32-bit
+    whole numbers, all on the host or all on the device; n_tokens: tokens that the batch's arrays have room
+    for; max_new: no sequence has more of them (0: not known)."""
+
+    def __init__(self, start, len, table, n_tokens: int, max_new: int = 0):  # noqa: A002
+        if table is None or tuple(table.shape) != (len.shape[0], table.shape[-1]):
+            raise InvalidError("table: [sequences, blocks] expected")
+        n = int(len.shape[0])
+        self.start, self.len, self.table = _words(start, n + 1, "start"), _words(len, n, "len"), table
+        _words(table, n * int(table.shape[1]), "table")
+        self.n_seqs, self.n_tokens, self.max_blocks, self.max_new = n, int(n_tokens), int(table.shape[1]), int(max_new)
+
+    def struct(self):
+        """(lt_kv_batch, is_host)"""
+        ps = [_ptr(a) for a in (self.start, self.len, self.table)]
+        if len({h for _, h in ps}) > 1:
+            raise InvalidError("mix of host and device arrays")
+        return KvBatchStruct(self.n_seqs, self.n_tokens, self.max_blocks, self.max_new, *(p for p, _ in ps)), ps[0][1]
+
+
+class KvCache:
+    """One layer's keys and values in 8-bit blocks (lt_kv_create)."""
+
+    def __init__(self, ctx: "Context", handle, n_blocks, n_kv_heads, head_dim, n_seqs):
+        self.ctx, self.handle = ctx, handle
+        self.n_blocks, self.n_kv_heads, self.head_dim, self.n_seqs = n_blocks, n_kv_heads, head_dim, n_seqs
+
+    @property
+    def nbytes(self) -> int:
+        return int(self.ctx.lib.lt_kv_bytes(self.handle))
+
+    def append(self, k, v, batch: KvBatch):
+        """The batch's tokens' keys and values ([n_tokens, n_kv_heads, head_dim]) into the cache."""
+        b, host = batch.struct()
+        got = [self._mine(a, w, batch.n_tokens) for a, w in ((k, "k"), (v, "v"))]
+        if {host} != {g[1] for g in got}:
+            raise InvalidError("mix of host and device arrays")
+        c = self.ctx
+        c._check(c.lib.lt_kv_append(c.ptr, self.handle, got[0][0], got[1][0], got[0][5], got[1][5], C.byref(b),
+                                    LT_HOST_IO if host else 0))
+
+    def read(self, k_out, v_out, slots):
+        """The values that slots stand for, into k_out and v_out [n, n_kv_heads, head_dim]."""
+        n = int(np.prod(tuple(slots.shape)))
+        _words(slots, n, "slots")
+        for a, w in ((k_out, "k_out"), (v_out, "v_out")):
+            if self._mine(a, w, n)[5] != self.n_kv_heads * self.head_dim:
+                raise InvalidError(f"{w}: must be contiguous")
+        c = self.ctx
+        c._check(c.lib.lt_kv_read(c.ptr, _ptr(k_out)[0], _ptr(v_out)[0], self.handle, _ptr(slots)[0], n,
+                                  c._io(k_out, v_out, slots)))
+
+    def _mine(self, a, what, tokens):
+        got = _heads(a, what)
+        if got[2:5] != (tokens, self.n_kv_heads, self.head_dim):
+            raise InvalidError(f"{what}: {tuple(a.shape)}, {(tokens, self.n_kv_heads, self.head_dim)} expected")
+        return got
+
+    def free(self):
+        if self.handle:
+            self.ctx.lib.lt_kv_free(self.ctx.ptr, self.handle)
             self.handle = None
 
 
@@ -341,6 +470,84 @@ class Context:
         self._check(self.lib.lt_moe_forward_noalloc(self.ptr, _ptr(out)[0], _ptr(x)[0], router.handle, _ptr(bias)[0],
                                                     gate_up.handle, down.handle, sg, su, sd, k, d_expert, act,
                                                     fl, _ptr(out_ids)[0], _ptr(out_w)[0]))
+        return out
+
+    def rope(self, head_dim: int, n_rot: int | None = None, base: float = 10000.0, style: int = ROPE_NEOX,
+             freq_factors=None) -> Rope:
+        """What qk_norm_rope rotates by; n_rot: elements that are rotated (None: all)."""
+        n_rot = head_dim if n_rot is None else n_rot
+        f = None
+        if freq_factors is not None:
+            f = np.ascontiguousarray(freq_factors, np.float32)
+            if f.shape != (n_rot // 2,):
+                raise InvalidError(f"freq_factors: {f.shape}, {n_rot // 2} expected")
+        h = C.c_void_p()
+        self._check(self.lib.lt_rope_create(self.ptr, head_dim, n_rot, base, None if f is None else f.ctypes.data, style,
+                                            C.byref(h)))
+        return Rope(self, h, head_dim)
+
+    def qk_norm_rope(self, q_out, k_out, q, k, wq, wk, positions, rope: Rope, eps=1e-6, norm=True, one_plus_w=False):
+        """Norms of queries and keys [tokens, heads, head_dim] for each head and the rotation, in one pass
+        (lt_qk_norm_rope).  k and k_out may be None; weights may be None (not multiplied); norm=False: rotate only."""
+        given = [("q", q), ("q_out", q_out)] + ([("k", k), ("k_out", k_out)] if k is not None or k_out is not None else [])
+        if any(a is None for _, a in given):
+            raise InvalidError("an input without its output")
+        got = {w: _heads(a, w) for w, a in given}
+        T = got["q"][2]
+        for w, g in got.items():
+            if (g[2], g[4]) != (T, rope.head_dim) or g[3] != got[w[0]][3]:
+                raise InvalidError(f"{w}: {g[2:5]}, {T} tokens of heads of {rope.head_dim} expected")
+        for w, a in (("wq", wq), ("wk", wk)):
+            if a is not None and (tuple(a.shape) != (rope.head_dim,) or str(a.dtype).replace("torch.", "") != "float32"):
+                raise InvalidError(f"{w}: float32 [{rope.head_dim}] expected")
+        _words(positions, T, "positions")
+        rest = [_ptr(a) for a in (wq, wk, positions)]
+        hosts = {g[1] for g in got.values()} | {h for _, h in rest if h is not None}
+        if len(hosts) > 1:
+            raise InvalidError("mix of host and device arrays")
+        none = (None, None, 0, 0, 0, 0)
+        gk, gko = got.get("k", none), got.get("k_out", none)
+        fl = (LT_HOST_IO if hosts == {True} else 0) | (0 if norm else LT_ROPE_NO_NORM)
+        fl |= LT_NORM_ONE_PLUS_W if one_plus_w else 0
+        self._check(self.lib.lt_qk_norm_rope(self.ptr, got["q_out"][0], gko[0], got["q"][0], gk[0], rest[0][0], rest[1][0],
+                                             rest[2][0], rope.handle, T, got["q"][3], gk[3], got["q"][5], gk[5],
+                                             got["q_out"][5], gko[5], eps, fl))
+
+    def kv_cache(self, n_blocks: int, n_kv_heads: int, head_dim: int, n_seqs: int = 1) -> KvCache:
+        """An empty cache of n_blocks blocks of 32 tokens for one layer and up to n_seqs sequences."""
+        h = C.c_void_p()
+        self._check(self.lib.lt_kv_create(self.ptr, n_blocks, n_kv_heads, head_dim, n_seqs, C.byref(h)))
+        return KvCache(self, h, n_blocks, n_kv_heads, head_dim, n_seqs)
+
+    def kv_plan(self, batch: KvBatch, len_in, n_new, free_blocks, used_in, used_out, positions, slots):
+        """A step's batch (start, len, new entries of table), positions and slots from the sequences'
+        lengths and a list of free blocks (lt_kv_plan)."""
+        b, host = batch.struct()
+        n_free = int(np.prod(tuple(free_blocks.shape)))
+        arrays = [_words(len_in, batch.n_seqs, "len_in"), _words(n_new, batch.n_seqs, "n_new"),
+                  _words(free_blocks, n_free, "free_blocks"), _words(used_in, 1, "used_in"), _words(used_out, 1, "used_out"),
+                  _words(positions, batch.n_tokens, "positions"), _words(slots, batch.n_tokens, "slots")]
+        ps = [_ptr(a) for a in arrays]
+        if {h for _, h in ps} != {host}:
+            raise InvalidError("mix of host and device arrays")
+        p = [x for x, _ in ps]
+        self._check(self.lib.lt_kv_plan(self.ptr, C.byref(b), p[0], p[1], p[2], n_free, p[3], p[4], p[5], p[6],
+                                        LT_HOST_IO if host else 0))
+
+    def attention(self, out, q, cache: KvCache, batch: KvBatch, scale: float, window: int = 0):
+        """out [n_tokens, heads, head_dim]: the queries over the cache, causal (lt_attention)."""
+        b, host = batch.struct()
+        gq, go = _heads(q, "q"), _heads(out, "out")
+        T, H, D = gq[2:5]
+        if T != batch.n_tokens or D != cache.head_dim or go[2:5] != gq[2:5]:
+            raise InvalidError(f"q {tuple(q.shape)} and out {tuple(out.shape)} for {batch.n_tokens} tokens of heads of "
+                               f"{cache.head_dim}")
+        if go[5] != H * D:
+            raise InvalidError("out: must be contiguous")
+        if {gq[1], go[1]} != {host}:
+            raise InvalidError("mix of host and device arrays")
+        self._check(self.lib.lt_attention(self.ptr, go[0], gq[0], cache.handle, C.byref(b), H, gq[5], scale, window,
+                                          LT_HOST_IO if host else 0))
         return out
 
     def moe_prefill(self, out, X, router: Tensor, gate_up: Tensor, down: Tensor, k: int, d_expert: int,
