@@ -107,6 +107,8 @@ struct lt_ctx {
     };
     std::vector<MxHand> mx_hands;
     uint32_t mx_wait = lt::kMxWaitTicks;
+    // arrival tickets of the attention's parts, zeroed once at init like the router's
+    uint32_t *attn_tickets = nullptr;
     // hand-over memory of the single-launch dense FFN (allocated by lt_init)
     void *ffn = nullptr;
     lt::FfnScratch ffsc{};
@@ -676,9 +678,12 @@ extern "C" int lt_init(int device, lt_ctx **out_ctx) {
     }
     hipError_t e = hipMalloc((void **)&ctx->ticket, 256);
     if (e == hipSuccess) e = hipMemset(ctx->ticket, 0, 256);
+    if (e == hipSuccess) e = hipMalloc((void **)&ctx->attn_tickets, lt::kAttnTickets * 4);
+    if (e == hipSuccess) e = hipMemset(ctx->attn_tickets, 0, lt::kAttnTickets * 4);
     if (e == hipSuccess) e = init_device_state(ctx);
     if (e != hipSuccess) {
         if (ctx->ticket) (void)hipFree(ctx->ticket);
+        if (ctx->attn_tickets) (void)hipFree(ctx->attn_tickets);
         if (ctx->pin) (void)hipHostFree(ctx->pin);
         if (ctx->fused_err) (void)hipHostFree(ctx->fused_err);
         if (ctx->prof.stamps) (void)hipFree(ctx->prof.stamps);
@@ -708,6 +713,7 @@ extern "C" void lt_destroy(lt_ctx *ctx) {
     for (hipEvent_t e : ctx->prof.free_events) (void)hipEventDestroy(e);
     if (ctx->prof.stamps) (void)hipFree(ctx->prof.stamps);
     if (ctx->ticket) (void)hipFree(ctx->ticket);
+    if (ctx->attn_tickets) (void)hipFree(ctx->attn_tickets);
     if (ctx->fused) (void)hipFree(ctx->fused);
     for (const lt_ctx::MxHand &m : ctx->mx_hands) (void)hipFree(m.p);
     if (ctx->ffn) (void)hipFree(ctx->ffn);
@@ -2211,7 +2217,7 @@ extern "C" int lt_attention(lt_ctx *ctx, float *out, const float *q, const lt_kv
     a.kv = kv->d, a.b = batch_dev(*batch), a.q = q, a.out = out, a.q_stride = q_stride;
     a.n_heads = n_heads, a.group = n_heads / n_kv, a.window = window, a.scale = scale, a.err = ctx->err_dev;
     if ((rc = ensure(ctx, ctx->attn, lt::attention_workspace(a)))) return rc;
-    a.work = ctx->attn.p;
+    a.work = ctx->attn.p, a.tickets = ctx->attn_tickets;
     if (!host) return launch_rc(ctx, lt::launch_attention(a, ctx->stream), "attention");
     HostArrays io(ctx);
     const int iq = io.add(q, a.b.n_tokens, width, q_stride), oo = io.add(out, a.b.n_tokens, width);

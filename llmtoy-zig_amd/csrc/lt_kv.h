@@ -116,8 +116,10 @@ struct AttnArgs {
     uint32_t n_heads, group, window;
     float scale;
     void *work;
+    uint32_t *tickets;  // kAttnTickets words, zero between launches
     uint32_t *err;
 };
+constexpr size_t kAttnTickets = 8192;
 bool attention_head_dim(uint32_t D);
 size_t attention_workspace(const AttnArgs &a);
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
