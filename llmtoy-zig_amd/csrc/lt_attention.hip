@@ -24,17 +24,12 @@
 // number of blocks, as many as fill the chip; the part that arrives last at a
 // tile joins them.
 #include "llmtoy_hip.h"
-#include "lt_kv.h"
+#include "lt_attn.h"
 
 namespace lt {
 
 namespace {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kThinRows = 16;
 // Wavefronts of a workgroup: eight take a tile's blocks in turn; heads of 512
 // need the registers and the LDS of twice as much.
@@ -62,23 +57,6 @@ struct ThinArgs {
     uint32_t *err;
 };
 
-// A byte code + 128 is the f16 number 1024 + 128 + code with the byte 0x64 above it.
-__device__ __forceinline__ half8 codes8(uint32_t a, uint32_t b) {
-    union {
-        uint32_t u[4];
-        half2v h[4];
-        half8 v;
-    } r;
-    r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
-    r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
-    r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
-    r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
-    const half2v off = {(_Float16)1152.0f, (_Float16)1152.0f};
-#pragma unroll
-    for (int i = 0; i < 4; i++) r.h[i] = r.h[i] - off;
-    return r.v;
-}
-
 // How a sequence's rows are cut: `tiles` tiles of 16 rows, over the blocks lo ..
 // lo + blocks - 1.
 struct ThinRow {
@@ -91,7 +69,7 @@ __device__ __forceinline__ ThinRow thin_row(const ThinArgs &a, uint32_t r) {
     t.k = kv_row_of(a.b, r);
     // (beyond max_new: as many as the grid has room for, and those get NaN)
     const uint32_t n = a.b.max_new && t.k.n > a.b.max_new ? a.b.max_new : t.k.n;
-    t.tiles = (n * a.group + kThinRows - 1) / kThinRows;
+    t.tiles = n * a.group > kThinMost ? 0 : (n * a.group + kThinRows - 1) / kThinRows;
     t.lo = 0;
     t.blocks = 1;
     if (!t.k.bad && t.k.n) {
@@ -125,8 +103,6 @@ __device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, uint32_t least
     const float each = ceilf(sum * (float)a.n_kv / (float)kThinTarget);
     return each < (float)least ? least : each > 1e9f ? 1000000000u : (uint32_t)each;
 }
-
-__device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index, uint32_t least) {
     ThinWork w{};
@@ -180,25 +156,6 @@ __device__ __forceinline__ float row_max(float v) {
     v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
     const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
-}
-
-// Partial results go past the L2s (agent scope): another XCD reads them.
-__device__ __forceinline__ void put4(float *p, f32x4 v) {
-    uint64_t *q = reinterpret_cast<uint64_t *>(p);
-    __hip_atomic_store(q, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(q + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x4 get4(const float *p) {
-    const uint64_t *q = reinterpret_cast<const uint64_t *>(p);
-    const float2 a = __builtin_bit_cast(float2, __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    const float2 b = __builtin_bit_cast(float2, __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    return f32x4{a.x, a.y, b.x, b.y};
-}
-
-// What an output is of its sums: 2^(mo - m) / l, without the weights' 2^15; no
-// key seen: 0.
-__device__ __forceinline__ float out_scale(float m, float l, float mo) {
-    return l > 0.0f || l != l ? (mo == kNegInf ? 0.0f : exp2f(mo - m - 15.0f)) / l : 0.0f;
 }
 
 // Joins `count` partial results that lie `step` floats apart into a row's sums: T
@@ -458,7 +415,7 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
             lt_ += mi == kNegInf ? li : li * exp2f(mi - mt);  // (l is 0 or NaN without a largest)
             fo[i] = moi == kNegInf ? 1.0f : exp2f(moi - mot);
         }
-        const float scale = w.splits > 1 ? 1.0f : w.bad ? __builtin_nanf("") : out_scale(mt, lt_, mot);
+        const float scale = w.splits > 1 ? 1.0f : w.bad ? __builtin_nanf("") : out_scale(mt, lt_, mot, 15.0f);
 #pragma unroll
         for (int i = 0; i < (D + 4 * T - 1) / (4 * T); i++) {
             const uint32_t d = 4 * (part + T * i);
@@ -515,7 +472,7 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
         if (rr < rows_in) sums.run(from, used_groups, step * in_group, part);
     }
     if (rr < rows_in) {
-        const float scale = out_scale(sums.m, sums.l, sums.mo);
+        const float scale = out_scale(sums.m, sums.l, sums.mo, 15.0f);
 #pragma unroll
         for (int k = 0; k < Joined<D, T>::N; k++) {
             const uint32_t d = 4 * (part + T * k);
@@ -529,10 +486,9 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
 uint32_t thin_tiles(const AttnArgs &a) {
     const uint64_t rows = (uint64_t)a.b.n_tokens * a.group;
     uint64_t tiles = rows / kThinRows + a.b.n_seqs;
-    if (a.b.max_new) {
-        const uint64_t most = (uint64_t)a.b.n_seqs * (((uint64_t)a.b.max_new * a.group + kThinRows - 1) / kThinRows);
-        if (most < tiles) tiles = most;
-    }
+    const uint64_t each = a.b.max_new && (uint64_t)a.b.max_new * a.group < kThinMost ? a.b.max_new * a.group : kThinMost;
+    const uint64_t most = (uint64_t)a.b.n_seqs * ((each + kThinRows - 1) / kThinRows);
+    if (most < tiles) tiles = most;
     if (rows < tiles) tiles = rows;
     return (uint32_t)tiles;
 }
@@ -548,11 +504,20 @@ void go(const ThinArgs &t, uint32_t tiles, hipStream_t s) {
 
 bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D == 192 || D == 256 || D == 512; }
 
+// Whether a sequence may have rows for the wide kernel.
+static bool wide(const AttnArgs &a) { return (uint64_t)(a.b.max_new ? a.b.max_new : a.b.n_tokens) * a.group > kThinMost; }
+
 size_t attention_workspace(const AttnArgs &a) {
-    return (size_t)a.kv.n_kv * thin_slots(a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
+    const size_t thin = (size_t)a.kv.n_kv * thin_slots(a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
+    const size_t more = wide(a) ? attention_wide_workspace(a.kv.D) : 0;
+    return thin < more ? more : thin;
 }
 
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
+    if (wide(a)) {
+        const hipError_t e = launch_attention_wide(a, s);
+        if (e != hipSuccess) return e;
+    }
     ThinArgs t{};
     t.codes = a.kv.codes, t.scales = a.kv.scales, t.n_blocks = a.kv.n_blocks, t.n_kv = a.kv.n_kv, t.b = a.b;
     t.q = a.q, t.out = a.out, t.q_stride = a.q_stride, t.n_heads = a.n_heads, t.group = a.group, t.window = a.window;

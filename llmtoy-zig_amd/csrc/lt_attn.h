@@ -1,0 +1,61 @@
+// lt_attn.h -- what the attention's two kernels share (lt_attention.hip: few rows,
+// lt_attention_wide.hip: many).
+#pragma once
+#include "lt_kv.h"
+
+#ifdef __HIPCC__
+
+namespace lt {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Rows (tokens times heads of a group) of a sequence up to which lt_attention.hip's
+// kernel takes it; the other kernel takes those with more.  By the sequence alone, so
+// that what else is in the batch does not change its results.
+constexpr uint32_t kThinMost = 32;
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// A byte code + 128 is the f16 number 1024 + 128 + code with the byte 0x64 above it.
+__device__ __forceinline__ half8 codes8(uint32_t a, uint32_t b) {
+    union {
+        uint32_t u[4];
+        half2v h[4];
+        half8 v;
+    } r;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    const half2v off = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.h[i] = r.h[i] - off;
+    return r.v;
+}
+
+// Partial results go past the L2s (agent scope): another XCD reads them.
+__device__ __forceinline__ void put4(float *p, f32x4 v) {
+    uint64_t *q = reinterpret_cast<uint64_t *>(p);
+    __hip_atomic_store(q, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(q + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4 get4(const float *p) {
+    const uint64_t *q = reinterpret_cast<const uint64_t *>(p);
+    const float2 a = __builtin_bit_cast(float2, __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    const float2 b = __builtin_bit_cast(float2, __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    return f32x4{a.x, a.y, b.x, b.y};
+}
+
+// What an output is of its sums: 2^(mo - m) / l, without the weights' 2^bits; no
+// key seen: 0.
+__device__ __forceinline__ float out_scale(float m, float l, float mo, float bits) {
+    return l > 0.0f || l != l ? (mo == kNegInf ? 0.0f : exp2f(mo - m - bits)) / l : 0.0f;
+}
+
+}  // namespace lt
+
+#endif  // __HIPCC__

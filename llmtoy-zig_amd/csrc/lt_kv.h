@@ -123,5 +123,7 @@ constexpr size_t kAttnTickets = 8192;
 bool attention_head_dim(uint32_t D);
 size_t attention_workspace(const AttnArgs &a);
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
+size_t attention_wide_workspace(uint32_t D);
+hipError_t launch_attention_wide(const AttnArgs &a, hipStream_t s);
 
 }  // namespace lt
