@@ -129,6 +129,52 @@ __device__ __forceinline__ float row_max2(float v) {
     return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
 
+// v, but what is computed from it stays in its branch (the compiler would rather always do it and select).
+template <typename T>
+__device__ __forceinline__ T in_branch(T v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ half2v pair(float a, float b) { return __builtin_convertvector((f32x2{a, b}), half2v); }
+
+// N operands read from LDS one after the other, the i-th for use(i, operand): kAhead of
+// them under way before the first product (the compiler, short of registers, would
+// read one and wait for it).
+constexpr int kAhead = 4;
+struct Feed {
+    half8 x[kAhead];
+    const half8 *from;
+    __device__ __forceinline__ void open(const half8 *f) {
+        from = f;
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) x[i] = from[i * kWave];
+    }
+    template <int N, typename F>
+    __device__ __forceinline__ void run(F use) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            use(i, x[i % kAhead]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + kAhead < N) x[i % kAhead] = from[(i + kAhead) * kWave];
+        }
+    }
+};
+
+// What is left of p beside h's first or second half, in one instruction.
+__device__ __forceinline__ float rest0(half2v h, float p) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
+__device__ __forceinline__ float rest1(half2v h, float p) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
+
 template <int D>
 __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attention_wide(WideArgs a) {
     using Sh = Shape<D>;
@@ -343,15 +389,15 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
             const half8 *kv = s_kv[(j - b0) % 2];
             const bool on = !idle && (int)(j * kKvBlock) <= pos1 && (int)(j * kKvBlock + kKvBlock) > low0;
             f32x16 acc;
+            Feed keys, values;
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[e] = 0.0f;
             if (on) {
-#pragma unroll
-                for (int s = 0; s < S; s++) {
-                    const half8 k = kv[(cut * S + s) * kWave + lane];
+                keys.open(kv + cut * S * kWave + lane);
+                keys.run<S>([&](int s, half8 k) {
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[s], acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[s], acc, 0, 0, 0);
-                }
+                });
             }
             if (SPLIT > 1) {
 #pragma unroll
@@ -366,14 +412,16 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
                 }
             }
             if (on) {
+                values.open(kv + 4 * D + cut * CB * 2 * kWave + lane);  // (there by the time of the weights)
                 const float ks = __uint_as_float(from_lane(__float_as_uint(ks_l), (j - b0) % kWave));
                 const float lv = __uint_as_float(from_lane(__float_as_uint(lv_l), (j - b0) % kWave));
                 // keys 32 j + 4 half + 8 (e / 4) + e % 4
                 const bool edge = (int)(j * kKvBlock + kKvBlock - 1) > pos0 || (int)(j * kKvBlock) < low1;
                 if (edge) {
+                    const int key0 = in_branch((int)(j * kKvBlock + 4 * half));
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const int key = (int)(j * kKvBlock + 4 * half) + 8 * (e / 4) + e % 4;
+                        const int key = key0 + 8 * (e / 4) + e % 4;
                         if (key > pos || key < low) acc[e] = kNegInf;
                     }
                 }
@@ -399,9 +447,10 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
 #pragma unroll
                 for (int e = 0; e < 16; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(acc[e], c, eb));
                 if (edge) {
+                    const float none = in_branch(kNegInf);
 #pragma unroll
                     for (int e = 0; e < 16; e++)
-                        if (acc[e] == kNegInf) p[e] = 0.0f;  // (what is not seen adds nothing, whatever its scale)
+                        if (acc[e] == none) p[e] = 0.0f;  // (what is not seen adds nothing, whatever its scale)
                 }
 #pragma unroll
                 for (int e = 0; e < 16; e++) sum += p[e];
@@ -409,21 +458,17 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
                 // operand u: the keys 4 half + 16 u' + 8 u .. + 3 for u' = 0, 1, as a value's codes lie
                 half8 ph[2], pl[2];
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
+                for (int e = 0; e < 16; e += 2) {
                     const int w = e / 4 % 2, i = e % 4 + 4 * (e / 8);
-                    const _Float16 hi = (_Float16)p[e];
-                    ph[w][i] = hi;
-                    pl[w][i] = (_Float16)(p[e] - (float)hi);
+                    const half2v hi = pair(p[e], p[e + 1]);
+                    const half2v lo = pair(rest0(hi, p[e]), rest1(hi, p[e + 1]));
+                    ph[w][i] = hi[0], ph[w][i + 1] = hi[1];
+                    pl[w][i] = lo[0], pl[w][i + 1] = lo[1];
                 }
-#pragma unroll
-                for (int k = 0; k < CB; k++) {
-#pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const half8 v = kv[4 * D + ((cut * CB + k) * 2 + w) * kWave + lane];
-                        o[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[w], o[k], 0, 0, 0);
-                        o[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[w], o[k], 0, 0, 0);
-                    }
-                }
+                values.run<2 * CB>([&](int i, half8 v) {
+                    o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i % 2], o[i / 2], 0, 0, 0);
+                    o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i % 2], o[i / 2], 0, 0, 0);
+                });
             }
             __syncthreads();
         }
