@@ -51,10 +51,15 @@ struct WideArgs {
     uint32_t *err;
 };
 
-// Wavefronts a head is cut over, wavefronts a workgroup, workgroups a CU.
+// Wavefronts a head is cut over, wavefronts a workgroup, workgroups a CU.  Measured on
+// 512 queries of 16 or 32 heads (us): heads of 64 4 wavefronts three times a CU 319, twice 335, 8 345;
+// of 96 8 230, 4 twice a CU 238; of 128 8 501, 4 twice 523; of 192 cut, 4 twice 280, 8 288;
+// of 256 whole 363, cut 475.  (Products of the next block between this one's
+// exponentials: slower for 64 to 128 and 512, 5% faster for 192.)
 template <int D>
 struct Shape {
-    static constexpr int kSplit = D <= 128 ? 1 : 2, kWaves = 4, kPerCu = D <= 192 ? 2 : 1;
+    static constexpr int kSplit = D == 192 || D == 512 ? 2 : 1, kWaves = D == 96 || D == 128 ? 8 : 4;
+    static constexpr int kPerCu = D == 64 ? 3 : D == 192 ? 2 : 1;
     static constexpr int kThreads = kWaves * kWave, kRows = 32 * kWaves / kSplit;
     static constexpr int DW = D / kSplit, S = DW / 16, CB = DW / 32;
     static constexpr size_t kPart = (size_t)kWaves * (CB * 4 + 1) * kWave * 4;  // floats
