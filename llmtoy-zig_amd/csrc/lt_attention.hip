@@ -30,15 +30,26 @@ namespace lt {
 
 namespace {
 
+#ifndef TGT
+#define TGT 3
+#endif
 constexpr int kThinRows = 16;
-// Wavefronts of a workgroup: eight take a tile's blocks in turn; heads of 512
-// need the registers and the LDS of twice as much.
+// Wavefronts of a workgroup that a block's channels are cut over, wavefronts, workgroups a
+// CU, blocks a wavefront has under way.
 template <int D>
-constexpr int kThinWaves = D <= 256 ? 8 : 4;
-// Workgroups that a launch's work is split into, where there are fewer tiles: one
-// on each CU.
-constexpr uint32_t kThinTarget = 256;
-// Parts of a tile that are joined at once; more are joined in groups first.
+struct Shape {
+    static constexpr int kSplit = D <= 256 ? 1 : 2, kWaves = 4, kPerCu = D <= 128 ? 3 : D <= 256 ? 2 : 1, kTarget = kPerCu < TGT ? kPerCu : TGT, kDepth = D <= 64 ? 4 : 1;
+    static constexpr int kThreads = kWaves * kWave, kBlocks = kWaves / kSplit;  // blocks a round
+    static constexpr int DW = D / kSplit, C = DW / 32;
+    static constexpr bool kQueriesInLds = DW >= 256;
+};
+// Blocks that a part is worth having for.
+#ifndef LEAST
+#define LEAST 8
+#endif
+constexpr uint32_t kLeast = LEAST;
+// Parts of a tile that are joined at once; more are joined in groups first, and no tile
+// has more than kJoin groups of kJoin.
 constexpr uint32_t kJoin = 16;
 
 struct ThinArgs {
@@ -51,9 +62,9 @@ struct ThinArgs {
     size_t q_stride;
     uint32_t n_heads, group, window;
     float scale2;  // scale * log2(e)
-    float *part;        // [n_kv][slots][16][D + 4]: sums, then m, l, mo
+    float *part;        // [n_kv][slots]: [16][D] sums, then [16][4] m, l, mo
     uint32_t *tickets;  // [n_kv][slots][2]: groups, tiles; zero between launches
-    uint32_t slots;
+    uint32_t slots, target;  // parts of all heads that the work is cut into, about
     uint32_t *err;
 };
 
@@ -88,33 +99,42 @@ struct ThinWork {
     bool any, bad;
 };
 
-// Blocks a part: all of the batch's over the launch's workgroups, evenly, and one
-// a wavefront at least.  Every wavefront finds it for itself from the lengths
-// (one load and a sum for up to 64 sequences).
-__device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, uint32_t least) {
+// Blocks a part: all of the batch's (sum) over the launch's workgroups, evenly, and
+// kLeast at least.
+__device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, float sum) {
+    const float each = ceilf(sum * (float)a.n_kv / (float)a.target);
+    return each < (float)kLeast ? kLeast : each > 1e9f ? 1000000000u : (uint32_t)each;
+}
+
+// Every wavefront finds its work for itself from the lengths (one load and two sums for
+// up to 64 sequences).
+__device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index) {
+    ThinWork w{};
+    const uint32_t lane = threadIdx.x % kWave;
     float sum = 0.0f;  // (a count beyond 2^24 need not be exact)
-    for (uint32_t r = threadIdx.x % kWave; r < a.b.n_seqs; r += kWave) {
-        const ThinRow t = thin_row(a, r);
+    ThinRow t{};
+    for (uint32_t r0 = 0; r0 < a.b.n_seqs; r0 += kWave) {
+        const uint32_t r = r0 + lane;
+        if (r >= a.b.n_seqs) break;
+        t = thin_row(a, r);
         if (t.k.falls && blockIdx.x == 0 && blockIdx.y == 0) kv_report(a.err, kKvErrRows, r);
         sum += (float)t.tiles * (float)t.blocks;
     }
+    if (a.b.n_seqs > 1) {
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-    const float each = ceilf(sum * (float)a.n_kv / (float)kThinTarget);
-    return each < (float)least ? least : each > 1e9f ? 1000000000u : (uint32_t)each;
-}
-
-__device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index, uint32_t least) {
-    ThinWork w{};
-    const uint32_t lane = threadIdx.x % kWave, share = thin_share(a, least);
+        for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+    } else {
+        sum = __uint_as_float(from_lane(__float_as_uint(sum), 0));
+    }
+    const uint32_t share = thin_share(a, sum);
     uint32_t seen = 0, joined = 0;  // workgroups and joined parts of the rows before
     for (uint32_t r0 = 0; r0 < a.b.n_seqs; r0 += kWave) {
         const uint32_t r = r0 + lane;
-        ThinRow t{};
         uint32_t splits = 0;
+        if (a.b.n_seqs > kWave) t = r < a.b.n_seqs ? thin_row(a, r) : ThinRow{};
         if (r < a.b.n_seqs) {
-            t = thin_row(a, r);
             splits = (t.blocks + share - 1) / share;
+            if (splits > kJoin * kJoin) splits = kJoin * kJoin;
         }
         const uint32_t mine = t.tiles * splits, parts = splits > 1 ? mine : 0;
         uint32_t up = mine, pup = parts;
@@ -158,61 +178,22 @@ __device__ __forceinline__ float row_max(float v) {
     return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
-// Joins `count` partial results that lie `step` floats apart into a row's sums: T
-// threads a row, thread `part` the channels 4 part + 4 T i.
-template <int D, int T>
-struct Joined {
-    static constexpr int N = (D + 4 * T - 1) / (4 * T);
-    f32x4 sum[N];
-    float m, l, mo;
-    __device__ __forceinline__ void run(const float *from, uint32_t count, size_t step, uint32_t part) {
-        m = kNegInf, mo = kNegInf, l = 0.0f;
-#pragma unroll
-        for (int k = 0; k < N; k++) sum[k] = f32x4{0, 0, 0, 0};
-        // (the largest so far, as the softmax runs: one pass, four parts' loads at once)
-        for (uint32_t i = 0; i < count; i += 4) {
-            f32x4 st[4], v[4][N];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const float *p = from + (size_t)(i + u < count ? i + u : i) * step;
-                st[u] = get4(p + D);
-#pragma unroll
-                for (int k = 0; k < N; k++) {
-                    const uint32_t d = 4 * (part + T * k);
-                    v[u][k] = get4(p + (d < D ? d : 0));
-                }
-            }
-            float m1 = m, mo1 = mo;
-#pragma unroll
-            for (int u = 0; u < 4; u++) m1 = fmaxf(m1, st[u][0]), mo1 = fmaxf(mo1, st[u][2]);
-            l *= m == kNegInf ? 1.0f : exp2f(m - m1);  // (l is 0 or NaN then)
-            const float fall = mo == kNegInf ? 1.0f : exp2f(mo - mo1);
-#pragma unroll
-            for (int k = 0; k < N; k++) sum[k] *= fall;
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                if (i + u >= count) break;
-                l += st[u][0] == kNegInf ? st[u][1] : st[u][1] * exp2f(st[u][0] - m1);
-                const float f = st[u][2] == kNegInf ? 1.0f : exp2f(st[u][2] - mo1);  // (sums of 0 or NaN)
-#pragma unroll
-                for (int k = 0; k < N; k++) sum[k] += v[u][k] * f;
-            }
-            m = m1, mo = mo1;
-        }
-    }
-};
-
 template <int D>
-__global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_attention_thin(ThinArgs a) {
-    constexpr int C = D / 32, P = D + 4, W = kThinWaves<D>, T = W * kWave / kThinRows;  // P: floats of a joined row
-    // the wavefronts' sums; with heads of 256 and more the queries lie there before
-    constexpr bool kQueriesInLds = D >= 256;
-    __shared__ __align__(16) float s_o[W][kThinRows][D + 4];
-    __shared__ float s_m[3][W][kThinRows];
+__global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attention_thin(ThinArgs a) {
+    using Sh = Shape<D>;
+    constexpr int C = Sh::C, W = Sh::kWaves, NT = Sh::kThreads, SPLIT = Sh::kSplit, NB = Sh::kBlocks, DEPTH = Sh::kDepth;
+    constexpr bool kQueriesInLds = Sh::kQueriesInLds;
+    constexpr size_t P = kThinRows * (D + 4);  // floats of a part
+    // the wavefronts' sums; the queries lie there before, where they are in LDS
+    __shared__ __align__(16) float s_o[NB][kThinRows][D + 4];
+    __shared__ f32x4 s_x[SPLIT > 1 ? 2 : 1][SPLIT > 1 ? W * 2 * kWave : 1];  // parts of q k^T, rounds in turn
+    __shared__ f32x4 s_m[NB][kThinRows];
+    __shared__ float s_f[kJoin][kThinRows], s_top[2][W][kThinRows], s_sum[W][kThinRows];
     __shared__ uint32_t s_last;
-    const uint32_t lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), h = blockIdx.y;
-    const ThinWork w = thin_work(a, blockIdx.x, W);
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, g = lane / 16, n = lane % 16;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / kWave), h = blockIdx.y;
+    const uint32_t cut = wave % SPLIT, which = wave / SPLIT;  // channels, block of a round
+    const ThinWork w = thin_work(a, blockIdx.x);
     if (!w.any) return;
     const uint32_t row = w.row;
     const uint32_t rows = w.n * a.group - w.tile * kThinRows;  // of this tile (more: 16)
@@ -232,47 +213,73 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
         b1 = min(b1, (uint32_t)pos1 / kKvBlock + 1);
     } else {
         b1 = b0;
-        if (threadIdx.x == 0 && h == 0) kv_report(a.err, kKvErrRows, row);
+        if (tid == 0 && h == 0) kv_report(a.err, kKvErrRows, row);
     }
     const uint32_t *table = a.b.table + (size_t)row * a.b.max_blocks;
 
+    const uint32_t mine = b0 + which < b1 ? (b1 - b0 - which + NB - 1) / NB : 0;  // blocks of this wavefront
+    const uint32_t rounds = SPLIT == 1 ? mine : b0 < b1 ? (b1 - b0 + NB - 1) / NB : 0;
     // The pages and scales of a wavefront's next 64 blocks, a block a lane: i is block
-    // b0 + wave + W * i.  Keys' scale, and log2 of the values' (a block of zeros: any).
+    // b0 + which + NB * i.  lost: blocks that the cache does not have.
     uint32_t page_l = 0;
-    float ks_l = 0.0f, lv_l = 0.0f;
+    float2 scales_n = make_float2(0.0f, 0.0f), scales_l = scales_n;
+    uint64_t lost_n = 0, lost_l = 0;
     const auto pages = [&](uint32_t i) {
-        const uint32_t j = b0 + wave + W * i;
-        if (j >= b1) return;
-        page_l = table[j];
-        const bool lost = page_l >= a.n_blocks;
-        if (lost) {
-            page_l = 0;
-            if (h == 0) kv_report(a.err, kKvErrBlock, row);
+        page_l = table[b0 + which + NB * (i < mine ? i : mine - 1)];
+        lost_n = __ballot(page_l >= a.n_blocks);
+        if (lost_n) {
+            if (page_l >= a.n_blocks) {
+                page_l = 0;
+                if (h == 0) kv_report(a.err, kKvErrBlock, row);
+            }
         }
-        const float2 s = a.scales[(size_t)page_l * a.n_kv + h];
-        ks_l = lost ? __builtin_nanf("") : s.x;
-        lv_l = lost ? __builtin_nanf("") : s.y == 0.0f ? 0.0f : log2f(s.y);
+        scales_n = a.scales[(size_t)page_l * a.n_kv + h];
     };
-    pages(lane);
+    const auto load = [&](uint4 *to, uint32_t i, int of) {
+        const uint32_t page = from_lane(page_l, i % kWave);
+        const uint4 *p = reinterpret_cast<const uint4 *>(a.codes + (((size_t)page * a.n_kv + h) * 2 + of) * (kKvBlock * D)) +
+                         cut * C * kWave + lane;
+#pragma unroll
+        for (int c = 0; c < C; c++) to[c] = p[c * kWave];
+    };
+    const float *qp = a.q + (size_t)(w.first + token) * a.q_stride + (size_t)head * D + 8 * g;
+    float4 qx[C][2];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        qx[c][0] = *reinterpret_cast<const float4 *>(qp + 32 * (cut * C + c));
+        qx[c][1] = *reinterpret_cast<const float4 *>(qp + 32 * (cut * C + c) + 4);
+    }
+    if (mine) pages(lane);
+    uint4 kq[DEPTH][C], vq[DEPTH][C];
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+        if ((uint32_t)d < mine) {
+            load(kq[d], d, 0);
+            load(vq[d], d, 1);
+        }
 
     // the queries' two parts, scaled to 2^14 .. 2^15 by a power of two
     half8 qh[kQueriesInLds ? 1 : C], ql[kQueriesInLds ? 1 : C];
-    half8 *s_q = reinterpret_cast<half8 *>(&s_o[0][0][0]);  // [C][2][64]
+    half8 *s_q = reinterpret_cast<half8 *>(&s_o[0][0][0]);  // [SPLIT][C][2][64]
     float c_row;
     {
-        const float *qp = a.q + (size_t)(w.first + token) * a.q_stride + (size_t)head * D + 8 * g;
         float top = 0.0f;
         bool fine = true;
-        float x[C][8];
+        const auto look = [&](float4 v) {
+            const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const float4 u = *reinterpret_cast<const float4 *>(qp + 32 * c), v = *reinterpret_cast<const float4 *>(qp + 32 * c + 4);
-            const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[c][i] = e[i];
+            for (int i = 0; i < 4; i++) {
                 top = fmaxf(top, fabsf(e[i]));
                 fine &= fabsf(e[i]) <= 3.402823466e38f;
+            }
+        };
+#pragma unroll
+        for (int c = 0; c < C; c++) look(qx[c][0]), look(qx[c][1]);
+        if (SPLIT > 1) {  // (the other wavefront's channels too)
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                look(*reinterpret_cast<const float4 *>(qp + 32 * ((cut ^ 1) * C + c)));
+                look(*reinterpret_cast<const float4 *>(qp + 32 * ((cut ^ 1) * C + c) + 4));
             }
         }
         const bool bad = row_max(fine ? 0.0f : 1.0f) > 0.0f;
@@ -284,17 +291,18 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
         const bool minus = a.scale2 < 0.0f;  // (the logits' factor is not negative: the largest stays it)
 #pragma unroll
         for (int c = 0; c < C; c++) {
+            const float f[8] = {qx[c][0].x, qx[c][0].y, qx[c][0].z, qx[c][0].w, qx[c][1].x, qx[c][1].y, qx[c][1].z, qx[c][1].w};
             half8 hi, lo;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float y = bad ? 0.0f : ldexpf(minus ? -x[c][i] : x[c][i], e);
+                const float y = bad ? 0.0f : ldexpf(minus ? -f[i] : f[i], e);
                 hi[i] = (_Float16)y;
                 lo[i] = (_Float16)(y - (float)hi[i]);
             }
             if (!kQueriesInLds) {
                 qh[kQueriesInLds ? 0 : c] = hi, ql[kQueriesInLds ? 0 : c] = lo;
-            } else if (c % W == (int)wave) {
-                s_q[(c * 2) * kWave + lane] = hi, s_q[(c * 2 + 1) * kWave + lane] = lo;
+            } else if (c % NB == (int)which) {
+                s_q[((cut * C + c) * 2) * kWave + lane] = hi, s_q[((cut * C + c) * 2 + 1) * kWave + lane] = lo;
             }
         }
     }
@@ -305,144 +313,175 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
     for (int i = 0; i < 2 * C; i++) o[i] = f32x4{0, 0, 0, 0};
     float m = kNegInf, l = 0.0f, mo = kNegInf;
 
-    uint4 kq[C], vq[C];
-    const auto load = [&](uint4 *to, uint32_t page, int which) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(a.codes + (((size_t)page * a.n_kv + h) * 2 + which) * (kKvBlock * D)) + lane;
-#pragma unroll
-        for (int c = 0; c < C; c++) to[c] = p[c * kWave];
-    };
-    const uint32_t mine = b0 + wave < b1 ? (b1 - b0 - wave + W - 1) / W : 0;  // blocks of this wavefront
-    for (uint32_t i0 = 0; i0 < mine; i0 += kWave) {
-        if (i0) pages(i0 + lane);
-        const uint32_t here = mine - i0 < kWave ? mine - i0 : kWave;
-        load(kq, from_lane(page_l, 0), 0);
-        load(vq, from_lane(page_l, 0), 1);
-        for (uint32_t i = 0; i < here; i++) {
-            const uint32_t next = from_lane(page_l, i + 1 < here ? i + 1 : i);
-            const float ks = __uint_as_float(from_lane(__float_as_uint(ks_l), i));
-            const float lv = __uint_as_float(from_lane(__float_as_uint(lv_l), i));
-            f32x4 sa[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, sb[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    const auto block = [&](uint32_t i, uint4 (&kx)[C], uint4 (&vx)[C]) {
+        const bool on = i < mine;
+        if (i % kWave == 0) scales_l = scales_n, lost_l = lost_n;
+        f32x4 sa[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, sb[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+        if (on) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const half8 k0 = codes8(kq[c].x, kq[c].y), k1 = codes8(kq[c].z, kq[c].w);
-                const half8 hi = kQueriesInLds ? s_q[(c * 2) * kWave + lane] : qh[kQueriesInLds ? 0 : c];
-                const half8 lo = kQueriesInLds ? s_q[(c * 2 + 1) * kWave + lane] : ql[kQueriesInLds ? 0 : c];
+                const half8 k0 = codes8(kx[c].x, kx[c].y), k1 = codes8(kx[c].z, kx[c].w);
+                const half8 hi = kQueriesInLds ? s_q[((cut * C + c) * 2) * kWave + lane] : qh[kQueriesInLds ? 0 : c];
+                const half8 lo = kQueriesInLds ? s_q[((cut * C + c) * 2 + 1) * kWave + lane] : ql[kQueriesInLds ? 0 : c];
                 sa[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, hi, sa[0], 0, 0, 0);
                 sa[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, hi, sa[1], 0, 0, 0);
                 sb[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, lo, sb[0], 0, 0, 0);
                 sb[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, lo, sb[1], 0, 0, 0);
             }
-            if (i + 1 < here) load(kq, next, 0);
-            // keys 32 j + 16 (e / 4) + 4 g + e % 4
-            const uint32_t j = b0 + wave + W * (i0 + i);
-            float t[8];
+            sa[0] += sb[0], sa[1] += sb[1];
+        }
+        // (64 blocks on, page_l holds the next 64)
+        const bool more = i + DEPTH < mine;
+        if (more && (i + DEPTH) % kWave == 0) pages(i + DEPTH + lane);
+        if (more) load(kx, i + DEPTH, 0);
+        if (SPLIT > 1) {
+            s_x[i % 2][(wave * 2) * kWave + lane] = sa[0], s_x[i % 2][(wave * 2 + 1) * kWave + lane] = sa[1];
+            __syncthreads();
+            sa[0] += s_x[i % 2][((wave ^ 1) * 2) * kWave + lane], sa[1] += s_x[i % 2][((wave ^ 1) * 2 + 1) * kWave + lane];
+        }
+        if (!on) return;
+        // keys 32 j + 16 (e / 4) + 4 g + e % 4
+        const uint32_t j = b0 + which + NB * i;
+        float t[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) t[e] = sa[e / 4][e % 4] + sb[e / 4][e % 4];
-            const bool edge = (int)(j * kKvBlock + kKvBlock - 1) > pos0 || (int)(j * kKvBlock) < low1;
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int key = (int)(j * kKvBlock + 4 * g) + 16 * (e / 4) + e % 4;
-                    if (key > pos || key < low) t[e] = kNegInf;
-                }
-            }
-            const float c = c_row * ks;
-            float mb = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
-            mb = row_max(mb);
-            mb = mb == kNegInf ? mb : mb * c;
-            const float m1 = fmaxf(m, mb), mo1 = fmaxf(mo, mb + lv);
-            const float ms = m1 == kNegInf ? 0.0f : m1;  // (no key yet)
-            if (__any(m1 > m || mo1 > mo)) {
-                l *= __builtin_amdgcn_exp2f(m - ms);  // (0 before the first key)
-                const float fall = mo == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mo - mo1);
-#pragma unroll
-                for (int k = 0; k < 2 * C; k++) o[k] *= fall;
-            }
-            m = m1, mo = mo1;
-            // (a weight of less than 2^-60 of the largest need not be that small among the sums, but counts in l)
-            float e15 = fmaxf(lv - mo1, -60.0f - ms) + 15.0f;
-            if (lv != lv) e15 = lv;
-            float p[8], sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(t[e], c, e15));
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (t[e] == kNegInf) p[e] = 0.0f;  // (what is not seen adds nothing, whatever its scale)
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) sum += p[e];
-            if (mo1 != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-e15 - ms);
-            half8 ph, pl;
+        for (int e = 0; e < 8; e++) t[e] = sa[e / 4][e % 4];
+        const bool edge = (int)(j * kKvBlock + kKvBlock - 1) > pos0 || (int)(j * kKvBlock) < low1;
+        if (edge) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const _Float16 hi = (_Float16)p[e];
-                ph[e] = hi;
-                pl[e] = (_Float16)(p[e] - (float)hi);
+                const int key = (int)(j * kKvBlock + 4 * g) + 16 * (e / 4) + e % 4;
+                if (key > pos || key < low) t[e] = kNegInf;
             }
-#pragma unroll
-            for (int k = 0; k < C; k++) {
-                const half8 v0 = codes8(vq[k].x, vq[k].y), v1 = codes8(vq[k].z, vq[k].w);
-                o[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[2 * k], 0, 0, 0);
-                o[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[2 * k + 1], 0, 0, 0);
-                o[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, o[2 * k], 0, 0, 0);
-                o[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, o[2 * k + 1], 0, 0, 0);
-            }
-            if (i + 1 < here) load(vq, next, 1);
         }
+        // keys' scale, and log2 of the values' (a block of zeros: any)
+        const bool lost = lost_l >> (i % kWave) & 1;
+        const float ks = lost ? __builtin_nanf("") : __uint_as_float(from_lane(__float_as_uint(scales_l.x), i % kWave));
+        const float vs = lost ? __builtin_nanf("") : __uint_as_float(from_lane(__float_as_uint(scales_l.y), i % kWave));
+        const float lv = vs == 0.0f ? 0.0f : log2f(vs);
+        const float c = c_row * ks;
+        float mb = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+        mb = row_max(mb);
+        mb = mb == kNegInf ? mb : mb * c;
+        const float m1 = fmaxf(m, mb), mo1 = fmaxf(mo, mb + lv);
+        const float ms = m1 == kNegInf ? 0.0f : m1;  // (no key yet)
+        if (__any(m1 > m || mo1 > mo)) {
+            l *= __builtin_amdgcn_exp2f(m - ms);  // (0 before the first key)
+            const float fall = mo == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mo - mo1);
+#pragma unroll
+            for (int k = 0; k < 2 * C; k++) o[k] *= fall;
+        }
+        m = m1, mo = mo1;
+        // (a weight of less than 2^-60 of the largest need not be that small among the sums, but counts in l)
+        float e15 = fmaxf(lv - mo1, -60.0f - ms) + 15.0f;
+        if (lv != lv) e15 = lv;
+        float p[8], sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(t[e], c, e15));
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (t[e] == kNegInf) p[e] = 0.0f;  // (what is not seen adds nothing, whatever its scale)
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum += p[e];
+        if (mo1 != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-e15 - ms);
+        half8 ph, pl;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const _Float16 hi = (_Float16)p[e];
+            ph[e] = hi;
+            pl[e] = (_Float16)(p[e] - (float)hi);
+        }
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const half8 v0 = codes8(vx[k].x, vx[k].y), v1 = codes8(vx[k].z, vx[k].w);
+            o[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[2 * k], 0, 0, 0);
+            o[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[2 * k + 1], 0, 0, 0);
+            o[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, o[2 * k], 0, 0, 0);
+            o[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, o[2 * k + 1], 0, 0, 0);
+        }
+        if (more) load(vx, i + DEPTH, 1);
+    };
+    for (uint32_t i = 0; i < rounds; i += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+            if (DEPTH == 1 || i + d < rounds) block(i + d, kq[d], vq[d]);
     }
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
 
     // the wavefronts' parts joined through LDS
-    if (g == 0) s_m[0][wave][n] = m, s_m[1][wave][n] = l, s_m[2][wave][n] = mo;
+    if (g == 0 && cut == 0) s_m[which][n] = f32x4{m, l, mo, 0.0f};
     if (kQueriesInLds) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2 * C; i++) *reinterpret_cast<f32x4 *>(&s_o[wave][n][16 * i + 4 * g]) = o[i];
+    for (int i = 0; i < 2 * C; i++) *reinterpret_cast<f32x4 *>(&s_o[which][n][cut * Sh::DW + 16 * i + 4 * g]) = o[i];
     __syncthreads();
-    // a row's channels over T threads
-    const uint32_t rr = threadIdx.x / T, part = threadIdx.x % T;
-    const uint32_t r1 = w.tile * kThinRows + rr;
-    float *out = a.out + ((size_t)(w.first + r1 / a.group) * a.n_heads + h * a.group + r1 % a.group) * D;
-    float *mine_p = a.part + (((size_t)h * a.slots + w.slot) * kThinRows + rr) * P;
-    if (rr < rows_in) {
-        float mt = kNegInf, mot = kNegInf, lt_ = 0.0f, fo[W];
+    // Row rr's place among the sums and the outputs: its channels in fours, over the workgroup.
+    const auto out_of = [&](uint32_t rr) {
+        const uint32_t r1 = w.tile * kThinRows + rr;
+        return a.out + ((size_t)(w.first + r1 / a.group) * a.n_heads + h * a.group + r1 % a.group) * D;
+    };
+    const auto place = [&](uint32_t slot) { return a.part + ((size_t)h * a.slots + slot) * P; };
+    // Parts' m, l, mo to the rows' common ones: thread 16 i + row has part i's of a row.
+    // Leaves each part's factor in s_f, each row's m and mo in s_top and l's terms in s_sum, a wavefront's each.
+    static_assert(NT == kJoin * kThinRows, "a part and row a thread");
+    const auto weigh = [&](uint32_t count, f32x4 st) {
+        const uint32_t i = tid / kThinRows;
+        float tm = i < count ? st[0] : kNegInf, tmo = i < count ? st[2] : kNegInf;
 #pragma unroll
-        for (int i = 0; i < W; i++) mt = fmaxf(mt, s_m[0][i][rr]), mot = fmaxf(mot, s_m[2][i][rr]);
+        for (int off = 16; off < kWave; off <<= 1)
+            tm = fmaxf(tm, __shfl_xor(tm, off, kWave)), tmo = fmaxf(tmo, __shfl_xor(tmo, off, kWave));
+        if (g == 0) s_top[0][wave][n] = tm, s_top[1][wave][n] = tmo;
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const float mi = s_m[0][i][rr], moi = s_m[2][i][rr], li = s_m[1][i][rr];
-            lt_ += mi == kNegInf ? li : li * exp2f(mi - mt);  // (l is 0 or NaN without a largest)
-            fo[i] = moi == kNegInf ? 1.0f : exp2f(moi - mot);
+        for (int k = 0; k < W; k++) tm = fmaxf(tm, s_top[0][k][n]), tmo = fmaxf(tmo, s_top[1][k][n]);
+        float l_i = i < count ? st[0] == kNegInf ? st[1] : st[1] * exp2f(st[0] - tm) : 0.0f;  // (l is 0 or NaN without a largest)
+        s_f[i][n] = st[2] == kNegInf ? 1.0f : exp2f(st[2] - tmo);                             // (sums of 0 or NaN)
+#pragma unroll
+        for (int off = 16; off < kWave; off <<= 1) l_i += __shfl_xor(l_i, off, kWave);
+        if (g == 0) s_sum[wave][n] = l_i;
+        __syncthreads();
+    };
+    const auto stat_of = [&](uint32_t rr) {
+        f32x4 st = {kNegInf, 0.0f, kNegInf, 0.0f};
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            st[0] = fmaxf(st[0], s_top[0][k][rr]), st[2] = fmaxf(st[2], s_top[1][k][rr]);
+            st[1] += s_sum[k][rr];
         }
-        const float scale = w.splits > 1 ? 1.0f : w.bad ? __builtin_nanf("") : out_scale(mt, lt_, mot, 15.0f);
+        return st;
+    };
+    const auto stats_to = [&](float *p) {
+        if (tid < rows_in) put4(p + kThinRows * D + 4 * tid, stat_of(tid));
+    };
+    const auto scale_of = [&](uint32_t rr) {
+        const f32x4 st = stat_of(rr);
+        return w.bad ? __builtin_nanf("") : out_scale(st[0], st[1], st[2], 15.0f);
+    };
+    weigh(NB, s_m[tid / kThinRows % NB][n]);
+    for (uint32_t at = tid; at < rows_in * (D / 4); at += NT) {
+        const uint32_t rr = at / (D / 4), d = at % (D / 4) * 4;
+        f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < (D + 4 * T - 1) / (4 * T); i++) {
-            const uint32_t d = 4 * (part + T * i);
-            if (d >= D) break;
-            f32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-            for (int u = 0; u < W; u++) sum += *reinterpret_cast<const f32x4 *>(&s_o[u][rr][d]) * fo[u];
-            if (w.splits > 1) put4(mine_p + d, sum);
-            else *reinterpret_cast<f32x4 *>(out + d) = sum * scale;
-        }
-        if (w.splits > 1 && part == 0) put4(mine_p + D, f32x4{mt, lt_, mot, 0});
+        for (int i = 0; i < NB; i++) sum += *reinterpret_cast<const f32x4 *>(&s_o[i][rr][d]) * s_f[i][rr];
+        if (w.splits > 1) put4(place(w.slot) + rr * D + d, sum);
+        else *reinterpret_cast<f32x4 *>(out_of(rr) + d) = sum * scale_of(rr);
     }
     if (w.splits == 1) return;
+    stats_to(place(w.slot));
 
     // The part that is last at its group joins the group, the group that is last at its
     // tile the tile.  A part's stores are acknowledged before it counts; the one that
     // counts last reads past the L2s, and leaves the counters at zero.
-    const uint32_t groups = (w.splits + kJoin - 1) / kJoin, in_group = (w.splits + groups - 1) / groups;
-    const uint32_t grp = w.split / in_group, slot0 = w.slot - w.split;
-    const uint32_t g0 = slot0 + grp * in_group;
+    const uint32_t in_group = w.splits <= kJoin ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
+    const uint32_t grp = w.split / in_group, slot0 = w.slot - w.split, g0 = slot0 + grp * in_group;
     const uint32_t gn = w.splits - grp * in_group < in_group ? w.splits - grp * in_group : in_group;
-    const uint32_t used_groups = (w.splits + in_group - 1) / in_group;
+    const uint32_t groups = (w.splits + in_group - 1) / in_group;
     uint32_t *tickets = a.tickets + (size_t)h * a.slots * 2;
     const auto last = [&](uint32_t *t, uint32_t count) -> bool {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (tid == 0) {
             const bool is = __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == count - 1;
             if (is) __hip_atomic_store(t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             s_last = is;
@@ -450,35 +489,41 @@ __global__ __launch_bounds__(kThinWaves<D> *kWave, D <= 256 ? 2 : 1) void k_atte
         __syncthreads();
         return s_last;
     };
-    if (!last(tickets + 2 * g0, gn)) return;
-    Joined<D, T> sums;
-    const size_t step = (size_t)kThinRows * P;
-    const float *from = a.part + (((size_t)h * a.slots + g0) * kThinRows + rr) * P;
-    if (rr < rows_in) sums.run(from, gn, step, part);
-    if (used_groups > 1) {
-        // (the group's first part's place now holds the group's sums)
-        float *to = const_cast<float *>(from);
-        __syncthreads();
-        if (rr < rows_in) {
+    // Parts slot, slot + step, ..: their sums to `to`, or to the outputs.  The sums are under
+    // way before the factors are found.
+    const auto join = [&](uint32_t slot, uint32_t step, uint32_t count, float *to) {
+        const uint32_t i0 = tid / kThinRows;
+        const f32x4 st = get4(place(slot + (i0 < count ? i0 : 0) * step) + kThinRows * D + 4 * n);
+        f32x4 v[kJoin];
+        const auto fetch = [&](uint32_t at) {
 #pragma unroll
-            for (int k = 0; k < Joined<D, T>::N; k++) {
-                const uint32_t d = 4 * (part + T * k);
-                if (d < D) put4(to + d, sums.sum[k]);
+            for (uint32_t u = 0; u < kJoin; u++) {
+                if (u % 4 == 0 && u >= count) break;
+                v[u] = get4(place(slot + (u < count ? u : 0) * step) + 4 * at);
             }
-            if (part == 0) put4(to + D, f32x4{sums.m, sums.l, sums.mo, 0});
-        }
-        if (!last(tickets + 2 * slot0 + 1, used_groups)) return;
-        from = a.part + (((size_t)h * a.slots + slot0) * kThinRows + rr) * P;
-        if (rr < rows_in) sums.run(from, used_groups, step * in_group, part);
-    }
-    if (rr < rows_in) {
-        const float scale = out_scale(sums.m, sums.l, sums.mo, 15.0f);
+        };
+        const uint32_t all = rows_in * (D / 4);
+        if (tid < all) fetch(tid);
+        weigh(count, st);
+        for (uint32_t at = tid; at < all; at += NT) {
+            const uint32_t rr = at / (D / 4), d = at % (D / 4) * 4;
+            if (at != tid) fetch(at);
+            f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < Joined<D, T>::N; k++) {
-            const uint32_t d = 4 * (part + T * k);
-            if (d < D) *reinterpret_cast<f32x4 *>(out + d) = sums.sum[k] * scale;
+            for (uint32_t u = 0; u < kJoin; u++)
+                if (u < count) sum += v[u] * s_f[u][rr];
+            if (to) put4(to + rr * D + d, sum);
+            else *reinterpret_cast<f32x4 *>(out_of(rr) + d) = sum * scale_of(rr);
         }
+        if (to) stats_to(to);
+    };
+    if (!last(tickets + 2 * g0, gn)) return;
+    if (groups == 1) {
+        join(g0, 1, gn, nullptr);
+        return;
     }
+    join(g0, 1, gn, place(g0));  // (each thread has read its own of the group's first place before it writes there)
+    if (last(tickets + 2 * slot0 + 1, groups)) join(slot0, in_group, groups, nullptr);
 }
 
 // Workgroups of a head: a tile more or less a sequence, and the parts of those
@@ -492,12 +537,25 @@ uint32_t thin_tiles(const AttnArgs &a) {
     if (rows < tiles) tiles = rows;
     return (uint32_t)tiles;
 }
-uint32_t thin_slots(uint32_t n_kv) { return 2 * (kThinTarget / n_kv + 1) + 2; }
+uint32_t thin_slots(uint32_t target, uint32_t n_kv) { return 2 * (target / n_kv + 1) + 2; }
 
 template <int D>
-void go(const ThinArgs &t, uint32_t tiles, hipStream_t s) {
-    const dim3 grid(tiles + kThinTarget / t.n_kv + 1, t.n_kv);
-    hipLaunchKernelGGL(k_attention_thin<D>, grid, dim3(kThinWaves<D> * kWave), 0, s, t);
+void go(ThinArgs t, uint32_t tiles, hipStream_t s) {
+    const uint32_t each = (t.b.max_blocks + kLeast - 1) / kLeast;  // (a tile's parts, at most)
+    uint64_t x = tiles + t.target / t.n_kv + 1;
+    if ((uint64_t)tiles * each < x) x = (uint64_t)tiles * each;
+    hipLaunchKernelGGL(k_attention_thin<D>, dim3((uint32_t)x, t.n_kv), dim3(Shape<D>::kThreads), 0, s, t);
+}
+
+uint32_t thin_target(uint32_t D) {
+    switch (D) {
+    case 64: return 256 * Shape<64>::kTarget;
+    case 96: return 256 * Shape<96>::kTarget;
+    case 128: return 256 * Shape<128>::kTarget;
+    case 192: return 256 * Shape<192>::kTarget;
+    case 256: return 256 * Shape<256>::kTarget;
+    default: return 256 * Shape<512>::kTarget;
+    }
 }
 
 }  // namespace
@@ -508,7 +566,7 @@ bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D
 static bool wide(const AttnArgs &a) { return (uint64_t)(a.b.max_new ? a.b.max_new : a.b.n_tokens) * a.group > kThinMost; }
 
 size_t attention_workspace(const AttnArgs &a) {
-    const size_t thin = (size_t)a.kv.n_kv * thin_slots(a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
+    const size_t thin = (size_t)a.kv.n_kv * thin_slots(thin_target(a.kv.D), a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
     const size_t more = wide(a) ? attention_wide_workspace(a.kv.D) : 0;
     return thin < more ? more : thin;
 }
@@ -522,7 +580,8 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
     t.codes = a.kv.codes, t.scales = a.kv.scales, t.n_blocks = a.kv.n_blocks, t.n_kv = a.kv.n_kv, t.b = a.b;
     t.q = a.q, t.out = a.out, t.q_stride = a.q_stride, t.n_heads = a.n_heads, t.group = a.group, t.window = a.window;
     t.scale2 = a.scale * 1.4426950408889634f;
-    t.part = (float *)a.work, t.tickets = a.tickets, t.slots = thin_slots(t.n_kv), t.err = a.err;
+    t.part = (float *)a.work, t.tickets = a.tickets, t.err = a.err;
+    t.target = thin_target(a.kv.D), t.slots = thin_slots(t.target, t.n_kv);
     const uint32_t tiles = thin_tiles(a);
     switch (a.kv.D) {
     case 64: go<64>(t, tiles, s); break;
