@@ -30,26 +30,36 @@ namespace lt {
 
 namespace {
 
-#ifndef TGT
-#define TGT 3
-#endif
 constexpr int kThinRows = 16;
-// Wavefronts of a workgroup that a block's channels are cut over, wavefronts, workgroups a
+#ifndef ALONE
+#define ALONE 3
+#endif
+#ifndef WB
+#define WB 8
+#endif
+#ifndef DEP
+#define DEP 1
+#endif
+#ifndef LROUNDS
+#define LROUNDS 1
+#endif
+#ifndef TGT
+#define TGT 2
+#endif
+// Wavefronts a workgroup, wavefronts that a block's channels are cut over, workgroups a
 // CU, blocks a wavefront has under way.
 template <int D>
 struct Shape {
-    static constexpr int kSplit = D <= 256 ? 1 : 2, kWaves = 4, kPerCu = D <= 128 ? 3 : D <= 256 ? 2 : 1, kTarget = kPerCu < TGT ? kPerCu : TGT, kDepth = D <= 64 ? 4 : 1;
+    static constexpr int kWaves = D <= 128 ? 8 : D <= 256 ? WB : 8, kSplit = D <= 256 ? 1 : 2;
+    static constexpr int kPerCu = (D <= 128 ? 16 : 8) / kWaves, kTarget = kPerCu < TGT ? kPerCu : TGT;
+    static constexpr int kDepth = D <= 64 ? DEP : 1;
     static constexpr int kThreads = kWaves * kWave, kBlocks = kWaves / kSplit;  // blocks a round
     static constexpr int DW = D / kSplit, C = DW / 32;
-    static constexpr bool kQueriesInLds = DW >= 256;
+    static constexpr bool kQueriesInLds = DW >= 256 || D == 128;
+    static constexpr uint32_t kLeast = LROUNDS * kBlocks;  // blocks that a part is worth having for
 };
-// Blocks that a part is worth having for.
-#ifndef LEAST
-#define LEAST 8
-#endif
-constexpr uint32_t kLeast = LEAST;
-// Parts of a tile that are joined at once; more are joined in groups first, and no tile
-// has more than kJoin groups of kJoin.
+// Parts of a tile that are joined at once (or 8 for each time that the workgroup's threads
+// are more than a part's places); more are joined in groups first, and no tile has more than the square.
 constexpr uint32_t kJoin = 16;
 
 struct ThinArgs {
@@ -65,6 +75,7 @@ struct ThinArgs {
     float *part;        // [n_kv][slots]: [16][D] sums, then [16][4] m, l, mo
     uint32_t *tickets;  // [n_kv][slots][2]: groups, tiles; zero between launches
     uint32_t slots, target;  // parts of all heads that the work is cut into, about
+    uint32_t least;          // blocks a part, at least
     uint32_t *err;
 };
 
@@ -99,11 +110,19 @@ struct ThinWork {
     bool any, bad;
 };
 
-// Blocks a part: all of the batch's (sum) over the launch's workgroups, evenly, and
-// kLeast at least.
+// Blocks a part: all of the batch's (sum) over the launch's workgroups, evenly.
 __device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, float sum) {
     const float each = ceilf(sum * (float)a.n_kv / (float)a.target);
-    return each < (float)kLeast ? kLeast : each > 1e9f ? 1000000000u : (uint32_t)each;
+    return each < (float)a.least ? a.least : each > 1e9f ? 1000000000u : (uint32_t)each;
+}
+
+// A tile's parts.  None where a workgroup has its blocks done before parts are joined; parts of
+// `least` where there are few, for their latency; else no more parts than the chip has room for at once.
+__device__ __forceinline__ uint32_t thin_splits(const ThinArgs &a, uint32_t blocks, uint32_t share) {
+    if (blocks <= ALONE * a.least) return 1;
+    uint32_t n = share > a.least ? blocks / share : (blocks + share - 1) / share;
+    if (n == 0) n = 1;
+    return n < kJoin * kJoin ? n : kJoin * kJoin;
 }
 
 // Every wavefront finds its work for itself from the lengths (one load and two sums for
@@ -133,8 +152,7 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
         uint32_t splits = 0;
         if (a.b.n_seqs > kWave) t = r < a.b.n_seqs ? thin_row(a, r) : ThinRow{};
         if (r < a.b.n_seqs) {
-            splits = (t.blocks + share - 1) / share;
-            if (splits > kJoin * kJoin) splits = kJoin * kJoin;
+            splits = thin_splits(a, t.blocks, share);
         }
         const uint32_t mine = t.tiles * splits, parts = splits > 1 ? mine : 0;
         uint32_t up = mine, pup = parts;
@@ -178,17 +196,41 @@ __device__ __forceinline__ float row_max(float v) {
     return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
+// Sums of parts and what they are sums to.
+struct Joint {
+    f32x4 sum;
+    float m, l, mo;
+    __device__ __forceinline__ void clear() { sum = f32x4{0, 0, 0, 0}, m = kNegInf, mo = kNegInf, l = 0.0f; }
+    // `count` parts more (N at most): their m, l, mo and sums
+    template <int N>
+    __device__ __forceinline__ void add(const f32x4 (&st)[N], const f32x4 (&v)[N], uint32_t count) {
+        float m1 = m, mo1 = mo;
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            if (i < count) m1 = fmaxf(m1, st[i][0]), mo1 = fmaxf(mo1, st[i][2]);
+        l *= m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m1);  // (l is 0 or NaN without a largest)
+        sum *= mo == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mo - mo1);  // (sums of 0 or NaN)
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            if (i < count) {
+                l += st[i][0] == kNegInf ? st[i][1] : st[i][1] * __builtin_amdgcn_exp2f(st[i][0] - m1);
+                sum += v[i] * (st[i][2] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(st[i][2] - mo1));
+            }
+        m = m1, mo = mo1;
+    }
+};
+
 template <int D>
-__global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attention_thin(ThinArgs a) {
+__global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_attention_thin(ThinArgs a) {
     using Sh = Shape<D>;
-    constexpr int C = Sh::C, W = Sh::kWaves, NT = Sh::kThreads, SPLIT = Sh::kSplit, NB = Sh::kBlocks, DEPTH = Sh::kDepth;
+    constexpr int W = Sh::kWaves, C = Sh::C, NT = Sh::kThreads, SPLIT = Sh::kSplit, NB = Sh::kBlocks, DEPTH = Sh::kDepth;
     constexpr bool kQueriesInLds = Sh::kQueriesInLds;
+    constexpr uint32_t kBatch = D <= 128 ? 8 : 16;  // parts that a thread reads at once
     constexpr size_t P = kThinRows * (D + 4);  // floats of a part
     // the wavefronts' sums; the queries lie there before, where they are in LDS
     __shared__ __align__(16) float s_o[NB][kThinRows][D + 4];
-    __shared__ f32x4 s_x[SPLIT > 1 ? 2 : 1][SPLIT > 1 ? W * 2 * kWave : 1];  // parts of q k^T, rounds in turn
     __shared__ f32x4 s_m[NB][kThinRows];
-    __shared__ float s_f[kJoin][kThinRows], s_top[2][W][kThinRows], s_sum[W][kThinRows];
+    __shared__ float s_top[SPLIT > 1 ? W : 1][kThinRows];
     __shared__ uint32_t s_last;
     const uint32_t tid = threadIdx.x, lane = tid % kWave, g = lane / 16, n = lane % 16;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / kWave), h = blockIdx.y;
@@ -222,8 +264,9 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
     // The pages and scales of a wavefront's next 64 blocks, a block a lane: i is block
     // b0 + which + NB * i.  lost: blocks that the cache does not have.
     uint32_t page_l = 0;
-    float2 scales_n = make_float2(0.0f, 0.0f), scales_l = scales_n;
-    uint64_t lost_n = 0, lost_l = 0;
+    float2 scales_n = make_float2(0.0f, 0.0f);
+    float ks_l = 0.0f, lv_l = 0.0f;  // keys' scale, and log2 of the values' (a block of zeros: any)
+    uint64_t lost_n = 0;
     const auto pages = [&](uint32_t i) {
         page_l = table[b0 + which + NB * (i < mine ? i : mine - 1)];
         lost_n = __ballot(page_l >= a.n_blocks);
@@ -261,6 +304,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
     // the queries' two parts, scaled to 2^14 .. 2^15 by a power of two
     half8 qh[kQueriesInLds ? 1 : C], ql[kQueriesInLds ? 1 : C];
     half8 *s_q = reinterpret_cast<half8 *>(&s_o[0][0][0]);  // [SPLIT][C][2][64]
+    f32x4 *s_x = reinterpret_cast<f32x4 *>(s_q + D * 4);    // parts of q k^T, two rounds in turn, [2][W][2][64]
+    static_assert(SPLIT == 1 || sizeof s_o >= (D * 4 + 4 * W * kWave) * 16, "both lie in s_o");
     float c_row;
     {
         float top = 0.0f;
@@ -275,15 +320,13 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         };
 #pragma unroll
         for (int c = 0; c < C; c++) look(qx[c][0]), look(qx[c][1]);
+        top = row_max(fine ? top : __builtin_inff());
         if (SPLIT > 1) {  // (the other wavefront's channels too)
-#pragma unroll
-            for (int c = 0; c < C; c++) {
-                look(*reinterpret_cast<const float4 *>(qp + 32 * ((cut ^ 1) * C + c)));
-                look(*reinterpret_cast<const float4 *>(qp + 32 * ((cut ^ 1) * C + c) + 4));
-            }
+            if (g == 0) s_top[wave][n] = top;
+            __syncthreads();
+            top = fmaxf(top, s_top[wave ^ 1][n]);
         }
-        const bool bad = row_max(fine ? 0.0f : 1.0f) > 0.0f;
-        top = row_max(top);
+        const bool bad = top > 3.402823466e38f;
         int e = 0;
         (void)frexpf(top, &e);
         e = top > 0.0f ? 15 - e : 0;
@@ -315,29 +358,33 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
 
     const auto block = [&](uint32_t i, uint4 (&kx)[C], uint4 (&vx)[C]) {
         const bool on = i < mine;
-        if (i % kWave == 0) scales_l = scales_n, lost_l = lost_n;
-        f32x4 sa[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, sb[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+        if (i % kWave == 0) {
+            const bool lost = lost_n >> lane & 1;
+            ks_l = lost ? __builtin_nanf("") : scales_n.x;
+            lv_l = lost ? __builtin_nanf("") : scales_n.y == 0.0f ? 0.0f : log2f(scales_n.y);
+        }
+        f32x4 sa[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
         if (on) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 const half8 k0 = codes8(kx[c].x, kx[c].y), k1 = codes8(kx[c].z, kx[c].w);
                 const half8 hi = kQueriesInLds ? s_q[((cut * C + c) * 2) * kWave + lane] : qh[kQueriesInLds ? 0 : c];
                 const half8 lo = kQueriesInLds ? s_q[((cut * C + c) * 2 + 1) * kWave + lane] : ql[kQueriesInLds ? 0 : c];
+                sa[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, lo, sa[0], 0, 0, 0);
+                sa[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, lo, sa[1], 0, 0, 0);
                 sa[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, hi, sa[0], 0, 0, 0);
                 sa[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, hi, sa[1], 0, 0, 0);
-                sb[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, lo, sb[0], 0, 0, 0);
-                sb[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, lo, sb[1], 0, 0, 0);
             }
-            sa[0] += sb[0], sa[1] += sb[1];
         }
         // (64 blocks on, page_l holds the next 64)
         const bool more = i + DEPTH < mine;
         if (more && (i + DEPTH) % kWave == 0) pages(i + DEPTH + lane);
         if (more) load(kx, i + DEPTH, 0);
         if (SPLIT > 1) {
-            s_x[i % 2][(wave * 2) * kWave + lane] = sa[0], s_x[i % 2][(wave * 2 + 1) * kWave + lane] = sa[1];
+            f32x4 *x = s_x + i % 2 * (W * 2 * kWave) + lane;
+            x[wave * 2 * kWave] = sa[0], x[(wave * 2 + 1) * kWave] = sa[1];
             __syncthreads();
-            sa[0] += s_x[i % 2][((wave ^ 1) * 2) * kWave + lane], sa[1] += s_x[i % 2][((wave ^ 1) * 2 + 1) * kWave + lane];
+            sa[0] += x[(wave ^ 1) * 2 * kWave], sa[1] += x[((wave ^ 1) * 2 + 1) * kWave];
         }
         if (!on) return;
         // keys 32 j + 16 (e / 4) + 4 g + e % 4
@@ -353,11 +400,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
                 if (key > pos || key < low) t[e] = kNegInf;
             }
         }
-        // keys' scale, and log2 of the values' (a block of zeros: any)
-        const bool lost = lost_l >> (i % kWave) & 1;
-        const float ks = lost ? __builtin_nanf("") : __uint_as_float(from_lane(__float_as_uint(scales_l.x), i % kWave));
-        const float vs = lost ? __builtin_nanf("") : __uint_as_float(from_lane(__float_as_uint(scales_l.y), i % kWave));
-        const float lv = vs == 0.0f ? 0.0f : log2f(vs);
+        const float ks = __uint_as_float(from_lane(__float_as_uint(ks_l), i % kWave));
+        const float lv = __uint_as_float(from_lane(__float_as_uint(lv_l), i % kWave));
         const float c = c_row * ks;
         float mb = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
         mb = row_max(mb);
@@ -387,10 +431,10 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         if (mo1 != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-e15 - ms);
         half8 ph, pl;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const _Float16 hi = (_Float16)p[e];
-            ph[e] = hi;
-            pl[e] = (_Float16)(p[e] - (float)hi);
+        for (int e = 0; e < 8; e += 2) {
+            const half2v hi = pair(p[e], p[e + 1]), lo = pair(rest0(hi, p[e]), rest1(hi, p[e + 1]));
+            ph[e] = hi[0], ph[e + 1] = hi[1];
+            pl[e] = lo[0], pl[e + 1] = lo[1];
         }
 #pragma unroll
         for (int k = 0; k < C; k++) {
@@ -422,58 +466,34 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         return a.out + ((size_t)(w.first + r1 / a.group) * a.n_heads + h * a.group + r1 % a.group) * D;
     };
     const auto place = [&](uint32_t slot) { return a.part + ((size_t)h * a.slots + slot) * P; };
-    // Parts' m, l, mo to the rows' common ones: thread 16 i + row has part i's of a row.
-    // Leaves each part's factor in s_f, each row's m and mo in s_top and l's terms in s_sum, a wavefront's each.
-    static_assert(NT == kJoin * kThinRows, "a part and row a thread");
-    const auto weigh = [&](uint32_t count, f32x4 st) {
-        const uint32_t i = tid / kThinRows;
-        float tm = i < count ? st[0] : kNegInf, tmo = i < count ? st[2] : kNegInf;
-#pragma unroll
-        for (int off = 16; off < kWave; off <<= 1)
-            tm = fmaxf(tm, __shfl_xor(tm, off, kWave)), tmo = fmaxf(tmo, __shfl_xor(tmo, off, kWave));
-        if (g == 0) s_top[0][wave][n] = tm, s_top[1][wave][n] = tmo;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < W; k++) tm = fmaxf(tm, s_top[0][k][n]), tmo = fmaxf(tmo, s_top[1][k][n]);
-        float l_i = i < count ? st[0] == kNegInf ? st[1] : st[1] * exp2f(st[0] - tm) : 0.0f;  // (l is 0 or NaN without a largest)
-        s_f[i][n] = st[2] == kNegInf ? 1.0f : exp2f(st[2] - tmo);                             // (sums of 0 or NaN)
-#pragma unroll
-        for (int off = 16; off < kWave; off <<= 1) l_i += __shfl_xor(l_i, off, kWave);
-        if (g == 0) s_sum[wave][n] = l_i;
-        __syncthreads();
-    };
-    const auto stat_of = [&](uint32_t rr) {
-        f32x4 st = {kNegInf, 0.0f, kNegInf, 0.0f};
-#pragma unroll
-        for (int k = 0; k < W; k++) {
-            st[0] = fmaxf(st[0], s_top[0][k][rr]), st[2] = fmaxf(st[2], s_top[1][k][rr]);
-            st[1] += s_sum[k][rr];
+    // A row's four channels, to a part's place or to the outputs.
+    const auto put = [&](const Joint &x, uint32_t rr, uint32_t d, float *to) {
+        if (to) {
+            put4(to + rr * D + d, x.sum);
+            if (d == 0) put4(to + kThinRows * D + 4 * rr, f32x4{x.m, x.l, x.mo, 0.0f});
+        } else {
+            const float scale = w.bad ? __builtin_nanf("") : out_scale(x.m, x.l, x.mo, 15.0f);
+            *reinterpret_cast<f32x4 *>(out_of(rr) + d) = x.sum * scale;
         }
-        return st;
     };
-    const auto stats_to = [&](float *p) {
-        if (tid < rows_in) put4(p + kThinRows * D + 4 * tid, stat_of(tid));
-    };
-    const auto scale_of = [&](uint32_t rr) {
-        const f32x4 st = stat_of(rr);
-        return w.bad ? __builtin_nanf("") : out_scale(st[0], st[1], st[2], 15.0f);
-    };
-    weigh(NB, s_m[tid / kThinRows % NB][n]);
-    for (uint32_t at = tid; at < rows_in * (D / 4); at += NT) {
+    const uint32_t all = rows_in * (D / 4);
+    for (uint32_t at = tid; at < all; at += NT) {
         const uint32_t rr = at / (D / 4), d = at % (D / 4) * 4;
-        f32x4 sum = {0, 0, 0, 0};
+        f32x4 st[NB], v[NB];
 #pragma unroll
-        for (int i = 0; i < NB; i++) sum += *reinterpret_cast<const f32x4 *>(&s_o[i][rr][d]) * s_f[i][rr];
-        if (w.splits > 1) put4(place(w.slot) + rr * D + d, sum);
-        else *reinterpret_cast<f32x4 *>(out_of(rr) + d) = sum * scale_of(rr);
+        for (int i = 0; i < NB; i++) st[i] = s_m[i][rr], v[i] = *reinterpret_cast<const f32x4 *>(&s_o[i][rr][d]);
+        Joint x;
+        x.clear();
+        x.add(st, v, NB);
+        put(x, rr, d, w.splits > 1 ? place(w.slot) : nullptr);
     }
     if (w.splits == 1) return;
-    stats_to(place(w.slot));
 
     // The part that is last at its group joins the group, the group that is last at its
     // tile the tile.  A part's stores are acknowledged before it counts; the one that
     // counts last reads past the L2s, and leaves the counters at zero.
-    const uint32_t in_group = w.splits <= kJoin ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
+    const uint32_t hands = all < (uint32_t)NT ? NT / all : 1;
+    const uint32_t in_group = w.splits <= kJoin || w.splits <= 8 * hands ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
     const uint32_t grp = w.split / in_group, slot0 = w.slot - w.split, g0 = slot0 + grp * in_group;
     const uint32_t gn = w.splits - grp * in_group < in_group ? w.splits - grp * in_group : in_group;
     const uint32_t groups = (w.splits + in_group - 1) / in_group;
@@ -489,33 +509,40 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         __syncthreads();
         return s_last;
     };
-    // Parts slot, slot + step, ..: their sums to `to`, or to the outputs.  The sums are under
-    // way before the factors are found.
+    // Parts slot, slot + step, ..: their sums to `to`, or to the outputs.  Where there are more
+    // threads than a part has places, the parts are dealt out to `hands` of them, and what
+    // those make of them is joined through LDS.
     const auto join = [&](uint32_t slot, uint32_t step, uint32_t count, float *to) {
-        const uint32_t i0 = tid / kThinRows;
-        const f32x4 st = get4(place(slot + (i0 < count ? i0 : 0) * step) + kThinRows * D + 4 * n);
-        f32x4 v[kJoin];
-        const auto fetch = [&](uint32_t at) {
-#pragma unroll
-            for (uint32_t u = 0; u < kJoin; u++) {
-                if (u % 4 == 0 && u >= count) break;
-                v[u] = get4(place(slot + (u < count ? u : 0) * step) + 4 * at);
-            }
-        };
-        const uint32_t all = rows_in * (D / 4);
-        if (tid < all) fetch(tid);
-        weigh(count, st);
-        for (uint32_t at = tid; at < all; at += NT) {
+        const uint32_t hand = hands > 1 ? tid / all : 0;
+        for (uint32_t at0 = 0; at0 < all; at0 += NT) {
+            const uint32_t at = hands > 1 ? tid - hand * all : at0 + tid;
             const uint32_t rr = at / (D / 4), d = at % (D / 4) * 4;
-            if (at != tid) fetch(at);
-            f32x4 sum = {0, 0, 0, 0};
+            Joint x;
+            x.clear();
+            if (hand < hands && at < all)
+                for (uint32_t u0 = hand; u0 < count; u0 += kBatch * hands) {
+                    f32x4 st[kBatch], v[kBatch];
+                    const uint32_t n_here = (count - u0 + hands - 1) / hands;
 #pragma unroll
-            for (uint32_t u = 0; u < kJoin; u++)
-                if (u < count) sum += v[u] * s_f[u][rr];
-            if (to) put4(to + rr * D + d, sum);
-            else *reinterpret_cast<f32x4 *>(out_of(rr) + d) = sum * scale_of(rr);
+                    for (uint32_t u = 0; u < kBatch; u++) {
+                        if (u % 4 == 0 && u >= n_here) break;
+                        const float *p = place(slot + (u < n_here ? u0 + u * hands : u0) * step);
+                        st[u] = get4(p + kThinRows * D + 4 * rr), v[u] = get4(p + 4 * at);
+                    }
+                    x.add(st, v, n_here);
+                }
+            if (hands > 1) {
+                f32x4 *s_part = reinterpret_cast<f32x4 *>(&s_o[0][0][0]);
+                if (hand < hands) s_part[tid] = x.sum, s_part[NT + tid] = f32x4{x.m, x.l, x.mo, 0.0f};
+                __syncthreads();
+                if (hand) continue;  // (the only round)
+                for (uint32_t k = 1; k < hands; k++) {
+                    const f32x4 st[1] = {s_part[NT + k * all + at]}, v[1] = {s_part[k * all + at]};
+                    x.add(st, v, 1);
+                }
+            }
+            if (at < all) put(x, rr, d, to);
         }
-        if (to) stats_to(to);
     };
     if (!last(tickets + 2 * g0, gn)) return;
     if (groups == 1) {
@@ -541,22 +568,14 @@ uint32_t thin_slots(uint32_t target, uint32_t n_kv) { return 2 * (target / n_kv 
 
 template <int D>
 void go(ThinArgs t, uint32_t tiles, hipStream_t s) {
-    const uint32_t each = (t.b.max_blocks + kLeast - 1) / kLeast;  // (a tile's parts, at most)
+    using Sh = Shape<D>;
+    t.target = 256 * Sh::kTarget, t.slots = thin_slots(t.target, t.n_kv), t.least = Sh::kLeast;
+    const uint32_t each = (t.b.max_blocks + t.least - 1) / t.least;  // (a tile's parts, at most)
     uint64_t x = tiles + t.target / t.n_kv + 1;
     if ((uint64_t)tiles * each < x) x = (uint64_t)tiles * each;
-    hipLaunchKernelGGL(k_attention_thin<D>, dim3((uint32_t)x, t.n_kv), dim3(Shape<D>::kThreads), 0, s, t);
+    hipLaunchKernelGGL(k_attention_thin<D>, dim3((uint32_t)x, t.n_kv), dim3(Sh::kThreads), 0, s, t);
 }
-
-uint32_t thin_target(uint32_t D) {
-    switch (D) {
-    case 64: return 256 * Shape<64>::kTarget;
-    case 96: return 256 * Shape<96>::kTarget;
-    case 128: return 256 * Shape<128>::kTarget;
-    case 192: return 256 * Shape<192>::kTarget;
-    case 256: return 256 * Shape<256>::kTarget;
-    default: return 256 * Shape<512>::kTarget;
-    }
-}
+constexpr uint32_t kThinTarget = 512;  // the largest
 
 }  // namespace
 
@@ -566,7 +585,7 @@ bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D
 static bool wide(const AttnArgs &a) { return (uint64_t)(a.b.max_new ? a.b.max_new : a.b.n_tokens) * a.group > kThinMost; }
 
 size_t attention_workspace(const AttnArgs &a) {
-    const size_t thin = (size_t)a.kv.n_kv * thin_slots(thin_target(a.kv.D), a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
+    const size_t thin = (size_t)a.kv.n_kv * thin_slots(kThinTarget, a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
     const size_t more = wide(a) ? attention_wide_workspace(a.kv.D) : 0;
     return thin < more ? more : thin;
 }
@@ -581,7 +600,6 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
     t.q = a.q, t.out = a.out, t.q_stride = a.q_stride, t.n_heads = a.n_heads, t.group = a.group, t.window = a.window;
     t.scale2 = a.scale * 1.4426950408889634f;
     t.part = (float *)a.work, t.tickets = a.tickets, t.err = a.err;
-    t.target = thin_target(a.kv.D), t.slots = thin_slots(t.target, t.n_kv);
     const uint32_t tiles = thin_tiles(a);
     switch (a.kv.D) {
     case 64: go<64>(t, tiles, s); break;

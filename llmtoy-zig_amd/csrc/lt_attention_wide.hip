@@ -141,9 +141,6 @@ __device__ __forceinline__ T in_branch(T v) {
     return v;
 }
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ half2v pair(float a, float b) { return __builtin_convertvector((f32x2{a, b}), half2v); }
-
 // N operands read from LDS one after the other, the i-th for use(i, operand): kAhead of
 // them under way before the first product (the compiler, short of registers, would
 // read one and wait for it).
@@ -167,18 +164,6 @@ struct Feed {
         }
     }
 };
-
-// What is left of p beside h's first or second half, in one instruction.
-__device__ __forceinline__ float rest0(half2v h, float p) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
-    return r;
-}
-__device__ __forceinline__ float rest1(half2v h, float p) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
-    return r;
-}
 
 template <int D>
 __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attention_wide(WideArgs a) {

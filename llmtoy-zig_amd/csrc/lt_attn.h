@@ -37,6 +37,21 @@ __device__ __forceinline__ half8 codes8(uint32_t a, uint32_t b) {
     return r.v;
 }
 
+// Two numbers as f16, and what is left of them.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ half2v pair(float a, float b) { return __builtin_convertvector((f32x2{a, b}), half2v); }
+// What is left of p beside h's first or second half, in one instruction.
+__device__ __forceinline__ float rest0(half2v h, float p) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
+__device__ __forceinline__ float rest1(half2v h, float p) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
+
 // Partial results go past the L2s (agent scope): another XCD reads them.
 __device__ __forceinline__ void put4(float *p, f32x4 v) {
     uint64_t *q = reinterpret_cast<uint64_t *>(p);
