@@ -31,33 +31,19 @@ namespace lt {
 namespace {
 
 constexpr int kThinRows = 16;
-#ifndef ALONE
-#define ALONE 3
-#endif
-#ifndef WB
-#define WB 8
-#endif
-#ifndef DEP
-#define DEP 1
-#endif
-#ifndef LROUNDS
-#define LROUNDS 1
-#endif
-#ifndef TGT
-#define TGT 2
-#endif
-// Wavefronts a workgroup, wavefronts that a block's channels are cut over, workgroups a
-// CU, blocks a wavefront has under way.
+// Wavefronts a workgroup, wavefronts that a block's channels are cut over, parts that a
+// launch is cut into (more of them: 48 heads' caches of 220 MB 61.5 us with 512, 64 with 1,024; fewer:
+// 79 with 256, whose workgroups leave half of the registers unused).
 template <int D>
 struct Shape {
-    static constexpr int kWaves = D <= 128 ? 8 : D <= 256 ? WB : 8, kSplit = D <= 256 ? 1 : 2;
-    static constexpr int kPerCu = (D <= 128 ? 16 : 8) / kWaves, kTarget = kPerCu < TGT ? kPerCu : TGT;
-    static constexpr int kDepth = D <= 64 ? DEP : 1;
+    static constexpr int kWaves = 8, kSplit = D <= 256 ? 1 : 2, kTarget = D <= 128 ? 512 : 256;
     static constexpr int kThreads = kWaves * kWave, kBlocks = kWaves / kSplit;  // blocks a round
     static constexpr int DW = D / kSplit, C = DW / 32;
-    static constexpr bool kQueriesInLds = DW >= 256 || D == 128;
-    static constexpr uint32_t kLeast = LROUNDS * kBlocks;  // blocks that a part is worth having for
+    // (what a wavefront would not have the registers for: four on a SIMD up to heads of 128, then two)
+    static constexpr bool kQueriesInLds = DW >= 128;
 };
+constexpr uint32_t kThinTarget = 512;  // the largest
+
 // Parts of a tile that are joined at once (or 8 for each time that the workgroup's threads
 // are more than a part's places); more are joined in groups first, and no tile has more than the square.
 constexpr uint32_t kJoin = 16;
@@ -119,7 +105,7 @@ __device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, float sum) {
 // A tile's parts.  None where a workgroup has its blocks done before parts are joined; parts of
 // `least` where there are few, for their latency; else no more parts than the chip has room for at once.
 __device__ __forceinline__ uint32_t thin_splits(const ThinArgs &a, uint32_t blocks, uint32_t share) {
-    if (blocks <= ALONE * a.least) return 1;
+    if (blocks <= 3 * a.least) return 1;
     uint32_t n = share > a.least ? blocks / share : (blocks + share - 1) / share;
     if (n == 0) n = 1;
     return n < kJoin * kJoin ? n : kJoin * kJoin;
@@ -223,7 +209,7 @@ struct Joint {
 template <int D>
 __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_attention_thin(ThinArgs a) {
     using Sh = Shape<D>;
-    constexpr int W = Sh::kWaves, C = Sh::C, NT = Sh::kThreads, SPLIT = Sh::kSplit, NB = Sh::kBlocks, DEPTH = Sh::kDepth;
+    constexpr int W = Sh::kWaves, C = Sh::C, NT = Sh::kThreads, SPLIT = Sh::kSplit, NB = Sh::kBlocks;
     constexpr bool kQueriesInLds = Sh::kQueriesInLds;
     constexpr uint32_t kBatch = D <= 128 ? 8 : 16;  // parts that a thread reads at once
     constexpr size_t P = kThinRows * (D + 4);  // floats of a part
@@ -293,13 +279,11 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         qx[c][1] = *reinterpret_cast<const float4 *>(qp + 32 * (cut * C + c) + 4);
     }
     if (mine) pages(lane);
-    uint4 kq[DEPTH][C], vq[DEPTH][C];
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++)
-        if ((uint32_t)d < mine) {
-            load(kq[d], d, 0);
-            load(vq[d], d, 1);
-        }
+    uint4 kq[C], vq[C];
+    if (mine) {
+        load(kq, 0, 0);
+        load(vq, 0, 1);
+    }
 
     // the queries' two parts, scaled to 2^14 .. 2^15 by a power of two
     half8 qh[kQueriesInLds ? 1 : C], ql[kQueriesInLds ? 1 : C];
@@ -356,7 +340,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     for (int i = 0; i < 2 * C; i++) o[i] = f32x4{0, 0, 0, 0};
     float m = kNegInf, l = 0.0f, mo = kNegInf;
 
-    const auto block = [&](uint32_t i, uint4 (&kx)[C], uint4 (&vx)[C]) {
+    for (uint32_t i = 0; i < rounds; i++) {
         const bool on = i < mine;
         if (i % kWave == 0) {
             const bool lost = lost_n >> lane & 1;
@@ -367,7 +351,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         if (on) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const half8 k0 = codes8(kx[c].x, kx[c].y), k1 = codes8(kx[c].z, kx[c].w);
+                const half8 k0 = codes8(kq[c].x, kq[c].y), k1 = codes8(kq[c].z, kq[c].w);
                 const half8 hi = kQueriesInLds ? s_q[((cut * C + c) * 2) * kWave + lane] : qh[kQueriesInLds ? 0 : c];
                 const half8 lo = kQueriesInLds ? s_q[((cut * C + c) * 2 + 1) * kWave + lane] : ql[kQueriesInLds ? 0 : c];
                 sa[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, lo, sa[0], 0, 0, 0);
@@ -377,16 +361,16 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
             }
         }
         // (64 blocks on, page_l holds the next 64)
-        const bool more = i + DEPTH < mine;
-        if (more && (i + DEPTH) % kWave == 0) pages(i + DEPTH + lane);
-        if (more) load(kx, i + DEPTH, 0);
+        const bool more = i + 1 < mine;
+        if (more && (i + 1) % kWave == 0) pages(i + 1 + lane);
+        if (more) load(kq, i + 1, 0);
         if (SPLIT > 1) {
             f32x4 *x = s_x + i % 2 * (W * 2 * kWave) + lane;
             x[wave * 2 * kWave] = sa[0], x[(wave * 2 + 1) * kWave] = sa[1];
             __syncthreads();
             sa[0] += x[(wave ^ 1) * 2 * kWave], sa[1] += x[((wave ^ 1) * 2 + 1) * kWave];
         }
-        if (!on) return;
+        if (!on) continue;
         // keys 32 j + 16 (e / 4) + 4 g + e % 4
         const uint32_t j = b0 + which + NB * i;
         float t[8];
@@ -438,18 +422,13 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         }
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            const half8 v0 = codes8(vx[k].x, vx[k].y), v1 = codes8(vx[k].z, vx[k].w);
+            const half8 v0 = codes8(vq[k].x, vq[k].y), v1 = codes8(vq[k].z, vq[k].w);
             o[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[2 * k], 0, 0, 0);
             o[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[2 * k + 1], 0, 0, 0);
             o[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, o[2 * k], 0, 0, 0);
             o[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, o[2 * k + 1], 0, 0, 0);
         }
-        if (more) load(vx, i + DEPTH, 1);
-    };
-    for (uint32_t i = 0; i < rounds; i += DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++)
-            if (DEPTH == 1 || i + d < rounds) block(i + d, kq[d], vq[d]);
+        if (more) load(vq, i + 1, 1);
     }
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
@@ -569,14 +548,12 @@ uint32_t thin_slots(uint32_t target, uint32_t n_kv) { return 2 * (target / n_kv 
 template <int D>
 void go(ThinArgs t, uint32_t tiles, hipStream_t s) {
     using Sh = Shape<D>;
-    t.target = 256 * Sh::kTarget, t.slots = thin_slots(t.target, t.n_kv), t.least = Sh::kLeast;
+    t.target = Sh::kTarget, t.slots = thin_slots(t.target, t.n_kv), t.least = Sh::kBlocks;
     const uint32_t each = (t.b.max_blocks + t.least - 1) / t.least;  // (a tile's parts, at most)
     uint64_t x = tiles + t.target / t.n_kv + 1;
     if ((uint64_t)tiles * each < x) x = (uint64_t)tiles * each;
     hipLaunchKernelGGL(k_attention_thin<D>, dim3((uint32_t)x, t.n_kv), dim3(Sh::kThreads), 0, s, t);
 }
-constexpr uint32_t kThinTarget = 512;  // the largest
-
 }  // namespace
 
 bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D == 192 || D == 256 || D == 512; }

@@ -10,8 +10,10 @@
 // within half a turn, is exact enough for fp32.
 //
 // Bound by the reads and writes of the heads.  A group of lanes takes a token's
-// heads one after the other and finds the token's angles once; the angles of
+// heads, HB at a time, and finds the token's angles once; the angles of
 // one pair take about 60 instructions, 15 times those of turning it.
+// 4,095 tokens of 16 + 8 heads of 256, half of each turned: 48 us, 4.2 TB/s; one token of 36
+// heads of 128 3.3 us in a graph's row of 16.
 #include "llmtoy_hip.h"
 #include "lt_kv.h"
 
@@ -29,8 +31,17 @@ struct RopeArgs {
     float eps, bias;
 };
 
-// V consecutive pairs a lane and step, W lanes a head, KP steps.
-template <int V, int W, int KP>
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// (MANY: past the caches; 4,095 tokens of 24 heads of 256: 52 -> 48 us, of 36 of 128 36 -> 31)
+template <bool MANY>
+__device__ __forceinline__ void put(float *to, const float *v) {
+    const f32x4 x = {v[0], v[1], v[2], v[3]};
+    if (MANY) __builtin_nontemporal_store(x, reinterpret_cast<f32x4 *>(to));
+    else *reinterpret_cast<f32x4 *>(to) = x;
+}
+
+// V consecutive pairs a lane and step, W lanes a head, KP steps, HB heads at a time.
+template <int V, int W, int KP, int HB>
 __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs a) {
     const uint32_t lane = threadIdx.x % W;
     const size_t group = (size_t)blockIdx.x * (256 / W) + threadIdx.x / W;
@@ -40,8 +51,6 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs a) {
     const uint32_t half = a.n_rot / 2, pairs = a.D / 2;
     // the lane's 2 V elements: V in a row from at, V from to
     uint32_t at[KP], to[KP];
-    float cs[KP][V], sn[KP][V];
-    const uint32_t pos = a.pos[t];
 #pragma unroll
     for (int i = 0; i < KP; i++) {
         const uint32_t p = (lane + i * W) * V;
@@ -53,89 +62,101 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs a) {
             at[i] = 2 * p;
             to[i] = 2 * p + V;
         }
+    }
+    const auto get = [&](const float *x, int i, float (&u)[2 * V]) {
+        if ((lane + i * W) * V >= pairs) {
+#pragma unroll
+            for (int j = 0; j < 2 * V; j++) u[j] = 0.0f;
+        } else if constexpr (V == 4) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(x + at[i]), hi = *reinterpret_cast<const f32x4 *>(x + to[i]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) u[j] = lo[j], u[4 + j] = hi[j];
+        } else {
+            u[0] = x[at[i]], u[1] = x[to[i]];
+        }
+    };
+    const auto head_of = [&](uint32_t h) {
+        return h < a.n_heads ? a.q + (size_t)t * a.q_stride + (size_t)h * a.D
+                             : a.k + (size_t)t * a.k_stride + (size_t)(h - a.n_heads) * a.D;
+    };
+    // everything that is read first, side by side: the heads, the position and rates, the weights
+    float u[HB][KP][2 * V], g[2][KP][2 * V];
+    const auto fetch = [&](uint32_t h) {
+#pragma unroll
+        for (int b = 0; b < HB; b++)
+#pragma unroll
+            for (int i = 0; i < KP; i++) get(head_of(h + b < h1 ? h + b : h1 - 1), i, u[b][i]);
+    };
+    fetch(h0);
+    const uint32_t pos = a.pos[t];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float *w = k ? a.wk : a.wq;
+#pragma unroll
+        for (int i = 0; i < KP; i++) {
+            if (a.norm && w) get(w, i, g[k][i]);
+#pragma unroll
+            for (int j = 0; j < 2 * V; j++) g[k][i][j] = a.norm && w ? a.bias + g[k][i][j] : 1.0f;
+        }
+    }
+    float cs[KP][V], sn[KP][V];
+#pragma unroll
+    for (int i = 0; i < KP; i++) {
+        const uint32_t p = (lane + i * W) * V;
 #pragma unroll
         for (int j = 0; j < V; j++) {
             cs[i][j] = 1.0f, sn[i][j] = 0.0f;
-            if (turned) {
+            if (p < half) {
                 const double turn = (double)pos * a.turns[p + j];
                 sincospif(2.0f * (float)(turn - rint(turn)), &sn[i][j], &cs[i][j]);
             }
         }
     }
-    for (uint32_t h = h0; h < h1; h++) {
-        const bool is_q = h < a.n_heads;
-        const uint32_t hh = is_q ? h : h - a.n_heads;
-        const float *x = is_q ? a.q + (size_t)t * a.q_stride : a.k + (size_t)t * a.k_stride;
-        float *y = is_q ? a.q_out + (size_t)t * a.q_out_stride : a.k_out + (size_t)t * a.k_out_stride;
-        const float *w = is_q ? a.wq : a.wk;
-        x += (size_t)hh * a.D;
-        y += (size_t)hh * a.D;
-        float u[KP][2 * V];
-        float ss = 0.0f;
+    for (uint32_t h = h0; h < h1; h += HB) {
+        if (h != h0) fetch(h);
 #pragma unroll
-        for (int i = 0; i < KP; i++) {
-            const bool in = (lane + i * W) * V < pairs;
-            if (V == 4) {
-                const float4 z = make_float4(0, 0, 0, 0);
-                const float4 lo = in ? *reinterpret_cast<const float4 *>(x + at[i]) : z;
-                const float4 hi = in ? *reinterpret_cast<const float4 *>(x + to[i]) : z;
-                u[i][0] = lo.x, u[i][1 % (2 * V)] = lo.y, u[i][2 % (2 * V)] = lo.z, u[i][3 % (2 * V)] = lo.w;
-                u[i][4 % (2 * V)] = hi.x, u[i][5 % (2 * V)] = hi.y, u[i][6 % (2 * V)] = hi.z, u[i][7 % (2 * V)] = hi.w;
-            } else {
-                u[i][0] = in ? x[at[i]] : 0.0f;
-                u[i][1] = in ? x[to[i]] : 0.0f;
+        for (int b = 0; b < HB; b++) {
+            if (h + b >= h1) break;
+            const bool is_q = h + b < a.n_heads;
+            float *y = is_q ? a.q_out + (size_t)t * a.q_out_stride + (size_t)(h + b) * a.D
+                            : a.k_out + (size_t)t * a.k_out_stride + (size_t)(h + b - a.n_heads) * a.D;
+            float r = 1.0f;
+            if (a.norm) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < KP; i++)
+#pragma unroll
+                    for (int j = 0; j < 2 * V; j++) ss += u[b][i][j] * u[b][i][j];
+#pragma unroll
+                for (int off = W / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, W);
+                r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
             }
 #pragma unroll
-            for (int j = 0; j < 2 * V; j++) ss += u[i][j] * u[i][j];
-        }
-        float r = 1.0f;
-        if (a.norm) {
+            for (int i = 0; i < KP; i++) {
+                if ((lane + i * W) * V >= pairs) continue;
+                float v[2 * V], o[2 * V];
 #pragma unroll
-            for (int off = W / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, W);
-            r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-        }
+                for (int j = 0; j < 2 * V; j++) v[j] = u[b][i][j] * (r * (is_q ? g[0][i][j] : g[1][i][j]));
+                if (a.neox) {
 #pragma unroll
-        for (int i = 0; i < KP; i++) {
-            const bool in = (lane + i * W) * V < pairs;
-            if (!in) continue;
-            float g[2 * V];
-#pragma unroll
-            for (int j = 0; j < 2 * V; j++) g[j] = r;
-            if (a.norm && w) {
-                if (V == 4) {
-                    const float4 lo = *reinterpret_cast<const float4 *>(w + at[i]);
-                    const float4 hi = *reinterpret_cast<const float4 *>(w + to[i]);
-                    const float ww[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-                    for (int j = 0; j < 2 * V; j++) g[j] *= a.bias + ww[j];
+                    for (int j = 0; j < V; j++) {
+                        o[j] = v[j] * cs[i][j] - v[j + V] * sn[i][j];
+                        o[j + V] = v[j] * sn[i][j] + v[j + V] * cs[i][j];
+                    }
                 } else {
-                    g[0] *= a.bias + w[at[i]];
-                    g[1] *= a.bias + w[to[i]];
-                }
-            }
 #pragma unroll
-            for (int j = 0; j < 2 * V; j++) u[i][j] *= g[j];
-            float o[2 * V];
-            if (a.neox) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    o[j] = u[i][j] * cs[i][j] - u[i][j + V] * sn[i][j];
-                    o[j + V] = u[i][j] * sn[i][j] + u[i][j + V] * cs[i][j];
+                    for (int j = 0; j < V; j++) {
+                        o[2 * j] = v[2 * j] * cs[i][j] - v[2 * j + 1] * sn[i][j];
+                        o[2 * j + 1] = v[2 * j] * sn[i][j] + v[2 * j + 1] * cs[i][j];
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    o[2 * j] = u[i][2 * j] * cs[i][j] - u[i][2 * j + 1] * sn[i][j];
-                    o[2 * j + 1] = u[i][2 * j] * sn[i][j] + u[i][2 * j + 1] * cs[i][j];
+                if constexpr (V == 4) {
+                    put<(HB > 1)>(y + at[i], o);
+                    put<(HB > 1)>(y + to[i], o + 4);
+                } else {
+                    y[at[i]] = o[0];
+                    y[to[i]] = o[1];
                 }
-            }
-            if (V == 4) {
-                *reinterpret_cast<float4 *>(y + at[i]) = make_float4(o[0], o[1 % (2 * V)], o[2 % (2 * V)], o[3 % (2 * V)]);
-                *reinterpret_cast<float4 *>(y + to[i]) =
-                    make_float4(o[4 % (2 * V)], o[5 % (2 * V)], o[6 % (2 * V)], o[7 % (2 * V)]);
-            } else {
-                y[at[i]] = o[0];
-                y[to[i]] = o[1];
             }
         }
     }
@@ -149,7 +170,9 @@ void go(RopeArgs &a, hipStream_t s) {
     while (a.per < a.n_all && (uint64_t)a.T * ((a.n_all + 2 * a.per - 1) / (2 * a.per)) >= kEnough) a.per *= 2;
     a.parts = (a.n_all + a.per - 1) / a.per;
     const size_t groups = (size_t)a.T * a.parts;
-    hipLaunchKernelGGL((k_qk_norm_rope<V, W, KP>), dim3((unsigned)((groups + 256 / W - 1) / (256 / W))), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)((groups + 256 / W - 1) / (256 / W)));
+    if (a.per == 1) hipLaunchKernelGGL((k_qk_norm_rope<V, W, KP, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_qk_norm_rope<V, W, KP, (V == 4 ? 4 : 2)>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace

@@ -19,6 +19,8 @@ library must be built (make -C llmtoy-zig_amd) and a GPU must be present.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import math
 import os
 
 import numpy as np
@@ -159,12 +161,12 @@ def _ptr(a):
         if not a.flags["C_CONTIGUOUS"]:
             raise InvalidError("array must be C-contiguous")
         return a.ctypes.data, True
-    if hasattr(a, "ptr") and hasattr(a, "dtype"):  # hip.DeviceArray / DeviceView
-        return a.ptr, False
     if _is_torch(a):
         if not a.is_contiguous():
             raise InvalidError("tensor must be contiguous")
         return a.data_ptr(), not a.is_cuda
+    if hasattr(a, "ptr") and hasattr(a, "dtype"):  # hip.DeviceArray / DeviceView
+        return a.ptr, False
     raise TypeError(f"unsupported array type {type(a)}")
 
 
@@ -196,25 +198,35 @@ class Tensor:
             self.handle = None
 
 
+@functools.lru_cache(maxsize=None)
+def _kind(dtype) -> str:
+    """A numpy or torch type's name without its package."""
+    return str(np.dtype(dtype)) if isinstance(dtype, type) else str(dtype).replace("torch.", "")
+
+
+def _count(a) -> int:
+    return a.numel() if _is_torch(a) else math.prod(a.shape)
+
+
 def _words(a, n: int, what: str):
-    """A contiguous array of n 32-bit whole numbers."""
+    """(pointer, is_host) of a contiguous array of n 32-bit whole numbers."""
     if a is None:
         raise InvalidError(f"{what}: an array of {n} is needed")
-    if str(a.dtype).replace("torch.", "") not in ("int32", "uint32"):
+    if _kind(a.dtype) not in ("int32", "uint32"):
         raise InvalidError(f"{what}: 32-bit whole numbers expected, got {a.dtype}")
-    if int(np.prod(tuple(a.shape))) != n:
+    if _count(a) != n:
         raise InvalidError(f"{what}: {tuple(a.shape)}, {n} entries expected")
-    return a
+    return _ptr(a)
 
 
 def _heads(a, what: str):
     """(pointer, is_host, tokens, heads, head_dim, floats from token to token) of a float32 array
     [tokens, heads, head_dim] whose heads lie in a row; the tokens may be a stride apart."""
-    if a.dtype != np.float32 and str(a.dtype) != "torch.float32":
+    if _kind(a.dtype) != "float32":
         raise InvalidError(f"{what}: float32 expected, got {a.dtype}")
     if len(a.shape) != 3:
         raise InvalidError(f"{what}: [tokens, heads, head_dim] expected, got {tuple(a.shape)}")
-    T, H, D = (int(n) for n in a.shape)
+    T, H, D = a.shape
     if _is_torch(a):
         st, p, host = a.stride(), a.data_ptr(), not a.is_cuda
     elif isinstance(a, np.ndarray):
@@ -223,7 +235,7 @@ def _heads(a, what: str):
         st, (p, host) = (H * D, D, 1), _ptr(a)
     if T and (D > 1 and st[2] != 1 or H > 1 and st[1] != D or T > 1 and st[0] < H * D):
         raise InvalidError(f"{what}: a token's heads must lie in a row (strides {tuple(st)})")
-    return p, host, T, H, D, int(st[0]) if T > 1 else H * D
+    return p, host, T, H, D, st[0] if T > 1 else H * D
 
 
 class Rope:
@@ -247,16 +259,16 @@ class KvBatch:
         if table is None or tuple(table.shape) != (len.shape[0], table.shape[-1]):
             raise InvalidError("table: [sequences, blocks] expected")
         n = int(len.shape[0])
-        self.start, self.len, self.table = _words(start, n + 1, "start"), _words(len, n, "len"), table
-        _words(table, n * int(table.shape[1]), "table")
+        _words(start, n + 1, "start"), _words(len, n, "len"), _words(table, n * int(table.shape[1]), "table")
+        self.start, self.len, self.table = start, len, table
         self.n_seqs, self.n_tokens, self.max_blocks, self.max_new = n, int(n_tokens), int(table.shape[1]), int(max_new)
 
     def struct(self):
         """(lt_kv_batch, is_host)"""
-        ps = [_ptr(a) for a in (self.start, self.len, self.table)]
-        if len({h for _, h in ps}) > 1:
+        (s, host), (n, h1), (t, h2) = _ptr(self.start), _ptr(self.len), _ptr(self.table)
+        if host != h1 or host != h2:
             raise InvalidError("mix of host and device arrays")
-        return KvBatchStruct(self.n_seqs, self.n_tokens, self.max_blocks, self.max_new, *(p for p, _ in ps)), ps[0][1]
+        return KvBatchStruct(self.n_seqs, self.n_tokens, self.max_blocks, self.max_new, s, n, t), host
 
 
 class KvCache:
@@ -273,23 +285,24 @@ class KvCache:
     def append(self, k, v, batch: KvBatch):
         """The batch's tokens' keys and values ([n_tokens, n_kv_heads, head_dim]) into the cache."""
         b, host = batch.struct()
-        got = [self._mine(a, w, batch.n_tokens) for a, w in ((k, "k"), (v, "v"))]
-        if {host} != {g[1] for g in got}:
+        gk, gv = self._mine(k, "k", batch.n_tokens), self._mine(v, "v", batch.n_tokens)
+        if host != gk[1] or host != gv[1]:
             raise InvalidError("mix of host and device arrays")
         c = self.ctx
-        c._check(c.lib.lt_kv_append(c.ptr, self.handle, got[0][0], got[1][0], got[0][5], got[1][5], C.byref(b),
-                                    LT_HOST_IO if host else 0))
+        c._check(c.lib.lt_kv_append(c.ptr, self.handle, gk[0], gv[0], gk[5], gv[5], C.byref(b), LT_HOST_IO if host else 0))
 
     def read(self, k_out, v_out, slots):
         """The values that slots stand for, into k_out and v_out [n, n_kv_heads, head_dim]."""
-        n = int(np.prod(tuple(slots.shape)))
-        _words(slots, n, "slots")
-        for a, w in ((k_out, "k_out"), (v_out, "v_out")):
-            if self._mine(a, w, n)[5] != self.n_kv_heads * self.head_dim:
+        n = _count(slots)
+        p, host = _words(slots, n, "slots")
+        gk, gv = self._mine(k_out, "k_out", n), self._mine(v_out, "v_out", n)
+        for g, w in ((gk, "k_out"), (gv, "v_out")):
+            if g[5] != self.n_kv_heads * self.head_dim:
                 raise InvalidError(f"{w}: must be contiguous")
+        if host != gk[1] or host != gv[1]:
+            raise InvalidError("mix of host and device arrays")
         c = self.ctx
-        c._check(c.lib.lt_kv_read(c.ptr, _ptr(k_out)[0], _ptr(v_out)[0], self.handle, _ptr(slots)[0], n,
-                                  c._io(k_out, v_out, slots)))
+        c._check(c.lib.lt_kv_read(c.ptr, gk[0], gv[0], self.handle, p, n, LT_HOST_IO if host else 0))
 
     def _mine(self, a, what, tokens):
         got = _heads(a, what)
@@ -489,29 +502,31 @@ class Context:
     def qk_norm_rope(self, q_out, k_out, q, k, wq, wk, positions, rope: Rope, eps=1e-6, norm=True, one_plus_w=False):
         """Norms of queries and keys [tokens, heads, head_dim] for each head and the rotation, in one pass
         (lt_qk_norm_rope).  k and k_out may be None; weights may be None (not multiplied); norm=False: rotate only."""
-        given = [("q", q), ("q_out", q_out)] + ([("k", k), ("k_out", k_out)] if k is not None or k_out is not None else [])
-        if any(a is None for _, a in given):
+        if q is None or q_out is None or (k is None) != (k_out is None):
             raise InvalidError("an input without its output")
-        got = {w: _heads(a, w) for w, a in given}
-        T = got["q"][2]
-        for w, g in got.items():
-            if (g[2], g[4]) != (T, rope.head_dim) or g[3] != got[w[0]][3]:
-                raise InvalidError(f"{w}: {g[2:5]}, {T} tokens of heads of {rope.head_dim} expected")
-        for w, a in (("wq", wq), ("wk", wk)):
-            if a is not None and (tuple(a.shape) != (rope.head_dim,) or str(a.dtype).replace("torch.", "") != "float32"):
-                raise InvalidError(f"{w}: float32 [{rope.head_dim}] expected")
-        _words(positions, T, "positions")
-        rest = [_ptr(a) for a in (wq, wk, positions)]
-        hosts = {g[1] for g in got.values()} | {h for _, h in rest if h is not None}
-        if len(hosts) > 1:
-            raise InvalidError("mix of host and device arrays")
         none = (None, None, 0, 0, 0, 0)
-        gk, gko = got.get("k", none), got.get("k_out", none)
-        fl = (LT_HOST_IO if hosts == {True} else 0) | (0 if norm else LT_ROPE_NO_NORM)
-        fl |= LT_NORM_ONE_PLUS_W if one_plus_w else 0
-        self._check(self.lib.lt_qk_norm_rope(self.ptr, got["q_out"][0], gko[0], got["q"][0], gk[0], rest[0][0], rest[1][0],
-                                             rest[2][0], rope.handle, T, got["q"][3], gk[3], got["q"][5], gk[5],
-                                             got["q_out"][5], gko[5], eps, fl))
+        gq, gqo = _heads(q, "q"), _heads(q_out, "q_out")
+        gk, gko = (none, none) if k is None else (_heads(k, "k"), _heads(k_out, "k_out"))
+        T, host = gq[2], gq[1]
+        for w, g, first in (("q", gq, gq), ("q_out", gqo, gq), ("k", gk, gk), ("k_out", gko, gk)):
+            if g[0] is None:
+                continue
+            if g[2] != T or g[4] != rope.head_dim or g[3] != first[3]:
+                raise InvalidError(f"{w}: {g[2:5]}, {T} tokens of heads of {rope.head_dim} expected")
+            if g[1] != host:
+                raise InvalidError("mix of host and device arrays")
+        ps = []
+        for w, a in (("wq", wq), ("wk", wk)):
+            if a is not None and (tuple(a.shape) != (rope.head_dim,) or _kind(a.dtype) != "float32"):
+                raise InvalidError(f"{w}: float32 [{rope.head_dim}] expected")
+            ps.append(_ptr(a))
+        ps.append(_words(positions, T, "positions"))
+        for _, h in ps:
+            if h is not None and h != host:
+                raise InvalidError("mix of host and device arrays")
+        fl = (LT_HOST_IO if host else 0) | (0 if norm else LT_ROPE_NO_NORM) | (LT_NORM_ONE_PLUS_W if one_plus_w else 0)
+        self._check(self.lib.lt_qk_norm_rope(self.ptr, gqo[0], gko[0], gq[0], gk[0], ps[0][0], ps[1][0], ps[2][0], rope.handle,
+                                             T, gq[3], gk[3], gq[5], gk[5], gqo[5], gko[5], eps, fl))
 
     def kv_cache(self, n_blocks: int, n_kv_heads: int, head_dim: int, n_seqs: int = 1) -> KvCache:
         """An empty cache of n_blocks blocks of 32 tokens for one layer and up to n_seqs sequences."""
@@ -523,14 +538,15 @@ class Context:
         """A step's batch (start, len, new entries of table), positions and slots from the sequences'
         lengths and a list of free blocks (lt_kv_plan)."""
         b, host = batch.struct()
-        n_free = int(np.prod(tuple(free_blocks.shape)))
-        arrays = [_words(len_in, batch.n_seqs, "len_in"), _words(n_new, batch.n_seqs, "n_new"),
-                  _words(free_blocks, n_free, "free_blocks"), _words(used_in, 1, "used_in"), _words(used_out, 1, "used_out"),
-                  _words(positions, batch.n_tokens, "positions"), _words(slots, batch.n_tokens, "slots")]
-        ps = [_ptr(a) for a in arrays]
-        if {h for _, h in ps} != {host}:
-            raise InvalidError("mix of host and device arrays")
-        p = [x for x, _ in ps]
+        n_free = _count(free_blocks)
+        p = []
+        for w, a, n in (("len_in", len_in, batch.n_seqs), ("n_new", n_new, batch.n_seqs), ("free_blocks", free_blocks, n_free),
+                        ("used_in", used_in, 1), ("used_out", used_out, 1), ("positions", positions, batch.n_tokens),
+                        ("slots", slots, batch.n_tokens)):
+            at, h = _words(a, n, w)
+            if h != host:
+                raise InvalidError("mix of host and device arrays")
+            p.append(at)
         self._check(self.lib.lt_kv_plan(self.ptr, C.byref(b), p[0], p[1], p[2], n_free, p[3], p[4], p[5], p[6],
                                         LT_HOST_IO if host else 0))
 
@@ -544,7 +560,7 @@ class Context:
                                f"{cache.head_dim}")
         if go[5] != H * D:
             raise InvalidError("out: must be contiguous")
-        if {gq[1], go[1]} != {host}:
+        if gq[1] != host or go[1] != host:
             raise InvalidError("mix of host and device arrays")
         self._check(self.lib.lt_attention(self.ptr, go[0], gq[0], cache.handle, C.byref(b), H, gq[5], scale, window,
                                           LT_HOST_IO if host else 0))
