@@ -142,15 +142,63 @@ __host__ __device__ __forceinline__ uint32_t append_units(uint32_t n_tokens, uin
     return n_tokens / kKvBlock + 2 * n_seqs;
 }
 
+// The row that unit u belongs to, by a whole wavefront: up to 64 rows from one round of
+// loads, more in three.
+__device__ __forceinline__ uint32_t append_row(const KvBatchDev &b, uint32_t u, KvRow &row) {
+    const auto base = [&](uint32_t start, uint32_t i) { return (start < b.n_tokens ? start : b.n_tokens) / kKvBlock + 2 * i; };
+    uint32_t r;
+    if (b.n_seqs <= kWave) {
+        const uint32_t lane = threadIdx.x % kWave, i = lane < b.n_seqs ? lane : b.n_seqs - 1;
+        const KvRow k = kv_row_of(b, i);
+        const uint64_t below = __ballot(lane < b.n_seqs && base(b.start[i], i) <= u);
+        r = below ? 63 - __builtin_clzll(below) : 0;
+        row.first = __builtin_amdgcn_readlane(k.first, r), row.n = __builtin_amdgcn_readlane(k.n, r);
+        row.len = __builtin_amdgcn_readlane(k.len, r);
+        row.bad = __builtin_amdgcn_readlane(k.bad, r), row.falls = __builtin_amdgcn_readlane(k.falls, r);
+    } else {
+        r = kv_row(b.n_seqs, u, [&](uint32_t i) { return base(b.start[i], i); });
+        row = kv_row_of(b, r);
+    }
+    return r;
+}
+
 // round(x / s), ties to even, |x| <= 127.5 s: the product with 1 / s is at most
 // one code off, and what remains of x beside code * s is exact.
-__device__ __forceinline__ int kv_code(float x, float s, float inv) {
+__device__ __forceinline__ float kv_code(float x, float s, float inv) {
     float q = rintf(x * inv);
     q = fminf(fmaxf(q, -127.0f), 127.0f);
     const float r = fmaf(-q, s, x), h = 0.5f * s;
     if (r > h || (r == h && ((int)q & 1))) q += 1.0f;
     else if (r < -h || (r == -h && ((int)q & 1))) q -= 1.0f;
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+    return fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+// The codes + 128 of 16 values, s > 0 their block's scale (or 0: all 0).  Off a border between two
+// codes the product with 1 / s, off by 2^-16 at most, rounds as the quotient does; where one of a
+// wavefront's values is nearer to one (1 in 10,000 is), all are taken by kv_code.
+__device__ __forceinline__ uint4 kv_codes16(const float (&x)[16], float s) {
+    // (next to the subnormal numbers the remainders of kv_code would not be exact: scaled up by 2^100 they are)
+    const float up = s < 0x1p-100f ? 0x1p100f : 1.0f;
+    const float su = s * up, inv = s > 0.0f ? 1.0f / su : 0.0f;
+    float q[16], near = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const float y = x[e] * up * inv;
+        q[e] = rintf(y);
+        near = fmaxf(near, fabsf(y - q[e]));
+    }
+    if (__any(near > 0.4999f) || up != 1.0f) {  // (a subnormal scale may be too small by a half: kv_code's bounds)
+#pragma unroll
+        for (int e = 0; e < 16; e++) q[e] = s > 0.0f ? kv_code(x[e] * up, su, inv) : 0.0f;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        w[e] = 0;
+#pragma unroll
+        for (int f = 0; f < 4; f++) w[e] = __builtin_amdgcn_cvt_pk_u8_f32(q[4 * e + f] + 128.0f, f, w[e]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ size_t open_at(const KvDev &kv, uint32_t seq, uint32_t h, uint32_t which, uint32_t block) {
@@ -170,11 +218,8 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
                                                               size_t k_stride, size_t v_stride, uint32_t *err) {
     constexpr int kPieces = 2 * D, kSteps = (kPieces + kAppendThreads - 1) / kAppendThreads;
     const uint32_t h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
-    const uint32_t r = kv_row(b.n_seqs, blockIdx.x, [&](uint32_t i) {
-        const uint32_t s = b.start[i];
-        return (s < b.n_tokens ? s : b.n_tokens) / kKvBlock + 2 * i;
-    });
-    const KvRow row = kv_row_of(b, r);
+    KvRow row;
+    const uint32_t r = append_row(b, blockIdx.x, row);
     if (row.n == 0) {
         if (row.falls && tid == 0) kv_report(err, kKvErrRows, r);
         return;
@@ -186,9 +231,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
     const uint32_t begin = row.len - row.n, first = begin / kKvBlock, last = (row.len - 1) / kKvBlock;
     const uint32_t j = blockIdx.x - (row.first / kKvBlock + 2 * r) + first;
     if (j < first || j > last) return;  // (more units than blocks; start that falls)
-    const uint32_t page = b.table[(size_t)r * b.max_blocks + j];
-    const bool lost = page >= kv.n_blocks;
-    if (lost && tid == 0) kv_report(err, kKvErrBlock, r);
+    const uint32_t page = b.table[(size_t)r * b.max_blocks + j];  // (looked at behind the loads of the tokens)
     const float *src = which ? v : k;
     const size_t stride = which ? v_stride : k_stride;
     src += (size_t)row.first * stride + (size_t)h * D;  // token i of the row at i * stride
@@ -197,19 +240,14 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
     const uint32_t held = row.len - base < kKvBlock ? row.len - base : kKvBlock;
     uint2 *tag = kv.tags + (((size_t)r * kv.n_kv + h) * 2 + which) * 2;
     float *open = kv.open + open_at(kv, r, h, which, j);
-    bool stale = false;
-    if (from) {
-        const uint2 t = tag[j & 1];
-        stale = t.x != j || t.y < from;
-        if (stale && tid == 0) kv_report(err, kKvErrOpen, r);
-    }
+    const uint2 held_tag = tag[j & 1];
     // the block's tokens from before lie in the open block, the batch's in src; none: the first of them, to be cleared
     const auto at = [&](uint32_t token) -> const float * {
         return token < from ? open + (size_t)token * D : src + (size_t)(base + (token < held ? token : held - 1) - begin) * stride;
     };
     float x[kSteps][16];
     float top = 0.0f;
-    bool finite = !stale;
+    bool finite = true;
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
         const uint32_t p = tid + i * kAppendThreads, lane = p % kWave, c = p / kWave, g = lane / 16, n = lane % 16;
@@ -235,12 +273,19 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
                 x[i][8 + f] = token < held ? hi : 0.0f;
             }
         }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             finite &= fabsf(x[i][e]) <= 3.402823466e38f;
             top = fmaxf(top, fabsf(x[i][e]));
         }
-    }
+    const bool lost = page >= kv.n_blocks;
+    if (lost && tid == 0) kv_report(err, kKvErrBlock, r);
+    const bool stale = from && (held_tag.x != j || held_tag.y < from);
+    if (stale && tid == 0) kv_report(err, kKvErrOpen, r);
+    finite &= !stale;
     __shared__ float s_top[kAppendThreads / kWave];
     __shared__ int s_bad[kAppendThreads / kWave];
 #pragma unroll
@@ -253,27 +298,12 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
     for (int i = 0; i < kAppendThreads / kWave; i++) top = fmaxf(top, s_top[i]), bad |= s_bad[i] != 0;
     if (!lost) {
         const float s = bad ? __builtin_nanf("") : top / 127.0f;
-        const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-        // (next to the subnormal numbers the remainders of kv_code would not be exact: scaled up by 2^100 they are)
-        const bool tiny = s < 0x1p-100f;
         uint4 *out = reinterpret_cast<uint4 *>(kv.codes + (((size_t)page * kv.n_kv + h) * 2 + which) * kKvBlock * D);
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
             const uint32_t p = tid + i * kAppendThreads;
             if (p >= (uint32_t)kPieces) continue;
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                w[e] = 0;
-#pragma unroll
-                for (int f = 0; f < 4; f++) {
-                    const float y = x[i][4 * e + f];
-                    int code = 0;
-                    if (s > 0.0f) code = tiny ? kv_code(y * 0x1p100f, s * 0x1p100f, 1.0f / (s * 0x1p100f)) : kv_code(y, s, inv);
-                    w[e] |= (uint32_t)(code + 128) << (8 * f);
-                }
-            }
-            out[p] = make_uint4(w[0], w[1], w[2], w[3]);
+            out[p] = kv_codes16(x[i], s);
         }
         if (tid == 0) {
             float *sc = reinterpret_cast<float *>(kv.scales + (size_t)page * kv.n_kv + h);
