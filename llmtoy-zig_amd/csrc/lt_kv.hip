@@ -156,10 +156,13 @@ __device__ __forceinline__ uint32_t append_row(const KvBatchDev &b, uint32_t u, 
         row.len = __builtin_amdgcn_readlane(k.len, r);
         row.bad = __builtin_amdgcn_readlane(k.bad, r), row.falls = __builtin_amdgcn_readlane(k.falls, r);
     } else {
-        r = kv_row(b.n_seqs, u, [&](uint32_t i) { return base(b.start[i], i); });
-        row = kv_row_of(b, r);
+        r = __builtin_amdgcn_readfirstlane(kv_row(b.n_seqs, u, [&](uint32_t i) { return base(b.start[i], i); }));
+        const KvRow k = kv_row_of(b, r);
+        row.first = __builtin_amdgcn_readfirstlane(k.first), row.n = __builtin_amdgcn_readfirstlane(k.n);
+        row.len = __builtin_amdgcn_readfirstlane(k.len);
+        row.bad = __builtin_amdgcn_readfirstlane(k.bad), row.falls = __builtin_amdgcn_readfirstlane(k.falls);
     }
-    return r;
+    return r;  // (in scalar registers, as what follows from it)
 }
 
 // round(x / s), ties to even, |x| <= 127.5 s: the product with 1 / s is at most
@@ -168,14 +171,15 @@ __device__ __forceinline__ float kv_code(float x, float s, float inv) {
     float q = rintf(x * inv);
     q = fminf(fmaxf(q, -127.0f), 127.0f);
     const float r = fmaf(-q, s, x), h = 0.5f * s;
-    if (r > h || (r == h && ((int)q & 1))) q += 1.0f;
-    else if (r < -h || (r == -h && ((int)q & 1))) q -= 1.0f;
+    const float odd = fabsf(q) - 2.0f * floorf(0.5f * fabsf(q));  // 1 or 0
+    const float up = fabsf(r) > h ? 1.0f : fabsf(r) == h ? odd : 0.0f;
+    q += r < 0.0f ? -up : up;
     return fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
 // The codes + 128 of 16 values, s > 0 their block's scale (or 0: all 0).  Off a border between two
 // codes the product with 1 / s, off by 2^-16 at most, rounds as the quotient does; where one of a
-// wavefront's values is nearer to one (1 in 10,000 is), all are taken by kv_code.
+// wavefront's values is nearer to one (1 in 25,000 is), all are taken by kv_code.
 __device__ __forceinline__ uint4 kv_codes16(const float (&x)[16], float s) {
     // (next to the subnormal numbers the remainders of kv_code would not be exact: scaled up by 2^100 they are)
     const float up = s < 0x1p-100f ? 0x1p100f : 1.0f;
@@ -187,7 +191,7 @@ __device__ __forceinline__ uint4 kv_codes16(const float (&x)[16], float s) {
         q[e] = rintf(y);
         near = fmaxf(near, fabsf(y - q[e]));
     }
-    if (__any(near > 0.4999f) || up != 1.0f) {  // (a subnormal scale may be too small by a half: kv_code's bounds)
+    if (__any(near > 0.49998f) || up != 1.0f) {  // (a subnormal scale may be too small by a half: kv_code's bounds)
 #pragma unroll
         for (int e = 0; e < 16; e++) q[e] = s > 0.0f ? kv_code(x[e] * up, su, inv) : 0.0f;
     }
@@ -206,18 +210,19 @@ __device__ __forceinline__ size_t open_at(const KvDev &kv, uint32_t seq, uint32_
 }
 
 // Grid: units, heads, keys or values.  A workgroup takes the block's tokens into
-// registers as the layout's pieces (16 elements a thread and step: two runs of
+// registers as the layout's pieces (16 elements a thread: two runs of
 // eight channels for keys, two of eight tokens for values), finds the largest,
-// and writes the codes.  The unit of a row's first block alone keeps that
-// row's fp32 tokens, after it has read those from before.
+// and writes the codes.
 // Bound by the reads of the new tokens; a single token by its chain of
-// latencies.
-constexpr int kAppendThreads = 256;
+// latencies: the lengths, then the table, the tag and the tokens, the largest, the codes.
+// 4,103 tokens of 8 heads of 128: APPEND_FIG; one token each of 16 sequences 6 us.  (Keys
+// and values by one workgroup: slower by a third.)
 template <int D>
-__global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchDev b, const float *k, const float *v,
+__global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, const float *k, const float *v,
                                                               size_t k_stride, size_t v_stride, uint32_t *err) {
-    constexpr int kPieces = 2 * D, kSteps = (kPieces + kAppendThreads - 1) / kAppendThreads;
-    const uint32_t h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+    constexpr int kWaves = 2 * D / kWave;
+    const uint32_t h = blockIdx.y, tid = threadIdx.x, which = blockIdx.z;
+    const uint32_t lane = tid % kWave, c = tid / kWave, g = lane / 16, n = lane % 16;
     KvRow row;
     const uint32_t r = append_row(b, blockIdx.x, row);
     if (row.n == 0) {
@@ -232,92 +237,103 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
     const uint32_t j = blockIdx.x - (row.first / kKvBlock + 2 * r) + first;
     if (j < first || j > last) return;  // (more units than blocks; start that falls)
     const uint32_t page = b.table[(size_t)r * b.max_blocks + j];  // (looked at behind the loads of the tokens)
-    const float *src = which ? v : k;
-    const size_t stride = which ? v_stride : k_stride;
-    src += (size_t)row.first * stride + (size_t)h * D;  // token i of the row at i * stride
-    const uint32_t base = j * kKvBlock;                 // position of the block's first token
-    const uint32_t from = begin > base ? begin - base : 0;  // its first token in the batch
+    const uint32_t base = j * kKvBlock;                           // position of the block's first token
+    const uint32_t from = begin > base ? begin - base : 0;        // its first token in the batch
     const uint32_t held = row.len - base < kKvBlock ? row.len - base : kKvBlock;
     uint2 *tag = kv.tags + (((size_t)r * kv.n_kv + h) * 2 + which) * 2;
-    float *open = kv.open + open_at(kv, r, h, which, j);
     const uint2 held_tag = tag[j & 1];
-    // the block's tokens from before lie in the open block, the batch's in src; none: the first of them, to be cleared
-    const auto at = [&](uint32_t token) -> const float * {
-        return token < from ? open + (size_t)token * D : src + (size_t)(base + (token < held ? token : held - 1) - begin) * stride;
-    };
-    float x[kSteps][16];
-    float top = 0.0f;
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < kSteps; i++) {
-        const uint32_t p = tid + i * kAppendThreads, lane = p % kWave, c = p / kWave, g = lane / 16, n = lane % 16;
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[i][e] = 0.0f;
-        if (p >= (uint32_t)kPieces) continue;
+    const size_t stride = which ? v_stride : k_stride;
+    const float *src = (which ? v : k) + (size_t)row.first * stride + (size_t)h * D;  // token i of the row at i * stride
+    const float *open = kv.open + open_at(kv, r, h, which, j);
+    float x[16];
+    // The thread's piece, token t + more from at(t, more); tokens that nobody has are cleared.
+    const auto piece = [&](auto at, uint32_t n_held) {
         if (which == 0) {
 #pragma unroll
             for (int hi = 0; hi < 2; hi++) {
-                const float4 *row4 = reinterpret_cast<const float4 *>(at(n + 16 * hi) + 32 * c + 8 * g);
+                const float4 *row4 = reinterpret_cast<const float4 *>(at(n, 16 * hi) + 32 * c + 8 * g);
                 const float4 u = row4[0], w = row4[1];
                 const float e8[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int f = 0; f < 8; f++) x[i][8 * hi + f] = n + 16 * hi < held ? e8[f] : 0.0f;
+                for (int f = 0; f < 8; f++) x[8 * hi + f] = n + 16 * hi < n_held ? e8[f] : 0.0f;
             }
         } else {
 #pragma unroll
             for (int f = 0; f < 8; f++) {
-                const uint32_t token = 4 * g + f % 4 + 16 * (f / 4);
-                const float *row1 = at(token) + 32 * c + n;
+                const int more = f % 4 + 16 * (f / 4);
+                const float *row1 = at(4 * g, more) + 32 * c + n;
                 const float lo = row1[0], hi = row1[16];
-                x[i][f] = token < held ? lo : 0.0f;
-                x[i][8 + f] = token < held ? hi : 0.0f;
+                x[f] = 4 * g + more < n_held ? lo : 0.0f;
+                x[8 + f] = 4 * g + more < n_held ? hi : 0.0f;
             }
         }
+    };
+    // (a block that the batch fills: one stride between its tokens, no look at any)
+    if (from == 0 && held == kKvBlock) {
+        const float *block = src + (size_t)(base - begin) * stride;
+        piece([&](uint32_t t, int more) { return block + t * stride + more * stride; }, kKvBlock);
+    } else {
+        // the tokens from before lie in the open block, the batch's in src; none: the last of those
+        piece([&](uint32_t t, int more) -> const float * {
+            t += more;
+            return t < from ? open + (size_t)t * D : src + (size_t)(base + (t < held ? t : held - 1) - begin) * stride;
+        }, held);
     }
-#pragma unroll
-    for (int i = 0; i < kSteps; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            finite &= fabsf(x[i][e]) <= 3.402823466e38f;
-            top = fmaxf(top, fabsf(x[i][e]));
-        }
     const bool lost = page >= kv.n_blocks;
     if (lost && tid == 0) kv_report(err, kKvErrBlock, r);
     const bool stale = from && (held_tag.x != j || held_tag.y < from);
     if (stale && tid == 0) kv_report(err, kKvErrOpen, r);
-    finite &= !stale;
-    __shared__ float s_top[kAppendThreads / kWave];
-    __shared__ int s_bad[kAppendThreads / kWave];
+    float top = 0.0f, odd = 0.0f;  // odd: NaN with an infinity or a NaN among them
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        odd = fmaf(x[e], 0.0f, odd);
+        top = fmaxf(top, fabsf(x[e]));
+    }
+    if (odd != odd || stale) top = __builtin_inff();  // (all of the block becomes NaN)
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-    const bool all_finite = __all(finite);
-    if (tid % kWave == 0) s_top[tid / kWave] = top, s_bad[tid / kWave] = !all_finite;
+    __shared__ float s_top[kWaves];
+    if (lane == 0) s_top[c] = top;
     __syncthreads();  // (and every earlier token of the block is read)
-    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < kAppendThreads / kWave; i++) top = fmaxf(top, s_top[i]), bad |= s_bad[i] != 0;
+    for (int i = 0; i < kWaves; i++) top = fmaxf(top, s_top[i]);
     if (!lost) {
-        const float s = bad ? __builtin_nanf("") : top / 127.0f;
-        uint4 *out = reinterpret_cast<uint4 *>(kv.codes + (((size_t)page * kv.n_kv + h) * 2 + which) * kKvBlock * D);
-#pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            const uint32_t p = tid + i * kAppendThreads;
-            if (p >= (uint32_t)kPieces) continue;
-            out[p] = kv_codes16(x[i], s);
-        }
-        if (tid == 0) {
-            float *sc = reinterpret_cast<float *>(kv.scales + (size_t)page * kv.n_kv + h);
-            sc[which] = s;
-        }
+        const float s = top == __builtin_inff() ? __builtin_nanf("") : top / 127.0f;
+        reinterpret_cast<uint4 *>(kv.codes + (((size_t)page * kv.n_kv + h) * 2 + which) * kKvBlock * D)[tid] = kv_codes16(x, s);
+        if (tid == 0) reinterpret_cast<float *>(kv.scales + (size_t)page * kv.n_kv + h)[which] = s;
     }
-    if (j != first) return;
-    // the fp32 tokens of the row's last two blocks
+    // The fp32 tokens of the row's last two blocks: each by its own unit, unless that would
+    // overwrite, in the place that both share, tokens from before that the first block's
+    // unit reads; then by that one.
     for (uint32_t o = last > first ? last - 1 : last; o <= last; o++) {
+        const bool shared = begin % kKvBlock && o > first && (o - first) % 2 == 0;
+        if (j != (shared ? first : o)) continue;
         const uint32_t b0 = o * kKvBlock, f = begin > b0 ? begin - b0 : 0;
         const uint32_t e = row.len - b0 < kKvBlock ? row.len - b0 : kKvBlock;
         float *dst = kv.open + open_at(kv, r, h, which, o);
-        for (uint32_t i = f * D + tid; i < e * D; i += kAppendThreads)
-            dst[i] = src[(size_t)(b0 + i / D - begin) * stride + i % D];
+        if (shared) {
+            for (uint32_t i = f * D + tid; i < e * D; i += 2 * D)
+                dst[i] = src[(size_t)(b0 + i / D - begin) * stride + i % D];
+        } else if (which == 0) {
+#pragma unroll
+            for (int hi = 0; hi < 2; hi++) {
+                const uint32_t t = n + 16 * hi;
+                float4 *to = reinterpret_cast<float4 *>(dst + (size_t)t * D + 32 * c + 8 * g);
+                if (t >= f && t < e) {
+                    to[0] = make_float4(x[8 * hi], x[8 * hi + 1], x[8 * hi + 2], x[8 * hi + 3]);
+                    to[1] = make_float4(x[8 * hi + 4], x[8 * hi + 5], x[8 * hi + 6], x[8 * hi + 7]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const uint32_t t = 4 * g + u % 4 + 16 * (u / 4);
+                if (t >= f && t < e) {
+                    dst[(size_t)t * D + 32 * c + n] = x[u];
+                    dst[(size_t)t * D + 32 * c + n + 16] = x[8 + u];
+                }
+            }
+        }
         if (tid == 0 && !(o == first && stale)) tag[o & 1] = make_uint2(o, e);
     }
 }
@@ -325,31 +341,63 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvDev kv, KvBatchD
 // ------------------------------------------------------------------- reading
 // The values of single tokens: a thread four channels of a (slot, head).  Bound
 // by the writes.
-__global__ __launch_bounds__(256) void k_kv_read(KvDev kv, const uint32_t *slots, uint32_t n, float *k, float *v) {
-    const uint32_t quads = kv.D / 4;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)n * kv.n_kv * quads) return;
-    const uint32_t d = (uint32_t)(i % quads) * 4;
-    const size_t th = i / quads;
-    const uint32_t h = (uint32_t)(th % kv.n_kv), slot = slots[th / kv.n_kv], page = slot / kKvBlock, t = slot % kKvBlock;
-    const float nan = __builtin_nanf("");
-    float4 ko = make_float4(nan, nan, nan, nan), vo = ko;
-    if (page < kv.n_blocks) {
-        const float2 s = kv.scales[(size_t)page * kv.n_kv + h];
-        const uint8_t *kc = kv.codes + ((size_t)page * kv.n_kv + h) * 2 * kKvBlock * kv.D, *vc = kc + kKvBlock * kv.D;
-        const uint32_t c = d / 32;
-        // keys: four channels of one token in a row
-        const uint32_t kb = *reinterpret_cast<const uint32_t *>(
-            kc + (c * kWave + (d % 32) / 8 * 16 + t % 16) * 16 + (t / 16) * 8 + d % 8);
-        // values: token t is byte (t % 4) + 4 (t / 16) of lane group (t % 16) / 4
-        const uint8_t *vb = vc + (c * kWave + (t % 16) / 4 * 16 + d % 16) * 16 + (d % 32) / 16 * 8 + t % 4 + 4 * (t / 16);
-        const auto val = [](uint32_t byte, float scale) { return (float)((int)byte - 128) * scale; };
-        ko = make_float4(val(kb & 255, s.x), val(kb >> 8 & 255, s.x), val(kb >> 16 & 255, s.x), val(kb >> 24, s.x));
-        vo = make_float4(val(vb[0], s.y), val(vb[16], s.y), val(vb[32], s.y), val(vb[48], s.y));
+constexpr int kReadThreads = 256;
+template <int D, int U>
+__global__ __launch_bounds__(kReadThreads) void k_kv_read(KvDev kv, const uint32_t *slots, uint32_t n, float *k, float *v) {
+    constexpr uint32_t kQuads = D / 4, kPer = kReadThreads / kQuads;  // threads of a slot and head, those of a workgroup
+    const uint32_t th0 = blockIdx.x * (kPer * U) + threadIdx.x / kQuads, d = threadIdx.x % kQuads * 4, all = n * kv.n_kv;
+    if (threadIdx.x >= kPer * kQuads) return;
+    uint32_t page[U], slot[U], kb[U], vb[U][4];
+    float2 s[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t th = th0 + u * kPer < all ? th0 + u * kPer : all - 1;
+        slot[u] = slots[th / kv.n_kv];
     }
-    const size_t at = th * kv.D + d;
-    *reinterpret_cast<float4 *>(k + at) = ko;
-    *reinterpret_cast<float4 *>(v + at) = vo;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t th = th0 + u * kPer < all ? th0 + u * kPer : all - 1, h = th % kv.n_kv, t = slot[u] % kKvBlock, c = d / 32;
+        page[u] = slot[u] / kKvBlock;
+        const size_t at = (size_t)(page[u] < kv.n_blocks ? page[u] : 0) * kv.n_kv + h;
+        s[u] = kv.scales[at];
+        const uint8_t *kc = kv.codes + at * (2 * kKvBlock * D), *vc = kc + kKvBlock * D;
+        // keys: four channels of one token in a row
+        kb[u] = *reinterpret_cast<const uint32_t *>(kc + (c * kWave + (d % 32) / 8 * 16 + t % 16) * 16 + (t / 16) * 8 + d % 8);
+        // values: token t is byte (t % 4) + 4 (t / 16) of lane group (t % 16) / 4
+        const uint8_t *v0 = vc + (c * kWave + (t % 16) / 4 * 16 + d % 16) * 16 + (d % 32) / 16 * 8 + t % 4 + 4 * (t / 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) vb[u][e] = v0[16 * e];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t th = th0 + u * kPer;
+        if (th >= all) return;
+        if (page[u] >= kv.n_blocks) s[u] = make_float2(__builtin_nanf(""), __builtin_nanf(""));
+        const auto val = [](uint32_t byte, float scale) { return (float)((int)byte - 128) * scale; };
+        const size_t at = (size_t)th * D + d;
+        *reinterpret_cast<float4 *>(k + at) = make_float4(val(kb[u] & 255, s[u].x), val(kb[u] >> 8 & 255, s[u].x),
+                                                          val(kb[u] >> 16 & 255, s[u].x), val(kb[u] >> 24, s[u].x));
+        *reinterpret_cast<float4 *>(v + at) = make_float4(val(vb[u][0], s[u].y), val(vb[u][1], s[u].y), val(vb[u][2], s[u].y),
+                                                          val(vb[u][3], s[u].y));
+    }
+}
+
+template <int D>
+void go_append(const KvDev &kv, const KvBatchDev &b, const float *k, const float *v, size_t k_stride, size_t v_stride,
+               uint32_t *err, hipStream_t s) {
+    const uint32_t units = append_units(b.n_tokens, b.n_seqs);
+    hipLaunchKernelGGL(k_kv_append<D>, dim3(units, kv.n_kv, 2), dim3(2 * D), 0, s, kv, b, k, v, k_stride, v_stride, err);
+}
+
+template <int D>
+void go_read(const KvDev &kv, const uint32_t *slots, uint32_t n, float *k, float *v, hipStream_t s) {
+    constexpr uint32_t kPer = kReadThreads / (D / 4);
+    const uint32_t all = n * kv.n_kv;
+    // (enough for every CU: four a thread, side by side)
+    if (all / kPer >= 2048)
+        hipLaunchKernelGGL((k_kv_read<D, 4>), dim3((all + 4 * kPer - 1) / (4 * kPer)), dim3(kReadThreads), 0, s, kv, slots, n, k, v);
+    else
+        hipLaunchKernelGGL((k_kv_read<D, 1>), dim3((all + kPer - 1) / kPer), dim3(kReadThreads), 0, s, kv, slots, n, k, v);
 }
 
 }  // namespace
@@ -363,22 +411,29 @@ hipError_t launch_kv_plan(const KvPlanArgs &a, hipStream_t s) {
 
 hipError_t launch_kv_append(const KvDev &kv, const KvBatchDev &b, const float *k, const float *v, size_t k_stride,
                             size_t v_stride, uint32_t *err, hipStream_t s) {
-    const dim3 grid(append_units(b.n_tokens, b.n_seqs), kv.n_kv, 2), block(kAppendThreads);
     switch (kv.D) {
-    case 64: hipLaunchKernelGGL(k_kv_append<64>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
-    case 96: hipLaunchKernelGGL(k_kv_append<96>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
-    case 128: hipLaunchKernelGGL(k_kv_append<128>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
-    case 192: hipLaunchKernelGGL(k_kv_append<192>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
-    case 256: hipLaunchKernelGGL(k_kv_append<256>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
-    case 512: hipLaunchKernelGGL(k_kv_append<512>, grid, block, 0, s, kv, b, k, v, k_stride, v_stride, err); break;
+    case 64: go_append<64>(kv, b, k, v, k_stride, v_stride, err, s); break;
+    case 96: go_append<96>(kv, b, k, v, k_stride, v_stride, err, s); break;
+    case 128: go_append<128>(kv, b, k, v, k_stride, v_stride, err, s); break;
+    case 192: go_append<192>(kv, b, k, v, k_stride, v_stride, err, s); break;
+    case 256: go_append<256>(kv, b, k, v, k_stride, v_stride, err, s); break;
+    case 512: go_append<512>(kv, b, k, v, k_stride, v_stride, err, s); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
 }
 
 hipError_t launch_kv_read(const KvDev &kv, const uint32_t *slots, uint32_t n, float *k, float *v, hipStream_t s) {
-    const size_t threads = (size_t)n * kv.n_kv * (kv.D / 4);
-    hipLaunchKernelGGL(k_kv_read, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, kv, slots, n, k, v);
+    if ((uint64_t)n * kv.n_kv >= (1ull << 31)) return hipErrorInvalidValue;  // (slots and heads are counted in 32 bits)
+    switch (kv.D) {
+    case 64: go_read<64>(kv, slots, n, k, v, s); break;
+    case 96: go_read<96>(kv, slots, n, k, v, s); break;
+    case 128: go_read<128>(kv, slots, n, k, v, s); break;
+    case 192: go_read<192>(kv, slots, n, k, v, s); break;
+    case 256: go_read<256>(kv, slots, n, k, v, s); break;
+    case 512: go_read<512>(kv, slots, n, k, v, s); break;
+    default: return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
 
