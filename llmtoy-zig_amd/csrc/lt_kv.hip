@@ -215,13 +215,12 @@ __device__ __forceinline__ size_t open_at(const KvDev &kv, uint32_t seq, uint32_
 // and writes the codes.
 // Bound by the reads of the new tokens; a single token by its chain of
 // latencies: the lengths, then the table, the tag and the tokens, the largest, the codes.
-// 4,103 tokens of 8 heads of 128: APPEND_FIG; one token each of 16 sequences 6 us.  (Keys
-// and values by one workgroup: slower by a third.)
-template <int D>
-__global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, const float *k, const float *v,
-                                                              size_t k_stride, size_t v_stride, uint32_t *err) {
+// 4,103 tokens of 8 heads of 128 13.1 us (42 MB), 512 5.5; one token each of 16 sequences 6 us.  (Keys
+// and values by one workgroup: slower by a third.  A code for keys and one for values: 16.5 -> 13.1 us.)
+template <int D, int which>
+__device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b, const float *kv_src, size_t stride, uint32_t *err) {
     constexpr int kWaves = 2 * D / kWave;
-    const uint32_t h = blockIdx.y, tid = threadIdx.x, which = blockIdx.z;
+    const uint32_t h = blockIdx.y, tid = threadIdx.x;
     const uint32_t lane = tid % kWave, c = tid / kWave, g = lane / 16, n = lane % 16;
     KvRow row;
     const uint32_t r = append_row(b, blockIdx.x, row);
@@ -242,8 +241,7 @@ __global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, con
     const uint32_t held = row.len - base < kKvBlock ? row.len - base : kKvBlock;
     uint2 *tag = kv.tags + (((size_t)r * kv.n_kv + h) * 2 + which) * 2;
     const uint2 held_tag = tag[j & 1];
-    const size_t stride = which ? v_stride : k_stride;
-    const float *src = (which ? v : k) + (size_t)row.first * stride + (size_t)h * D;  // token i of the row at i * stride
+    const float *src = kv_src + (size_t)row.first * stride + (size_t)h * D;  // token i of the row at i * stride
     const float *open = kv.open + open_at(kv, r, h, which, j);
     float x[16];
     // The thread's piece, token t + more from at(t, more); tokens that nobody has are cleared.
@@ -336,6 +334,13 @@ __global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, con
         }
         if (tid == 0 && !(o == first && stale)) tag[o & 1] = make_uint2(o, e);
     }
+}
+
+template <int D>
+__global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, const float *k, const float *v, size_t k_stride,
+                                                     size_t v_stride, uint32_t *err) {
+    if (blockIdx.z == 0) append_unit<D, 0>(kv, b, k, k_stride, err);
+    else append_unit<D, 1>(kv, b, v, v_stride, err);
 }
 
 // ------------------------------------------------------------------- reading
