@@ -16,8 +16,8 @@
 // The softmax runs along: m is the largest logit so far (base 2), l the sum of
 // 2^(s - m).  A block's value scale meets the weights, not the sums: with mo the
 // largest of (block's largest logit + log2(scale)) so far, the weights are
-// 2^(s + log2(scale) - mo), at most 1, times 2^15 to use f16's range; their sum
-// times 2^(mo - log2(scale) - m) goes to l.  (Two maxima, because a block of small
+// 2^(s + log2(scale) - mo), times 2^kBits to use f16's range; their sum
+// times 2^(mo - log2(scale) - m) goes to l.  (Both are followed with some slack.)  (Two maxima, because a block of small
 // values may have the largest logit.)
 //
 // Work: a sequence's tiles are cut along the keys into parts of about the same
@@ -390,21 +390,23 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         float mb = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
         mb = row_max(mb);
         mb = mb == kNegInf ? mb : mb * c;
-        const float m1 = fmaxf(m, mb), mo1 = fmaxf(mo, mb + lv);
-        const float ms = m1 == kNegInf ? 0.0f : m1;  // (no key yet)
-        if (__any(m1 > m || mo1 > mo)) {
-            l *= __builtin_amdgcn_exp2f(m - ms);  // (0 before the first key)
-            const float fall = mo == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mo - mo1);
+        if (__any(mb > m + kSlack || mb + lv > mo + kSlack)) {
+            const float m1 = fmaxf(m, mb), mo1 = fmaxf(mo, mb + lv);
+            if (i) {  // (no sums before the first block)
+                l *= __builtin_amdgcn_exp2f(m - (m1 == kNegInf ? 0.0f : m1));  // (0 before the first key)
+                const float fall = mo == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mo - mo1);
 #pragma unroll
-            for (int k = 0; k < 2 * C; k++) o[k] *= fall;
+                for (int k = 0; k < 2 * C; k++) o[k] *= fall;
+            }
+            m = m1, mo = mo1;
         }
-        m = m1, mo = mo1;
+        const float ms = m == kNegInf ? 0.0f : m;  // (no key yet)
         // (a weight of less than 2^-60 of the largest need not be that small among the sums, but counts in l)
-        float e15 = fmaxf(lv - mo1, -60.0f - ms) + 15.0f;
-        if (lv != lv) e15 = lv;
+        float eb = fmaxf(lv - mo, -60.0f - ms) + kBits;
+        if (lv != lv) eb = lv;
         float p[8], sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(t[e], c, e15));
+        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(t[e], c, eb));
         if (edge) {
 #pragma unroll
             for (int e = 0; e < 8; e++)
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) sum += p[e];
-        if (mo1 != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-e15 - ms);
+        if (mo != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-eb - ms);
         half8 ph, pl;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -451,7 +453,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
             put4(to + rr * D + d, x.sum);
             if (d == 0) put4(to + kThinRows * D + 4 * rr, f32x4{x.m, x.l, x.mo, 0.0f});
         } else {
-            const float scale = w.bad ? __builtin_nanf("") : out_scale(x.m, x.l, x.mo, 15.0f);
+            const float scale = w.bad ? __builtin_nanf("") : out_scale(x.m, x.l, x.mo, kBits);
             *reinterpret_cast<f32x4 *>(out_of(rr) + d) = x.sum * scale;
         }
     };
@@ -471,8 +473,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     // The part that is last at its group joins the group, the group that is last at its
     // tile the tile.  A part's stores are acknowledged before it counts; the one that
     // counts last reads past the L2s, and leaves the counters at zero.
-    const uint32_t hands = all < (uint32_t)NT ? NT / all : 1;
-    const uint32_t in_group = w.splits <= kJoin || w.splits <= 8 * hands ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
+    const uint32_t most_hands = all < (uint32_t)NT ? NT / all : 1;
+    const uint32_t in_group = w.splits <= kJoin || w.splits <= 8 * most_hands ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
     const uint32_t grp = w.split / in_group, slot0 = w.slot - w.split, g0 = slot0 + grp * in_group;
     const uint32_t gn = w.splits - grp * in_group < in_group ? w.splits - grp * in_group : in_group;
     const uint32_t groups = (w.splits + in_group - 1) / in_group;
@@ -492,6 +494,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     // threads than a part has places, the parts are dealt out to `hands` of them, and what
     // those make of them is joined through LDS.
     const auto join = [&](uint32_t slot, uint32_t step, uint32_t count, float *to) {
+        const uint32_t hands = count <= kBatch ? 1 : most_hands;  // (one after the other: a thread reads them all at once)
         const uint32_t hand = hands > 1 ? tid / all : 0;
         for (uint32_t at0 = 0; at0 < all; at0 += NT) {
             const uint32_t at = hands > 1 ? tid - hand * all : at0 + tid;

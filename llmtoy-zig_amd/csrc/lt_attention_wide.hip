@@ -26,10 +26,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// The reference of the weights may lag behind the largest logit by this much
-// (base 2), so that sums are rarely scaled down; weights go in times 2^kBits, and
-// 2^(kBits + kSlack) is in f16's range.
-constexpr float kSlack = 3.0f, kBits = 12.0f;
 constexpr uint32_t kLeast = 8;      // blocks that a workgroup is worth having for
 constexpr uint32_t kMaxTiles = 1024;  // of a head, whose blocks are counted in LDS
 constexpr uint32_t kJoin = 16;      // parts joined at once; more are joined in groups first

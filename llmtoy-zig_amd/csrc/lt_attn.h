@@ -16,6 +16,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // that what else is in the batch does not change its results.
 constexpr uint32_t kThinMost = 32;
 
+// The reference of the weights may lag behind the largest logit by this much
+// (base 2), so that sums are rarely scaled down; weights go in times 2^kBits, and
+// 2^(kBits + kSlack) is in f16's range.
+constexpr float kSlack = 3.0f, kBits = 12.0f;
+
 constexpr float kNegInf = -__builtin_huge_valf();
 
 __device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
