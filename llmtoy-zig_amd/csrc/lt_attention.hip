@@ -212,7 +212,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     constexpr int W = Sh::kWaves, C = Sh::C, NT = Sh::kThreads, SPLIT = Sh::kSplit, NB = Sh::kBlocks;
     constexpr bool kQueriesInLds = Sh::kQueriesInLds;
     constexpr uint32_t kBatch = D <= 128 ? 8 : 16;  // parts that a thread reads at once
-    constexpr size_t P = kThinRows * (D + 4);  // floats of a part
+    constexpr uint32_t P = kThinRows * (D + 4);  // floats of a part
     // the wavefronts' sums; the queries lie there before, where they are in LDS
     __shared__ __align__(16) float s_o[NB][kThinRows][D + 4];
     __shared__ f32x4 s_m[NB][kThinRows];
@@ -446,12 +446,14 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         const uint32_t r1 = w.tile * kThinRows + rr;
         return a.out + ((size_t)(w.first + r1 / a.group) * a.n_heads + h * a.group + r1 % a.group) * D;
     };
-    const auto place = [&](uint32_t slot) { return a.part + ((size_t)h * a.slots + slot) * P; };
+    const Shared shared(a.part, a.n_kv * a.slots * P);
+    const auto place = [&](uint32_t slot) { return (h * a.slots + slot) * P; };
     // A row's four channels, to a part's place or to the outputs.
-    const auto put = [&](const Joint &x, uint32_t rr, uint32_t d, float *to) {
-        if (to) {
-            put4(to + rr * D + d, x.sum);
-            if (d == 0) put4(to + kThinRows * D + 4 * rr, f32x4{x.m, x.l, x.mo, 0.0f});
+    constexpr uint32_t kOut = 0xffffffffu;
+    const auto put = [&](const Joint &x, uint32_t rr, uint32_t d, uint32_t to) {
+        if (to != kOut) {
+            shared.put(to + rr * D + d, x.sum);
+            if (d == 0) shared.put(to + kThinRows * D + 4 * rr, f32x4{x.m, x.l, x.mo, 0.0f});
         } else {
             const float scale = w.bad ? __builtin_nanf("") : out_scale(x.m, x.l, x.mo, kBits);
             *reinterpret_cast<f32x4 *>(out_of(rr) + d) = x.sum * scale;
@@ -466,7 +468,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         Joint x;
         x.clear();
         x.add(st, v, NB);
-        put(x, rr, d, w.splits > 1 ? place(w.slot) : nullptr);
+        put(x, rr, d, w.splits > 1 ? place(w.slot) : kOut);
     }
     if (w.splits == 1) return;
 
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     // Parts slot, slot + step, ..: their sums to `to`, or to the outputs.  Where there are more
     // threads than a part has places, the parts are dealt out to `hands` of them, and what
     // those make of them is joined through LDS.
-    const auto join = [&](uint32_t slot, uint32_t step, uint32_t count, float *to) {
+    const auto join = [&](uint32_t slot, uint32_t step, uint32_t count, uint32_t to) {
         const uint32_t hands = count <= kBatch ? 1 : most_hands;  // (one after the other: a thread reads them all at once)
         const uint32_t hand = hands > 1 ? tid / all : 0;
         for (uint32_t at0 = 0; at0 < all; at0 += NT) {
@@ -508,8 +510,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
 #pragma unroll
                     for (uint32_t u = 0; u < kBatch; u++) {
                         if (u % 4 == 0 && u >= n_here) break;
-                        const float *p = place(slot + (u < n_here ? u0 + u * hands : u0) * step);
-                        st[u] = get4(p + kThinRows * D + 4 * rr), v[u] = get4(p + 4 * at);
+                        const uint32_t p = place(slot + (u < n_here ? u0 + u * hands : u0) * step);
+                        st[u] = shared.get(p + kThinRows * D + 4 * rr), v[u] = shared.get(p + 4 * at);
                     }
                     x.add(st, v, n_here);
                 }
@@ -528,11 +530,11 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     };
     if (!last(tickets + 2 * g0, gn)) return;
     if (groups == 1) {
-        join(g0, 1, gn, nullptr);
+        join(g0, 1, gn, kOut);
         return;
     }
     join(g0, 1, gn, place(g0));  // (each thread has read its own of the group's first place before it writes there)
-    if (last(tickets + 2 * slot0 + 1, groups)) join(slot0, in_group, groups, nullptr);
+    if (last(tickets + 2 * slot0 + 1, groups)) join(slot0, in_group, groups, kOut);
 }
 
 // Workgroups of a head: a tile more or less a sequence, and the parts of those

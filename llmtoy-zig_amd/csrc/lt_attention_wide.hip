@@ -58,7 +58,7 @@ struct Shape {
     static constexpr int kPerCu = D == 64 ? 3 : D == 192 ? 2 : 1;
     static constexpr int kThreads = kWaves * kWave, kRows = 32 * kWaves / kSplit;
     static constexpr int DW = D / kSplit, S = DW / 16, CB = DW / 32;
-    static constexpr size_t kPart = (size_t)kWaves * (CB * 4 + 1) * kWave * 4;  // floats
+    static constexpr uint32_t kPart = kWaves * (CB * 4 + 1) * kWave * 4;  // floats
 };
 
 struct Tile {
@@ -483,15 +483,16 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         while (f + 1 < pieces && total * (f + 1) / pieces <= first) f++;
         while (g + 1 < pieces && total * (g + 1) / pieces <= end - 1) g++;
         const uint32_t parts = g - f + 1, me = piece - f;
+        const Shared shared(a.part, 2 * a.pieces * Sh::kPart);
         const auto place = [&](uint32_t i) { return 2 * (f + i) + (i == 0); };
         const auto put = [&](uint32_t slot) {
-            float *to = a.part + slot * Sh::kPart + (size_t)wave * ((CB * 4 + 1) * kWave * 4) + lane * 4;
+            const uint32_t to = slot * Sh::kPart + wave * ((CB * 4 + 1) * kWave * 4) + lane * 4;
 #pragma unroll
             for (int k = 0; k < CB; k++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    put4(to + (k * 4 + i) * (kWave * 4), f32x4{o[k][4 * i], o[k][4 * i + 1], o[k][4 * i + 2], o[k][4 * i + 3]});
-            put4(to + CB * 4 * (kWave * 4), f32x4{m, l, mo, 0.0f});
+                    shared.put(to + (k * 4 + i) * (kWave * 4), f32x4{o[k][4 * i], o[k][4 * i + 1], o[k][4 * i + 2], o[k][4 * i + 3]});
+            shared.put(to + CB * 4 * (kWave * 4), f32x4{m, l, mo, 0.0f});
         };
         const auto join = [&](uint32_t from, uint32_t step, uint32_t count) {
 #pragma unroll
@@ -500,11 +501,11 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
                 for (int j = 0; j < 16; j++) o[k][j] = 0.0f;
             m = kNegInf, mo = kNegInf, l = 0.0f;
             for (uint32_t i = 0; i < count; i++) {
-                const float *p = a.part + place(from + i * step) * Sh::kPart + (size_t)wave * ((CB * 4 + 1) * kWave * 4) + lane * 4;
+                const uint32_t p = place(from + i * step) * Sh::kPart + wave * ((CB * 4 + 1) * kWave * 4) + lane * 4;
                 f32x4 v[CB * 4];
 #pragma unroll
-                for (int k = 0; k < CB * 4; k++) v[k] = get4(p + k * (kWave * 4));
-                const f32x4 st = get4(p + CB * 4 * (kWave * 4));
+                for (int k = 0; k < CB * 4; k++) v[k] = shared.get(p + k * (kWave * 4));
+                const f32x4 st = shared.get(p + CB * 4 * (kWave * 4));
                 const float m1 = fmaxf(m, st[0]), mo1 = fmaxf(mo, st[2]);
                 l *= m == kNegInf ? 1.0f : exp2f(m - m1);  // (l is 0 or NaN then)
                 l += st[0] == kNegInf ? st[1] : st[1] * exp2f(st[0] - m1);

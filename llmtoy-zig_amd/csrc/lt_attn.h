@@ -10,6 +10,7 @@ namespace lt {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Rows (tokens times heads of a group) of a sequence up to which lt_attention.hip's
 // kernel takes it; the other kernel takes those with more.  By the sequence alone, so
@@ -57,18 +58,19 @@ __device__ __forceinline__ float rest1(half2v h, float p) {
     return r;
 }
 
-// Partial results go past the L2s (agent scope): another XCD reads them.
-__device__ __forceinline__ void put4(float *p, f32x4 v) {
-    uint64_t *q = reinterpret_cast<uint64_t *>(p);
-    __hip_atomic_store(q, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(q + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x4 get4(const float *p) {
-    const uint64_t *q = reinterpret_cast<const uint64_t *>(p);
-    const float2 a = __builtin_bit_cast(float2, __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    const float2 b = __builtin_bit_cast(float2, __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    return f32x4{a.x, a.y, b.x, b.y};
-}
+// Partial results go past the L2s (sc1: agent scope), since another XCD reads them: 16 bytes a lane,
+// at a float's index from the workspace's begin.
+struct Shared {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ Shared(float *p, uint32_t floats) : r(__builtin_amdgcn_make_buffer_rsrc(p, 0, floats * 4, 0x00020000)) {}
+    __device__ __forceinline__ void put(uint32_t at, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at * 4, 0, kPast);
+    }
+    __device__ __forceinline__ f32x4 get(uint32_t at) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at * 4, 0, kPast));
+    }
+    static constexpr int kPast = 16;  // sc1
+};
 
 // What an output is of its sums: 2^(mo - m) / l, without the weights' 2^bits; no
 // key seen: 0.
