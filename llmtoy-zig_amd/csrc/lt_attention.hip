@@ -307,7 +307,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         top = row_max(fine ? top : __builtin_inff());
         if (SPLIT > 1) {  // (the other wavefront's channels too)
             if (g == 0) s_top[wave][n] = top;
-            __syncthreads();
+            lds_barrier();
             top = fmaxf(top, s_top[wave ^ 1][n]);
         }
         const bool bad = top > 3.402823466e38f;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
             }
         }
     }
-    if (kQueriesInLds) __syncthreads();
+    if (kQueriesInLds) lds_barrier();
 
     f32x4 o[2 * C];
 #pragma unroll
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         if (SPLIT > 1) {
             f32x4 *x = s_x + i % 2 * (W * 2 * kWave) + lane;
             x[wave * 2 * kWave] = sa[0], x[(wave * 2 + 1) * kWave] = sa[1];
-            __syncthreads();
+            lds_barrier();
             sa[0] += x[(wave ^ 1) * 2 * kWave], sa[1] += x[((wave ^ 1) * 2 + 1) * kWave];
         }
         if (!on) continue;

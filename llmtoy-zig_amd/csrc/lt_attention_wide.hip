@@ -363,11 +363,11 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
             for (int j = 0; j < 16; j++) o[i][j] = 0.0f;
         float m = kNegInf, l = 0.0f, mo = kNegInf;
 
-        __syncthreads();  // (the last segment's readers of s_kv)
+        lds_barrier();  // (the last segment's readers of s_kv)
         stage(b0);
         ks_l = ks_n, lv_l = lv_n;
         fetch(b0 + 1);
-        __syncthreads();
+        lds_barrier();
         for (uint32_t j = b0; j < b1; j++) {
             if ((j - b0) % kWave == 0) ks_l = ks_n, lv_l = lv_n;
             stage(j + 1);
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     s_x[(wave * 4 + e) * kWave + lane] = f32x4{acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]};
-                __syncthreads();
+                lds_barrier();
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const f32x4 v = s_x[((wave ^ 1) * 4 + e) * kWave + lane];
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
                     o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i % 2], o[i / 2], 0, 0, 0);
                 });
             }
-            __syncthreads();
+            lds_barrier();
         }
         l += __shfl_xor(l, 32, kWave);
 

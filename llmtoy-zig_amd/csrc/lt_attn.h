@@ -26,6 +26,10 @@ constexpr float kNegInf = -__builtin_huge_valf();
 
 __device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// A barrier behind which the workgroup's LDS accesses are done, and no more: __syncthreads
+// also waits for the loads from memory that are under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // A byte code + 128 is the f16 number 1024 + 128 + code with the byte 0x64 above it.
 __device__ __forceinline__ half8 codes8(uint32_t a, uint32_t b) {
     union {
