@@ -428,7 +428,8 @@ typedef struct lt_kv lt_kv;
  * i's last ones, at the positions len[i] - (start[i + 1] - start[i]) .. len[i] - 1;
  * position p lies in block table[i * max_blocks + p / LT_KV_BLOCK].  start does not
  * fall and ends at n_tokens or before; tokens behind the last sequence belong to nobody
- * and are left alone.  A sequence with no token in the batch is idle.  The pointers are
+ * and are left alone.  A sequence with no token in the batch is idle.  (Where start falls all the same,
+ * which is reported, sequences may overlap, and the tokens of any of them may be left out.)  The pointers are
  * host memory with LT_HOST_IO, device memory (4-byte aligned) otherwise. */
 typedef struct {
     uint32_t n_seqs;     /* 1 .. 4096 */

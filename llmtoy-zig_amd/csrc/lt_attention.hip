@@ -58,7 +58,7 @@ struct ThinArgs {
     size_t q_stride;
     uint32_t n_heads, group, window;
     float scale2;  // scale * log2(e)
-    float *part;        // [n_kv][slots]: [16][D] sums, then [16][4] m, l, mo
+    float *part;        // [n_kv][2][slots] of parts and of groups of them: [16][D] sums, then [16][4] m, l, mo
     uint32_t *tickets;  // [n_kv][slots][2]: groups, tiles; zero between launches
     uint32_t slots, target;  // parts of all heads that the work is cut into, about
     uint32_t least;          // blocks a part, at least
@@ -76,8 +76,8 @@ __device__ __forceinline__ ThinRow thin_row(const ThinArgs &a, uint32_t r) {
     ThinRow t;
     t.k = kv_row_of(a.b, r);
     // (beyond max_new: as many as the grid has room for, and those get NaN)
-    const uint32_t n = a.b.max_new && t.k.n > a.b.max_new ? a.b.max_new : t.k.n;
-    t.tiles = n * a.group > kThinMost ? 0 : (n * a.group + kThinRows - 1) / kThinRows;
+    if (a.b.max_new && t.k.n > a.b.max_new) t.k.n = a.b.max_new;
+    t.tiles = t.k.n * a.group > kThinMost ? 0 : (t.k.n * a.group + kThinRows - 1) / kThinRows;
     t.lo = 0;
     t.blocks = 1;
     if (!t.k.bad && t.k.n) {
@@ -105,7 +105,7 @@ __device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, float sum) {
 // A tile's parts.  None where a workgroup has its blocks done before parts are joined; parts of
 // `least` where there are few, for their latency; else no more parts than the chip has room for at once.
 __device__ __forceinline__ uint32_t thin_splits(const ThinArgs &a, uint32_t blocks, uint32_t share) {
-    if (blocks <= 3 * a.least) return 1;
+    if (blocks <= 3 * a.least || share == 0xffffffffu) return 1;
     uint32_t n = share > a.least ? blocks / share : (blocks + share - 1) / share;
     if (n == 0) n = 1;
     return n < kJoin * kJoin ? n : kJoin * kJoin;
@@ -117,12 +117,14 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
     ThinWork w{};
     const uint32_t lane = threadIdx.x % kWave;
     float sum = 0.0f;  // (a count beyond 2^24 need not be exact)
+    bool falls = false;
     ThinRow t{};
     for (uint32_t r0 = 0; r0 < a.b.n_seqs; r0 += kWave) {
         const uint32_t r = r0 + lane;
         if (r >= a.b.n_seqs) break;
         t = thin_row(a, r);
         if (t.k.falls && blockIdx.x == 0 && blockIdx.y == 0) kv_report(a.err, kKvErrRows, r);
+        falls |= t.k.falls;
         sum += (float)t.tiles * (float)t.blocks;
     }
     if (a.b.n_seqs > 1) {
@@ -131,7 +133,9 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
     } else {
         sum = __uint_as_float(from_lane(__float_as_uint(sum), 0));
     }
-    const uint32_t share = thin_share(a, sum);
+    // (where start falls, sequences may overlap and have more tiles than the grid has workgroups for: whole
+    // tiles, so that none waits for a part that nobody takes)
+    const uint32_t share = __any(falls) ? 0xffffffffu : thin_share(a, sum);
     uint32_t seen = 0, joined = 0;  // workgroups and joined parts of the rows before
     for (uint32_t r0 = 0; r0 < a.b.n_seqs; r0 += kWave) {
         const uint32_t r = r0 + lane;
@@ -446,8 +450,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         const uint32_t r1 = w.tile * kThinRows + rr;
         return a.out + ((size_t)(w.first + r1 / a.group) * a.n_heads + h * a.group + r1 % a.group) * D;
     };
-    const Shared shared(a.part, a.n_kv * a.slots * P);
-    const auto place = [&](uint32_t slot) { return (h * a.slots + slot) * P; };
+    const Shared shared(a.part, a.n_kv * 2 * a.slots * P);
+    const auto place = [&](uint32_t slot) { return (h * 2 * a.slots + slot) * P; };
     // A row's four channels, to a part's place or to the outputs.
     constexpr uint32_t kOut = 0xffffffffu;
     const auto put = [&](const Joint &x, uint32_t rr, uint32_t d, uint32_t to) {
@@ -533,8 +537,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         join(g0, 1, gn, kOut);
         return;
     }
-    join(g0, 1, gn, place(g0));  // (each thread has read its own of the group's first place before it writes there)
-    if (last(tickets + 2 * slot0 + 1, groups)) join(slot0, in_group, groups, kOut);
+    join(g0, 1, gn, place(a.slots + g0));
+    if (last(tickets + 2 * slot0 + 1, groups)) join(a.slots + slot0, in_group, groups, kOut);
 }
 
 // Workgroups of a head: a tile more or less a sequence, and the parts of those
@@ -567,7 +571,7 @@ bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D
 static bool wide(const AttnArgs &a) { return (uint64_t)(a.b.max_new ? a.b.max_new : a.b.n_tokens) * a.group > kThinMost; }
 
 size_t attention_workspace(const AttnArgs &a) {
-    const size_t thin = (size_t)a.kv.n_kv * thin_slots(kThinTarget, a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
+    const size_t thin = (size_t)a.kv.n_kv * 2 * thin_slots(kThinTarget, a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
     const size_t more = wide(a) ? attention_wide_workspace(a.kv.D) : 0;
     return thin < more ? more : thin;
 }

@@ -184,6 +184,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         if (k.falls && blockIdx.x == 0) kv_report(a.err, kKvErrRows, r);
     }
     uint32_t at = scan<W>(mine, s_sum32, all_tiles);
+    if (all_tiles > a.tiles) return;  // (start falls, sequences overlap; reported)
     // ---- what this workgroup takes: blocks u .. u1 - 1 of the line of heads and tiles, or a tile
     uint64_t u = 0, u1 = 1, line = 0, total = 0;
     uint32_t pieces = 1, piece = 0, head_kv = 0;
