@@ -40,7 +40,70 @@ def test_gpu_attention_in_many_parts(ctx, D, KV, G, past, new):
     c.free()
 
 
-@pytest.mark.parametrize("G,max_new,news", [(3, 1, [1, 30, 1]), (3, 12, [12, 30, 12])])
+# more than 512 rows a sequence, and just as many: whole tiles and pieces of them, windows, odd groups
+ROWS = [
+    (64, 1, 3, [0], [171], 0), (64, 1, 4, [500], [128], 0), (96, 1, 5, [77], [131], 0), (96, 2, 2, [0, 3], [300, 256], 40),
+    (128, 1, 7, [1000], [90], 300), (128, 2, 3, [0], [1500], 0), (192, 1, 4, [90], [150], 0), (192, 1, 9, [0], [60], 17),
+    (256, 1, 11, [333], [60], 0), (256, 2, 2, [0, 64], [270, 1], 0), (512, 1, 16, [100], [40], 0), (512, 1, 3, [40], [180], 64),
+    (64, 8, 1, [3000], [520], 0), (128, 1, 128, [31], [5], 0), (64, 2, 8, [0] * 12, [70] * 12, 0), (512, 2, 8, [6000], [65], 0),
+]
+
+
+@pytest.mark.parametrize("D,KV,G,past,new,window", ROWS)
+def test_gpu_attention_of_many_rows(ctx, D, KV, G, past, new, window):
+    print(f"rows {D} {KV}x{G} {past[:3]} {new[:3]} {window}", flush=True)
+    g, s, k, v, c, q, total, scale = _attend(ctx, D, KV, G, past, new, window, seed=4)
+    want, bound = _expect(k, v, q, total, new, scale, window)
+    b, qd = s.batch(total, new, len(q) + 2), dev(np.concatenate([q, q[:2]]))
+    first = None
+    for _ in range(2):
+        out = dev(np.full((len(q) + 2,) + q.shape[1:], 5, np.float32))
+        ctx.attention(out, qd, c, b, scale, window)
+        ctx.sync()
+        got = out.numpy()
+        first = got if first is None else first
+        assert np.array_equal(got, first)
+    close(first[:len(q)], want, bound)
+    assert (first[len(q):] == 5).all()
+    c.free()
+
+
+@pytest.mark.parametrize("G,new", [(8, 80), (4, 129)])
+def test_gpu_many_rows_see_no_further_than_their_mask(ctx, G, new):
+    print(f"many rows: NaN and infinities in and out of sight, nothing in sight but zeros {G} {new}", flush=True)
+    D, KV, window = 64, 1, 40
+    g, s, k, v, c, q, total, scale = _attend(ctx, D, KV, G, [200], [new], window)
+    c.free()
+    k[0][5, 0, 3], v[0][40, 0, 2] = np.inf, np.nan  # blocks 0 and 1: out of every window
+    v[0][170:240] = 0  # blocks of nothing
+    k[0][224:256] = 0
+    q[3] = 0
+    clean = [x.copy() for x in (k[0], v[0])]
+    for x in clean:
+        x[:64] = 0
+    want, bound = _expect([clean[0]], [clean[1]], q, total, [new], scale, window)
+    c = filled(ctx, s, k, v, KV, D)
+    out = DeviceArray(q.shape)
+    ctx.attention(out, dev(q), c, s.batch(total, [new]), scale, window)
+    ctx.sync()
+    close(out.numpy(), want, bound)
+    want, bound = _expect([clean[0]], [clean[1]], q, total, [new], 0.0, window)  # all keys alike
+    ctx.attention(out, dev(q), c, s.batch(total, [new]), 0.0, window)
+    ctx.sync()
+    close(out.numpy(), want, bound)
+    c.free()
+    k[0][225, 0, 1] = np.nan  # a block that some see
+    c = filled(ctx, s, k, v, KV, D)
+    ctx.attention(out, dev(q), c, s.batch(total, [new]), scale, window)
+    ctx.sync()
+    pos = np.arange(200, 200 + new)
+    sees = (pos >= 224) & (pos - window + 1 <= 255)
+    got = out.numpy()
+    assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
+    c.free()
+
+
+@pytest.mark.parametrize("G,max_new,news", [(3, 1, [1, 30, 1]), (3, 12, [12, 30, 12]), (30, 20, [20, 30, 20])])
 def test_gpu_tokens_beyond_max_new_are_left_alone(ctx, G, max_new, news):
     print(f"tokens beyond max_new {G} {max_new}", flush=True)
     g, s, k, v, c, q, total, scale = _attend(ctx, 64, 1, G, [100] * 3, news, 0)
@@ -56,7 +119,7 @@ def test_gpu_tokens_beyond_max_new_are_left_alone(ctx, G, max_new, news):
     c.free()
 
 
-@pytest.mark.parametrize("each,past", [(6, 3000), (40, 1000)])
+@pytest.mark.parametrize("each,past", [(6, 3000), (40, 1000), (160, 1000)])
 def test_gpu_overlapping_sequences_do_not_spoil_later_calls(ctx, each, past):
     print(f"overlapping sequences {each} {past}", flush=True)
     G, n = 4, 9
