@@ -63,10 +63,19 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
     if (lane == kWave - 1) s_wave[0][wave] = itok, s_wave[1][wave] = ineed;
     if (tid == 0) s_used = used;
     __syncthreads();  // (every length is read: len and len_in may be one array, so may used and used_in)
-    uint64_t btok = itok - tok, bneed = ineed - need;
-    for (uint32_t w = 0; w < wave; w++) btok += s_wave[0][w], bneed += s_wave[1][w];
-    uint64_t all = 0, fresh = 0;
-    for (uint32_t w = 0; w < kPlanThreads / kWave; w++) all += s_wave[0][w], fresh += s_wave[1][w];
+    // (the wavefronts' sums, a lane each: those before this one's, and all)
+    static_assert(kPlanThreads / kWave == 16, "");
+    uint64_t before[2], sum[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint64_t mine = s_wave[k][lane % 16];
+        uint64_t up = lane % 16 < wave ? mine : 0, every = mine;
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) up += __shfl_xor(up, off, kWave), every += __shfl_xor(every, off, kWave);
+        before[k] = up, sum[k] = every;
+    }
+    uint64_t btok = itok - tok + before[0], bneed = ineed - need + before[1];
+    const uint64_t all = sum[0], fresh = sum[1];
     uint32_t most = used;
     for (uint32_t i = 0; i < kPlanRows; i++) {
         const uint32_t r = tid * kPlanRows + i;
@@ -88,7 +97,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
         btok += add[i];
         bneed += b1 - b0;
     }
-    atomicMax(&s_used, most);
+    // (a wavefront's largest first: 1,024 atomics on one word took 3 us)
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) most = max(most, (uint32_t)__shfl_xor(most, off, kWave));
+    if (lane == 0) atomicMax(&s_used, most);
     __syncthreads();
     if (tid == 0) {
         a.start[a.n_seqs] = sat32(all);
@@ -102,17 +114,24 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
         if (b0 != kKvNone) a.table[(size_t)r * a.max_blocks + b0 + (k - s_need[r])] = a.free_blocks[used + k];
     }
     if (a.n_tokens > kPlanTokens) return;
-    __syncthreads();
-    __threadfence_block();
+    // (a new block's number from the list, not from the table, which is being written)
     const uint32_t end = (uint32_t)(all < a.n_tokens ? all : a.n_tokens);
     for (uint32_t t = tid; t < a.n_tokens; t += kPlanThreads) {
-        uint32_t pos = 0, slot = kKvNone;
+        uint64_t pos = 0;
+        uint32_t slot = kKvNone;
         if (t < end) {
             const uint32_t r = plan_row(s_first, a.n_seqs, t);
-            pos = s_pos[r] + (t - s_first[r]);
-            slot = plan_slot(a, r, pos);
+            pos = (uint64_t)s_pos[r] + (t - s_first[r]);
+            const uint64_t j = pos / kKvBlock, first_new = ((uint64_t)s_pos[r] + kKvBlock - 1) / kKvBlock;
+            uint32_t block = kKvNone;
+            if (j >= first_new) {
+                if (s_block[r] != kKvNone) block = a.free_blocks[used + s_need[r] + (uint32_t)(j - first_new)];
+            } else if (j < a.max_blocks) {
+                block = a.table[(size_t)r * a.max_blocks + j];
+            }
+            if (block < kKvNone / kKvBlock) slot = block * kKvBlock + (uint32_t)pos % kKvBlock;
         }
-        a.pos[t] = pos;
+        a.pos[t] = (uint32_t)pos;
         a.slot[t] = slot;
     }
 }
