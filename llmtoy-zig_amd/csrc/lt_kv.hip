@@ -13,8 +13,8 @@ namespace {
 // order, and their tokens lie in the batch in order.  Both are prefix sums over
 // the rows, which one workgroup takes (kPlanRows a thread); new blocks and
 // tokens then look their row up in the sums.  Bound by its chain of latencies:
-// the lengths, the sums, the table's entry, the slot (8 rows 7.2 us; 2,000 rows 8.4, and the
-// maps of 65,536 tokens 6.2 behind it).
+// the lengths, the sums, the table's entry, the slot (8 rows 5.1 us; 2,000 rows 6.2, and the
+// maps of 65,536 tokens 6.1 behind it).
 constexpr uint32_t kPlanThreads = 1024, kPlanRows = kKvMaxSeqs / kPlanThreads;
 // Tokens of a batch that the one workgroup maps; more go to a grid of their own
 // behind it (k_kv_slots).

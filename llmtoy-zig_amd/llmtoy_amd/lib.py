@@ -204,15 +204,28 @@ def _kind(dtype) -> str:
     return str(np.dtype(dtype)) if isinstance(dtype, type) else str(dtype).replace("torch.", "")
 
 
+_WORD = {}  # types seen: whether they are 32-bit whole numbers
+
+
+def _is_word(dtype) -> bool:
+    got = _WORD.get(dtype)
+    if got is None:
+        got = _WORD[dtype] = _kind(dtype) in ("int32", "uint32")
+    return got
+
+
 def _count(a) -> int:
     return a.numel() if _is_torch(a) else math.prod(a.shape)
 
 
 def _words(a, n: int, what: str):
     """(pointer, is_host) of a contiguous array of n 32-bit whole numbers."""
+    if type(a).__module__ == "torch":  # (the usual case of a step, ten times a call: nothing looked up twice)
+        if _is_word(a.dtype) and a.numel() == n and a.is_contiguous():
+            return a.data_ptr(), not a.is_cuda
     if a is None:
         raise InvalidError(f"{what}: an array of {n} is needed")
-    if _kind(a.dtype) not in ("int32", "uint32"):
+    if not _is_word(a.dtype):
         raise InvalidError(f"{what}: 32-bit whole numbers expected, got {a.dtype}")
     if _count(a) != n:
         raise InvalidError(f"{what}: {tuple(a.shape)}, {n} entries expected")
@@ -265,10 +278,13 @@ class KvBatch:
 
     def struct(self):
         """(lt_kv_batch, is_host)"""
-        (s, host), (n, h1), (t, h2) = _ptr(self.start), _ptr(self.len), _ptr(self.table)
+        n = self.n_seqs
+        p, host = _words(self.start, n + 1, "start")
+        q, h1 = _words(self.len, n, "len")
+        t, h2 = _words(self.table, n * self.max_blocks, "table")
         if host != h1 or host != h2:
             raise InvalidError("mix of host and device arrays")
-        return KvBatchStruct(self.n_seqs, self.n_tokens, self.max_blocks, self.max_new, s, n, t), host
+        return KvBatchStruct(n, self.n_tokens, self.max_blocks, self.max_new, p, q, t), host
 
 
 class KvCache:
@@ -539,12 +555,11 @@ class Context:
         lengths and a list of free blocks (lt_kv_plan)."""
         b, host = batch.struct()
         n_free = _count(free_blocks)
-        p = []
-        for w, a, n in (("len_in", len_in, batch.n_seqs), ("n_new", n_new, batch.n_seqs), ("free_blocks", free_blocks, n_free),
-                        ("used_in", used_in, 1), ("used_out", used_out, 1), ("positions", positions, batch.n_tokens),
-                        ("slots", slots, batch.n_tokens)):
+        p, T = [], batch.n_tokens
+        for w, a, n in (("len_in", len_in, b.n_seqs), ("n_new", n_new, b.n_seqs), ("free_blocks", free_blocks, n_free),
+                        ("used_in", used_in, 1), ("used_out", used_out, 1), ("positions", positions, T), ("slots", slots, T)):
             at, h = _words(a, n, w)
-            if h != host:
+            if h is not host:
                 raise InvalidError("mix of host and device arrays")
             p.append(at)
         self._check(self.lib.lt_kv_plan(self.ptr, C.byref(b), p[0], p[1], p[2], n_free, p[3], p[4], p[5], p[6],
