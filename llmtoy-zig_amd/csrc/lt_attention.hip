@@ -28,7 +28,8 @@
 // of which the loads take 18 and the two rounds of joining 7); else by instructions (a block of heads of 64
 // takes a wavefront about 250, of 128 400, of 256 650, 4 cycles each) and the chain of one launch: one
 // token of 14 heads over 1,500 keys 7.6 us, of which lengths 1.3, table 0.7, queries 0.6, codes 0.9, products and the
-// wavefronts' sums 1.5, arrival 0.9, joining 1.6.
+// wavefronts' sums 1.5, arrival 0.9, joining 1.6 (taken with integer divisions in lengths, queries and joining; 0.35 less
+// without: a graph of 12 layers 107.5 -> 103.2).
 #include "llmtoy_hip.h"
 #include "lt_attn.h"
 
@@ -51,8 +52,9 @@ struct Shape {
 constexpr uint32_t kThinTarget = 512;  // the largest
 
 // Parts of a tile that are joined at once (or 8 for each time that the workgroup's threads
-// are more than a part's places); more are joined in groups first, and no tile has more than the square.
-constexpr uint32_t kJoin = 16;
+// are more than a part's places); more are joined in groups first, and no tile has more than
+// the square (less one: 2^24 blocks times parts stay in 32 bits).
+constexpr uint32_t kJoin = 16, kMostParts = kJoin * kJoin - 1;
 
 struct ThinArgs {
     const uint8_t *codes;
@@ -64,6 +66,7 @@ struct ThinArgs {
     size_t q_stride;
     uint32_t n_heads, group, window;
     float scale2;  // scale * log2(e)
+    float per_group;  // 1 / group
     float *part;        // [n_kv][2][slots] of parts and of groups of them: [16][D] sums, then [16][4] m, l, mo
     uint32_t *tickets;  // [n_kv][slots][2]: groups, tiles; zero between launches
     uint32_t slots, target;  // parts of all heads that the work is cut into, about
@@ -114,7 +117,7 @@ __device__ __forceinline__ uint32_t thin_splits(const ThinArgs &a, uint32_t bloc
     if (blocks <= 3 * a.least || share == 0xffffffffu) return 1;
     uint32_t n = share > a.least ? blocks / share : (blocks + share - 1) / share;
     if (n == 0) n = 1;
-    return n < kJoin * kJoin ? n : kJoin * kJoin;
+    return n < kMostParts ? n : kMostParts;
 }
 
 // Every wavefront finds its work for itself from the lengths (one load and two sums for
@@ -167,12 +170,12 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
             w.any = true;
             w.row = r0 + l;
             w.splits = from_lane(splits, l);
-            w.tile = in / w.splits;
-            w.split = in % w.splits;
+            w.tile = w.splits == 1 ? in : in / w.splits;
+            w.split = in - w.tile * w.splits;
             const uint32_t lo = from_lane(t.lo, l), blocks = from_lane(t.blocks, l);
             // as even as whole blocks go
-            w.b0 = lo + (uint32_t)((uint64_t)blocks * w.split / w.splits);
-            w.b1 = lo + (uint32_t)((uint64_t)blocks * (w.split + 1) / w.splits);
+            w.b0 = lo + (w.splits == 1 ? 0 : blocks * w.split / w.splits);
+            w.b1 = lo + (w.splits == 1 ? blocks : blocks * (w.split + 1) / w.splits);
             w.slot = joined + from_lane(pup - parts, l) + in;
             w.first = from_lane(t.k.first, l), w.n = from_lane(t.k.n, l), w.len = from_lane(t.k.len, l);
             w.bad = from_lane(t.k.bad, l);
@@ -182,6 +185,13 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
         joined += from_lane(pup, kWave - 1);
     }
     return w;
+}
+
+// A row's token, among its sequence's.  (row + 1/2) / group is 1 / (2 group) from a whole number at
+// least, and the product is off by (row + 1/2) / group * 2^-23 at most: exact for rows below 2^22, where
+// kThinMost and a tile are the most.  (A quotient of integers takes some 20 instructions.)
+__device__ __forceinline__ uint32_t token_of(const ThinArgs &a, uint32_t row) {
+    return (uint32_t)(((float)row + 0.5f) * a.per_group);
 }
 
 // The largest of the four lanes that share a row.
@@ -236,12 +246,12 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     const uint32_t row = w.row;
     const uint32_t rows = w.n * a.group - w.tile * kThinRows;  // of this tile (more: 16)
     const uint32_t rho = w.tile * kThinRows + (n < rows ? n : 0);
-    const uint32_t token = rho / a.group, head = h * a.group + rho % a.group;
+    const uint32_t token = token_of(a, rho), head = h * a.group + rho - token * a.group;
     const int pos = (int)(w.len - w.n + token);
     const int low = a.window && (uint32_t)pos + 1 > a.window ? pos + 1 - (int)a.window : 0;
     // positions that every row of the tile sees the keys between
-    const uint32_t tok0 = w.tile * kThinRows / a.group, rows_in = rows < kThinRows ? rows : kThinRows;
-    const uint32_t tok1 = (w.tile * kThinRows + rows_in - 1) / a.group;
+    const uint32_t tok0 = token_of(a, w.tile * kThinRows), rows_in = rows < kThinRows ? rows : kThinRows;
+    const uint32_t tok1 = token_of(a, w.tile * kThinRows + rows_in - 1);
     const int pos0 = (int)(w.len - w.n + tok0), pos1 = (int)(w.len - w.n + tok1);
     const int low1 = a.window && (uint32_t)pos1 + 1 > a.window ? pos1 + 1 - (int)a.window : 0;
     const int low0 = a.window && (uint32_t)pos0 + 1 > a.window ? pos0 + 1 - (int)a.window : 0;
@@ -453,8 +463,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     __syncthreads();
     // Row rr's place among the sums and the outputs: its channels in fours, over the workgroup.
     const auto out_of = [&](uint32_t rr) {
-        const uint32_t r1 = w.tile * kThinRows + rr;
-        return a.out + ((size_t)(w.first + r1 / a.group) * a.n_heads + h * a.group + r1 % a.group) * D;
+        const uint32_t r1 = w.tile * kThinRows + rr, t = token_of(a, r1);
+        return a.out + ((size_t)(w.first + t) * a.n_heads + h * a.group + r1 - t * a.group) * D;
     };
     const Shared shared(a.part, a.n_kv * 2 * a.slots * P);
     const auto place = [&](uint32_t slot) { return (h * 2 * a.slots + slot) * P; };
@@ -487,9 +497,10 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     // counts last reads past the L2s, and leaves the counters at zero.
     const uint32_t most_hands = all < (uint32_t)NT ? NT / all : 1;
     const uint32_t in_group = w.splits <= kJoin || w.splits <= 8 * most_hands ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
-    const uint32_t grp = w.split / in_group, slot0 = w.slot - w.split, g0 = slot0 + grp * in_group;
+    const bool one = in_group == w.splits;
+    const uint32_t grp = one ? 0 : w.split / in_group, slot0 = w.slot - w.split, g0 = slot0 + grp * in_group;
     const uint32_t gn = w.splits - grp * in_group < in_group ? w.splits - grp * in_group : in_group;
-    const uint32_t groups = (w.splits + in_group - 1) / in_group;
+    const uint32_t groups = one ? 1 : (w.splits + in_group - 1) / in_group;
     uint32_t *tickets = a.tickets + (size_t)h * a.slots * 2;
     const auto last = [&](uint32_t *t, uint32_t count) -> bool {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -590,7 +601,7 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
     ThinArgs t{};
     t.codes = a.kv.codes, t.scales = a.kv.scales, t.n_blocks = a.kv.n_blocks, t.n_kv = a.kv.n_kv, t.b = a.b;
     t.q = a.q, t.out = a.out, t.q_stride = a.q_stride, t.n_heads = a.n_heads, t.group = a.group, t.window = a.window;
-    t.scale2 = a.scale * 1.4426950408889634f;
+    t.scale2 = a.scale * 1.4426950408889634f, t.per_group = 1.0f / (float)a.group;
     t.part = (float *)a.work, t.tickets = a.tickets, t.err = a.err;
     const uint32_t tiles = thin_tiles(a);
     switch (a.kv.D) {

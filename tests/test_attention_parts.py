@@ -3,6 +3,7 @@ once, places of parts that no two parts share, and as many as the workspace has.
 import math
 import random
 
+import numpy as np
 import pytest
 
 JOIN = 16
@@ -12,7 +13,7 @@ def thin_splits(blocks, share, least):
     if blocks <= 3 * least:
         return 1
     n = blocks // share if share > least else -(-blocks // share)
-    return min(max(n, 1), JOIN * JOIN)
+    return min(max(n, 1), JOIN * JOIN - 1)
 
 
 @pytest.mark.parametrize("target,least", [(512, 8), (256, 8), (256, 4)])
@@ -39,6 +40,13 @@ def test_few_row_parts_fit_grid_and_workspace(target, least):
                 each = s if s <= JOIN or s <= 8 * hands else math.ceil(math.sqrt(s))
                 groups = -(-s // each)
                 assert each * groups >= s and (groups == 1 or groups <= JOIN and each <= JOIN)
+
+
+def test_tokens_of_rows_by_a_product():
+    f = np.float32
+    for group in range(1, 600):
+        rows = np.arange(512 + 16)
+        assert np.array_equal(((rows.astype(f) + f(0.5)) * (f(1) / f(group))).astype(np.uint32), rows // group)
 
 
 def test_many_row_pieces_cover_every_tile_once():
