@@ -37,24 +37,19 @@ namespace lt {
 
 namespace {
 
-constexpr int kThinRows = 16;
 // Wavefronts a workgroup, wavefronts that a block's channels are cut over, parts that a
 // launch is cut into (more of them: 48 heads' caches of 220 MB 61.5 us with 512, 64 with 1,024; fewer:
 // 79 with 256, whose workgroups leave half of the registers unused).
 template <int D>
 struct Shape {
-    static constexpr int kWaves = 8, kSplit = D <= 256 ? 1 : 2, kTarget = D <= 128 ? 512 : 256;
+    static constexpr int kWaves = 8, kSplit = D <= 256 ? 1 : 2, kTarget = thin_target(D);
     static constexpr int kThreads = kWaves * kWave, kBlocks = kWaves / kSplit;  // blocks a round
     static constexpr int DW = D / kSplit, C = DW / 32;
+    static_assert(kBlocks == (int)thin_least(D), "");
     // (what a wavefront would not have the registers for: four on a SIMD up to heads of 128, then two)
     static constexpr bool kQueriesInLds = DW >= 128;
 };
 constexpr uint32_t kThinTarget = 512;  // the largest
-
-// Parts of a tile that are joined at once (or 8 for each time that the workgroup's threads
-// are more than a part's places); more are joined in groups first, and no tile has more than
-// the square (less one: 2^24 blocks times parts stay in 32 bits).
-constexpr uint32_t kJoin = 16, kMostParts = kJoin * kJoin - 1;
 
 struct ThinArgs {
     const uint8_t *codes;
@@ -84,9 +79,8 @@ struct ThinRow {
 __device__ __forceinline__ ThinRow thin_row(const ThinArgs &a, uint32_t r) {
     ThinRow t;
     t.k = kv_row_of(a.b, r);
-    // (beyond max_new: as many as the grid has room for, and those get NaN)
-    if (a.b.max_new && t.k.n > a.b.max_new) t.k.n = a.b.max_new;
-    t.tiles = t.k.n * a.group > kThinMost ? 0 : (t.k.n * a.group + kThinRows - 1) / kThinRows;
+    t.k.n = cut_tokens(t.k.n, a.b.max_new);
+    t.tiles = thin_row_tiles(t.k.n, a.group);
     t.lo = 0;
     t.blocks = 1;
     if (!t.k.bad && t.k.n) {
@@ -104,21 +98,6 @@ struct ThinWork {
     uint32_t first, n, len;
     bool any, bad;
 };
-
-// Blocks a part: all of the batch's (sum) over the launch's workgroups, evenly.
-__device__ __forceinline__ uint32_t thin_share(const ThinArgs &a, float sum) {
-    const float each = ceilf(sum * (float)a.n_kv / (float)a.target);
-    return each < (float)a.least ? a.least : each > 1e9f ? 1000000000u : (uint32_t)each;
-}
-
-// A tile's parts.  None where a workgroup has its blocks done before parts are joined; parts of
-// `least` where there are few, for their latency; else no more parts than the chip has room for at once.
-__device__ __forceinline__ uint32_t thin_splits(const ThinArgs &a, uint32_t blocks, uint32_t share) {
-    if (blocks <= 3 * a.least || share == 0xffffffffu) return 1;
-    uint32_t n = share > a.least ? blocks / share : (blocks + share - 1) / share;
-    if (n == 0) n = 1;
-    return n < kMostParts ? n : kMostParts;
-}
 
 // Every wavefront finds its work for itself from the lengths (one load and two sums for
 // up to 64 sequences).
@@ -144,14 +123,14 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
     }
     // (where start falls, sequences may overlap and have more tiles than the grid has workgroups for: whole
     // tiles, so that none waits for a part that nobody takes)
-    const uint32_t share = __any(falls) ? 0xffffffffu : thin_share(a, sum);
+    const uint32_t share = __any(falls) ? 0xffffffffu : thin_share(sum, a.n_kv, a.target, a.least);
     uint32_t seen = 0, joined = 0;  // workgroups and joined parts of the rows before
     for (uint32_t r0 = 0; r0 < a.b.n_seqs; r0 += kWave) {
         const uint32_t r = r0 + lane;
         uint32_t splits = 0;
         if (a.b.n_seqs > kWave) t = r < a.b.n_seqs ? thin_row(a, r) : ThinRow{};
         if (r < a.b.n_seqs) {
-            splits = thin_splits(a, t.blocks, share);
+            splits = thin_splits(t.blocks, share, a.least);
         }
         const uint32_t mine = t.tiles * splits, parts = splits > 1 ? mine : 0;
         uint32_t up = mine, pup = parts;
@@ -496,7 +475,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     // tile the tile.  A part's stores are acknowledged before it counts; the one that
     // counts last reads past the L2s, and leaves the counters at zero.
     const uint32_t most_hands = all < (uint32_t)NT ? NT / all : 1;
-    const uint32_t in_group = w.splits <= kJoin || w.splits <= 8 * most_hands ? w.splits : (uint32_t)ceilf(sqrtf((float)w.splits));
+    const uint32_t in_group = thin_in_group(w.splits, most_hands);
     const bool one = in_group == w.splits;
     const uint32_t grp = one ? 0 : w.split / in_group, slot0 = w.slot - w.split, g0 = slot0 + grp * in_group;
     const uint32_t gn = w.splits - grp * in_group < in_group ? w.splits - grp * in_group : in_group;
@@ -558,34 +537,18 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     if (last(tickets + 2 * slot0 + 1, groups)) join(a.slots + slot0, in_group, groups, kOut);
 }
 
-// Workgroups of a head: a tile more or less a sequence, and the parts of those
-// that are split (at most the target and one more a tile).
-uint32_t thin_tiles(const AttnArgs &a) {
-    const uint64_t rows = (uint64_t)a.b.n_tokens * a.group;
-    uint64_t tiles = rows / kThinRows + a.b.n_seqs;
-    const uint64_t each = a.b.max_new && (uint64_t)a.b.max_new * a.group < kThinMost ? a.b.max_new * a.group : kThinMost;
-    const uint64_t most = (uint64_t)a.b.n_seqs * ((each + kThinRows - 1) / kThinRows);
-    if (most < tiles) tiles = most;
-    if (rows < tiles) tiles = rows;
-    return (uint32_t)tiles;
-}
-uint32_t thin_slots(uint32_t target, uint32_t n_kv) { return 2 * (target / n_kv + 1) + 2; }
-
 template <int D>
 void go(ThinArgs t, uint32_t tiles, hipStream_t s) {
     using Sh = Shape<D>;
     t.target = Sh::kTarget, t.slots = thin_slots(t.target, t.n_kv), t.least = Sh::kBlocks;
-    const uint32_t each = (t.b.max_blocks + t.least - 1) / t.least;  // (a tile's parts, at most)
-    uint64_t x = tiles + t.target / t.n_kv + 1;
-    if ((uint64_t)tiles * each < x) x = (uint64_t)tiles * each;
-    hipLaunchKernelGGL(k_attention_thin<D>, dim3((uint32_t)x, t.n_kv), dim3(Sh::kThreads), 0, s, t);
+    const uint32_t x = thin_grid(tiles, t.b.max_blocks, t.n_kv, t.target, t.least);
+    hipLaunchKernelGGL(k_attention_thin<D>, dim3(x, t.n_kv), dim3(Sh::kThreads), 0, s, t);
 }
 }  // namespace
 
 bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D == 192 || D == 256 || D == 512; }
 
-// Whether a sequence may have rows for the wide kernel.
-static bool wide(const AttnArgs &a) { return (uint64_t)(a.b.max_new ? a.b.max_new : a.b.n_tokens) * a.group > kThinMost; }
+static bool wide(const AttnArgs &a) { return any_wide(a.b.n_tokens, a.b.max_new, a.group); }
 
 size_t attention_workspace(const AttnArgs &a) {
     const size_t thin = (size_t)a.kv.n_kv * 2 * thin_slots(kThinTarget, a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
@@ -603,7 +566,7 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
     t.q = a.q, t.out = a.out, t.q_stride = a.q_stride, t.n_heads = a.n_heads, t.group = a.group, t.window = a.window;
     t.scale2 = a.scale * 1.4426950408889634f, t.per_group = 1.0f / (float)a.group;
     t.part = (float *)a.work, t.tickets = a.tickets, t.err = a.err;
-    const uint32_t tiles = thin_tiles(a);
+    const uint32_t tiles = thin_tiles(a.b.n_tokens, a.b.n_seqs, a.b.max_new, a.group);
     switch (a.kv.D) {
     case 64: go<64>(t, tiles, s); break;
     case 96: go<96>(t, tiles, s); break;

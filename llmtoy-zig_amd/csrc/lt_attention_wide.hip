@@ -29,8 +29,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr uint32_t kLeast = 8;      // blocks that a workgroup is worth having for
-constexpr uint32_t kMaxTiles = 1024;  // of a head, whose blocks are counted in LDS
 constexpr uint32_t kJoin = 16;      // parts joined at once; more are joined in groups first
 
 struct WideArgs {
@@ -71,8 +69,7 @@ struct Tile {
 };
 
 __device__ __forceinline__ uint32_t row_rows(const WideArgs &a, const KvRow &k) {
-    // (beyond max_new: as many as the grid has room for, and those get NaN)
-    const uint32_t rows = (a.b.max_new && k.n > a.b.max_new ? a.b.max_new : k.n) * a.group;
+    const uint32_t rows = cut_tokens(k.n, a.b.max_new) * a.group;
     return rows > kThinMost ? rows : 0;
 }
 
@@ -228,8 +225,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
             if (tid * per2 + i < all_tiles) s_first[tid * per2 + i] += before;
         __syncthreads();
         total = line * a.n_kv;
-        pieces = total / kLeast < a.pieces ? (uint32_t)(total / kLeast) : a.pieces;
-        if (pieces == 0) pieces = 1;
+        pieces = wide_cut(total, a.pieces);
         // (an XCD's workgroups side by side in the line: their L2 has the blocks)
         piece = blockIdx.x;
         if (pieces == a.pieces && pieces % 8 == 0) piece = piece % 8 * (pieces / 8) + piece / 8;
@@ -555,29 +551,16 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
 }
 
 template <int D>
-uint32_t tiles_of(const AttnArgs &a) {
-    const uint64_t rows = (uint64_t)a.b.n_tokens * a.group, R = Shape<D>::kRows;
-    const uint64_t most_rows = rows / (kThinMost + 1);  // (sequences that this kernel takes, at most)
-    uint64_t tiles = rows / R + (most_rows < a.b.n_seqs ? most_rows : a.b.n_seqs);
-    if (a.b.max_new) {
-        const uint64_t most = (uint64_t)a.b.n_seqs * (((uint64_t)a.b.max_new * a.group + R - 1) / R);
-        if (most < tiles) tiles = most;
-    }
-    return (uint32_t)tiles;
-}
-
-template <int D>
 hipError_t go(const AttnArgs &a, hipStream_t s) {
     WideArgs t{};
     t.codes = a.kv.codes, t.scales = a.kv.scales, t.n_blocks = a.kv.n_blocks, t.n_kv = a.kv.n_kv, t.b = a.b;
     t.q = a.q, t.out = a.out, t.q_stride = a.q_stride, t.n_heads = a.n_heads, t.group = a.group, t.window = a.window;
     t.scale2 = a.scale * 1.4426950408889634f;
     t.part = (float *)a.work, t.tickets = a.tickets, t.err = a.err;
-    t.tiles = tiles_of<D>(a);
+    t.tiles = wide_tiles(a.b.n_tokens, a.b.n_seqs, a.b.max_new, a.group, Shape<D>::kRows);
     const uint32_t fit = 256 * Shape<D>::kPerCu;
     const uint64_t all = (uint64_t)t.tiles * t.n_kv;
-    // (two tiles and more for every place: the hardware's order evens them out)
-    t.pieces = all >= 2 * fit || t.tiles > kMaxTiles || a.b.n_seqs > kMaxTiles ? 0 : fit;
+    t.pieces = wide_pieces(t.tiles, a.b.n_seqs, t.n_kv, fit);
     if (all * Shape<D>::kThreads >= (1ull << 32)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(k_attention_wide<D>, dim3(t.pieces ? fit : (uint32_t)all), dim3(Shape<D>::kThreads), 0, s, t);
     return hipGetLastError();

@@ -12,13 +12,6 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Rows (tokens times heads of a group) of a sequence up to which lt_attention.hip's
-// kernel takes it; the other kernel takes those with more.  With 8 heads of 128 a group, few-row kernel
-// and many-row kernel in us: 48 rows 23 and 54, 256 rows over 4,000 keys 22 and 66, 512 rows over 16,000
-// keys 60 and 79, 8 sequences of 512 rows over 4,000 keys 87 and 80; from there on the latter's
-// tiles of 64 to 256 rows pay.
-constexpr uint32_t kThinMost = 512;
-
 // The reference of the weights may lag behind the largest logit by this much
 // (base 2), so that sums are rarely scaled down; weights go in times 2^kBits, and
 // 2^(kBits + kSlack) is in f16's range.

@@ -18,6 +18,7 @@
 // by the parity of the block's index), so that a block is coded from its tokens
 // and never from codes, however they come.
 #pragma once
+#include "lt_cut.h"
 #include "lt_internal.h"
 
 namespace lt {
@@ -119,7 +120,6 @@ struct AttnArgs {
     uint32_t *tickets;  // kAttnTickets words, zero between launches
     uint32_t *err;
 };
-constexpr size_t kAttnTickets = 8192;
 bool attention_head_dim(uint32_t D);
 size_t attention_workspace(const AttnArgs &a);
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
