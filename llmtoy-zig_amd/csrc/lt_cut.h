@@ -92,9 +92,10 @@ LT_CUT uint32_t thin_slots(uint32_t target, uint32_t n_kv) { return 2 * (target 
 constexpr uint32_t kLeast = 8;        // blocks that a workgroup is worth having for
 constexpr uint32_t kMaxTiles = 1024;  // of a head, whose blocks are counted in LDS
 
-// Whether a sequence of the batch may have rows for the many-row kernel.
+// Whether a sequence of the batch may have rows for the many-row kernel: not where max_new allows them and the
+// batch has too few tokens (wide_tiles would be 0, and a launch empty).
 LT_CUT bool any_wide(uint32_t n_tokens, uint32_t max_new, uint32_t group) {
-    return (uint64_t)(max_new ? max_new : n_tokens) * group > kThinMost;
+    return (uint64_t)cut_tokens(n_tokens, max_new) * group > kThinMost;
 }
 
 LT_CUT uint32_t wide_row_tiles(uint32_t n, uint32_t group, uint32_t tile) {

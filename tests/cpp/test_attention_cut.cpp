@@ -46,10 +46,10 @@ static uint32_t blocks_of(const Batch &b, const Seq &s) {
 static Batch draw() {
     Batch b;
     const uint32_t seqs = pick_log(1, 4096), most = pick_log(1, pick(0, 3) ? 40 : 3000), past = pick_log(1, 200000);
-    const bool sparse = pick(0, 2) == 0;
+    const bool sparse = pick(0, 2) == 0, rare = pick(0, 3) == 0;  // (rare: a few tokens of all the sequences)
     uint32_t top = 0;
     for (uint32_t i = 0; i < seqs; i++) {
-        const uint32_t n = sparse && pick(0, 9) ? 0 : pick(0, most);
+        const uint32_t n = (rare && pick(0, seqs) > 3) || (sparse && pick(0, 9)) ? 0 : pick(0, most);
         b.seqs.push_back({n, n + pick(0, past)});
         b.n_tokens += n;
         top = std::max(top, n);
@@ -120,6 +120,7 @@ static void many(const Batch &b, uint32_t tile, uint32_t per_cu) {
     const uint32_t room = wide_tiles(b.n_tokens, seqs, b.max_new, b.group, tile);
     CHECK(tiles.size() <= room);
     const uint32_t pieces = wide_pieces(room, seqs, b.n_kv, fit);
+    CHECK(pieces || (uint64_t)room * b.n_kv > 0);  // (no launch without a workgroup)
     if (!pieces) return;
     CHECK(room <= kMaxTiles && seqs <= kMaxTiles && 3 * pieces <= kAttnTickets);
     uint64_t line = 0;

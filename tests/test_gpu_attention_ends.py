@@ -1,0 +1,40 @@
+"""What attention's operators do at their ends: many sequences and few tokens, blocks of nothing, tiles that cross a
+block of NaN, full rows of a table, sequences in another row, reports; against the 64-bit reference
+(attn_reference.py)."""
+import numpy as np
+import pytest
+
+import attn_reference as ref
+import llmtoy_amd as lt
+from llmtoy_amd import ggml
+from llmtoy_amd.hip import DeviceArray, Graph
+from llmtoy_amd.lib import DeviceError, rmsnorm
+from test_gpu_attention import Seqs, _attend, _expect, close, dev, filled, gen, heads, read, same, u32
+
+pytestmark = pytest.mark.gpu
+
+
+# sequences of a batch, those with tokens in it, tokens before, max_new (0: not known)
+FEW_OF_MANY = [(2000, [1] * 16, 90, 128), (1025, [1], 40, 4096), (2000, [3, 1], 33, 0), (4096, [1] * 5, 20, 1 << 24),
+               (1500, [100, 1, 1], 50, 100), (1500, [100, 1, 70], 50, 0)]
+
+
+@pytest.mark.parametrize("n,new,past,max_new", FEW_OF_MANY)
+def test_gpu_few_tokens_of_many_sequences(ctx, n, new, past, max_new):
+    """More sequences than the many-row kernel cuts in pieces for, and fewer rows than a tile of it."""
+    print(f"few of many {n} {new} {past} {max_new}", flush=True)
+    D, KV, G = 128, 1, 8
+    g = gen(n, len(new), 21)
+    rows = np.sort(g.permutation(n)[:len(new)])
+    total, adds = np.zeros(n, int), np.zeros(n, int)
+    total[rows], adds[rows] = past + np.array(new), new
+    s = Seqs(g, total)
+    k, v = ([heads(g, m, KV, D) for m in total] for _ in range(2))
+    c = filled(ctx, s, k, v, KV, D)
+    q = g.standard_normal((sum(new), KV * G, D)).astype(np.float32)
+    want, bound = _expect(k, v, q, total, adds, D ** -0.5, 0)
+    out = dev(np.full(q.shape, 5, np.float32))
+    ctx.attention(out, dev(q), c, s.batch(total, adds, max_new=max_new), D ** -0.5)
+    ctx.sync()
+    close(out.numpy(), want, bound)
+    c.free()
