@@ -250,7 +250,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
     // b0 + which + NB * i.  lost: blocks that the cache does not have.
     uint32_t page_l = 0;
     float2 scales_n = make_float2(0.0f, 0.0f);
-    float ks_l = 0.0f, lv_l = 0.0f;  // keys' scale, and log2 of the values' (a block of zeros: any)
+    float ks_l = 0.0f, lv_l = 0.0f;  // keys' scale, and log2 of the values'
     uint64_t lost_n = 0;
     const auto pages = [&](uint32_t i) {
         page_l = table[b0 + which + NB * (i < mine ? i : mine - 1)];
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         if (i % kWave == 0) {
             const bool lost = lost_n >> lane & 1;
             ks_l = lost ? __builtin_nanf("") : scales_n.x;
-            lv_l = lost ? __builtin_nanf("") : scales_n.y == 0.0f ? 0.0f : log2f(scales_n.y);
+            lv_l = lost ? __builtin_nanf("") : log2_scale(scales_n.y);
         }
         f32x4 sa[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
         if (on) {

@@ -294,7 +294,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
             }
             const float2 s = a.scales[(size_t)page_l * a.n_kv + h];
             ks_n = lost ? __builtin_nanf("") : s.x;
-            lv_n = lost ? __builtin_nanf("") : s.y == 0.0f ? 0.0f : log2f(s.y);
+            lv_n = lost ? __builtin_nanf("") : log2_scale(s.y);
         };
         uint4 raw[GPW];
         const auto fetch = [&](uint32_t j) {

@@ -19,6 +19,10 @@ constexpr float kSlack = 3.0f, kBits = 12.0f;
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
+// log2 of a block's value scale.  A block of zeros has none: below every real one (2^-149 at least), so that its
+// logits count in the softmax's sum and never set the reference that real values' weights are held against.
+__device__ __forceinline__ float log2_scale(float s) { return s == 0.0f ? -200.0f : log2f(s); }
+
 __device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // A barrier behind which the workgroup's LDS accesses are done, and no more: __syncthreads

@@ -38,3 +38,38 @@ def test_gpu_few_tokens_of_many_sequences(ctx, n, new, past, max_new):
     ctx.sync()
     close(out.numpy(), want, bound)
     c.free()
+
+
+@pytest.mark.parametrize("D,new", [(64, 1), (64, 90), (512, 2), (128, 80)])
+@pytest.mark.parametrize("size,lift", [(1e-6, 0.0), (1e-8, 0.0), (1e-10, 0.0), (1.0, 15.0), (1.0, 40.0), (1e-6, 15.0)])
+def test_gpu_attention_beside_a_block_of_nothing(ctx, D, new, size, lift):
+    """A block whose values are all zero beside others of `size`; its logits higher than theirs by about `lift`."""
+    print(f"block of nothing {D} {new} {size} {lift}", flush=True)
+    KV, G, past, scale = 1, 8, 600, D ** -0.5  # (past: two blocks and more a wavefront)
+    g = gen(D, new, int(lift), 22)
+    n = past + new
+    s = Seqs(g, [n])
+    k, v, q = heads(g, n, KV, D), size * heads(g, n, KV, D), 0.3 * g.standard_normal((new, KV * G, D)).astype(np.float32)
+    way = np.ones(D, np.float32)  # (every query has sqrt(D) of it)
+    q += way
+    k[32:64] += lift / (D * scale) * way
+    v[32:64] = 0
+    v = v.astype(np.float32)
+    c = filled(ctx, s, [k], [v], KV, D)
+    want, bound = _expect([k], [v], q, [n], [new], scale, 0)
+    out = DeviceArray(q.shape)
+    ctx.attention(out, dev(q), c, s.batch([n], [new]), scale)
+    ctx.sync()
+    close(out.numpy(), want, bound)
+    # nothing but such blocks in sight
+    w = np.zeros_like(v)
+    w[:32] = v[:32]
+    c.append(dev(k), dev(w), s.batch([n], [n]))
+    want, bound = _expect([k], [w], q, [n], [new], scale, 0)
+    ctx.attention(out, dev(q), c, s.batch([n], [new]), scale)
+    ctx.sync()
+    close(out.numpy(), want, bound)
+    ctx.attention(out, dev(q), c, s.batch([n], [new]), scale, 64)
+    ctx.sync()
+    assert (out.numpy() == 0).all()
+    c.free()
