@@ -413,7 +413,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, (D <= 128 ? 4 : 2)) void k_atte
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) sum += p[e];
-        if (mo != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-eb - ms);
+        if (sum != 0.0f) l += sum * __builtin_amdgcn_exp2f(-eb - ms);  // (0: none in sight, and eb may be NaN)
         half8 ph, pl;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {

@@ -440,7 +440,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
                 }
 #pragma unroll
                 for (int e = 0; e < 16; e++) sum += p[e];
-                if (mo != kNegInf || sum != sum) l += sum * __builtin_amdgcn_exp2f(-eb - ms);
+                if (sum != 0.0f) l += sum * __builtin_amdgcn_exp2f(-eb - ms);  // (0: none in sight, and eb may be NaN)
                 // operand u: the keys 4 half + 16 u' + 8 u .. + 3 for u' = 0, 1, as a value's codes lie
                 half8 ph[2], pl[2];
 #pragma unroll

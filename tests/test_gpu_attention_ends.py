@@ -73,3 +73,39 @@ def test_gpu_attention_beside_a_block_of_nothing(ctx, D, new, size, lift):
     ctx.sync()
     assert (out.numpy() == 0).all()
     c.free()
+
+
+@pytest.mark.parametrize("D,G,past,new,window", [
+    (64, 4, 222, 4, 40), (64, 4, 229, 4, 40), (64, 4, 478, 4, 0), (128, 8, 479, 2, 0), (512, 4, 478, 4, 0), (64, 4, 521, 4, 300),
+    (64, 4, 198, 130, 40), (128, 8, 221, 70, 40), (512, 8, 222, 66, 40), (128, 8, 221, 70, 0)])
+@pytest.mark.parametrize("what", ["keys", "values", "lost"])
+def test_gpu_rows_of_a_tile_before_a_block_of_nan(ctx, D, G, past, new, window, what):
+    """Rows that do not see a block which others of their tile see: it changes nothing for them."""
+    print(f"block of NaN {D} {G} {past} {new} {window} {what}", flush=True)
+    KV, n, scale = 1, past + new, D ** -0.5
+    g, s, k, v, c, q, total, _ = _attend(ctx, D, KV, G, [past], [new], window, seed=23)
+    pos = np.arange(past, n)
+    c.free()
+    for block in {b for b in (past // 32, past // 32 + 1, (past - window + 2) // 32 if window else 0) if b * 32 < n}:
+        sees = (pos >= block * 32) & (pos - (window or n) + 1 < block * 32 + 32)
+        k1, v1, table = k[0].copy(), v[0].copy(), s.table
+        if what == "keys":
+            k1[block * 32, 0, 3] = np.nan
+        elif what == "values":
+            v1[block * 32, 0, 3] = np.inf
+        c = filled(ctx, s, [k1], [v1], KV, D)
+        if what == "lost":
+            s.table = table.copy()
+            s.table[0, block] = ref.NONE
+        want, bound = _expect(k, v, q, total, [new], scale, window)
+        out = DeviceArray(q.shape)
+        ctx.attention(out, dev(q), c, s.batch(total, [new]), scale, window)
+        if what == "lost" and sees.any():
+            with pytest.raises(DeviceError, match="sequence 0: the table has no block"):
+                ctx.sync()
+        ctx.sync()
+        s.table = table
+        got = out.numpy()
+        assert np.isnan(got[sees]).all()
+        close(got[~sees], want[~sees], bound[~sees])
+        c.free()
