@@ -484,10 +484,15 @@ size_t lt_kv_bytes(const lt_kv *kv);
  *   positions, slots          [batch->n_tokens]: each token's position, and block *
  *                             LT_KV_BLOCK + offset (tokens behind the last sequence: 0 and LT_KV_NONE)
  * len_in may be batch->len and used_in used_out: a replayed graph then moves on by
- * itself.  A sequence whose blocks free_blocks does not have, or whose row of the
- * table is full, gets LT_KV_NONE for all its new blocks and its tokens there, and so do the later
- * ones that need blocks; its length counts on (the caller that is told sets it
- * back).  Tokens beyond n_tokens have no place in the maps.  Both are reported.
+ * itself.  A sequence whose blocks free_blocks does not have gets LT_KV_NONE for all its new
+ * blocks and its tokens there, and so do the later ones that need blocks.  One whose row of the table
+ * is too short for them gets LT_KV_NONE too, but takes nothing from the list, and the later ones are
+ * served (unless its length passes 2^32 - 1, which the arrays' own fault is: behind it nobody gets a
+ * block).  Their lengths count on (the caller that is told sets them back).  Every entry that
+ * used_out counts is in the table.  Tokens beyond n_tokens have no place in the maps.  All of
+ * this is reported.  A sequence that was shortened to len_in tokens gets new blocks from index
+ * ceil(len_in / LT_KV_BLOCK) on: what the table had there goes back to the caller's list before the call,
+ * or is lost to it.
  * flags: LT_HOST_IO. */
 int lt_kv_plan(lt_ctx *ctx, const lt_kv_batch *batch, const uint32_t *len_in, const uint32_t *n_new,
                const uint32_t *free_blocks, uint32_t n_free, const uint32_t *used_in, uint32_t *used_out,

@@ -10,7 +10,8 @@ namespace {
 // ------------------------------------------------------------------- the plan
 // With total = len + n_new of a row, it needs blocks for the indices
 // ceil(len / 32) .. ceil(total / 32) - 1; the rows take them from the free list in
-// order, and their tokens lie in the batch in order.  Both are prefix sums over
+// order, and their tokens lie in the batch in order.  A row whose table has no room for them
+// takes none.  Both are prefix sums over
 // the rows, which one workgroup takes (kPlanRows a thread); new blocks and
 // tokens then look their row up in the sums.  Bound by its chain of latencies:
 // the lengths, the sums, the table's entry, the slot (8 rows 5.1 us; 2,000 rows 6.2, and the
@@ -19,6 +20,16 @@ constexpr uint32_t kPlanThreads = 1024, kPlanRows = kKvMaxSeqs / kPlanThreads;
 // Tokens of a batch that the one workgroup maps; more go to a grid of their own
 // behind it (k_kv_slots).
 constexpr uint32_t kPlanTokens = 2048;
+
+// Blocks that a row takes from the list: none where its table has no room; where even the
+// length passes 32 bits, more than any list has, so that none is handed out behind it.
+constexpr uint64_t kBeyondAny = 1ull << 40;
+__device__ __forceinline__ uint64_t plan_need(uint32_t len, uint32_t add, uint32_t max_blocks) {
+    const uint64_t total = (uint64_t)len + add;
+    if (total >> 32) return kBeyondAny;
+    const uint64_t b0 = ((uint64_t)len + kKvBlock - 1) / kKvBlock, b1 = (total + kKvBlock - 1) / kKvBlock;
+    return b1 <= max_blocks ? b1 - b0 : 0;
+}
 
 __device__ __forceinline__ uint32_t sat32(uint64_t v) { return v < kKvNone ? (uint32_t)v : kKvNone; }
 
@@ -52,7 +63,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
         len[i] = r < a.n_seqs ? a.len_in[r] : 0;
         add[i] = r < a.n_seqs ? a.n_new[r] : 0;
         tok += add[i];
-        need += ((uint64_t)len[i] + add[i] + kKvBlock - 1) / kKvBlock - ((uint64_t)len[i] + kKvBlock - 1) / kKvBlock;
+        need += plan_need(len[i], add[i], a.max_blocks);
     }
     // sums before this thread's rows
     uint64_t itok = tok, ineed = need;
@@ -87,15 +98,15 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
             s_first[r] = sat32(btok);
             s_pos[r] = len[i];
             s_need[r] = sat32(bneed);
-            const bool room = b1 <= a.max_blocks, served = room && used + bneed + (b1 - b0) <= a.n_free;
+            const bool room = b1 <= a.max_blocks && !(total >> 32), served = room && used + bneed + (b1 - b0) <= a.n_free;
             s_block[r] = served ? (uint32_t)b0 : kKvNone;
             if (served) most = max(most, (uint32_t)(used + bneed + (b1 - b0)));
-            else if (b1 > b0) kv_report(a.err, kKvErrPool, r);
+            else if (b1 > b0 || (!room && add[i])) kv_report(a.err, kKvErrPool, r);
             if (!served)  // (its new entries: nothing; the entries of a served row are written below)
                 for (uint64_t j = b0; j < b1 && j < a.max_blocks; j++) a.table[(size_t)r * a.max_blocks + j] = kKvNone;
         }
         btok += add[i];
-        bneed += b1 - b0;
+        bneed += plan_need(len[i], add[i], a.max_blocks);
     }
     // (a wavefront's largest first: 1,024 atomics on one word took 3 us)
 #pragma unroll

@@ -109,3 +109,90 @@ def test_gpu_rows_of_a_tile_before_a_block_of_nan(ctx, D, G, past, new, window, 
         assert np.isnan(got[sees]).all()
         close(got[~sees], want[~sees], bound[~sees])
         c.free()
+
+
+def plan(past, new, table, free, used):
+    """(table, used) of lt_kv_plan where every length fits 32 bits: a sequence whose row is full takes no blocks; from
+    one that the list is too short for on, none does."""
+    table, at, short = np.array(table, np.int64), used, False
+    for i in range(len(past)):
+        b0, b1 = -(-int(past[i]) // 32), -(-int(past[i] + new[i]) // 32)
+        full = b1 > table.shape[1]
+        if not full and b1 > b0:
+            short |= at + b1 - b0 > len(free)
+        take = not full and not short
+        for j in range(b0, min(b1, table.shape[1])):
+            table[i, j] = free[at + j - b0] if take else ref.NONE
+        at += b1 - b0 if take else 0
+    return u32(table), at
+
+
+@pytest.mark.parametrize("n,width,most", [(3, 4, 40), (9, 4, 70), (200, 6, 100), (1500, 5, 60)])
+@pytest.mark.parametrize("short", [False, True])
+def test_gpu_plan_with_full_rows_among_others(ctx, n, width, most, short):
+    print(f"plan with full rows {n} {width} {most} {short}", flush=True)
+    g = gen(n, width, short, 24)
+    past = g.integers(0, width * 32 + 1, n)
+    new = g.integers(0, most, n)
+    past[0], new[0] = width * 32, 33
+    new[1] = 1 << 30  # far beyond any row
+    past[2], new[2] = 31, 2
+    held, after = -(-past // 32), -(-(past + new) // 32)
+    order = g.permutation(int(held.sum() + after[after <= width].sum()) + 9)
+    table = np.full((n, width), ref.NONE, np.int64)
+    for i in range(n):
+        table[i, :held[i]] = order[held[:i].sum():held[:i + 1].sum()]
+    need = int((after - held)[after <= width].sum())
+    free = order[held.sum():held.sum() + (need * 2 // 3 if short else need + 3) + 2]
+    tokens = new.copy()
+    tokens[1] = 0
+    want, used = plan(past, tokens, table, free, 2)
+    if not short:
+        assert used == 2 + need
+    room = int(new[0]) + 70  # (the second sequence has all of the others' room)
+    b = lt.KvBatch(DeviceArray((n + 1,), np.uint32), DeviceArray((n,), np.uint32), dev(table, np.uint32), room)
+    us, pos, sl = DeviceArray((1,), np.uint32), DeviceArray((room,), np.uint32), DeviceArray((room,), np.uint32)
+    ctx.kv_plan(b, dev(past, np.uint32), dev(new, np.uint32), dev(free, np.uint32), dev([2], np.uint32), us, pos, sl)
+    with pytest.raises(DeviceError, match="plan"):
+        ctx.sync()
+    got = b.table.numpy()
+    # (the second sequence's: those before its full row are none)
+    for j in range(held[1], width):
+        want[1, j] = ref.NONE
+    assert np.array_equal(got, want) and us.numpy()[0] == used
+    fresh = (got != u32(table)) & (got != ref.NONE)
+    assert fresh.sum() == used - 2  # what counts as taken is in a table
+    assert (sl.numpy()[:new[0]] == ref.NONE).all()
+
+
+@pytest.mark.parametrize("n,most", [(5, 3), (300, 40)])
+def test_gpu_plan_again_and_again_loses_no_block(ctx, n, most):
+    """A replayed plan beside a sequence whose row is full: every block that counts as taken is in a table."""
+    print(f"plan replayed beside a full row {n} {most}", flush=True)
+    g = gen(n, 25)
+    width, steps = 6, 12
+    past = u32(g.integers(0, 20, n))
+    past[1] = width * 32 - 1
+    new = u32(g.integers(1, most + 1, n))
+    new[1] = 20  # (full from the first step on)
+    free = u32(g.permutation(n * width * 2))
+    room = int(new.sum())
+    table = np.full((n, width), ref.NONE, np.uint32)
+    for i in range(n):
+        h = -(-int(past[i]) // 32)
+        table[i, :h] = 100000 + 10 * i + np.arange(h)
+    ln, used = dev(past), dev(u32([0]))
+    b = lt.KvBatch(DeviceArray((n + 1,), np.uint32), ln, dev(table), room)
+    pos, slots, nd, fd = DeviceArray((room,), np.uint32), DeviceArray((room,), np.uint32), dev(new), dev(free)
+    graph = Graph(ctx.stream, lambda: ctx.kv_plan(b, ln, nd, fd, used, used, pos, slots))
+    at = past.astype(int)
+    for _ in range(steps):
+        graph.launch()
+        with pytest.raises(DeviceError, match="no room in the table's row"):
+            ctx.sync()
+        at = at + new
+        fresh = b.table.numpy()
+        fresh = fresh[(fresh != ref.NONE) & (fresh < 100000)]
+        assert used.numpy()[0] == len(fresh) == len(set(fresh.tolist()))
+        assert np.array_equal(ln.numpy(), at)
+    graph.destroy()
