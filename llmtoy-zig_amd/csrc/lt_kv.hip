@@ -337,6 +337,7 @@ __device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b
     for (uint32_t o = last > first ? last - 1 : last; o <= last; o++) {
         const bool shared = begin % kKvBlock && o > first && (o - first) % 2 == 0;
         if (j != (shared ? first : o)) continue;
+        if (o == first && stale) continue;  // (its place holds another block's, or a beginning without a gap)
         const uint32_t b0 = o * kKvBlock, f = begin > b0 ? begin - b0 : 0;
         const uint32_t e = row.len - b0 < kKvBlock ? row.len - b0 : kKvBlock;
         float *dst = kv.open + open_at(kv, r, h, which, o);
@@ -363,7 +364,7 @@ __device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b
                 }
             }
         }
-        if (tid == 0 && !(o == first && stale)) tag[o & 1] = make_uint2(o, e);
+        if (tid == 0) tag[o & 1] = make_uint2(o, e);
     }
 }
 

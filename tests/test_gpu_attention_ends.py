@@ -196,3 +196,56 @@ def test_gpu_plan_again_and_again_loses_no_block(ctx, n, most):
         assert used.numpy()[0] == len(fresh) == len(set(fresh.tolist()))
         assert np.array_equal(ln.numpy(), at)
     graph.destroy()
+
+
+@pytest.mark.parametrize("D", [64, 192])
+@pytest.mark.parametrize("wrong,tokens", [(10, 3), (10, 40), (1, 90)])
+def test_gpu_a_refused_append_spoils_no_held_tokens(ctx, D, wrong, tokens):
+    """A length set back too far is told; set right, the sequence goes on with the tokens that it held."""
+    print(f"append: set back too far {D} {wrong} {tokens}", flush=True)
+    g, kv, n = gen(28, D, tokens), 2, 64 + 20
+    s = Seqs(g, [n + 10])
+    k = heads(g, n + 10, kv, D)
+    c = ctx.kv_cache(s.pool, kv, D, 1)
+    c.append(dev(k[:n]), dev(k[:n]), s.batch([n], [n]))
+    if tokens == 3:
+        x = heads(g, tokens, kv, D)
+        c.append(dev(x), dev(x), s.batch([wrong + tokens], [tokens]))
+        with pytest.raises(DeviceError, match="sequence 0: append: the block's earlier tokens are not held"):
+            ctx.sync()
+        c.append(dev(k[n:n + 1]), dev(k[n:n + 1]), s.batch([n + 1], [1]))
+        ctx.sync()
+        assert same(read(c, s.slots(0, 64, n + 1))[0], ref.values(k[64:n + 1]))
+    else:  # later blocks were begun anew: those are held
+        x = heads(g, tokens, kv, D)
+        c.append(dev(x), dev(x), s.batch([wrong + tokens], [tokens]))
+        with pytest.raises(DeviceError, match="sequence 0: append: the block's earlier tokens are not held"):
+            ctx.sync()
+        end = wrong + tokens
+        more = heads(g, 2, kv, D)
+        c.append(dev(more), dev(more), s.batch([end + 2], [2]))
+        ctx.sync()
+        a, _ = read(c, s.slots(0, 0, end + 2))
+        assert np.isnan(a[:32]).all()
+        assert same(a[32:], ref.values(np.concatenate([x[32 - wrong:], more])))
+    c.free()
+
+
+def test_gpu_a_block_that_is_not_there_leaves_the_held_tokens(ctx):
+    print("append: no block for a token, then one", flush=True)
+    g, kv, D = gen(29), 1, 128
+    s = Seqs(g, [70])
+    k = heads(g, 70, kv, D)
+    c = ctx.kv_cache(s.pool, kv, D, 1)
+    c.append(dev(k[:60]), dev(k[:60]), s.batch([60], [60]))
+    good, s.table = s.table, s.table.copy()
+    s.table[0, 1] = ref.NONE
+    x = heads(g, 1, kv, D)
+    c.append(dev(x), dev(x), s.batch([61], [1]))
+    with pytest.raises(DeviceError, match="sequence 0: the table has no block"):
+        ctx.sync()
+    s.table = good
+    c.append(dev(k[60:]), dev(k[60:]), s.batch([70], [10]))
+    ctx.sync()
+    assert same(read(c, s.slots(0, 0, 70))[0], ref.values(k))
+    c.free()
