@@ -502,7 +502,8 @@ int lt_kv_plan(lt_ctx *ctx, const lt_kv_batch *batch, const uint32_t *len_in, co
  * tokens begin inside a block, that block's earlier tokens are taken from their
  * fp32 copies, which are there for the last two blocks that were appended to: a
  * sequence may be shortened (len set back) by up to LT_KV_BLOCK tokens, or to the start of any block, and go
- * on from there (until then its last block stays coded beside the tokens taken back).  A block that is appended to must be in one sequence's table only; full
+ * on from there (until then its last block stays coded beside the tokens taken back).  The copies belong to the sequence's
+ * row of the batch and to the block: a sequence keeps its row, and moves to another only where its next token begins a block.  A block that is appended to must be in one sequence's table only; full
  * blocks may be shared.  Codes, scales and copies of the tokens appended are
  * written, nothing else.  A sequence that contradicts itself (more tokens than len, ...) or has more than
  * max_new of them is left out and reported; a block that is not in the cache

@@ -575,7 +575,7 @@ int check_kv_err(lt_ctx *ctx) {
         "plan: no blocks left in the free list, or no room in the table's row",
         "plan: more tokens than the maps have room for",
         "the table has no block of the cache for a token",
-        "append: the block's earlier tokens are not held (shortened too far, or never appended)",
+        "append: the block's earlier tokens are not held (shortened too far, never appended, or in another row of the batch)",
         "the batch contradicts itself: start falls or passes n_tokens, len is less than the tokens or more than the "
         "table holds, or more tokens than max_new",
     };
@@ -2071,23 +2071,24 @@ extern "C" int lt_kv_create(lt_ctx *ctx, uint32_t n_blocks, uint32_t n_kv_heads,
     const size_t bh = (size_t)n_blocks * n_kv_heads, sh = (size_t)n_seqs * n_kv_heads;
     const size_t codes = round(bh * 2 * lt::kKvBlock * head_dim), scales = round(bh * sizeof(float2));
     const size_t open = round(sh * 4 * lt::kKvBlock * head_dim * 4), tags = round(sh * 4 * sizeof(uint2));
+    const size_t owner = round((size_t)n_blocks * 4);
     OnDevice dev(ctx);
     LT_HIP(ctx, dev.e);
     lt_kv *kv = new (std::nothrow) lt_kv{};
     if (!kv) return fail(ctx, LT_ERR_OOM, "host allocation failed");
     uint8_t *p = nullptr;
-    hipError_t e = hipMalloc((void **)&p, codes + scales + open + tags);
+    hipError_t e = hipMalloc((void **)&p, codes + scales + open + tags + owner);
     // no token is held yet; behind what is enqueued, and waited for
-    if (e == hipSuccess) e = hipMemsetAsync(p + codes + scales + open, 0, tags, ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(p + codes + scales + open, 0, tags + owner, ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) {
         if (p) (void)hipFree(p);
         delete kv;
         return hip_fail(ctx, e, "cache");
     }
-    kv->bytes = codes + scales + open + tags;
+    kv->bytes = codes + scales + open + tags + owner;
     kv->d = {p, (float2 *)(p + codes), (float *)(p + codes + scales), (uint2 *)(p + codes + scales + open),
-             n_blocks, n_kv_heads, head_dim, n_seqs};
+             (uint32_t *)(p + codes + scales + open + tags), n_blocks, n_kv_heads, head_dim, n_seqs};
     *out_kv = kv;
     return LT_OK;
 }

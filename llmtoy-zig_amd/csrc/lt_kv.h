@@ -15,8 +15,10 @@
 // product's operand as they stand.
 //
 // The tokens of a sequence's last two blocks are also kept in fp32 (KvDev::open,
-// by the parity of the block's index), so that a block is coded from its tokens
-// and never from codes, however they come.
+// by its row of the batch and the parity of the block's index), so that a block is coded from its tokens
+// and never from codes, however they come.  A tag says whose they are: the block of the cache, and
+// how many.  A block that is begun anew takes itself out of the tags of the row that had it
+// (KvDev::owner), so that a tag never names a block that another sequence, or the same one anew, has written since.
 #pragma once
 #include "lt_cut.h"
 #include "lt_internal.h"
@@ -35,7 +37,8 @@ struct KvDev {
     uint8_t *codes;   // [n_blocks][n_kv][2][32 * D]
     float2 *scales;   // [n_blocks][n_kv]: keys', values'
     float *open;      // [n_seqs][n_kv][2 keys, values][2 parity][32][D]
-    uint2 *tags;      // [n_seqs][n_kv][2][2]: block index, tokens held (0: none)
+    uint2 *tags;      // [n_seqs][n_kv][2][2]: block of the cache, tokens held (0: none)
+    uint32_t *owner;  // [n_blocks]: row + 1 that began the block last (0: none)
     uint32_t n_blocks, n_kv, D, n_seqs;
 };
 

@@ -240,6 +240,22 @@ __device__ __forceinline__ size_t open_at(const KvDev &kv, uint32_t seq, uint32_
     return ((((size_t)seq * kv.n_kv + h) * 2 + which) * 2 + (block & 1)) * kKvBlock * kv.D;
 }
 
+// Block `page` is begun anew by row r: the tags of the row that had it last (former; 0: none) forget it, but for
+// those that this launch writes (parity `own` of row r; 2: none).  Where another workgroup of the launch writes
+// such a tag, whichever comes first, its own value stays.
+__device__ __forceinline__ void forget(const KvDev &kv, uint32_t page, uint32_t former, uint32_t r, uint32_t own, uint32_t threads) {
+    if (threadIdx.x == 0 && former != r + 1) kv.owner[page] = r + 1;
+    if (former == 0 || former > kv.n_seqs) return;
+    uint2 *tags = kv.tags + (size_t)(former - 1) * kv.n_kv * 4;
+    for (uint32_t i = threadIdx.x; i < kv.n_kv * 4; i += threads) {
+        const uint2 t = tags[i];
+        if (t.x != page || t.y == 0 || (former - 1 == r && i % 2 == own)) continue;
+        unsigned long long was = t.x | (unsigned long long)t.y << 32;
+        (void)__hip_atomic_compare_exchange_strong(reinterpret_cast<unsigned long long *>(tags + i), &was, (unsigned long long)page,
+                                                   __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
 // Grid: units, heads, keys or values.  A workgroup takes the block's tokens into
 // registers as the layout's pieces (16 elements a thread: two runs of
 // eight channels for keys, two of eight tokens for values), finds the largest,
@@ -310,8 +326,10 @@ __device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b
     }
     const bool lost = page >= kv.n_blocks;
     if (lost && tid == 0) kv_report(err, kKvErrBlock, r);
-    const bool stale = from && (held_tag.x != j || held_tag.y < from);
+    const bool stale = from && !lost && (held_tag.x != page || held_tag.y < from);
     if (stale && tid == 0) kv_report(err, kKvErrOpen, r);
+    const bool begins = which == 0 && h == 0 && from == 0 && !lost;  // (once for all heads)
+    const uint32_t former = begins ? kv.owner[page] : 0;
     float top = 0.0f, odd = 0.0f;  // odd: NaN with an infinity or a NaN among them
 #pragma unroll
     for (int e = 0; e < 16; e++) {
@@ -338,6 +356,8 @@ __device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b
         const bool shared = begin % kKvBlock && o > first && (o - first) % 2 == 0;
         if (j != (shared ? first : o)) continue;
         if (o == first && stale) continue;  // (its place holds another block's, or a beginning without a gap)
+        const uint32_t of = shared ? b.table[(size_t)r * b.max_blocks + o] : page;
+        if (of >= kv.n_blocks) continue;
         const uint32_t b0 = o * kKvBlock, f = begin > b0 ? begin - b0 : 0;
         const uint32_t e = row.len - b0 < kKvBlock ? row.len - b0 : kKvBlock;
         float *dst = kv.open + open_at(kv, r, h, which, o);
@@ -364,8 +384,9 @@ __device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b
                 }
             }
         }
-        if (tid == 0) tag[o & 1] = make_uint2(o, e);
+        if (tid == 0) tag[o & 1] = make_uint2(of, e);
     }
+    if (begins) forget(kv, page, former, r, j + 1 >= last ? j & 1 : 2, 2 * D);
 }
 
 template <int D>

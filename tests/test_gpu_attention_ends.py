@@ -198,6 +198,101 @@ def test_gpu_plan_again_and_again_loses_no_block(ctx, n, most):
     graph.destroy()
 
 
+def test_gpu_a_sequence_in_another_row(ctx):
+    """The open block's tokens are the row's: a sequence that goes on in another row is told, and never gets the tokens
+    of the row's last sequence; at a block's border it may move."""
+    print("append: a sequence in another row", flush=True)
+    g, kv, D = gen(26), 2, 64
+    for case in ("same index", "same block", "both"):
+        total = [40, 36, 64]
+        s = Seqs(g, total)
+        k = [heads(g, n, kv, D) for n in total]
+        spare = next(p for p in range(s.pool) if p not in s.table)
+        c = ctx.kv_cache(s.pool, kv, D, 3)
+        if case == "same block":  # the first sequence ends, and its last block becomes the second one's
+            first = s.table[0].copy()
+            c.append(dev(k[0]), dev(k[0]), s.batch([40, 0, 0], [40, 0, 0]))
+            s.table[1, 1] = first[1]
+            c.append(dev(np.concatenate(k[1:])), dev(np.concatenate(k[1:])), s.batch([40, 36, 64], [0, 36, 64]))
+        else:
+            c.append(dev(np.concatenate(k)), dev(np.concatenate(k)), s.batch(total, total))
+        if case == "both":  # the other way round too: two sequences change places
+            s.table[[0, 1]] = s.table[[1, 0]]
+            one = heads(g, 2, kv, D)
+            c.append(dev(one), dev(one), s.batch([37, 41, 64], [1, 1, 0]))
+            rows = [(0, 37), (1, 41)]
+        else:
+            s.table[0] = s.table[1]
+            one = heads(g, 1, kv, D)
+            c.append(dev(one), dev(one), s.batch([37, 0, 64], [1, 0, 0]))
+            rows = [(0, 37)]
+        with pytest.raises(DeviceError, match="append: the block's earlier tokens are not held"):
+            ctx.sync()
+        for i, n in rows:
+            a, b = read(c, s.slots(i, 32, n))
+            assert np.isnan(a).all() and np.isnan(b).all()
+            assert np.isfinite(read(c, s.slots(i, 0, 32))[0]).all()
+        # a whole block: no tokens from before are needed
+        s.table[1] = s.table[2]
+        s.table[1, 2] = spare
+        more = heads(g, 3, kv, D)
+        c.append(dev(more), dev(more), s.batch([0, 67, 64], [0, 3, 0]))
+        c.append(dev(more[:1]), dev(more[:1]), s.batch([0, 68, 64], [0, 1, 0]))
+        ctx.sync()
+        assert same(read(c, s.slots(1, 0, 68))[0], ref.values(np.concatenate([k[2], more, more[:1]])))
+        c.free()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_gpu_rows_and_blocks_used_again(ctx, new):
+    """Rows and blocks of sequences that ended, for others: nothing is left of the former."""
+    print(f"append: rows and blocks used again {new}", flush=True)
+    g, kv, D, n = gen(27, new), 2, 96, 3
+    s = Seqs(g, [160] * n, extra=0)
+    c = ctx.kv_cache(s.pool, kv, D, n)
+    order = s.table.copy()
+    for turn in range(4):
+        s.table = order[np.roll(np.arange(n), turn)]  # each row gets the blocks that another had
+        at, k = np.zeros(n, int), [heads(g, 160, kv, D) for _ in range(n)]
+        stop = np.array([47, 90, 160]) - turn
+        while (at < stop).any():
+            m = np.minimum([new, 1 + new // 2, 33], stop - at)
+            x = np.concatenate([k[i][at[i]:at[i] + m[i]] for i in range(n)])
+            at += m
+            c.append(dev(x), dev(x), s.batch(at, m))
+        ctx.sync()
+        for i in range(n):
+            a, b = read(c, s.slots(i, 0, stop[i]))
+            assert same(a, ref.values(k[i][:stop[i]])) and same(b, a), (turn, i)
+    c.free()
+
+
+def test_gpu_a_block_begun_anew_in_the_same_row(ctx):
+    """The tokens of a row's last sequence are not held any more once their block is begun anew, even where the new
+    sequence's last block has no place."""
+    print("append: a block begun anew in its row", flush=True)
+    g, kv, D = gen(33), 2, 64
+    s = Seqs(g, [96])
+    old, new = heads(g, 20, kv, D), heads(g, 71, kv, D)
+    c = ctx.kv_cache(s.pool, kv, D, 1)
+    c.append(dev(old), dev(old), s.batch([20], [20]))
+    good, s.table = s.table, s.table.copy()
+    s.table[0, 2] = ref.NONE
+    c.append(dev(new[:70]), dev(new[:70]), s.batch([70], [70]))
+    with pytest.raises(DeviceError, match="sequence 0: the table has no block"):
+        ctx.sync()
+    s.table = good
+    assert same(read(c, s.slots(0, 0, 64))[0], ref.values(new[:64]))
+    c.append(dev(new[20:21]), dev(new[20:21]), s.batch([21], [1]))
+    with pytest.raises(DeviceError, match="sequence 0: append: the block's earlier tokens are not held"):
+        ctx.sync()
+    assert np.isnan(read(c, s.slots(0, 0, 21))[0]).all()
+    c.append(dev(new), dev(new), s.batch([71], [71]))
+    ctx.sync()
+    assert same(read(c, s.slots(0, 0, 71))[0], ref.values(new))
+    c.free()
+
+
 @pytest.mark.parametrize("D", [64, 192])
 @pytest.mark.parametrize("wrong,tokens", [(10, 3), (10, 40), (1, 90)])
 def test_gpu_a_refused_append_spoils_no_held_tokens(ctx, D, wrong, tokens):
