@@ -111,7 +111,7 @@ __device__ __forceinline__ ThinWork thin_work(const ThinArgs &a, uint32_t index)
         const uint32_t r = r0 + lane;
         if (r >= a.b.n_seqs) break;
         t = thin_row(a, r);
-        if (t.k.falls && blockIdx.x == 0 && blockIdx.y == 0) kv_report(a.err, kKvErrRows, r);
+        if ((t.k.falls || t.k.behind) && blockIdx.x == 0 && blockIdx.y == 0) kv_report(a.err, kKvErrRows, r);
         falls |= t.k.falls;
         sum += (float)t.tiles * (float)t.blocks;
     }

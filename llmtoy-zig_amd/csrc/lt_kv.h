@@ -49,10 +49,10 @@ struct KvBatchDev {
 
 // One sequence's part of a batch: its tokens first .. first + n - 1, at the
 // positions len - n .. len - 1.  bad: the arrays contradict themselves; falls: by a
-// start that falls, so that n is 0.
+// start that falls, so that n is 0; behind: by tokens that all lie behind n_tokens, so that n is 0 too.
 struct KvRow {
     uint32_t first, n, len;
-    bool bad, falls;
+    bool bad, falls, behind;
 };
 
 #ifdef __HIPCC__
@@ -69,6 +69,7 @@ __device__ __forceinline__ KvRow kv_row_of(const KvBatchDev &b, uint32_t r) {
     k.n = end > k.first ? end - k.first : 0;
     k.len = b.len[r];
     k.falls = s1 < s0;
+    k.behind = s0 >= room && s1 > s0;
     k.bad = s1 > room || k.len < k.n || k.len > b.max_blocks * kKvBlock || (b.max_new && k.n > b.max_new);
     return k;
 }

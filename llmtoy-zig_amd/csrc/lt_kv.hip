@@ -174,7 +174,7 @@ __host__ __device__ __forceinline__ uint32_t append_units(uint32_t n_tokens, uin
 }
 
 // The row that unit u belongs to, by a whole wavefront: up to 64 rows from one round of
-// loads, more in three.
+// loads, more in three.  (row.falls: or behind)
 __device__ __forceinline__ uint32_t append_row(const KvBatchDev &b, uint32_t u, KvRow &row) {
     const auto base = [&](uint32_t start, uint32_t i) { return (start < b.n_tokens ? start : b.n_tokens) / kKvBlock + 2 * i; };
     uint32_t r;
@@ -185,13 +185,13 @@ __device__ __forceinline__ uint32_t append_row(const KvBatchDev &b, uint32_t u, 
         r = below ? 63 - __builtin_clzll(below) : 0;
         row.first = __builtin_amdgcn_readlane(k.first, r), row.n = __builtin_amdgcn_readlane(k.n, r);
         row.len = __builtin_amdgcn_readlane(k.len, r);
-        row.bad = __builtin_amdgcn_readlane(k.bad, r), row.falls = __builtin_amdgcn_readlane(k.falls, r);
+        row.bad = __builtin_amdgcn_readlane(k.bad, r), row.falls = __builtin_amdgcn_readlane(k.falls || k.behind, r);
     } else {
         r = __builtin_amdgcn_readfirstlane(kv_row(b.n_seqs, u, [&](uint32_t i) { return base(b.start[i], i); }));
         const KvRow k = kv_row_of(b, r);
         row.first = __builtin_amdgcn_readfirstlane(k.first), row.n = __builtin_amdgcn_readfirstlane(k.n);
         row.len = __builtin_amdgcn_readfirstlane(k.len);
-        row.bad = __builtin_amdgcn_readfirstlane(k.bad), row.falls = __builtin_amdgcn_readfirstlane(k.falls);
+        row.bad = __builtin_amdgcn_readfirstlane(k.bad), row.falls = __builtin_amdgcn_readfirstlane(k.falls || k.behind);
     }
     return r;  // (in scalar registers, as what follows from it)
 }

@@ -344,3 +344,32 @@ def test_gpu_a_block_that_is_not_there_leaves_the_held_tokens(ctx):
     ctx.sync()
     assert same(read(c, s.slots(0, 0, 70))[0], ref.values(k))
     c.free()
+
+
+@pytest.mark.parametrize("n,each", [(2, 3), (70, 2), (3, 200)])
+def test_gpu_sequences_wholly_behind_the_batch_are_told(ctx, n, each):
+    print(f"sequences behind n_tokens {n} {each}", flush=True)
+    D, KV, G = 64, 1, 4
+    g, s, k, v, c, q, total, scale = _attend(ctx, D, KV, G, [40] * n, [each] * n, 0, seed=30)
+    room = each * (n - 1)  # the last one has no place
+    want, bound = _expect(k, v, q, total, [each] * n, scale, 0)
+    b = s.batch(total, [each] * n, room=room)
+    c.free()
+    c = ctx.kv_cache(s.pool, KV, D, n)
+    first = [np.concatenate([x[:40] for x in a]) for a in (k, v)]
+    c.append(dev(first[0]), dev(first[1]), s.batch([40] * n, [40] * n))
+    c.append(dev(np.concatenate([x[40:] for x in k])[:room]), dev(np.concatenate([x[40:] for x in v])[:room]), b)
+    with pytest.raises(DeviceError, match=f"sequence {n - 1}: the batch contradicts itself"):
+        ctx.sync()
+    out = DeviceArray((room, *q.shape[1:]))
+    ctx.attention(out, dev(q[:room]), c, b, scale)
+    with pytest.raises(DeviceError, match=f"sequence {n - 1}: the batch contradicts itself"):
+        ctx.sync()
+    close(out.numpy(), want[:room], bound[:room])
+    # an idle one behind is nobody's fault
+    start = np.minimum(np.arange(n + 1) * each, room)
+    idle = lt.KvBatch(dev(start, np.uint32), dev(total, np.uint32), dev(s.table), room)
+    ctx.attention(out, dev(q[:room]), c, idle, scale)
+    ctx.sync()
+    close(out.numpy(), want[:room], bound[:room])
+    c.free()
