@@ -25,7 +25,8 @@
  * Errors found on the device.  The single-launch MoE kernel bounds each of
  * its waits (200 ms); a wait that runs out makes that call's outputs NaN and
  * sets an error word.  A device-pointer call returns before that is known:
- * the next lt_sync (or LT_HOST_IO call) returns LT_ERR_DEVICE and clears it.
+ * the next lt_sync (or LT_HOST_IO call, whose own results are there all the same)
+ * returns LT_ERR_DEVICE and clears it.  What several calls reported comes in one text.
  * Callers that use device pointers should check lt_sync.
  *
  * Reference citations are paths in the llmtoy-zig tree.

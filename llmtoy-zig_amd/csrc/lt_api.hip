@@ -433,7 +433,7 @@ ptrdiff_t pin_slot(lt_ctx *ctx, size_t bytes) {
     return (ptrdiff_t)at;
 }
 
-// The end of an LT_HOST_IO call.
+// An LT_HOST_IO call's wait for the device.
 int host_sync(lt_ctx *ctx) {
     LT_HIP(ctx, hipStreamSynchronize(ctx->stream));
     ctx->pin_used = 0;
@@ -624,6 +624,30 @@ int check_fused_err(lt_ctx *ctx) {
                 v, (int)d[0] - 1, d[1], word, d[4]);
 }
 
+// Everything that kernels have reported since the last look, in one text.
+int check_reports(lt_ctx *ctx) {
+    const int fused = check_fused_err(ctx);
+    std::string text;
+    if (fused) text.swap(ctx->err);
+    const int kv = check_kv_err(ctx);
+    if (!fused) return kv;
+    text.swap(ctx->err);  // (text: the cache's, where there is one)
+    if (kv) {
+        try {
+            ctx->err += "; " + text;
+        } catch (...) {
+            return fail(ctx, LT_ERR_OOM, "host allocation failed");
+        }
+    }
+    return fused;
+}
+
+// The end of an LT_HOST_IO call, its stream idle and its results copied.
+int host_end(lt_ctx *ctx) {
+    prof_harvest(ctx);
+    return check_reports(ctx);
+}
+
 int matvec_dev(lt_ctx *ctx, const DevTensor &W, const float *x, float *y) {
     hipError_t e;
     switch (W.type) {
@@ -728,12 +752,8 @@ extern "C" const char *lt_last_error(const lt_ctx *ctx) { return ctx ? ctx->err.
 
 extern "C" int lt_sync(lt_ctx *ctx) {
     if (!ctx) return LT_ERR_INVALID;
-    int rc = host_sync(ctx);
-    if (rc) return rc;
-    prof_harvest(ctx);
-    const int kv = check_kv_err(ctx);
-    rc = check_fused_err(ctx);
-    return rc ? rc : kv;
+    const int rc = host_sync(ctx);
+    return rc ? rc : host_end(ctx);
 }
 
 extern "C" void *lt_stream(lt_ctx *ctx) { return ctx ? (void *)ctx->stream : nullptr; }
@@ -864,7 +884,7 @@ extern "C" int lt_matvec(lt_ctx *ctx, float *out, const lt_tensor *W, const floa
     if ((rc = matvec_dev(ctx, T, dx, dy))) return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dy, T.total_rows * 4))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -893,7 +913,7 @@ extern "C" int lt_quantize(lt_ctx *ctx, lt_tensor *t, const float *x, size_t row
     if ((rc = launch_rc(ctx, lt::launch_mx_quantize(t->t, dx, row0, rows, ctx->stream), "quantize"))) return rc;
     if (flags & LT_HOST_IO) {
         if ((rc = host_sync(ctx))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -912,7 +932,7 @@ extern "C" int lt_dequantize(lt_ctx *ctx, float *out, const lt_tensor *t, size_t
     if ((rc = launch_rc(ctx, lt::launch_mx_dequantize(t->t, dy, row0, rows, ctx->stream), "dequantize"))) return rc;
     if (flags & LT_HOST_IO) {
         if ((rc = host_out(ctx, out, dy, bytes))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -956,7 +976,7 @@ extern "C" int lt_matmul(lt_ctx *ctx, float *out, const lt_tensor *W, const floa
     if ((rc = launch_rc(ctx, lt::launch_matmul_mx(w, dx, T, ctx->mx.p, dy, ctx->stream), "matmul"))) return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dy, bytes))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -983,7 +1003,7 @@ extern "C" int lt_matmul_quantized(lt_ctx *ctx, float *out, const lt_tensor *W, 
     if ((rc = launch_rc(ctx, lt::launch_matmul_mx_mx(w, x, T, dy, ctx->stream), "matmul_quantized"))) return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dy, bytes))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1064,7 +1084,7 @@ extern "C" int lt_ffn_dense(lt_ctx *ctx, float *out, const lt_tensor *Wg, const 
     if ((rc = ffn_dense_dev(ctx, Wg->t, Wu->t, Wd->t, dx, act, dy, (flags & LT_MOE_UNFUSED) != 0))) return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dy, D * 4))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1247,7 +1267,7 @@ extern "C" int lt_moe_router_topk(lt_ctx *ctx, const lt_tensor *router, const fl
         if (scores)
             LT_HIP(ctx, hipMemcpyAsync(scores, dscores, R.total_rows * 4, hipMemcpyDeviceToHost, ctx->stream));
         if ((rc = host_sync(ctx))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1285,7 +1305,7 @@ extern "C" int lt_expert_gate_up_id(lt_ctx *ctx, const lt_tensor *gate_up, const
     if ((rc = gate_up_dev(ctx, GU, dx, dids, k, d_expert, down_cols, act, dh))) return rc;
     if (host) {
         if ((rc = host_out(ctx, h, dh, (size_t)k * down_cols * 4))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1328,7 +1348,7 @@ extern "C" int lt_expert_down_id(lt_ctx *ctx, const lt_tensor *down, const float
         return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dout, D.rows * 4))) return rc;
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1483,8 +1503,7 @@ extern "C" int lt_moe_forward(lt_ctx *ctx, float *out, const float *x, const lt_
     if ((rc = copy_routing_out(ctx, k, out_ids, out_w, host))) return rc;
     if (host) {
         if ((rc = host_out(ctx, out, dout, d_model * 4))) return rc;
-        prof_harvest(ctx);
-        return check_fused_err(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1594,8 +1613,7 @@ extern "C" int lt_moe_prefill(lt_ctx *ctx, float *out, const float *X, uint32_t 
             LT_HIP(ctx, hipMemcpyAsync(out_w, wsp + logits_b + ids_b, (size_t)T * k * 4, hipMemcpyDeviceToHost,
                                        ctx->stream));
         if ((rc = host_sync(ctx))) return rc;
-        prof_harvest(ctx);
-        return check_fused_err(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1678,7 +1696,7 @@ int rmsnorm_entry(lt_ctx *ctx, int op, float *out, const float *a, const float *
     if (host) {
         LT_HIP(ctx, hipMemcpyAsync(out, dout, len * 4, hipMemcpyDeviceToHost, ctx->stream));
         LT_HIP(ctx, hipStreamSynchronize(ctx->stream));
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1721,7 +1739,7 @@ extern "C" int lt_rmsnorm_weighted_raw_scaled(lt_ctx *ctx, float *weighted_out, 
         LT_HIP(ctx, hipMemcpyAsync(weighted_out, dwo, (size_t)n * 4, hipMemcpyDeviceToHost, ctx->stream));
         LT_HIP(ctx, hipMemcpyAsync(raw_scaled_out, dro, (size_t)n * 4, hipMemcpyDeviceToHost, ctx->stream));
         LT_HIP(ctx, hipStreamSynchronize(ctx->stream));
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1750,7 +1768,7 @@ extern "C" int lt_moe_tail(lt_ctx *ctx, float *x, const float *moe, const float 
     if (host) {
         LT_HIP(ctx, hipMemcpyAsync(x, xo, (size_t)n * 4, hipMemcpyDeviceToHost, ctx->stream));
         LT_HIP(ctx, hipStreamSynchronize(ctx->stream));
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1818,8 +1836,7 @@ extern "C" int lt_gemma4_moe_block(lt_ctx *ctx, float *x, const float *dense_ffn
             if (host) {
                 LT_HIP(ctx, hipMemcpyAsync(x, xio, n * 4, hipMemcpyDeviceToHost, ctx->stream));
                 LT_HIP(ctx, hipStreamSynchronize(ctx->stream));
-                prof_harvest(ctx);
-                return check_fused_err(ctx);
+                return host_end(ctx);
             }
             return LT_OK;
         }
@@ -1852,7 +1869,7 @@ extern "C" int lt_gemma4_moe_block(lt_ctx *ctx, float *x, const float *dense_ffn
     if (host) {
         LT_HIP(ctx, hipMemcpyAsync(x, xio, n * 4, hipMemcpyDeviceToHost, ctx->stream));
         LT_HIP(ctx, hipStreamSynchronize(ctx->stream));
-        prof_harvest(ctx);
+        return host_end(ctx);
     }
     return LT_OK;
 }
@@ -1911,9 +1928,7 @@ struct HostArrays {
     }
     int finish() {
         const int rc = host_sync(ctx);
-        if (rc) return rc;
-        prof_harvest(ctx);
-        return check_kv_err(ctx);
+        return rc ? rc : host_end(ctx);
     }
 };
 

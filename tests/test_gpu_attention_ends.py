@@ -373,3 +373,70 @@ def test_gpu_sequences_wholly_behind_the_batch_are_told(ctx, n, each):
     ctx.sync()
     close(out.numpy(), want[:room], bound[:room])
     c.free()
+
+
+def _short_plan(c):
+    """A plan that finds no block (device arrays: nothing is told yet)."""
+    z = lambda *s: dev(np.zeros(s), np.uint32)  # noqa: E731
+    c.kv_plan(lt.KvBatch(z(2), z(1), z(1, 2), 1), z(1), dev([1], np.uint32), z(0), z(1), z(1), z(1), z(1))
+
+
+def test_gpu_every_synchronising_call_tells(ctx):
+    """What was found wrong on the device comes with the next lt_sync or LT_HOST_IO call, whichever that is, once, and the
+    call's own results are there."""
+    print("reports of host calls", flush=True)
+    g = gen(31)
+    D = 256
+    w = g.standard_normal((D, D)).astype(np.float32)
+    x = g.standard_normal(D).astype(np.float32)
+    t = ctx.upload(w, ggml.F32, D, D)
+    mx = ctx.create(ggml.MXFP4, 4, D)
+    y = np.zeros(D, np.float32)
+    rope = ctx.rope(64)
+    h, pos = g.standard_normal((3, 2, 64)).astype(np.float32), np.zeros(3, np.uint32)
+    calls = {
+        "matvec": lambda: ctx.quant_matvec(y, t, x),
+        "rmsnorm": lambda: rmsnorm(ctx, y[None], x[None]),
+        "quantize": lambda: ctx.quantize(mx, np.zeros((4, D), np.float32)),
+        "rotation": lambda: ctx.qk_norm_rope(np.zeros_like(h), None, h, None, None, None, pos, rope),
+        "sync": ctx.sync,
+    }
+    for name, call in calls.items():
+        _short_plan(ctx)
+        y[:] = 0
+        with pytest.raises(DeviceError, match="sequence 0: plan: no blocks left"):
+            call()
+        call()  # (told once)
+        if name == "matvec":
+            assert np.linalg.norm(y - w @ x) < 1e-4 * np.linalg.norm(y)
+    ctx.sync()
+    for a in (t, mx, rope):
+        a.free()
+
+
+def test_gpu_two_kinds_of_reports_at_once(ctx, monkeypatch):
+    print("a wait that ran out and a plan that found no blocks", flush=True)
+    from test_gpu_mxfp4_layer import layer
+    g = gen(32)
+    E, D, F, k = 128, 2048, 768, 8
+    x = g.standard_normal(D).astype(np.float32)
+    monkeypatch.setenv("LT_MX_WAIT_TICKS", "0")
+    with lt.Context(0) as c:
+        ts = layer(c, g, E, D, F)
+        out, ids, w = DeviceArray((D,)), DeviceArray((k,), np.uint32), DeviceArray((k,))
+        with pytest.raises(DeviceError, match="wait timed out"):  # (the hand-over memory's first call)
+            c.moe_forward(np.zeros(D, np.float32), x, *ts, k, F)
+        c.moe_forward(out, dev(x), *ts, k, F, out_ids=ids, out_w=w)
+        _short_plan(c)
+        with pytest.raises(DeviceError, match="(?s)wait timed out.*sequence 0: plan: no blocks left"):
+            c.sync()
+        c.sync()
+        # an attention call on host arrays tells of a layer's wait too
+        c.moe_forward(out, dev(x), *ts, k, F, out_ids=ids, out_w=w)
+        rope = c.rope(64)
+        h = g.standard_normal((1, 2, 64)).astype(np.float32)
+        with pytest.raises(DeviceError, match="wait timed out"):
+            c.qk_norm_rope(np.zeros_like(h), None, h, None, None, None, np.zeros(1, np.uint32), rope)
+        c.sync()
+        for t in (*ts, rope):
+            t.free()
