@@ -49,7 +49,6 @@ struct Shape {
     // (what a wavefront would not have the registers for: four on a SIMD up to heads of 128, then two)
     static constexpr bool kQueriesInLds = DW >= 128;
 };
-constexpr uint32_t kThinTarget = 512;  // the largest
 
 struct ThinArgs {
     const uint8_t *codes;
@@ -551,7 +550,7 @@ bool attention_head_dim(uint32_t D) { return D == 64 || D == 96 || D == 128 || D
 static bool wide(const AttnArgs &a) { return any_wide(a.b.n_tokens, a.b.max_new, a.group); }
 
 size_t attention_workspace(const AttnArgs &a) {
-    const size_t thin = (size_t)a.kv.n_kv * 2 * thin_slots(kThinTarget, a.kv.n_kv) * kThinRows * (a.kv.D + 4) * 4;
+    const size_t thin = thin_workspace(a.kv.D, a.kv.n_kv);
     const size_t more = wide(a) ? attention_wide_workspace(a.kv.D) : 0;
     return thin < more ? more : thin;
 }

@@ -88,6 +88,11 @@ LT_CUT uint32_t thin_grid(uint32_t tiles, uint32_t max_blocks, uint32_t n_kv, ui
 // Places for a head's parts; as many for groups of them.
 LT_CUT uint32_t thin_slots(uint32_t target, uint32_t n_kv) { return 2 * (target / n_kv + 1) + 2; }
 
+// Their bytes: 16 rows of D sums, then m, l, mo of each.
+LT_CUT size_t thin_workspace(uint32_t D, uint32_t n_kv) {
+    return (size_t)n_kv * 2 * thin_slots(thin_target(D), n_kv) * kThinRows * (D + 4) * 4;
+}
+
 // ------------------------------------------------------------------- many rows
 constexpr uint32_t kLeast = 8;        // blocks that a workgroup is worth having for
 constexpr uint32_t kMaxTiles = 1024;  // of a head, whose blocks are counted in LDS

@@ -95,6 +95,10 @@ static void few(const Batch &b, uint32_t D) {
     CHECK(work <= grid);
     CHECK(parts <= slots);
     CHECK((uint64_t)2 * slots * b.n_kv <= kAttnTickets);
+    // (two places a slot, of which the kernel's last float is in 32 bits of bytes; no more than this head size's parts need)
+    const uint64_t bytes = thin_workspace(D, b.n_kv), part = 16 * (D + 4) * 4;
+    CHECK(bytes >= 2 * part * slots * b.n_kv && bytes < 1ull << 32);
+    CHECK(bytes <= 2 * part * (2 * target + 4 * b.n_kv));
     // (none to do: then no sequence has rows for this kernel)
     if (b.n_tokens && grid == 0) CHECK(work == 0);
 }
