@@ -243,12 +243,12 @@ def _heads(a, what: str):
     if _is_torch(a):
         st, p, host = a.stride(), a.data_ptr(), not a.is_cuda
     elif isinstance(a, np.ndarray):
-        st, p, host = [n // 4 for n in a.strides], a.ctypes.data, True
+        st, p, host = [n / 4 for n in a.strides], a.ctypes.data, True
     else:
         st, (p, host) = (H * D, D, 1), _ptr(a)
-    if T and (D > 1 and st[2] != 1 or H > 1 and st[1] != D or T > 1 and st[0] < H * D):
+    if T and (D > 1 and st[2] != 1 or H > 1 and st[1] != D or T > 1 and (st[0] < H * D or st[0] % 1)):
         raise InvalidError(f"{what}: a token's heads must lie in a row (strides {tuple(st)})")
-    return p, host, T, H, D, st[0] if T > 1 else H * D
+    return p, host, T, H, D, int(st[0]) if T > 1 else H * D
 
 
 class Rope:
