@@ -90,19 +90,19 @@ __device__ __forceinline__ Tile tile_of(const WideArgs &a, uint32_t row, uint32_
 }
 
 // The sum of v over the threads before this one, and over all.
-template <int WAVES, typename T>
-__device__ __forceinline__ T scan(T v, T *s_sum, T &all) {
+template <int WAVES>
+__device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t *s_sum, uint64_t &all) {
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    T up = v;
+    uint64_t up = v;
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
-        const T p = __shfl_up(up, off, kWave);
+        const uint64_t p = __shfl_up(up, off, kWave);
         if ((int)lane >= off) up += p;
     }
     __syncthreads();
     if (lane == kWave - 1) s_sum[wave] = up;
     __syncthreads();
-    T before = up - v;
+    uint64_t before = up - v;
     all = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) {
@@ -169,13 +169,13 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
     __shared__ half8 s_kv[2][8 * D];
     __shared__ f32x4 s_x[SPLIT > 1 ? W * 4 * kWave : 1];
     __shared__ uint64_t s_first[kMaxTiles], s_sum[W];
-    __shared__ uint32_t s_base[kMaxTiles], s_sum32[W], s_hit[2], s_last;
+    __shared__ uint32_t s_base[kMaxTiles], s_hit[2], s_last;
     const uint32_t tid = threadIdx.x, lane = tid % kWave, half = lane / 32, n = lane % 32;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / kWave), cut = wave % SPLIT, rg = wave / SPLIT;
 
     // ---- the rows' tiles
     const uint32_t per = (a.b.n_seqs + NT - 1) / NT;
-    uint32_t mine = 0, all_tiles;
+    uint64_t mine = 0, every;  // (sequences that overlap may have 2^32 tiles and more)
     for (uint32_t i = 0; i < per; i++) {
         const uint32_t r = tid * per + i;
         if (r >= a.b.n_seqs) break;
@@ -183,8 +183,10 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         mine += (row_rows(a, k) + R - 1) / R;
         if (k.falls && blockIdx.x == 0) kv_report(a.err, kKvErrRows, r);
     }
-    uint32_t at = scan<W>(mine, s_sum32, all_tiles);
-    if (all_tiles > a.tiles) return;  // (start falls, sequences overlap; reported)
+    const uint64_t before0 = scan<W>(mine, s_sum, every);
+    if (every > a.tiles) return;  // (start falls, sequences overlap; reported)
+    const uint32_t all_tiles = (uint32_t)every;
+    uint32_t at = (uint32_t)before0;
     // ---- what this workgroup takes: blocks u .. u1 - 1 of the line of heads and tiles, or a tile
     uint64_t u = 0, u1 = 1, line = 0, total = 0;
     uint32_t pieces = 1, piece = 0, head_kv = 0;
