@@ -218,22 +218,43 @@ def _count(a) -> int:
     return a.numel() if _is_torch(a) else math.prod(a.shape)
 
 
+# Where an array lies: host memory, device memory that names no device (hip.DeviceArray), or a torch
+# device's number.
+HOST, SOME_DEVICE = -1, -2
+
+
+def _place(a, is_host: bool) -> int:
+    return HOST if is_host else a.get_device() if _is_torch(a) else SOME_DEVICE
+
+
+def _all_host(ctx: "Context", places: set) -> bool:
+    """Whether a call's arrays are host memory; all of them or none, and none on another device than the context's."""
+    if HOST in places:
+        if len(places) > 1:
+            raise InvalidError("mix of host and device arrays")
+        return True
+    if not places <= ctx.places:
+        raise InvalidError(f"an array on device {max(places - ctx.places)}, the context is on {ctx.device}")
+    return False
+
+
 def _words(a, n: int, what: str):
-    """(pointer, is_host) of a contiguous array of n 32-bit whole numbers."""
+    """(pointer, place) of a contiguous array of n 32-bit whole numbers."""
     if type(a).__module__ == "torch":  # (the usual case of a step, ten times a call: nothing looked up twice)
         if _is_word(a.dtype) and a.numel() == n and a.is_contiguous():
-            return a.data_ptr(), not a.is_cuda
+            return a.data_ptr(), a.get_device()
     if a is None:
         raise InvalidError(f"{what}: an array of {n} is needed")
     if not _is_word(a.dtype):
         raise InvalidError(f"{what}: 32-bit whole numbers expected, got {a.dtype}")
     if _count(a) != n:
         raise InvalidError(f"{what}: {tuple(a.shape)}, {n} entries expected")
-    return _ptr(a)
+    p, host = _ptr(a)
+    return p, _place(a, host)
 
 
 def _heads(a, what: str):
-    """(pointer, is_host, tokens, heads, head_dim, floats from token to token) of a float32 array
+    """(pointer, place, tokens, heads, head_dim, floats from token to token) of a float32 array
     [tokens, heads, head_dim] whose heads lie in a row; the tokens may be a stride apart."""
     if _kind(a.dtype) != "float32":
         raise InvalidError(f"{what}: float32 expected, got {a.dtype}")
@@ -241,14 +262,15 @@ def _heads(a, what: str):
         raise InvalidError(f"{what}: [tokens, heads, head_dim] expected, got {tuple(a.shape)}")
     T, H, D = a.shape
     if _is_torch(a):
-        st, p, host = a.stride(), a.data_ptr(), not a.is_cuda
+        st, p, place = a.stride(), a.data_ptr(), a.get_device()
     elif isinstance(a, np.ndarray):
-        st, p, host = [n / 4 for n in a.strides], a.ctypes.data, True
+        st, p, place = [n / 4 for n in a.strides], a.ctypes.data, HOST
     else:
         st, (p, host) = (H * D, D, 1), _ptr(a)
+        place = _place(a, host)
     if T and (D > 1 and st[2] != 1 or H > 1 and st[1] != D or T > 1 and (st[0] < H * D or st[0] % 1)):
         raise InvalidError(f"{what}: a token's heads must lie in a row (strides {tuple(st)})")
-    return p, host, T, H, D, int(st[0]) if T > 1 else H * D
+    return p, place, T, H, D, int(st[0]) if T > 1 else H * D
 
 
 class Rope:
@@ -277,14 +299,12 @@ class KvBatch:
         self.n_seqs, self.n_tokens, self.max_blocks, self.max_new = n, int(n_tokens), int(table.shape[1]), int(max_new)
 
     def struct(self):
-        """(lt_kv_batch, is_host)"""
+        """(lt_kv_batch, the places of its arrays)"""
         n = self.n_seqs
-        p, host = _words(self.start, n + 1, "start")
+        p, h0 = _words(self.start, n + 1, "start")
         q, h1 = _words(self.len, n, "len")
         t, h2 = _words(self.table, n * self.max_blocks, "table")
-        if host != h1 or host != h2:
-            raise InvalidError("mix of host and device arrays")
-        return KvBatchStruct(n, self.n_tokens, self.max_blocks, self.max_new, p, q, t), host
+        return KvBatchStruct(n, self.n_tokens, self.max_blocks, self.max_new, p, q, t), {h0, h1, h2}
 
 
 class KvCache:
@@ -300,24 +320,22 @@ class KvCache:
 
     def append(self, k, v, batch: KvBatch):
         """The batch's tokens' keys and values ([n_tokens, n_kv_heads, head_dim]) into the cache."""
-        b, host = batch.struct()
+        b, places = batch.struct()
         gk, gv = self._mine(k, "k", batch.n_tokens), self._mine(v, "v", batch.n_tokens)
-        if host != gk[1] or host != gv[1]:
-            raise InvalidError("mix of host and device arrays")
         c = self.ctx
+        host = _all_host(c, places | {gk[1], gv[1]})
         c._check(c.lib.lt_kv_append(c.ptr, self.handle, gk[0], gv[0], gk[5], gv[5], C.byref(b), LT_HOST_IO if host else 0))
 
     def read(self, k_out, v_out, slots):
         """The values that slots stand for, into k_out and v_out [n, n_kv_heads, head_dim]."""
         n = _count(slots)
-        p, host = _words(slots, n, "slots")
+        p, place = _words(slots, n, "slots")
         gk, gv = self._mine(k_out, "k_out", n), self._mine(v_out, "v_out", n)
         for g, w in ((gk, "k_out"), (gv, "v_out")):
             if g[5] != self.n_kv_heads * self.head_dim:
                 raise InvalidError(f"{w}: must be contiguous")
-        if host != gk[1] or host != gv[1]:
-            raise InvalidError("mix of host and device arrays")
         c = self.ctx
+        host = _all_host(c, {place, gk[1], gv[1]})
         c._check(c.lib.lt_kv_read(c.ptr, gk[0], gv[0], self.handle, p, n, LT_HOST_IO if host else 0))
 
     def _mine(self, a, what, tokens):
@@ -342,6 +360,7 @@ class Context:
         if rc != LT_OK:
             raise _ERRS.get(rc, LtError)(f"lt_init({device}) failed with status {rc}", rc)
         self.ptr = p
+        self.device, self.places = device, {device, SOME_DEVICE}  # (places: of device arrays that it takes)
 
     def close(self):
         if self.ptr:
@@ -523,25 +542,26 @@ class Context:
         none = (None, None, 0, 0, 0, 0)
         gq, gqo = _heads(q, "q"), _heads(q_out, "q_out")
         gk, gko = (none, none) if k is None else (_heads(k, "k"), _heads(k_out, "k_out"))
-        T, host = gq[2], gq[1]
+        T, places = gq[2], set()
         for w, g, first in (("q", gq, gq), ("q_out", gqo, gq), ("k", gk, gk), ("k_out", gko, gk)):
             if g[0] is None:
                 continue
             if g[2] != T or g[4] != rope.head_dim or g[3] != first[3]:
                 raise InvalidError(f"{w}: {g[2:5]}, {T} tokens of heads of {rope.head_dim} expected")
-            if g[1] != host:
-                raise InvalidError("mix of host and device arrays")
+            places.add(g[1])
         ps = []
         for w, a in (("wq", wq), ("wk", wk)):
             if a is not None and (tuple(a.shape) != (rope.head_dim,) or _kind(a.dtype) != "float32"):
                 raise InvalidError(f"{w}: float32 [{rope.head_dim}] expected")
-            ps.append(_ptr(a))
-        ps.append(_words(positions, T, "positions"))
-        for _, h in ps:
-            if h is not None and h != host:
-                raise InvalidError("mix of host and device arrays")
+            p, h = _ptr(a)
+            ps.append(p)
+            if a is not None:
+                places.add(_place(a, h))
+        p, h = _words(positions, T, "positions")
+        places.add(h)
+        host = _all_host(self, places)
         fl = (LT_HOST_IO if host else 0) | (0 if norm else LT_ROPE_NO_NORM) | (LT_NORM_ONE_PLUS_W if one_plus_w else 0)
-        self._check(self.lib.lt_qk_norm_rope(self.ptr, gqo[0], gko[0], gq[0], gk[0], ps[0][0], ps[1][0], ps[2][0], rope.handle,
+        self._check(self.lib.lt_qk_norm_rope(self.ptr, gqo[0], gko[0], gq[0], gk[0], ps[0], ps[1], p, rope.handle,
                                              T, gq[3], gk[3], gq[5], gk[5], gqo[5], gko[5], eps, fl))
 
     def kv_cache(self, n_blocks: int, n_kv_heads: int, head_dim: int, n_seqs: int = 1) -> KvCache:
@@ -553,21 +573,21 @@ class Context:
     def kv_plan(self, batch: KvBatch, len_in, n_new, free_blocks, used_in, used_out, positions, slots):
         """A step's batch (start, len, new entries of table), positions and slots from the sequences'
         lengths and a list of free blocks (lt_kv_plan)."""
-        b, host = batch.struct()
+        b, places = batch.struct()
         n_free = _count(free_blocks)
         p, T = [], batch.n_tokens
         for w, a, n in (("len_in", len_in, b.n_seqs), ("n_new", n_new, b.n_seqs), ("free_blocks", free_blocks, n_free),
                         ("used_in", used_in, 1), ("used_out", used_out, 1), ("positions", positions, T), ("slots", slots, T)):
             at, h = _words(a, n, w)
-            if h is not host:
-                raise InvalidError("mix of host and device arrays")
+            places.add(h)
             p.append(at)
+        host = _all_host(self, places)
         self._check(self.lib.lt_kv_plan(self.ptr, C.byref(b), p[0], p[1], p[2], n_free, p[3], p[4], p[5], p[6],
                                         LT_HOST_IO if host else 0))
 
     def attention(self, out, q, cache: KvCache, batch: KvBatch, scale: float, window: int = 0):
         """out [n_tokens, heads, head_dim]: the queries over the cache, causal (lt_attention)."""
-        b, host = batch.struct()
+        b, places = batch.struct()
         gq, go = _heads(q, "q"), _heads(out, "out")
         T, H, D = gq[2:5]
         if T != batch.n_tokens or D != cache.head_dim or go[2:5] != gq[2:5]:
@@ -575,8 +595,7 @@ class Context:
                                f"{cache.head_dim}")
         if go[5] != H * D:
             raise InvalidError("out: must be contiguous")
-        if gq[1] != host or go[1] != host:
-            raise InvalidError("mix of host and device arrays")
+        host = _all_host(self, places | {gq[1], go[1]})
         self._check(self.lib.lt_attention(self.ptr, go[0], gq[0], cache.handle, C.byref(b), H, gq[5], scale, window,
                                           LT_HOST_IO if host else 0))
         return out
