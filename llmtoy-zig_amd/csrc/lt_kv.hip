@@ -57,13 +57,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
     const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const uint32_t used = a.used_in[0];
     uint32_t len[kPlanRows], add[kPlanRows];
-    uint64_t tok = 0, need = 0;
+    uint64_t take[kPlanRows], tok = 0, need = 0;
     for (uint32_t i = 0; i < kPlanRows; i++) {
         const uint32_t r = tid * kPlanRows + i;
         len[i] = r < a.n_seqs ? a.len_in[r] : 0;
         add[i] = r < a.n_seqs ? a.n_new[r] : 0;
         tok += add[i];
-        need += plan_need(len[i], add[i], a.max_blocks);
+        take[i] = plan_need(len[i], add[i], a.max_blocks);
+        need += take[i];
     }
     // sums before this thread's rows
     uint64_t itok = tok, ineed = need;
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(KvPlanArgs a) {
                 for (uint64_t j = b0; j < b1 && j < a.max_blocks; j++) a.table[(size_t)r * a.max_blocks + j] = kKvNone;
         }
         btok += add[i];
-        bneed += plan_need(len[i], add[i], a.max_blocks);
+        bneed += take[i];
     }
     // (a wavefront's largest first: 1,024 atomics on one word took 3 us)
 #pragma unroll
