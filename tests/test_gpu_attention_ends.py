@@ -440,3 +440,72 @@ def test_gpu_two_kinds_of_reports_at_once(ctx, monkeypatch):
         c.sync()
         for t in (*ts, rope):
             t.free()
+
+
+@pytest.mark.parametrize("D,KV,G,window,seed", [(64, 2, 2, 0, 1), (128, 1, 4, 50, 2), (64, 1, 8, 0, 3)])
+def test_gpu_serving_with_rows_and_blocks_used_again(ctx, D, KV, G, window, seed):
+    """Sequences that come, go on by tokens and by parts of prompts, are taken back and end, over a small pool: plan,
+    append and attention at every step, the cache bit for bit and the outputs against 64 bits."""
+    print(f"serving {D} {KV}x{G} {window} {seed}", flush=True)
+    g = gen(D, seed, 34)
+    n, width, pool, steps = 6, 5, 22, 60
+    c = ctx.kv_cache(pool, KV, D, n)
+    table = np.full((n, width), ref.NONE, np.uint32)
+    free = list(g.permutation(pool))
+    k, v = ([np.zeros((0, KV, D), np.float32) for _ in range(n)] for _ in range(2))
+    held = [[None, None] for _ in range(n)]  # the blocks whose tokens a row has in fp32, by their parity
+
+    def cut(i, length):
+        """Sequence i keeps `length` tokens; blocks behind them go back."""
+        keep = -(-length // 32)
+        free.extend(int(b) for b in table[i, keep:] if b != ref.NONE)
+        table[i, keep:] = ref.NONE
+        k[i], v[i] = k[i][:length], v[i][:length]
+
+    for step in range(steps):
+        new = np.zeros(n, int)
+        for i in range(n):
+            what = g.random()
+            if what < 0.06:
+                cut(i, 0)
+                held[i] = [None, None]
+            elif what < 0.2 and len(k[i]):
+                to = len(k[i]) - int(g.integers(1, min(32, len(k[i])) + 1))
+                if to % 32 == 0 or held[i][to // 32 % 2] == to // 32:
+                    cut(i, to)
+            new[i] = int(g.choice([0, 1, 1, 1, 2, 3, 33, 70])) if len(k[i]) else int(g.integers(0, 70))
+            new[i] = min(new[i], width * 32 - len(k[i]))
+        past = np.array([len(x) for x in k])
+        need = -(-(past + new) // 32) - -(-past // 32)
+        for i in range(n):
+            if need[:i + 1].sum() > len(free):
+                new[i] = need[i] = 0
+        free = [int(b) for b in g.permutation(free)]
+        T = int(new.sum())
+        room = T + 2
+        b = lt.KvBatch(DeviceArray((n + 1,), np.uint32), DeviceArray((n,), np.uint32), dev(table), room, int(new.max()))
+        used, pos, slots = dev([0], np.uint32), DeviceArray((room,), np.uint32), DeviceArray((room,), np.uint32)
+        ctx.kv_plan(b, dev(past, np.uint32), dev(new, np.uint32), dev(free, np.uint32), used, used, pos, slots)
+        x, y = heads(g, room, KV, D), heads(g, room, KV, D)
+        q = g.standard_normal((room, KV * G, D)).astype(np.float32)
+        out = dev(np.full(q.shape, 5, np.float32))
+        c.append(dev(x), dev(y), b)
+        ctx.attention(out, dev(q), c, b, D ** -0.5, window)
+        ctx.sync()
+        table = b.table.numpy()
+        free = free[int(used.numpy()[0]):]
+        t, got = 0, out.numpy()
+        for i in range(n):
+            k[i], v[i] = (np.concatenate([o, e[t:t + new[i]]]) for o, e in ((k[i], x), (v[i], y)))
+            if new[i]:
+                for j in range(max(past[i] // 32, (len(k[i]) - 1) // 32 - 1), (len(k[i]) - 1) // 32 + 1):
+                    held[i][j % 2] = j
+                at = np.arange(len(k[i]))
+                a, w = read(c, u32(table[i, at // 32].astype(np.int64) * 32 + at % 32))
+                assert same(a, ref.values(k[i])) and same(w, ref.values(v[i])), (step, i)
+                close(got[t:t + new[i]], *ref.attention(q[t:t + new[i]], a, w, np.arange(past[i], len(k[i])), D ** -0.5, window))
+            t += new[i]
+        assert (got[T:] == 5).all()
+        taken = table[table != ref.NONE]
+        assert len(set(taken.tolist())) == len(taken) and len(taken) + len(free) == pool
+    c.free()
