@@ -470,7 +470,7 @@ def timeline_report(args, w, xs, n=200):
         ctx.moe_forward(out, X.row(i % len(xs)), *copies[i % args.copies], K, F, norm_topk=True)
         ctx.sync()
     rep = ctx.profile_report()
-    head = (f"Command (GPU box, repo root): python3 {' '.join(sys.argv)}\n"
+    head = (f"Command (repo root): python3 {' '.join(sys.argv)}\n"
             f"Workload: config-3 decode layer, {n} eager launches, {args.copies} weight copies rotated, "
             f"x pool of {len(xs)}; LT_PROFILE=timeline adds one store per workgroup at its end.\n\n")
     with open(args.timeline, "w") as f:
@@ -748,7 +748,7 @@ def timeline_cfg4(args, c, w, xs, n=200):
         ctx.moe_forward(out, X.row(i % len(xs)), *t[:3], K, G4_F, act=lt.ACT_GELU_TANH, shared=t[3:])
         ctx.sync()
     rep = ctx.profile_report()
-    head = (f"Command (GPU box, repo root): python3 {' '.join(sys.argv)}\n"
+    head = (f"Command (repo root): python3 {' '.join(sys.argv)}\n"
             f"Workload: config-4 layer (shared FFN in the same launch), {n} eager launches, {args.copies} weight "
             f"copies rotated, x pool of {len(xs)}; LT_PROFILE=timeline adds one store per workgroup at its end.\n\n")
     with open(args.timeline, "w") as f:
@@ -934,7 +934,7 @@ def timeline_gemma4(args, c, w, X, dense, dn, n=200):
                                c["eps"])
         ctx.sync()
     rep = ctx.profile_report()
-    head = (f"Command (GPU box, repo root): python3 {' '.join(sys.argv)}\n"
+    head = (f"Command (repo root): python3 {' '.join(sys.argv)}\n"
             f"Workload: Gemma4 block (config-4 layer, router-input prep, MoE tail in the same launch), {n} eager "
             f"launches, {len(copies)} weight copies rotated, x pool of {args.xpool}; LT_PROFILE=timeline adds one "
             f"store per workgroup at its end.\n\n")

@@ -457,8 +457,8 @@ int lt_rope_free(lt_ctx *ctx, lt_rope *rope);
  * alignment).  q, q_out: n_tokens x n_heads heads; k, k_out: n_tokens x n_kv_heads
  * (either number may be 0, then its pointers are not used).  positions:
  * [n_tokens].  Outputs may be their inputs where the strides are alike; otherwise they must
- * not overlap.  Angles are taken in 64 bits, so positions up to 2^32 - 1 keep fp32's
- * accuracy.  Pointers need 4-byte alignment (16, with strides of whole 4 floats and
+ * not overlap.  Angles are counted in 64 bits (what is left of whole turns is rounded to 32 before its
+ * sine), so positions up to 2^32 - 1 keep fp32's accuracy.  Pointers need 4-byte alignment (16, with strides of whole 4 floats and
  * head_dim and n_rot of whole 8, are faster).  flags: LT_HOST_IO,
  * LT_NORM_ONE_PLUS_W, LT_ROPE_NO_NORM.  Replaces the per-head norms and rotations of
  * gemma4/forward.zig (rmsnorm_perhead, rope_* pipelines). */
@@ -508,7 +508,7 @@ int lt_kv_plan(lt_ctx *ctx, const lt_kv_batch *batch, const uint32_t *len_in, co
  * blocks may be shared.  Codes, scales and copies of the tokens appended are
  * written, nothing else.  A sequence that contradicts itself (more tokens than len, ...) or has more than
  * max_new of them is left out and reported; a block that is not in the cache
- * is not written, a block whose earlier tokens are not held becomes all NaN, both are reported.
+ * is not written (nor are its tokens kept), a block whose earlier tokens are not held becomes all NaN, both are reported.
  * flags: LT_HOST_IO. */
 int lt_kv_append(lt_ctx *ctx, lt_kv *kv, const float *k, const float *v, size_t k_stride, size_t v_stride,
                  const lt_kv_batch *batch, uint32_t flags);
@@ -523,8 +523,11 @@ int lt_kv_read(lt_ctx *ctx, float *k_out, float *v_out, const lt_kv *kv, const u
  * max(0, p - window + 1) .. p with window > 0.  The batch's own tokens have been appended.
  * q: n_tokens x n_heads heads; heads h * n_heads / n_kv_heads .. share the cache's head
  * h (n_heads up to 128 times n_kv_heads).  Products take queries and weights to 2^-22 of the largest of a
- * row and are summed in fp32.  NaN comes out where a query, or a key or value that it sees, is not finite (a block
- * is all NaN then); what it does not see changes nothing.  Where the table has no block of the cache for a key,
+ * row and are summed in fp32; a logit (scale * q k) of size s moves an output by up to s 2^-23 of itself, and s should
+ * stay below 10^6.  NaN comes out where a query, or a key or value that it sees, is not finite (a block
+ * is all NaN then).  What it does not see changes nothing but the codes of a block that it sees in part: their
+ * scale is over all tokens of the block so far, so a prompt's outputs depend within the 8 bits on how many
+ * tokens come at a time.  Where the table has no block of the cache for a key,
  * the queries that see it get NaN; so do the tokens of a sequence that contradicts itself (those
  * beyond max_new: are left as they were); both are reported.  out must not overlap q.  flags:
  * LT_HOST_IO.  Replaces sdpAttn (ops/attn.zig:13-44) over all heads, and the attn_* pipelines. */

@@ -24,8 +24,9 @@
 // number of blocks, as many as fill the chip; the part that arrives last at a
 // tile joins them.
 //
-// Bound by memory where the cache is large (48 sequences' caches of 220 MB: 54 us, 4.1 TB/s; one of 134 MB: 32 us,
-// of which the loads take 18 and the two rounds of joining 7); else by instructions (a block of heads of 64
+// Bound by memory where the cache is large (48 sequences' caches of 220 MB: 54 us, 4.1 TB/s; one of 134 MB: 37 us, or 32
+// where the last call's keys are still in the chip's last cache, of which the loads take 18 and the two rounds of
+// joining 7); else by instructions (a block of heads of 64
 // takes a wavefront about 250, of 128 400, of 256 650, 4 cycles each) and the chain of one launch: one
 // token of 14 heads over 1,500 keys 7.6 us, of which lengths 1.3, table 0.7, queries 0.6, codes 0.9, products and the
 // wavefronts' sums 1.5, arrival 0.9, joining 1.6 (taken with integer divisions in lengths, queries and joining; 0.35 less

@@ -15,7 +15,7 @@
 // sixth of them exponentials), 940 cycles.  The two do not run side by side here: together they are
 // what a CU is busy for, with two wavefronts a SIMD of one workgroup or of two, with and
 // without priorities, and with the next block's products between this one's exponentials.  4,095
-// tokens of 32 heads of 128: 267 us, 1.03 PFLOP/s of f16 products (a library's product of 8192^3: 1.14).
+// tokens of 32 heads of 128: 262 us, 1.05 PFLOP/s of f16 products (a library's product of 8192^3: 1.14).
 //
 // Work: whole tiles, the longest first, where there are enough of them; else all
 // tiles' blocks in one line, cut into as many equal pieces as workgroups fit on

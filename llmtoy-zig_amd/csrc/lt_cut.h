@@ -16,10 +16,12 @@
 namespace lt {
 
 // Rows (tokens times heads of a group) of a sequence up to which lt_attention.hip's
-// kernel takes it; the other kernel takes those with more.  With 8 heads of 128 a group, few-row kernel
-// and many-row kernel in us: 48 rows 23 and 54, 256 rows over 4,000 keys 22 and 66, 512 rows over 16,000
-// keys 60 and 79, 8 sequences of 512 rows over 4,000 keys 87 and 80; from there on the latter's
-// tiles of 64 to 256 rows pay.
+// kernel takes it; the other kernel takes those with more.  Few-row and many-row kernel in us, a sequence of
+// 512 rows over 4,000 keys: heads of 64 (2 groups of 7) 16 and 33, of 128 (4 of 8) 29 and 64, 192 (4 of 4) 42 and 62,
+// 256 (8 of 2) 61 and 86, 512 (2 of 8) 50 and 93.  The many-row kernel's tiles of 64 to 256 rows pay with many
+// sequences: 8 of them of 512 rows 40 and 49, 104 and 87, 166 and 161, 407 and 338, 195 and 232; of 1,024 rows 69 and
+// 66, 190 and 157, 322 and 280, 816 and 697, 377 and 403 (one of 1,024: 20 and 35, 51 and 66, 49 and 75, 108 and 118,
+// 95 and 106).  One border for all, between what a sequence alone and what many would have.
 constexpr uint32_t kThinMost = 512;
 
 // The tokens of a sequence that are served: beyond max_new, as many as the grid has room for (and those get NaN).

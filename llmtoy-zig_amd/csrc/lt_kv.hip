@@ -263,7 +263,8 @@ __device__ __forceinline__ void forget(const KvDev &kv, uint32_t page, uint32_t 
 // and writes the codes.
 // Bound by the reads of the new tokens; a single token by its chain of
 // latencies: the lengths, then the table, the tag and the tokens, the largest, the codes.
-// 4,103 tokens of 8 heads of 128 13.1 us (42 MB), 512 5.5; one token each of 16 sequences 6 us.  (Keys
+// 4,103 tokens of 8 heads of 128 12.1 us (42 MB; at a copy's rate 8.1: the values' loads are of 4 bytes, 16 a thread),
+// 512 5.5; one token each of 16 sequences 6 us.  (Keys
 // and values by one workgroup: slower by a third.  A code for keys and one for values: 16.5 -> 13.1 us.)
 template <int D, int which>
 __device__ __forceinline__ void append_unit(const KvDev &kv, const KvBatchDev &b, const float *kv_src, size_t stride, uint32_t *err) {
@@ -398,8 +399,9 @@ __global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, con
 }
 
 // ------------------------------------------------------------------- reading
-// The values of single tokens: a thread four channels of a (slot, head).  Bound
-// by the writes.
+// The values of single tokens: a thread four channels of a (slot, head).  A few tokens are a
+// chain of latencies (one of 16 sequences 4 us); 4,103 tokens of 8 heads of 128 take 14 us for 42 MB, where a copy's
+// rate would take 8.1: a value's four channels are four loads of a byte, 16 bytes apart.
 constexpr int kReadThreads = 256;
 template <int D, int U>
 __global__ __launch_bounds__(kReadThreads) void k_kv_read(KvDev kv, const uint32_t *slots, uint32_t n, float *k, float *v) {

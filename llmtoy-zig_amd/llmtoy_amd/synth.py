@@ -2,7 +2,7 @@
 
 Every tensor is drawn from its own numpy PCG64 stream seeded with
 [0x1A70000 + config, tensor_id], so any tensor can be regenerated alone and
-the GPU box and this container produce identical bytes.  Quantised weights
+every machine produces identical bytes.  Quantised weights
 are raw GGUF block bytes (llmtoy-zig src/quant/dequant.zig layouts);
 f16 fields are round-to-nearest-even conversions of the fp32 draws.
 
