@@ -14,8 +14,8 @@ namespace {
 // takes none.  Both are prefix sums over
 // the rows, which one workgroup takes (kPlanRows a thread); new blocks and
 // tokens then look their row up in the sums.  Bound by its chain of latencies:
-// the lengths, the sums, the table's entry, the slot (8 rows 5.1 us; 2,000 rows 6.2, and the
-// maps of 65,536 tokens 6.1 behind it).
+// the lengths, the sums, the table's entry, the slot (8 rows 5.1 us; 2,000 rows 6.1, and the
+// maps of 65,536 tokens 6.5 behind it).
 constexpr uint32_t kPlanThreads = 1024, kPlanRows = kKvMaxSeqs / kPlanThreads;
 // Tokens of a batch that the one workgroup maps; more go to a grid of their own
 // behind it (k_kv_slots).
@@ -263,7 +263,7 @@ __device__ __forceinline__ void forget(const KvDev &kv, uint32_t page, uint32_t 
 // and writes the codes.
 // Bound by the reads of the new tokens; a single token by its chain of
 // latencies: the lengths, then the table, the tag and the tokens, the largest, the codes.
-// 4,103 tokens of 8 heads of 128 12.1 us (42 MB; at a copy's rate 8.1: the values' loads are of 4 bytes, 16 a thread),
+// 4,103 tokens of 8 heads of 128 12.5 us (42 MB; at a copy's rate 8.1: the values' loads are of 4 bytes, 16 a thread),
 // 512 5.5; one token each of 16 sequences 6 us.  (Keys
 // and values by one workgroup: slower by a third.  A code for keys and one for values: 16.5 -> 13.1 us.)
 template <int D, int which>
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(2 * D) void k_kv_append(KvDev kv, KvBatchDev b, con
 
 // ------------------------------------------------------------------- reading
 // The values of single tokens: a thread four channels of a (slot, head).  A few tokens are a
-// chain of latencies (one of 16 sequences 4 us); 4,103 tokens of 8 heads of 128 take 14 us for 42 MB, where a copy's
+// chain of latencies (one of 16 sequences 4 us); 4,103 tokens of 8 heads of 128 take 13.7 us for 42 MB, where a copy's
 // rate would take 8.1: a value's four channels are four loads of a byte, 16 bytes apart.
 constexpr int kReadThreads = 256;
 template <int D, int U>
