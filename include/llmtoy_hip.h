@@ -523,7 +523,7 @@ int lt_kv_read(lt_ctx *ctx, float *k_out, float *v_out, const lt_kv *kv, const u
  * max(0, p - window + 1) .. p with window > 0.  The batch's own tokens have been appended.
  * q: n_tokens x n_heads heads; heads h * n_heads / n_kv_heads .. share the cache's head
  * h (n_heads up to 128 times n_kv_heads).  Products take queries and weights to 2^-22 of the largest of a
- * row and are summed in fp32; a logit (scale * q k) of size s moves an output by up to s 2^-23 of itself, and s should
+ * row and are summed in fp32; a logit (scale * q k) of size s moves an output by up to s 2^-20 of itself, and s should
  * stay below 10^6.  NaN comes out where a query, or a key or value that it sees, is not finite (a block
  * is all NaN then).  What it does not see changes nothing but the codes of a block that it sees in part: their
  * scale is over all tokens of the block so far, so a prompt's outputs depend within the 8 bits on how many

@@ -68,16 +68,16 @@ struct Tile {
     uint32_t lo, hi;    // blocks lo .. hi - 1
 };
 
-__device__ __forceinline__ uint32_t row_rows(const WideArgs &a, const KvRow &k) {
-    const uint32_t rows = cut_tokens(k.n, a.b.max_new) * a.group;
-    return rows > kThinMost ? rows : 0;
+template <int R>
+__device__ __forceinline__ uint32_t row_tiles(const WideArgs &a, uint32_t row) {
+    return wide_row_tiles(cut_tokens(kv_row_of(a.b, row).n, a.b.max_new), a.group, R);
 }
 
 template <int R>
 __device__ __forceinline__ Tile tile_of(const WideArgs &a, uint32_t row, uint32_t t) {
     Tile x;
     x.k = kv_row_of(a.b, row);
-    const uint32_t all = row_rows(a, x.k);
+    const uint32_t all = cut_tokens(x.k.n, a.b.max_new) * a.group;
     x.r0 = t * R;
     x.rows = all - x.r0 < R ? all - x.r0 : R;
     x.lo = 0, x.hi = 1;
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         const uint32_t r = tid * per + i;
         if (r >= a.b.n_seqs) break;
         const KvRow k = kv_row_of(a.b, r);
-        mine += (row_rows(a, k) + R - 1) / R;
+        mine += wide_row_tiles(cut_tokens(k.n, a.b.max_new), a.group, R);
         if (k.falls && blockIdx.x == 0) kv_report(a.err, kKvErrRows, r);
     }
     const uint64_t before0 = scan<W>(mine, s_sum, every);
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
         for (uint32_t i = 0; i < per; i++) {
             const uint32_t r = tid * per + i;
             if (r >= a.b.n_seqs) break;
-            const uint32_t c = (row_rows(a, kv_row_of(a.b, r)) + R - 1) / R;
+            const uint32_t c = row_tiles<R>(a, r);
             if (t >= at && t < at + c) s_hit[0] = r, s_hit[1] = t - at;
             at += c;
         }
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, Shape<D>::kPerCu) void k_attent
             const uint32_t r = tid * per + i;
             if (r >= a.b.n_seqs) break;
             s_base[r] = at;
-            at += (row_rows(a, kv_row_of(a.b, r)) + R - 1) / R;
+            at += row_tiles<R>(a, r);
         }
         __syncthreads();
         const uint32_t per2 = (all_tiles + NT - 1) / NT;

@@ -227,14 +227,23 @@ def _place(a, is_host: bool) -> int:
     return HOST if is_host else a.get_device() if _is_torch(a) else SOME_DEVICE
 
 
-def _all_host(ctx: "Context", places: set) -> bool:
-    """Whether a call's arrays are host memory; all of them or none, and none on another device than the context's."""
-    if HOST in places:
-        if len(places) > 1:
-            raise InvalidError("mix of host and device arrays")
+def _meet(p: int, q: int) -> int:
+    """The place of arrays at p and at q."""
+    if p == q:
+        return p
+    if HOST in (p, q):
+        raise InvalidError("mix of host and device arrays")
+    if SOME_DEVICE in (p, q):
+        return max(p, q)
+    raise InvalidError(f"an array on device {max(p, q)}, another on device {min(p, q)}")
+
+
+def _is_host(ctx: "Context", place: int) -> bool:
+    """Whether a call's arrays are host memory; on another device than the context's they are refused."""
+    if place == HOST:
         return True
-    if not places <= ctx.places:
-        raise InvalidError(f"an array on device {max(places - ctx.places)}, the context is on {ctx.device}")
+    if place != ctx.device and place != SOME_DEVICE:
+        raise InvalidError(f"an array on device {place}, the context is on {ctx.device}")
     return False
 
 
@@ -299,12 +308,12 @@ class KvBatch:
         self.n_seqs, self.n_tokens, self.max_blocks, self.max_new = n, int(n_tokens), int(table.shape[1]), int(max_new)
 
     def struct(self):
-        """(lt_kv_batch, the places of its arrays)"""
+        """(lt_kv_batch, the place of its arrays)"""
         n = self.n_seqs
         p, h0 = _words(self.start, n + 1, "start")
         q, h1 = _words(self.len, n, "len")
         t, h2 = _words(self.table, n * self.max_blocks, "table")
-        return KvBatchStruct(n, self.n_tokens, self.max_blocks, self.max_new, p, q, t), {h0, h1, h2}
+        return KvBatchStruct(n, self.n_tokens, self.max_blocks, self.max_new, p, q, t), h0 if h0 == h1 == h2 else _meet(_meet(h0, h1), h2)
 
 
 class KvCache:
@@ -320,10 +329,10 @@ class KvCache:
 
     def append(self, k, v, batch: KvBatch):
         """The batch's tokens' keys and values ([n_tokens, n_kv_heads, head_dim]) into the cache."""
-        b, places = batch.struct()
+        b, place = batch.struct()
         gk, gv = self._mine(k, "k", batch.n_tokens), self._mine(v, "v", batch.n_tokens)
         c = self.ctx
-        host = _all_host(c, places | {gk[1], gv[1]})
+        host = _is_host(c, _meet(_meet(place, gk[1]), gv[1]))
         c._check(c.lib.lt_kv_append(c.ptr, self.handle, gk[0], gv[0], gk[5], gv[5], C.byref(b), LT_HOST_IO if host else 0))
 
     def read(self, k_out, v_out, slots):
@@ -335,7 +344,7 @@ class KvCache:
             if g[5] != self.n_kv_heads * self.head_dim:
                 raise InvalidError(f"{w}: must be contiguous")
         c = self.ctx
-        host = _all_host(c, {place, gk[1], gv[1]})
+        host = _is_host(c, _meet(_meet(place, gk[1]), gv[1]))
         c._check(c.lib.lt_kv_read(c.ptr, gk[0], gv[0], self.handle, p, n, LT_HOST_IO if host else 0))
 
     def _mine(self, a, what, tokens):
@@ -360,7 +369,7 @@ class Context:
         if rc != LT_OK:
             raise _ERRS.get(rc, LtError)(f"lt_init({device}) failed with status {rc}", rc)
         self.ptr = p
-        self.device, self.places = device, {device, SOME_DEVICE}  # (places: of device arrays that it takes)
+        self.device = device
 
     def close(self):
         if self.ptr:
@@ -542,13 +551,13 @@ class Context:
         none = (None, None, 0, 0, 0, 0)
         gq, gqo = _heads(q, "q"), _heads(q_out, "q_out")
         gk, gko = (none, none) if k is None else (_heads(k, "k"), _heads(k_out, "k_out"))
-        T, places = gq[2], set()
+        T, place = gq[2], gq[1]
         for w, g, first in (("q", gq, gq), ("q_out", gqo, gq), ("k", gk, gk), ("k_out", gko, gk)):
             if g[0] is None:
                 continue
             if g[2] != T or g[4] != rope.head_dim or g[3] != first[3]:
                 raise InvalidError(f"{w}: {g[2:5]}, {T} tokens of heads of {rope.head_dim} expected")
-            places.add(g[1])
+            place = _meet(place, g[1])
         ps = []
         for w, a in (("wq", wq), ("wk", wk)):
             if a is not None and (tuple(a.shape) != (rope.head_dim,) or _kind(a.dtype) != "float32"):
@@ -556,10 +565,9 @@ class Context:
             p, h = _ptr(a)
             ps.append(p)
             if a is not None:
-                places.add(_place(a, h))
+                place = _meet(place, _place(a, h))
         p, h = _words(positions, T, "positions")
-        places.add(h)
-        host = _all_host(self, places)
+        host = _is_host(self, _meet(place, h))
         fl = (LT_HOST_IO if host else 0) | (0 if norm else LT_ROPE_NO_NORM) | (LT_NORM_ONE_PLUS_W if one_plus_w else 0)
         self._check(self.lib.lt_qk_norm_rope(self.ptr, gqo[0], gko[0], gq[0], gk[0], ps[0], ps[1], p, rope.handle,
                                              T, gq[3], gk[3], gq[5], gk[5], gqo[5], gko[5], eps, fl))
@@ -573,21 +581,22 @@ class Context:
     def kv_plan(self, batch: KvBatch, len_in, n_new, free_blocks, used_in, used_out, positions, slots):
         """A step's batch (start, len, new entries of table), positions and slots from the sequences'
         lengths and a list of free blocks (lt_kv_plan)."""
-        b, places = batch.struct()
+        b, place = batch.struct()
         n_free = _count(free_blocks)
         p, T = [], batch.n_tokens
         for w, a, n in (("len_in", len_in, b.n_seqs), ("n_new", n_new, b.n_seqs), ("free_blocks", free_blocks, n_free),
                         ("used_in", used_in, 1), ("used_out", used_out, 1), ("positions", positions, T), ("slots", slots, T)):
             at, h = _words(a, n, w)
-            places.add(h)
+            if h != place:
+                place = _meet(place, h)
             p.append(at)
-        host = _all_host(self, places)
+        host = _is_host(self, place)
         self._check(self.lib.lt_kv_plan(self.ptr, C.byref(b), p[0], p[1], p[2], n_free, p[3], p[4], p[5], p[6],
                                         LT_HOST_IO if host else 0))
 
     def attention(self, out, q, cache: KvCache, batch: KvBatch, scale: float, window: int = 0):
         """out [n_tokens, heads, head_dim]: the queries over the cache, causal (lt_attention)."""
-        b, places = batch.struct()
+        b, place = batch.struct()
         gq, go = _heads(q, "q"), _heads(out, "out")
         T, H, D = gq[2:5]
         if T != batch.n_tokens or D != cache.head_dim or go[2:5] != gq[2:5]:
@@ -595,7 +604,7 @@ class Context:
                                f"{cache.head_dim}")
         if go[5] != H * D:
             raise InvalidError("out: must be contiguous")
-        host = _all_host(self, places | {gq[1], go[1]})
+        host = _is_host(self, _meet(_meet(place, gq[1]), go[1]))
         self._check(self.lib.lt_attention(self.ptr, go[0], gq[0], cache.handle, C.byref(b), H, gq[5], scale, window,
                                           LT_HOST_IO if host else 0))
         return out

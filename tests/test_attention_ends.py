@@ -41,7 +41,7 @@ _Elsewhere.__module__ = "torch"
 def test_arrays_on_another_device_or_on_none():
     f32, i32 = torch.float32, torch.int32
     c = ltlib.Context.__new__(ltlib.Context)  # (no device is asked: every call is refused before)
-    c.ptr, c.lib, c.device, c.places = None, None, 0, {0, ltlib.SOME_DEVICE}
+    c.ptr, c.lib, c.device = None, None, 0
     cache, rope = ltlib.KvCache(c, None, 4, 2, 64, 3), ltlib.Rope(c, None, 64)
     t = _Elsewhere
     batch = lambda d: ltlib.KvBatch(t((4,), i32, d), t((3,), i32, d), t((3, 2), i32, d), 5)  # noqa: E731
