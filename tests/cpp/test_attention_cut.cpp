@@ -99,8 +99,8 @@ static void few(const Batch &b, uint32_t D) {
     const uint64_t bytes = thin_workspace(D, b.n_kv), part = 16 * (D + 4) * 4;
     CHECK(bytes >= 2 * part * slots * b.n_kv && bytes < 1ull << 32);
     CHECK(bytes <= 2 * part * (2 * target + 4 * b.n_kv));
-    // (none to do: then no sequence has rows for this kernel)
-    if (b.n_tokens && grid == 0) CHECK(work == 0);
+    // (no launch without a workgroup)
+    CHECK(!b.n_tokens || grid > 0);
 }
 
 // Many rows.
